@@ -6,7 +6,10 @@
 // i = row, j = column < cols/2, gate_off = cols/2.  Column-major input (the reference's "fall back
 // to 2D" path, memory [cols][ld]): i = column < cols/2, j = row, gate_off = (cols/2)*ld.
 // A lane owns 8 consecutive j (16-byte accesses for 16-bit types) when the extents allow it.
-#include "tf24_common.hpp"
+//
+// The second pair of kernels keeps the input in 8 bits only (checkpoint8.hpp: as a matrix of 2 * rows rows, x and gate of a row one after the
+// other): the forward pass encodes what it reads, and on request what it writes, the backward pass decodes it.
+#include "checkpoint8.hpp"
 
 namespace tf24 {
 namespace {
@@ -77,6 +80,61 @@ gelu_glu_bwd(const T* __restrict__ grad_out, int64_t ld_go, const T* __restrict_
   }
   gx.store_stream(grad_in + i * ld_gi + j);
   gg.store_stream(grad_in + i * ld_gi + j + gate_off_gi);
+}
+
+// Row-major input, `half` columns of x and as many of gate in each row; a lane owns a unit of the output's columns.  What is kept of the
+// input has units and blocks of 2 * rows rows, that of the output of `rows` rows (numbered as the lanes are).
+template <typename T, bool KEEP_OUT>
+__global__ void __launch_bounds__(kThreads)
+gelu_glu_fwd_keep(const T* __restrict__ in, int64_t ld_in, int half, UnitRows by, uint32_t total, T* __restrict__ out, int64_t ld_out, uint8_t* __restrict__ values,
+                  uint8_t* __restrict__ scales, uint8_t* __restrict__ out_values, uint8_t* __restrict__ out_scales) {
+  const uint32_t u = blockIdx.x * kThreads + threadIdx.x;
+  if (u >= total) return;                                        // (a multiple of 4: whole blocks)
+  const uint32_t row = row_of_unit(by, u), first = row * by.units, col = (u - first) * kKeptUnit;
+  const int n = min(max(half - (int)col, 0), 8);
+  float x[8], g[8], o[8];
+  load_up_to_8(in + (int64_t)row * ld_in + col, n, x);
+  load_up_to_8(in + (int64_t)row * ld_in + half + col, n, g);
+#pragma unroll
+  for (int e = 0; e < 8; e++) o[e] = glu_terms<false>(g[e]).gelu * x[e];
+  store_up_to_8(out + (int64_t)row * ld_out + col, n, o);
+  const Kept8 kx = keep_8<T>(x), kg = keep_8<T>(g);
+  const uint64_t ux = (uint64_t)u + first, ug = ux + by.units;  // rows 2 row and 2 row + 1
+  *reinterpret_cast<uint2*>(values + ux * 8) = kx.values;
+  *reinterpret_cast<uint2*>(values + ug * 8) = kg.values;
+  if ((u & 3) == 0) {
+    scales[ux >> 2] = (uint8_t)kx.scale;
+    scales[ug >> 2] = (uint8_t)kg.scale;
+  }
+  if constexpr (KEEP_OUT) {
+    const Kept8 ko = keep_8<T>(o);
+    *reinterpret_cast<uint2*>(out_values + (uint64_t)u * 8) = ko.values;
+    if ((u & 3) == 0) out_scales[u >> 2] = (uint8_t)ko.scale;
+  }
+}
+
+template <typename T>
+__global__ void __launch_bounds__(kThreads)
+gelu_glu_bwd_kept(const T* __restrict__ grad_out, int64_t ld_go, const uint8_t* __restrict__ values, const uint8_t* __restrict__ scales, int half, UnitRows by,
+                  uint32_t total, T* __restrict__ grad_in, int64_t ld_gi) {
+  const uint32_t u = blockIdx.x * kThreads + threadIdx.x;
+  if (u >= total) return;
+  const uint32_t row = row_of_unit(by, u), first = row * by.units, col = (u - first) * kKeptUnit;
+  const int n = min(half - (int)col, 8);
+  if (n <= 0) return;
+  const uint64_t ux = (uint64_t)u + first, ug = ux + by.units;
+  float go[8], x[8], g[8], gx[8], gg[8];
+  load_up_to_8(grad_out + (int64_t)row * ld_go + col, n, go);
+  kept_to_float(*reinterpret_cast<const uint2*>(values + ux * 8), scales[ux >> 2], x);
+  kept_to_float(*reinterpret_cast<const uint2*>(values + ug * 8), scales[ug >> 2], g);
+#pragma unroll
+  for (int e = 0; e < 8; e++) {
+    const GluTerms t = glu_terms<true>(g[e]);
+    gx[e] = go[e] * t.gelu;
+    gg[e] = go[e] * x[e] * t.dgelu;
+  }
+  store_up_to_8(grad_in + (int64_t)row * ld_gi + col, n, gx);
+  store_up_to_8(grad_in + (int64_t)row * ld_gi + half + col, n, gg);
 }
 
 struct View {
@@ -170,4 +228,66 @@ extern "C" int tf24_gelu_glu_backward(const void* grad_out, int64_t ld_grad_out,
     case TF24_F16: return backward<f16_t>(grad_out, ld_grad_out, in, layout, ld_in, rows, cols, grad_in, ld_grad_in, s);
     default: return backward<bf16_t>(grad_out, ld_grad_out, in, layout, ld_in, rows, cols, grad_in, ld_grad_in, s);
   }
+}
+
+namespace tf24 {
+namespace {
+
+int check_kept(const char* fn, int dtype, int64_t rows, int64_t cols, int64_t ld_full, int64_t ld_half) {
+  if (dtype != TF24_F32 && dtype != TF24_F16 && dtype != TF24_BF16) return fail(TF24_ERR_DTYPE, "%s: unsupported dtype %d", fn, dtype);
+  if (rows < 0 || cols < 2 || cols % 2 || cols > (int64_t)1 << 30)
+    return fail(TF24_ERR_SHAPE, "%s: shape (%lld, %lld) is not supported: the last dimension must be even", fn, (long long)rows, (long long)cols);
+  if (rows > 0x7fffffffLL / (kept_blocks(cols / 2) * kKeptLanes)) return fail(TF24_ERR_SHAPE, "%s: tensor too large", fn);
+  if (rows > 1 && (ld_full < cols || ld_half < cols / 2))
+    return fail(TF24_ERR_STRIDE, "%s: leading dimensions %lld, %lld too small", fn, (long long)ld_full, (long long)ld_half);
+  return TF24_OK;
+}
+
+template <typename T>
+int forward_keep(const void* in, int64_t ld_in, int64_t rows, int64_t cols, void* out, int64_t ld_out, void* values, void* scales, void* out_values, void* out_scales,
+                 hipStream_t s) {
+  const UnitRows by = unit_rows(cols / 2);
+  const uint32_t total = (uint32_t)rows * by.units;
+  auto* kernel = out_values ? gelu_glu_fwd_keep<T, true> : gelu_glu_fwd_keep<T, false>;
+  hipLaunchKernelGGL(kernel, dim3((total + kThreads - 1) / kThreads), dim3(kThreads), 0, s, (const T*)in, ld_in, (int)(cols / 2), by, total, (T*)out, ld_out,
+                     (uint8_t*)values, (uint8_t*)scales, (uint8_t*)out_values, (uint8_t*)out_scales);
+  return check_launch("tf24_gelu_glu_forward_checkpoint");
+}
+
+template <typename T>
+int backward_kept(const void* go, int64_t ld_go, const void* values, const void* scales, int64_t rows, int64_t cols, void* gi, int64_t ld_gi, hipStream_t s) {
+  const UnitRows by = unit_rows(cols / 2);
+  const uint32_t total = (uint32_t)rows * by.units;
+  hipLaunchKernelGGL(gelu_glu_bwd_kept<T>, dim3((total + kThreads - 1) / kThreads), dim3(kThreads), 0, s, (const T*)go, ld_go, (const uint8_t*)values,
+                     (const uint8_t*)scales, (int)(cols / 2), by, total, (T*)gi, ld_gi);
+  return check_launch("tf24_gelu_glu_backward_checkpoint");
+}
+
+}  // namespace
+}  // namespace tf24
+
+extern "C" int tf24_gelu_glu_forward_checkpoint(const void* in, int dtype, int64_t ld_in, int64_t rows, int64_t cols, void* out, int64_t ld_out, void* values,
+                                                void* scales, void* out_values, void* out_scales, void* stream) {
+  using namespace tf24;
+  const char* fn = "tf24_gelu_glu_forward_checkpoint";
+  if (int rc = check_kept(fn, dtype, rows, cols, ld_in, ld_out)) return rc;
+  if (!rows) return TF24_OK;
+  if (!in || !out || !values || !scales || !out_values != !out_scales) return fail(TF24_ERR_ARG, "%s: null pointer", fn);
+  if (int rc = check_aligned(fn, dtype_size(dtype), {in, out})) return rc;
+  if (int rc = check_aligned(fn, 16, {values, out_values})) return rc;
+  auto* go = dtype == TF24_F32 ? forward_keep<float> : dtype == TF24_F16 ? forward_keep<f16_t> : forward_keep<bf16_t>;
+  return go(in, ld_in, rows, cols, out, ld_out, values, scales, out_values, out_scales, (hipStream_t)stream);
+}
+
+extern "C" int tf24_gelu_glu_backward_checkpoint(const void* grad_out, int64_t ld_grad_out, const void* values, const void* scales, int dtype, int64_t rows,
+                                                 int64_t cols, void* grad_in, int64_t ld_grad_in, void* stream) {
+  using namespace tf24;
+  const char* fn = "tf24_gelu_glu_backward_checkpoint";
+  if (int rc = check_kept(fn, dtype, rows, cols, ld_grad_in, ld_grad_out)) return rc;
+  if (!rows) return TF24_OK;
+  if (!grad_out || !values || !scales || !grad_in) return fail(TF24_ERR_ARG, "%s: null pointer", fn);
+  if (int rc = check_aligned(fn, dtype_size(dtype), {grad_out, grad_in})) return rc;
+  if (int rc = check_aligned(fn, 16, {values})) return rc;
+  auto* go = dtype == TF24_F32 ? backward_kept<float> : dtype == TF24_F16 ? backward_kept<f16_t> : backward_kept<bf16_t>;
+  return go(grad_out, ld_grad_out, values, scales, rows, cols, grad_in, ld_grad_in, (hipStream_t)stream);
 }

@@ -15,7 +15,9 @@ from .dense_ops import (soft_threshold24, sparse24, MVUE24_approx,
                         soft_threshold24_torch, sparse24_torch, MVUE24_approx_torch)
 from .sparse_linear_transpose import SparseLinearTranspose, sparse_linear_transpose
 from .sparse_semi_structured_linear import sparse_semi_structured_linear
-from .GELUglu import GELUglu, gelu_glu
+from .GELUglu import GELUglu, gelu_glu, gelu_glu_checkpoint
+from .activation_checkpoint import ActivationCheckpoint, checkpoint_activation
+from .block_norm import BlockNorm, ResidualNorm, block_norm, residual_norm
 from .sparse_ops import MyLinear, SparseLinear, SoftThreshold, SoftThresholdLinear, Sparse24
 
 __all__ = [
@@ -28,6 +30,8 @@ __all__ = [
     "soft_threshold24_torch", "sparse24_torch", "MVUE24_approx_torch",
     "SparseLinearTranspose", "sparse_linear_transpose",
     "sparse_semi_structured_linear",
-    "GELUglu", "gelu_glu",
+    "GELUglu", "gelu_glu", "gelu_glu_checkpoint",
+    "ActivationCheckpoint", "checkpoint_activation",
+    "BlockNorm", "ResidualNorm", "block_norm", "residual_norm",
     "MyLinear", "SparseLinear", "SoftThreshold", "SoftThresholdLinear", "Sparse24",
 ]

@@ -19,6 +19,7 @@ ROW_MAJOR, COL_MAJOR = 0, 1
 PRUNE_MAGNITUDE, PRUNE_MASK, PRUNE_MVUE, PRUNE_MVUE_PACKED, PRUNE_MVUE_SEEDED, PRUNE_MVUE_SEEDED_DEVICE = 0, 1, 2, 3, 4, 5
 ACT_NONE, ACT_RELU, ACT_SILU, ACT_GELU = 0, 1, 2, 3
 BIAS_F32 = 0x100                                   # or-ed to the activation of a product
+NORM_NONE, NORM_RMS, NORM_LAYER = 0, 1, 2
 COMPRESSED_CANONICAL, COMPRESSED_PANEL, COMPRESSED_CUTLASS = 0, 1, 2
 
 _DTYPES = {
@@ -60,6 +61,15 @@ _SIGNATURES = {
     "tf24_adamw_masked_decay_list": (_i, [_p, _i, _i, _i, _d, _d, _d, _d, _d, _d, _i64, _p]),
     "tf24_gelu_glu_forward": (_i, [_p, _i, _i, _i64, _i64, _i64, _p, _i64, _p]),
     "tf24_gelu_glu_backward": (_i, [_p, _i64, _p, _i, _i, _i64, _i64, _i64, _p, _i64, _p]),
+    "tf24_checkpoint_blocks": (_i64, [_i64]),
+    "tf24_checkpoint_encode": (_i, [_p, _i, _i64, _i64, _i64, _p, _p, _p]),
+    "tf24_checkpoint_decode": (_i, [_p, _p, _i64, _i64, _p, _i, _i64, _p]),
+    "tf24_gelu_glu_forward_checkpoint": (_i, [_p, _i, _i64, _i64, _i64, _p, _i64, _p, _p, _p, _p, _p]),
+    "tf24_gelu_glu_backward_checkpoint": (_i, [_p, _i64, _p, _p, _i, _i64, _i64, _p, _i64, _p]),
+    "tf24_block_norm_forward": (_i, [_p, _i64, _p, _i64, _i, _i, _i64, _i64, _p, _i, _i64, _i64, _p, _p, _p, _p, _i, _i, _i, _f, _f, _p, _p, _p, _p, _p, _p]),
+    "tf24_block_norm_backward": (_i, [_p, _i64, _p, _i64, _p, _i64, _p, _i64, _i, _i, _i64, _i64, _p, _i, _i64, _i64, _p, _p, _p, _i, _i, _i, _i, _f,
+                                      _p, _p, _p, _p, _p, _p, _p, _p, _p, _i64, _p]),
+    "tf24_block_norm_backward_workspace_bytes": (_i64, [_i64, _i64, _i64]),
     "tf24_adamw_step": (_i, [_p, _p, _i, _p, _p, _p, _p, _i64, _d, _d, _d, _d, _d, _i64, _p, _i, _p]),
     "tf24_adamw_step_partials": (_i64, [_i64]),
     "tf24_spmm": (_i, [_p, _p, _i, _i, _i64, _i64, _p, _i, _i64, _i64, _p, _i, _i, _i64, _p, _f, _i, _p, _i64, _p]),
@@ -137,6 +147,15 @@ def check(rc):
         raise RuntimeError(lib().tf24_last_error().decode() or f"tf24 call failed with code {rc}")
 
 
+def launch(tensor, call, *arguments):
+    """call(*arguments, stream) on the current stream of the tensor's device, whichever device is the current one."""
+    if tensor.get_device() == torch.cuda.current_device():
+        check(call(*arguments, stream_ptr()))
+    else:
+        with torch.cuda.device(tensor.device):
+            check(call(*arguments, stream_ptr()))
+
+
 _raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None)
 
 
@@ -210,6 +229,17 @@ def as_matrix(t, like=None):
     if lay is None or t.data_ptr() % 16 or lay[1] % 8:
         return t.contiguous()
     return t
+
+
+def as_rows(t):
+    """t as a matrix [rows, columns] whose rows are contiguous, and its leading dimension (0 or more: rows may overlap); a copy where
+    its storage does not allow that."""
+    if t.is_neg():
+        t = t.resolve_neg()
+    flat = t if t.dim() == 2 else t.reshape(-1, t.shape[-1])
+    if flat.shape[1] > 1 and flat.stride(1) != 1:
+        flat = flat.contiguous()
+    return flat, flat.stride(0)
 
 
 def ptr(t):

@@ -1,0 +1,81 @@
+"""Activations kept in 8 bits for the backward pass.
+
+    checkpoint_activation(x)      -> ActivationCheckpoint: x in blocks of 32 columns, float8 values and a power of two each
+    ActivationCheckpoint.decode() -> the values that are kept
+
+What a layer keeps of its input between the two passes is most of a training step's memory.  A checkpoint takes 33/64 of a 16-bit
+matrix, and a gradient formed from it differs from the exact one by what rounding to 4 bits of mantissa does to the input
+(at most 2^-4 of each element, 2^-5.6 of the whole in the mean).  The layers keep one of their input when asked to (SparseLinearTranspose,
+SoftThresholdLinear, GELUglu with checkpoint=True); the operators in front of a layer write one along with their output
+(block_norm, residual_norm, GELUglu), which saves the pass that reads the input again.  The reference keeps its activations
+as they are.
+"""
+import torch
+
+from . import _native as N
+
+__all__ = ["ActivationCheckpoint", "checkpoint_activation"]
+
+_BLOCK = 32
+_TYPES = (torch.float32, torch.float16, torch.bfloat16)
+
+
+class ActivationCheckpoint:
+    """A tensor kept in 8 bits: `values` (float8_e4m3fn, [rows, 32 * blocks]) times 2^(`scales` - 127) (uint8, [rows, blocks]); a
+    row is one of the tensor's last dimension, filled up with zeros.  `shape` and `dtype` are the tensor's.  Infinities and NaNs
+    are kept as NaNs.  It is data: no gradient passes through it."""
+
+    __slots__ = ("values", "scales", "shape", "dtype")
+
+    def __init__(self, values, scales, shape, dtype):
+        shape = torch.Size(shape)
+        rows, blocks = shape[:-1].numel(), (shape[-1] + _BLOCK - 1) // _BLOCK
+        if (values.shape != (rows, _BLOCK * blocks) or scales.shape != (rows, blocks) or values.dtype != torch.float8_e4m3fn
+                or scales.dtype != torch.uint8 or values.device != scales.device or not values.is_contiguous() or not scales.is_contiguous()
+                or dtype not in _TYPES):
+            raise RuntimeError(f"ActivationCheckpoint: values {tuple(values.shape)} {values.dtype} and scales {tuple(scales.shape)} {scales.dtype} "
+                               f"do not hold a tensor {tuple(shape)} {dtype}")
+        self.values, self.scales, self.shape, self.dtype = values, scales, shape, dtype
+
+    @property
+    def device(self):
+        return self.values.device
+
+    @property
+    def nbytes(self):
+        return self.values.numel() + self.scales.numel()
+
+    def decode(self, dtype=None):
+        """The kept values, in the type of the tensor that was kept (exact) or in another one (rounded)."""
+        dtype = self.dtype if dtype is None else dtype
+        if dtype not in _TYPES:
+            raise RuntimeError(f"ActivationCheckpoint.decode: dtype {dtype} is not supported")
+        out = torch.empty(self.shape, dtype=dtype, device=self.values.device)
+        rows, cols = self.values.shape[0], self.shape[-1]
+        N.launch(out, N.lib().tf24_checkpoint_decode, self.values.data_ptr(), self.scales.data_ptr(), rows, cols, out.data_ptr(), N.dtype_code(dtype), cols)
+        return out
+
+    def __repr__(self):
+        return f"ActivationCheckpoint(shape={tuple(self.shape)}, dtype={self.dtype}, device={self.device})"
+
+
+def empty_checkpoint(rows, cols, device):
+    """(values, scales) for a matrix of rows x cols"""
+    blocks = (cols + _BLOCK - 1) // _BLOCK
+    return (torch.empty((rows, _BLOCK * blocks), dtype=torch.float8_e4m3fn, device=device),
+            torch.empty((rows, blocks), dtype=torch.uint8, device=device))
+
+
+def checkpoint_activation(x):
+    """x (float32, float16 or bfloat16, on a GPU, at least one dimension and one column) kept in 8 bits."""
+    if not x.is_cuda:
+        raise RuntimeError("checkpoint_activation: only CUDA tensors are supported")
+    if x.dtype not in _TYPES:
+        raise RuntimeError(f"checkpoint_activation: dtype {x.dtype} is not supported")
+    if x.dim() == 0 or x.shape[-1] == 0:
+        raise RuntimeError(f"checkpoint_activation: shape {tuple(x.shape)} has no columns")
+    flat, ld = N.as_rows(x.detach())
+    rows, cols = flat.shape
+    values, scales = empty_checkpoint(rows, cols, x.device)
+    N.launch(x, N.lib().tf24_checkpoint_encode, flat.data_ptr(), N.dtype_code(x.dtype), ld, rows, cols, values.data_ptr(), scales.data_ptr())
+    return ActivationCheckpoint(values, scales, x.shape, x.dtype)

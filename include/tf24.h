@@ -426,6 +426,65 @@ int tf24_gelu_glu_backward(const void* grad_out, int64_t ld_grad_out, const void
                            void* stream);
 
 /*
+ * Activations kept in 8 bits for the backward pass.  A matrix [rows, cols] (F32|F16|BF16, row-major, leading dimension ld, any
+ * alignment of its elements) is kept as blocks of 32 adjacent columns of a row, the last block of a row filled up with zeros:
+ *     values  rows * blocks * 32 bytes of OCP e4m3 (16-byte aligned), scales  rows * blocks bytes;  blocks = tf24_checkpoint_blocks(cols)
+ * A scale byte b stands for 2^(b - 127), a value for e4m3 * 2^(b - 127).  The scale is the power of two for which the largest
+ * finite magnitude of the block lies in (224, 448] scales, and at least 2^-117; values are rounded to nearest even.  Magnitudes over
+ * 1.875 * 2^Emax (of `dtype`) are held there, so that the decoded matrix is finite; infinities and NaNs become NaNs.
+ * decode writes the values in any of the three types (exact in the type that was encoded, and in F32).
+ * The reference keeps activations as they are; these calls have no counterpart in it.
+ */
+int64_t tf24_checkpoint_blocks(int64_t cols);
+int tf24_checkpoint_encode(const void* x, int dtype, int64_t ld, int64_t rows, int64_t cols, void* values, void* scales, void* stream);
+int tf24_checkpoint_decode(const void* values, const void* scales, int64_t rows, int64_t cols, void* out, int dtype, int64_t ld, void* stream);
+
+/*
+ * GELU-GLU (row-major) whose backward pass reads its input from 8 bits: `forward` writes, besides out, `in` [rows, cols] as a kept matrix of
+ * 2 * rows rows and cols / 2 columns (x and gate of a row one after the other), and with out_values and out_scales (both or neither) `out`
+ * [rows, cols / 2] as another; `backward` gives the gradient at the kept values.
+ */
+int tf24_gelu_glu_forward_checkpoint(const void* in, int dtype, int64_t ld_in, int64_t rows, int64_t cols, void* out, int64_t ld_out, void* values,
+                                     void* scales, void* out_values, void* out_scales, void* stream);
+int tf24_gelu_glu_backward_checkpoint(const void* grad_out, int64_t ld_grad_out, const void* values, const void* scales, int dtype, int64_t rows,
+                                      int64_t cols, void* grad_in, int64_t ld_grad_in, void* stream);
+
+typedef enum { TF24_NORM_NONE = 0, TF24_NORM_RMS = 1, TF24_NORM_LAYER = 2 } tf24_norm_kind;
+
+/*
+ * Norms before and behind the blocks of a transformer, with the gate and the residual addition between them:
+ *     z = N_post(y) (post_kind NONE: y),   out = scale * x + gate * z,   n = N_pre(out) (pre_kind NONE: not formed)
+ *     RMS: N(v) = v / sqrt(mean(v^2) + eps) * weight + bias,  LAYER: N(v) = (v - mean(v)) / sqrt(var(v) + eps) * weight + bias
+ * x, out [rows, cols] of stream_dtype, y, n of block_dtype (stream F32 with any block type, or both the same 16-bit type); leading
+ * dimensions ld_x, ld_y (rows may overlap; out and n are contiguous), any alignment of the elements, 1 to 16384 columns.
+ * y NULL: n = N_pre(x) alone (no out, gate or post norm).  out is rounded to its type before it is normalised.
+ *   weights, biases [cols] of param_dtype F32|F16|BF16; NULL: ones, zeros
+ *   gate    NULL, or rows / rows_per_gate rows of cols (leading dimension ld_gate), each for rows_per_gate adjacent rows: rows_per_gate = rows
+ *           is a gate per channel, 1 a gate per row
+ *   stats   NULL, or float32 [4][rows] for the backward pass (16-byte aligned)
+ *   values, scales  NULL, or where n is kept in 8 bits (see tf24_checkpoint_encode)
+ * The reference has no such operators: its recipe trains models that bring their own (README.md:56-118).
+ */
+int tf24_block_norm_forward(const void* x, int64_t ld_x, const void* y, int64_t ld_y, int stream_dtype, int block_dtype, int64_t rows, int64_t cols,
+                            const void* gate, int gate_dtype, int64_t ld_gate, int64_t rows_per_gate, const void* post_weight, const void* post_bias,
+                            const void* pre_weight, const void* pre_bias, int param_dtype, int post_kind, int pre_kind, float scale, float eps, void* out,
+                            void* n, float* stats, void* values, void* scales, void* stream);
+/*
+ * Its backward pass: from the gradients of out (NULL: zero) and n, with h = out (residual 0: the x of a call without y) and y as they were and
+ * the stats of the forward pass.  Every result may be NULL: grad_x, grad_y (contiguous), the gradients of weights and biases (of param_dtype),
+ * grad_gate (of gate_dtype, contiguous).  y is read where there is a norm of it or grad_gate is wanted, h where pre_kind is not NONE.
+ *   workspace  for the gradients of parameters and of gates that rows share: tf24_block_norm_backward_workspace_bytes(rows, cols, rows_per_gate or rows)
+ * Sums over rows are float32 in a fixed order, rounded once.  rows >= 1.
+ */
+int tf24_block_norm_backward(const void* grad_out, int64_t ld_grad_out, const void* grad_n, int64_t ld_grad_n, const void* h, int64_t ld_h, const void* y,
+                             int64_t ld_y, int stream_dtype, int block_dtype, int64_t rows, int64_t cols, const void* gate, int gate_dtype, int64_t ld_gate,
+                             int64_t rows_per_gate, const void* post_weight, const void* post_bias, const void* pre_weight, int param_dtype, int post_kind,
+                             int pre_kind, int residual, float scale, const float* stats, void* grad_x, void* grad_y, void* grad_gate,
+                             void* grad_post_weight, void* grad_post_bias, void* grad_pre_weight, void* grad_pre_bias, void* workspace,
+                             int64_t workspace_bytes, void* stream);
+int64_t tf24_block_norm_backward_workspace_bytes(int64_t rows, int64_t cols, int64_t rows_per_gate);
+
+/*
  * Weight and bias gradient of a linear layer whose weight is dense:
  *     dw[i, j] = sum_t g[t, i] * x[t, j],  db[i] = sum_t g[t, i]   (t < tokens, i < m, j < n)
  * g [tokens, m] and x [tokens, n] row-major F16 or BF16 with leading dimensions ldg, ldx (multiples of 8, 16-byte aligned);

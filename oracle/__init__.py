@@ -18,6 +18,7 @@ Pinning status (what fixes each function independently of this file):
   adamw_masked_decay     step-1 closed forms, torch.optim.AdamW over several steps
   adamw_step_update      torch.optim.AdamW (amsgrad on/off) in phase 1, phase 1 at eps = 0 in phase 2, step-1 closed forms of Z
   gelu_glu_forward/_backward  torch's gelu(approximate='tanh') * x and autograd's gradient of it
+  kept, norm, norm_backward   torch's float8_e4m3fn cast; torch's layer_norm / rms_norm in float64 and autograd's gradients
   spmm_ref               dense masked fp32 product (definition); parity of the reference's CUTLASS
                          GEMM itself is unpinned (CUTLASS is an un-vendored, unpinned submodule)
 """
@@ -35,4 +36,5 @@ from .philox import philox4x32_10, mvue_uniforms  # noqa: F401
 from .adamw import adamw_masked_decay  # noqa: F401
 from .adamw_step import adamw_step_update, variance_change_statistic  # noqa: F401
 from .gelu_glu import gelu_glu_forward, gelu_glu_backward  # noqa: F401
+from .block_ops import kept, kept_fast, kept_scale, norm, norm_backward, statistics  # noqa: F401
 from .spmm import spmm_ref, spmm_ref_int, linear_ref  # noqa: F401
