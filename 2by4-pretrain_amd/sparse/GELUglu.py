@@ -86,7 +86,7 @@ class gelu_glu_checkpoint(autograd.Function):
         if input.dtype not in (torch.float32, torch.float16, torch.bfloat16):
             raise RuntimeError(f"gelu_glu_checkpoint: dtype {input.dtype} is not supported")
         x2, ld = N.as_rows(input)
-        rows, cols = x2.shape
+        rows, cols = input.shape[:-1].numel(), input.shape[-1]
         half = cols // 2
         out = torch.empty((*input.shape[:-1], half), dtype=input.dtype, device=input.device)
         values, scales = empty_checkpoint(2 * rows, half, input.device)
@@ -110,8 +110,8 @@ class gelu_glu_checkpoint(autograd.Function):
             return None, None
         values, scales = ctx.saved_tensors
         cols = ctx.shape[-1]
-        go, ld = N.as_rows(grad_output.to(ctx.dtype))
-        rows, half = go.shape
+        go, ld = N.as_rows(grad_output if grad_output.dtype == ctx.dtype else grad_output.to(ctx.dtype))
+        rows, half = ctx.shape[:-1].numel(), cols // 2
         if rows > 1 and ld < half:
             go, ld = go.contiguous(), half
         grad_in = torch.empty(ctx.shape, dtype=ctx.dtype, device=values.device)

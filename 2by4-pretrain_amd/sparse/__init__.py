@@ -17,7 +17,7 @@ from .sparse_linear_transpose import SparseLinearTranspose, sparse_linear_transp
 from .sparse_semi_structured_linear import sparse_semi_structured_linear
 from .GELUglu import GELUglu, gelu_glu, gelu_glu_checkpoint
 from .activation_checkpoint import ActivationCheckpoint, checkpoint_activation
-from .block_norm import BlockNorm, ResidualNorm, block_norm, residual_norm
+from .norms import BlockNorm, ResidualNorm, block_norm, residual_norm
 from .sparse_ops import MyLinear, SparseLinear, SoftThreshold, SoftThresholdLinear, Sparse24
 
 __all__ = [

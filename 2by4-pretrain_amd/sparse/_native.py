@@ -233,9 +233,11 @@ def as_matrix(t, like=None):
 
 def as_rows(t):
     """t as a matrix [rows, columns] whose rows are contiguous, and its leading dimension (0 or more: rows may overlap); a copy where
-    its storage does not allow that."""
+    its storage does not allow that.  (A contiguous tensor of any shape is given back as it is.)"""
     if t.is_neg():
         t = t.resolve_neg()
+    if t.is_contiguous():
+        return t, t.shape[-1]
     flat = t if t.dim() == 2 else t.reshape(-1, t.shape[-1])
     if flat.shape[1] > 1 and flat.stride(1) != 1:
         flat = flat.contiguous()

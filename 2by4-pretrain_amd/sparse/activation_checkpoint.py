@@ -74,8 +74,9 @@ def checkpoint_activation(x):
         raise RuntimeError(f"checkpoint_activation: dtype {x.dtype} is not supported")
     if x.dim() == 0 or x.shape[-1] == 0:
         raise RuntimeError(f"checkpoint_activation: shape {tuple(x.shape)} has no columns")
-    flat, ld = N.as_rows(x.detach())
-    rows, cols = flat.shape
+    flat, ld = N.as_rows(x)
+    cols = x.shape[-1]
+    rows = x.shape[:-1].numel()
     values, scales = empty_checkpoint(rows, cols, x.device)
     N.launch(x, N.lib().tf24_checkpoint_encode, flat.data_ptr(), N.dtype_code(x.dtype), ld, rows, cols, values.data_ptr(), scales.data_ptr())
     return ActivationCheckpoint(values, scales, x.shape, x.dtype)

@@ -26,25 +26,27 @@ _MAX_COLS = 16384
 def _forward(x, y, gate, rows_per_gate, post_weight, post_bias, pre_weight, pre_bias, scale, post_kind, pre_kind, eps, block_dtype, keep, with_stats):
     """(out, n, stats, values, scales), None for what is not formed"""
     flat, ld = N.as_rows(x)
-    rows, cols = flat.shape
+    shape = x.shape
+    rows, cols = shape[:-1].numel(), shape[-1]
     y2 = out = n = stats = values = scales = None
     ld_y = ld_gate = 0
-    param = next((p for p in (post_weight, post_bias, pre_weight, pre_bias) if p is not None), None)
+    param = post_weight if post_weight is not None else post_bias if post_bias is not None else pre_weight if pre_weight is not None else pre_bias
     if y is not None:
         y2, ld_y = N.as_rows(y)
-        out = torch.empty(x.shape, dtype=x.dtype, device=x.device)
+        out = torch.empty_like(x, memory_format=torch.contiguous_format)
     if gate is not None:
         gate, ld_gate = N.as_rows(gate)
     if pre_kind:
-        n = torch.empty(x.shape, dtype=block_dtype, device=x.device)
+        n = torch.empty_like(x if y is None else y, dtype=block_dtype, memory_format=torch.contiguous_format)
         if keep:
             values, scales = empty_checkpoint(rows, cols, x.device)
     if with_stats and (post_kind or pre_kind):
         stats = torch.empty((4, rows), dtype=torch.float32, device=x.device)
-    N.launch(x, N.lib().tf24_block_norm_forward, flat.data_ptr(), ld, N.ptr(y2), ld_y, N.dtype_code(x.dtype), N.dtype_code(block_dtype), rows, cols,
-             N.ptr(gate), N.F32 if gate is None else N.dtype_code(gate.dtype), ld_gate, rows_per_gate, N.ptr(post_weight), N.ptr(post_bias), N.ptr(pre_weight),
-             N.ptr(pre_bias), N.F32 if param is None else N.dtype_code(param.dtype), post_kind, pre_kind, scale, eps, N.ptr(out), N.ptr(n), N.ptr(stats),
-             N.ptr(values), N.ptr(scales))
+    code, ptr = N.dtype_codes, N.ptr
+    N.launch(x, N.lib().tf24_block_norm_forward, flat.data_ptr(), ld, ptr(y2), ld_y, code[x.dtype], code[block_dtype], rows, cols,
+             ptr(gate), N.F32 if gate is None else code[gate.dtype], ld_gate, rows_per_gate, ptr(post_weight), ptr(post_bias), ptr(pre_weight),
+             ptr(pre_bias), N.F32 if param is None else code[param.dtype], post_kind, pre_kind, scale, eps, ptr(out), ptr(n), ptr(stats),
+             ptr(values), ptr(scales))
     return out, n, stats, values, scales
 
 
@@ -54,11 +56,10 @@ class _block_norm(autograd.Function):
         ctx.set_materialize_grads(False)
         out, n, stats, values, scales = _forward(x, y, gate, rows_per_gate, post_weight, post_bias, pre_weight, pre_bias, scale, post_kind, pre_kind, eps,
                                                  block_dtype, keep, True)
-        ctx.residual = y is not None
-        needs_y = post_kind or (gate is not None and ctx.needs_input_grad[2])
-        ctx.save_for_backward((out if ctx.residual else x) if pre_kind else None, y if needs_y else None, gate, post_weight, post_bias, pre_weight, stats)
-        ctx.types = x.dtype, block_dtype, None if pre_bias is None else pre_bias.dtype
-        ctx.shape, ctx.call = x.shape, (rows_per_gate, scale, post_kind, pre_kind)
+        residual = y is not None
+        ctx.save_for_backward((out if residual else x) if pre_kind else None, y if post_kind or (gate is not None and ctx.needs_input_grad[2]) else None, gate,
+                              post_weight, post_bias, pre_weight, stats)
+        ctx.call = x.shape, x.dtype, block_dtype, None if pre_bias is None else pre_bias.dtype, residual, rows_per_gate, scale, post_kind, pre_kind
         if values is not None:
             ctx.mark_non_differentiable(values, scales)
         return out, n, values, scales
@@ -67,69 +68,62 @@ class _block_norm(autograd.Function):
     @once_differentiable
     def backward(ctx, grad_out, grad_n, _values, _scales):
         h, y, gate, post_weight, post_bias, pre_weight, stats = ctx.saved_tensors
-        rows_per_gate, scale, post_kind, pre_kind = ctx.call
-        stream_dtype, block_dtype, pre_bias_dtype = ctx.types
-        needs, shape = ctx.needs_input_grad, ctx.shape
+        shape, stream_dtype, block_dtype, pre_bias_dtype, residual, rows_per_gate, scale, post_kind, pre_kind = ctx.call
+        needs = ctx.needs_input_grad
         if grad_n is None:
             pre_kind = N.NORM_NONE                                 # only the stream goes on
             if grad_out is None:
                 return (None,) * 14
         device = (grad_out if grad_n is None else grad_n).device
-        cols = shape[-1]
-        rows = shape[:-1].numel()
-        param = next((p for p in (post_weight, post_bias, pre_weight) if p is not None), None)
+        rows, cols = shape[:-1].numel(), shape[-1]
+        param = post_weight if post_weight is not None else post_bias if post_bias is not None else pre_weight
         param_dtype = pre_bias_dtype if param is None else param.dtype
         make = torch.empty if rows else torch.zeros                # (sums over no rows)
         grad_x = torch.empty(shape, dtype=stream_dtype, device=device) if needs[0] else None
         grad_y = torch.empty(shape, dtype=block_dtype, device=device) if needs[1] else None
         grad_gate = make(gate.shape, dtype=gate.dtype, device=device) if needs[2] else None
-        grad_post_weight, grad_post_bias = (make(cols, dtype=param_dtype, device=device) if needs[i] and post_kind else None for i in (3, 4))
-        grad_pre_weight, grad_pre_bias = (make(cols, dtype=param_dtype, device=device) if needs[i] and pre_kind else None for i in (5, 6))
+        grads = [make(cols, dtype=param_dtype, device=device) if need and kind else None for need, kind in zip(needs[3:7], (post_kind, post_kind, pre_kind, pre_kind))]
+        sums = any(needs[2:7])
         if rows:
-            lib = N.lib()
+            lib, code, ptr = N.lib(), N.dtype_codes, N.ptr
             dout = dn = h2 = y2 = gate2 = workspace = None
             ld_dout = ld_dn = ld_h = ld_y = ld_gate = nbytes = 0
             if grad_out is not None:
-                dout, ld_dout = N.as_rows(grad_out.to(stream_dtype))
+                dout, ld_dout = N.as_rows(grad_out if grad_out.dtype == stream_dtype else grad_out.to(stream_dtype))
             if pre_kind:
-                dn, ld_dn = N.as_rows(grad_n.to(block_dtype))
+                dn, ld_dn = N.as_rows(grad_n if grad_n.dtype == block_dtype else grad_n.to(block_dtype))
                 h2, ld_h = N.as_rows(h)
             if y is not None:
                 y2, ld_y = N.as_rows(y)
             if gate is not None:
                 gate2, ld_gate = N.as_rows(gate)
-            if needs[2] or needs[3] or needs[4] or needs[5] or needs[6]:
+            if sums:
                 nbytes = lib.tf24_block_norm_backward_workspace_bytes(rows, cols, rows if gate is None else rows_per_gate)
                 workspace = torch.empty(nbytes, dtype=torch.uint8, device=device)
-            N.launch(workspace if dn is None and dout is None else dout if dn is None else dn, lib.tf24_block_norm_backward,
-                     N.ptr(dout), ld_dout, N.ptr(dn), ld_dn, N.ptr(h2), ld_h, N.ptr(y2), ld_y,
-                     N.dtype_code(stream_dtype), N.dtype_code(block_dtype), rows, cols, N.ptr(gate2), N.F32 if gate is None else N.dtype_code(gate.dtype),
-                     ld_gate, rows_per_gate, N.ptr(post_weight), N.ptr(post_bias), N.ptr(pre_weight),
-                     N.F32 if param_dtype is None else N.dtype_code(param_dtype), post_kind, pre_kind, ctx.residual, scale, N.ptr(stats), N.ptr(grad_x),
-                     N.ptr(grad_y), N.ptr(grad_gate), N.ptr(grad_post_weight), N.ptr(grad_post_bias), N.ptr(grad_pre_weight), N.ptr(grad_pre_bias),
-                     N.ptr(workspace), nbytes)
-        return grad_x, grad_y, grad_gate, grad_post_weight, grad_post_bias, grad_pre_weight, grad_pre_bias, None, None, None, None, None, None, None
+            N.launch(dout if dn is None else dn, lib.tf24_block_norm_backward,
+                     ptr(dout), ld_dout, ptr(dn), ld_dn, ptr(h2), ld_h, ptr(y2), ld_y,
+                     code[stream_dtype], code[block_dtype], rows, cols, ptr(gate2), N.F32 if gate is None else code[gate.dtype],
+                     ld_gate, rows_per_gate, ptr(post_weight), ptr(post_bias), ptr(pre_weight),
+                     N.F32 if param_dtype is None else code[param_dtype], post_kind, pre_kind, residual, scale, ptr(stats), ptr(grad_x),
+                     ptr(grad_y), ptr(grad_gate), ptr(grads[0]), ptr(grads[1]), ptr(grads[2]), ptr(grads[3]), ptr(workspace), nbytes)
+        return grad_x, grad_y, grad_gate, *grads, None, None, None, None, None, None, None
 
 
 def _parameters(fn, x, *params):
     """The parameters, contiguous and all of one type (float32 where they differ)."""
-    cols, dtype, mixed = x.shape[-1], None, False
+    cols, device, dtype, plain = x.shape[-1], x.get_device(), None, True
     for p in params:
         if p is None:
             continue
-        if p.shape != (cols,) or p.dtype not in _TYPES or p.device != x.device:
+        own = p.dtype
+        if p.shape != (cols,) or own not in _TYPES or p.get_device() != device:
             raise RuntimeError(f"{fn}: a weight or bias {tuple(p.shape)} {p.dtype} on {p.device} does not suit {cols} columns on {x.device}")
-        mixed = mixed or (dtype is not None and p.dtype != dtype)
-        dtype = p.dtype
-    plain = []
-    for p in params:
-        if p is not None:
-            if mixed:
-                p = p.float()
-            if not p.is_contiguous() or p.is_neg():
-                p = p.resolve_neg().contiguous()
-        plain.append(p)
-    return plain
+        plain = plain and (dtype is None or own == dtype) and p.is_contiguous() and not p.is_neg()
+        dtype = own
+    if plain:
+        return params
+    mixed = any(p is not None and p.dtype != dtype for p in params)
+    return [None if p is None else (p.float() if mixed else p).resolve_neg().contiguous() for p in params]
 
 
 def _gate(fn, gate, y):
@@ -137,6 +131,8 @@ def _gate(fn, gate, y):
     cols, lead = y.shape[-1], y.shape[:-1]
     if gate.dtype not in _TYPES or gate.device != y.device:
         raise RuntimeError(f"{fn}: a gate {gate.dtype} on {gate.device} does not suit a tensor on {y.device}")
+    if gate.shape == (cols,):
+        return gate, lead.numel()
     if gate.dim() > y.dim() or any(g not in (1, s) for g, s in zip(gate.shape[::-1], y.shape[::-1])):
         raise RuntimeError(f"{fn}: a gate {tuple(gate.shape)} does not broadcast to {tuple(y.shape)}")
     if gate.dim() == 0 or gate.shape[-1] != cols:
@@ -148,10 +144,7 @@ def _gate(fn, gate, y):
         shared -= 1
     if own[:shared] != lead[:shared]:
         gate, shared = gate.expand(y.shape), len(lead)
-    rows_per_gate = 1
-    for s in lead[shared:]:
-        rows_per_gate *= s
-    return gate.reshape(-1, cols), rows_per_gate
+    return gate, lead[shared:].numel()
 
 
 def _call(x, y, gate, rows_per_gate, post_weight, post_bias, pre_weight, pre_bias, scale, post_kind, pre_kind, eps, block_dtype, keep):
