@@ -16,7 +16,7 @@ from .dense_ops import (soft_threshold24, sparse24, MVUE24_approx,
 from .sparse_linear_transpose import SparseLinearTranspose, sparse_linear_transpose
 from .sparse_semi_structured_linear import sparse_semi_structured_linear
 from .GELUglu import GELUglu, gelu_glu, gelu_glu_checkpoint
-from .activation_checkpoint import ActivationCheckpoint, checkpoint_activation
+from .activation_checkpoint import ActivationCheckpoint, checkpoint_activation, checkpoint_weight_gradient
 from .norms import BlockNorm, ResidualNorm, block_norm, residual_norm
 from .sparse_ops import MyLinear, SparseLinear, SoftThreshold, SoftThresholdLinear, Sparse24
 
@@ -31,7 +31,7 @@ __all__ = [
     "SparseLinearTranspose", "sparse_linear_transpose",
     "sparse_semi_structured_linear",
     "GELUglu", "gelu_glu", "gelu_glu_checkpoint",
-    "ActivationCheckpoint", "checkpoint_activation",
+    "ActivationCheckpoint", "checkpoint_activation", "checkpoint_weight_gradient",
     "BlockNorm", "ResidualNorm", "block_norm", "residual_norm",
     "MyLinear", "SparseLinear", "SoftThreshold", "SoftThresholdLinear", "Sparse24",
 ]

@@ -66,6 +66,8 @@ _SIGNATURES = {
     "tf24_checkpoint_decode": (_i, [_p, _p, _i64, _i64, _p, _i, _i64, _p]),
     "tf24_gelu_glu_forward_checkpoint": (_i, [_p, _i, _i64, _i64, _i64, _p, _i64, _p, _p, _p, _p, _p]),
     "tf24_gelu_glu_backward_checkpoint": (_i, [_p, _i64, _p, _p, _i, _i64, _i64, _p, _i64, _p]),
+    "tf24_checkpoint_weight_grad": (_i, [_p, _i64, _i, _p, _p, _i64, _i64, _i64, _p, _p, _i, _p, _i64, _p]),
+    "tf24_checkpoint_weight_grad_workspace_bytes": (_i64, [_i64, _i64, _i64]),
     "tf24_block_norm_forward": (_i, [_p, _i64, _p, _i64, _i, _i, _i64, _i64, _p, _i, _i64, _i64, _p, _p, _p, _p, _i, _i, _i, _f, _f, _p, _p, _p, _p, _p, _p]),
     "tf24_block_norm_backward": (_i, [_p, _i64, _p, _i64, _p, _i64, _p, _i64, _i, _i, _i64, _i64, _p, _i, _i64, _i64, _p, _p, _p, _i, _i, _i, _i, _f,
                                       _p, _p, _p, _p, _p, _p, _p, _p, _p, _i64, _p]),

@@ -2,6 +2,7 @@
 
     checkpoint_activation(x)      -> ActivationCheckpoint: x in blocks of 32 columns, float8 values and a power of two each
     ActivationCheckpoint.decode() -> the values that are kept
+    checkpoint_weight_gradient(g, checkpoint) -> the gradients of a linear layer's weight and bias, from its input as it was kept
 
 What a layer keeps of its input between the two passes is most of a training step's memory.  A checkpoint takes 33/64 of a 16-bit
 matrix, and a gradient formed from it differs from the exact one by what rounding to 4 bits of mantissa does to the input
@@ -14,7 +15,7 @@ import torch
 
 from . import _native as N
 
-__all__ = ["ActivationCheckpoint", "checkpoint_activation"]
+__all__ = ["ActivationCheckpoint", "checkpoint_activation", "checkpoint_weight_gradient"]
 
 _BLOCK = 32
 _TYPES = (torch.float32, torch.float16, torch.bfloat16)
@@ -80,3 +81,38 @@ def checkpoint_activation(x):
     values, scales = empty_checkpoint(rows, cols, x.device)
     N.launch(x, N.lib().tf24_checkpoint_encode, flat.data_ptr(), N.dtype_code(x.dtype), ld, rows, cols, values.data_ptr(), scales.data_ptr())
     return ActivationCheckpoint(values, scales, x.shape, x.dtype)
+
+
+def checkpoint_weight_gradient(grad_output, checkpoint, bias=False, dtype=None):
+    """(dW, db) of y = x W^T + b: dW = grad_output^T x with x as `checkpoint` keeps it, db the sum of grad_output's rows with bias=True, otherwise None.
+    grad_output [..., out_features] is float16 or bfloat16, x of the same type and leading dimensions; dW [out_features, in_features] and db
+    are of that type or, with dtype=torch.float32, float32 (sums that are not rounded).  Without a graph: for backward passes."""
+    g = grad_output.detach()
+    if not g.is_cuda or g.get_device() != checkpoint.values.get_device():
+        raise RuntimeError(f"checkpoint_weight_gradient: grad_output on {g.device} and a checkpoint on {checkpoint.device} are not on one GPU")
+    if g.dtype not in (torch.float16, torch.bfloat16) or g.dtype != checkpoint.dtype:
+        raise RuntimeError(f"checkpoint_weight_gradient: grad_output {g.dtype} with a checkpoint of {checkpoint.dtype} is not supported (float16 or bfloat16, both the same)")
+    dtype = g.dtype if dtype is None else dtype
+    if dtype not in (g.dtype, torch.float32):
+        raise RuntimeError(f"checkpoint_weight_gradient: results of {dtype} are not supported ({g.dtype}, float32)")
+    shape = checkpoint.shape
+    if g.dim() == 0 or g.shape[:-1] != shape[:-1] or g.shape[-1] == 0:
+        raise RuntimeError(f"checkpoint_weight_gradient: grad_output {tuple(g.shape)} does not suit a checkpoint of {tuple(shape)}")
+    tokens, m, n = checkpoint.values.shape[0], g.shape[-1], shape[-1]
+    if tokens == 0:
+        return torch.zeros((m, n), dtype=dtype, device=g.device), torch.zeros(m, dtype=dtype, device=g.device) if bias else None
+    g, ld = N.as_rows(g)
+    padded = (m + 7) // 8 * 8
+    if padded != m:                                                # (the kernel's outputs come in eights)
+        g = torch.nn.functional.pad(g.reshape(tokens, m), (0, padded - m))
+        ld = padded
+    elif ld < m or ld % 8 or g.data_ptr() % 16:
+        g, ld = g.reshape(tokens, m).clone(memory_format=torch.contiguous_format), m
+    dw = torch.empty((padded, n), dtype=dtype, device=g.device)
+    db = torch.empty(padded, dtype=dtype, device=g.device) if bias else None
+    lib = N.lib()
+    nbytes = lib.tf24_checkpoint_weight_grad_workspace_bytes(tokens, padded, n)
+    workspace = torch.empty(nbytes, dtype=torch.uint8, device=g.device) if nbytes else None
+    N.launch(g, lib.tf24_checkpoint_weight_grad, g.data_ptr(), ld, N.dtype_codes[g.dtype], checkpoint.values.data_ptr(), checkpoint.scales.data_ptr(), tokens, padded, n,
+             dw.data_ptr(), N.ptr(db), N.dtype_codes[dtype], N.ptr(workspace), nbytes)
+    return dw[:m] if padded != m else dw, db[:m] if bias and padded != m else db

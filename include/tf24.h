@@ -449,6 +449,19 @@ int tf24_gelu_glu_forward_checkpoint(const void* in, int dtype, int64_t ld_in, i
 int tf24_gelu_glu_backward_checkpoint(const void* grad_out, int64_t ld_grad_out, const void* values, const void* scales, int dtype, int64_t rows,
                                       int64_t cols, void* grad_in, int64_t ld_grad_in, void* stream);
 
+/*
+ * Weight and bias gradient of a linear layer whose input x [tokens, n] was kept in 8 bits (tf24_checkpoint_encode):
+ *     dw[i, j] = sum_t g[t, i] * x[t, j],  db[i] = sum_t g[t, i]   (t < tokens, i < m, j < n)
+ * g [tokens, m] row-major F16 or BF16 (leading dimension a multiple of 8, 16-byte aligned), which should hold the kept values: what was kept of
+ * a float16 matrix for F16, of a bfloat16 one for BF16.  dw [m, n] and db [m] (NULL: not wanted) contiguous, of g's type or F32; sums in
+ * float32, rounded once.  m a multiple of 8, any n, at most 2^20; tokens >= 1.
+ *   workspace  16-byte aligned scratch; with tf24_checkpoint_weight_grad_workspace_bytes(tokens, m, n) bytes the token axis is cut into the
+ *              number of pieces that suits the shape (0: one piece), with less or none into fewer.  Deterministic either way.
+ */
+int tf24_checkpoint_weight_grad(const void* g, int64_t ldg, int dtype, const void* values, const void* scales, int64_t tokens, int64_t m, int64_t n, void* dw,
+                                void* db, int out_dtype, void* workspace, int64_t workspace_bytes, void* stream);
+int64_t tf24_checkpoint_weight_grad_workspace_bytes(int64_t tokens, int64_t m, int64_t n);
+
 typedef enum { TF24_NORM_NONE = 0, TF24_NORM_RMS = 1, TF24_NORM_LAYER = 2 } tf24_norm_kind;
 
 /*

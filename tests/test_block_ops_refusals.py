@@ -37,6 +37,21 @@ def test_glu_checkpoint_arguments(lib):
     assert backward(rows=0) == 0 and backward(ld=31) == STRIDE and backward(ld_gi=63) == STRIDE and backward(gi=None) == ARG and backward(cols=2 << 30) == SHAPE
 
 
+def test_weight_gradient_arguments(lib):
+    from sparse import _native as N
+
+    def call(g=A, ldg=64, dtype=N.F16, values=B, scales=C, tokens=100, m=64, n=33, dw=A, db=None, out=N.F16, ws=None, ws_bytes=0):
+        return lib.tf24_checkpoint_weight_grad(g, ldg, dtype, values, scales, tokens, m, n, dw, db, out, ws, ws_bytes, None)
+
+    assert call(dtype=N.F32) == DTYPE and call(out=N.BF16) == DTYPE and call(dtype=N.BF16) == DTYPE
+    assert call(tokens=0) == SHAPE and call(m=60) == SHAPE and call(m=0) == SHAPE and call(n=0) == SHAPE and call(n=(1 << 20) + 1) == SHAPE
+    assert call(ldg=56) == STRIDE and call(ldg=68) == STRIDE and call(ldg=(1 << 23) + 8) == STRIDE
+    assert call(g=None) == ARG and call(values=None) == ARG and call(scales=None) == ARG and call(dw=None) == ARG and call(ws_bytes=-1) == ARG
+    assert call(g=A + 8) == STRIDE and call(values=B + 8) == STRIDE and call(ws=A + 8) == STRIDE and call(dw=A + 2, out=N.F32) == STRIDE
+    need = lib.tf24_checkpoint_weight_grad_workspace_bytes
+    assert need(0, 64, 64) == 0 and need(64, 8192, 8192) == 0 and need(8192, 768, 768) > 0
+
+
 def test_block_norm_arguments(lib):
     from sparse import _native as N
 

@@ -178,12 +178,121 @@ def test_gated_activation_keeps_the_signs_of_trouble(cuda):
     assert bad == [6, 67, 70]      # the gate's slope at x = inf, and both gradients where the gate is a NaN
 
 
+# ------------------------------------------------------------------ gradients of weight and bias
+def check_weight_gradient(cuda, tokens, m, n, dtype, wide=False, bias=True, lead=None):
+    """Sums of float32 products in float32 (an instruction adds 32 of them to its accumulator, pieces are added in order): off by less than
+    (tokens / 32 + 48) u of the sum of the magnitudes, then one rounding."""
+    import sparse
+    x, g = draw(tokens, tokens, n, dtype=dtype), draw(m, tokens, m, dtype=dtype, std=0.1)
+    shape = lead or (tokens,)
+    kept = sparse.checkpoint_activation(x.to(cuda).view(*shape, n))
+    dw, db = sparse.checkpoint_weight_gradient(g.to(cuda).view(*shape, m), kept, bias=bias, dtype=F32 if wide else None)
+    out = F32 if wide else dtype
+    assert dw.shape == (m, n) and dw.dtype == out and (db is None) == (not bias)
+    g64, x64 = g.double().to(cuda), kept.decode().double().view(tokens, n)
+    for got, want, size in ((dw, g64.t().contiguous() @ x64, g64.abs().t().contiguous() @ x64.abs()),) + (((db, g64.sum(0), g64.abs().sum(0)),) if bias else ()):
+        tolerance = (tokens / 32 + 48) * U * size + torch.finfo(out).eps / 2 * want.abs() * 1.01 + 2.0 ** -25 * (out == F16)
+        off = (got.double() - want).abs()
+        assert (off <= tolerance).all(), (off / tolerance).max().item()
+    again, _ = sparse.checkpoint_weight_gradient(g.to(cuda).view(*shape, m), kept, bias=False, dtype=F32 if wide else None)
+    assert torch.equal(again, dw)
+
+
+@pytest.mark.parametrize("dtype", [F16, BF16])
+@pytest.mark.parametrize("tokens,m,n", [(1, 8, 1), (1, 8, 8), (2, 16, 33), (31, 200, 100), (63, 128, 128), (64, 192, 192), (65, 8, 257), (127, 264, 40), (128, 384, 193),
+                                        (129, 136, 384), (300, 512, 512), (1003, 768, 520), (2047, 256, 1000), (5000, 64, 96), (4096, 1024, 1536)])
+def test_weight_gradient(cuda, tokens, m, n, dtype):
+    check_weight_gradient(cuda, tokens, m, n, dtype)
+    check_weight_gradient(cuda, tokens, m, n, dtype, wide=True, bias=False)
+
+
+@pytest.mark.parametrize("m", [1, 7, 100, 1001])
+def test_weight_gradient_of_any_number_of_outputs(cuda, m):
+    check_weight_gradient(cuda, 77, m, 130, BF16, lead=(7, 11))
+
+
+def test_weight_gradient_of_strided_gradients(cuda):
+    import sparse
+    x, g = draw(1, 90, 200, dtype=BF16).to(cuda), draw(2, 90, 64, dtype=BF16).to(cuda)
+    kept = sparse.checkpoint_activation(x)
+    want, want_b = sparse.checkpoint_weight_gradient(g, kept, bias=True)
+    wide = torch.full((90, 80), float("nan"), dtype=BF16, device=cuda)
+    odd = torch.full((90, 69), float("nan"), dtype=BF16, device=cuda)
+    wide[:, 8:72], odd[:, 3:67] = g, g
+    for view in (wide[:, 8:72], odd[:, 3:67], g.t().contiguous().t(), torch._neg_view(-g)):
+        dw, db = sparse.checkpoint_weight_gradient(view, kept, bias=True)
+        assert torch.equal(dw, want) and torch.equal(db, want_b)
+    ones, one = torch.ones((), dtype=BF16, device=cuda).expand(90, 64), torch.ones(90, 64, dtype=BF16, device=cuda)
+    assert torch.equal(sparse.checkpoint_weight_gradient(ones, kept)[0], sparse.checkpoint_weight_gradient(one, kept)[0])
+    empty = sparse.checkpoint_weight_gradient(g[:0], sparse.checkpoint_activation(x[:0]), bias=True)
+    assert empty[0].shape == (64, 200) and empty[1].shape == (64,) and not empty[0].any() and not empty[1].any()
+
+
+@pytest.mark.parametrize("dtype", [F16, BF16])
+@pytest.mark.parametrize("tokens,m,n", [(64, 192, 192), (333, 264, 200), (1100, 128, 640)])
+def test_weight_gradient_of_integers_is_exact(cuda, tokens, m, n, dtype):
+    """Sums of products of small integers are exact in float32, in any order; each operand's rows and columns are its own, a row of one token shows
+    where it goes; infinities and NaNs stay in their rows and columns."""
+    import sparse
+    gen = torch.Generator().manual_seed(tokens)
+    x, g = (torch.randint(-4, 5, (tokens, c), generator=gen).to(dtype) for c in (n, m))
+    kept = sparse.checkpoint_activation(x.to(cuda))
+    assert torch.equal(kept.decode().cpu(), x)
+    dw, db = sparse.checkpoint_weight_gradient(g.to(cuda), kept, bias=True, dtype=F32)
+    assert torch.equal(dw.cpu().double(), g.double().t() @ x.double()) and torch.equal(db.cpu().double(), g.double().sum(0))
+    x[tokens - 1, 5], g[0, 3] = float("nan"), float("inf")
+    dw, db = sparse.checkpoint_weight_gradient(g.to(cuda), sparse.checkpoint_activation(x.to(cuda)), bias=True, dtype=F32)
+    want = g.double().t() @ x.double()
+    assert torch.equal(dw.cpu().isfinite(), want.isfinite()) and torch.equal(dw.cpu().double()[want.isfinite()], want[want.isfinite()])
+    assert torch.equal(db.cpu().isfinite(), g.double().sum(0).isfinite())
+
+
+def test_weight_gradient_at_every_scale(cuda):
+    """Blocks of magnitudes from the smallest to the largest that a type holds, one token each: the gradient is that row."""
+    import sparse
+    for dtype, low, high in ((F16, -24, 15), (BF16, -126, 126)):
+        exponents = torch.arange(low, high + 1)
+        x = (torch.linspace(1, 1.9, 64, dtype=torch.float64)[None] * 2.0 ** exponents.double()[:, None]).to(dtype)
+        g = torch.zeros(len(x), (len(x) + 7) // 8 * 8, dtype=dtype)
+        g[torch.arange(len(x)), torch.arange(len(x))] = 1
+        kept = sparse.checkpoint_activation(x.to(cuda))
+        dw, _ = sparse.checkpoint_weight_gradient(g.to(cuda), kept, dtype=F32)
+        want = kept.decode(F32)
+        if dtype == BF16:                                          # (matrix instructions flush what float32 holds as subnormal)
+            want = torch.where(want.abs() < 2.0 ** -126, 0, want)
+        assert torch.equal(dw[:len(x)], want), dtype
+
+
+def test_weight_gradient_without_a_workspace(cuda):
+    """Through the C ABI with less scratch than the cut into pieces asks for, and none: fewer pieces, the same sums (of integers)."""
+    import sparse
+    from sparse import _native as N
+    gen = torch.Generator().manual_seed(4)
+    tokens, m, n = 3000, 200, 160
+    x, g = (torch.randint(-4, 5, (tokens, c), generator=gen).to(F16).to(cuda) for c in (n, m))
+    kept = sparse.checkpoint_activation(x)
+    full = N.lib().tf24_checkpoint_weight_grad_workspace_bytes(tokens, m, n)
+    assert full > 0
+    want = (g.double().t().contiguous() @ x.double()).float()
+    for nbytes in (full, full // 2, 1000, 0):
+        dw, db = torch.empty(m, n, device=cuda), torch.empty(m, device=cuda)
+        ws = torch.full((max(nbytes, 1),), 255, dtype=torch.uint8, device=cuda)
+        N.check(N.lib().tf24_checkpoint_weight_grad(g.data_ptr(), m, N.F16, kept.values.data_ptr(), kept.scales.data_ptr(), tokens, m, n, dw.data_ptr(), db.data_ptr(), N.F32,
+                                                    ws.data_ptr() if nbytes else None, nbytes, N.stream_ptr()))
+        assert torch.equal(dw, want) and torch.equal(db.double(), g.double().sum(0)), nbytes
+
+
 def test_refusals(cuda):
     import sparse
+    g = torch.zeros(4, 8, device=cuda, dtype=F16)
     for call in (lambda: sparse.checkpoint_activation(torch.zeros(4, 8, device=cuda, dtype=torch.int32)), lambda: sparse.checkpoint_activation(torch.zeros((), device=cuda)),
                  lambda: sparse.checkpoint_activation(torch.zeros(4, 0, device=cuda)), lambda: sparse.gelu_glu_checkpoint.apply(torch.zeros(4, 7, device=cuda)),
                  lambda: sparse.gelu_glu_checkpoint.apply(torch.zeros(4, 8, device=cuda, dtype=torch.float64)),
-                 lambda: sparse.checkpoint_activation(torch.zeros(4, 8, device=cuda)).decode(torch.float64)):
+                 lambda: sparse.checkpoint_activation(torch.zeros(4, 8, device=cuda)).decode(torch.float64),
+                 lambda: sparse.checkpoint_weight_gradient(g, sparse.checkpoint_activation(g[:3])), lambda: sparse.checkpoint_weight_gradient(g.bfloat16(), sparse.checkpoint_activation(g)),
+                 lambda: sparse.checkpoint_weight_gradient(g.float(), sparse.checkpoint_activation(g.float())), lambda: sparse.checkpoint_weight_gradient(g[:, :0], sparse.checkpoint_activation(g)),
+                 lambda: sparse.checkpoint_weight_gradient(g.cpu(), sparse.checkpoint_activation(g)),
+                 lambda: sparse.checkpoint_weight_gradient(g, sparse.checkpoint_activation(g), dtype=BF16)):
         with pytest.raises(RuntimeError):
             call()
     leaf = torch.randn(2, 2, 8, device=cuda, requires_grad=True)
@@ -194,12 +303,13 @@ def test_refusals(cuda):
 
 def test_captured_and_on_another_stream(cuda):
     import sparse
-    x, dy = draw(7, 3, 40, 512, dtype=BF16).to(cuda), draw(8, 3, 40, 256, dtype=BF16).to(cuda)
+    x, dy = draw(7, 3, 400, 512, dtype=BF16).to(cuda), draw(8, 3, 400, 256, dtype=BF16).to(cuda)
 
     def step():
         leaf = x.detach().requires_grad_()
         out, kept = sparse.GELUglu(True, True)(leaf)
-        return [out.detach(), kept.decode(), sparse.checkpoint_activation(x).decode(), torch.autograd.grad(out, leaf, dy)[0]]
+        return [out.detach(), kept.decode(), sparse.checkpoint_activation(x).decode(), torch.autograd.grad(out, leaf, dy)[0],
+                *sparse.checkpoint_weight_gradient(dy, sparse.checkpoint_activation(x), bias=True)]
 
     want = step()
     side = torch.cuda.Stream()
