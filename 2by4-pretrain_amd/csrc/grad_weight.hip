@@ -81,10 +81,12 @@ __device__ __forceinline__ float widen(f16_t, short h) { return to_float(f16_t{(
 __device__ __forceinline__ float widen(bf16_t, short h) { return to_float(bf16_t{(uint16_t)h}); }
 
 // a sum rounded to the operands' type, as it is stored (float32 results hold the same values: a pass of its own that widens
-// them, and one for db, are 5 us each)
+// them, and one for db, are 5 us each), or as it is
+struct sum_t { float v; };
 template <typename T, typename OutT>
 __device__ __forceinline__ OutT rounded(float v) {
-  if constexpr (std::is_same<OutT, float>::value) return to_float(from_float<T>(v));
+  if constexpr (std::is_same<OutT, sum_t>::value) return sum_t{v};
+  else if constexpr (std::is_same<OutT, float>::value) return to_float(from_float<T>(v));
   else return from_float<T>(v);
 }
 
@@ -414,9 +416,16 @@ extern "C" int64_t tf24_grad_weight_workspace_bytes(int64_t tokens, int64_t m, i
 }
 
 namespace tf24 {
-namespace {
-int run(const char* fn, bool f32, const void* g, int64_t ldg, const void* x, int64_t ldx, int dtype, int64_t tokens, int64_t m, int64_t n,
-        void* dw, void* db, void* workspace, int64_t workspace_bytes, void* stream) {
+
+int64_t dense_weight_grad_workspace_bytes(int64_t tokens, int64_t m, int64_t n) { return tf24_grad_weight_workspace_bytes(tokens, m, n); }
+
+double dense_weight_grad_us(int64_t tokens, int64_t m, int64_t n) {
+  const int64_t any = (int64_t)1 << 40;
+  return takes_square(tokens, m, n, any) ? choose_pieces<Square>(tokens, m, n, any).us : choose_pieces<Wide>(tokens, m, n, any).us;
+}
+
+int dense_weight_grad(const char* fn, GradResults results, const void* g, int64_t ldg, const void* x, int64_t ldx, int dtype, int64_t tokens, int64_t m, int64_t n,
+                      void* dw, void* db, void* workspace, int64_t workspace_bytes, void* stream) {
   if (dtype != TF24_F16 && dtype != TF24_BF16) return fail(TF24_ERR_DTYPE, "%s: unsupported dtype %d", fn, dtype);
   if (tokens <= 0 || tokens > 0x7fffffffLL) return fail(TF24_ERR_SHAPE, "%s: bad number of tokens %lld", fn, (long long)tokens);
   if (m <= 0 || m % 8 || n <= 0 || n % 8 || m > (1 << 20) || n > (1 << 20))
@@ -427,21 +436,22 @@ int run(const char* fn, bool f32, const void* g, int64_t ldg, const void* x, int
   if (!g || !x || !dw) return fail(TF24_ERR_ARG, "%s: null pointer", fn);
   if (workspace_bytes < 0) return fail(TF24_ERR_ARG, "%s: negative workspace size", fn);
   if (int rc = check_aligned(fn, 16, {g, x, workspace})) return rc;
-  if (int rc = check_aligned(fn, f32 ? 4 : 2, {dw, db})) return rc;
+  if (int rc = check_aligned(fn, results == GRAD_AS_OPERANDS ? 2 : 4, {dw, db})) return rc;
   hipStream_t s = (hipStream_t)stream;
-  auto* go = dtype == TF24_F16 ? (f32 ? launch_either<f16_t, float> : launch_either<f16_t, f16_t>)
-                               : (f32 ? launch_either<bf16_t, float> : launch_either<bf16_t, bf16_t>);
+  auto* go = dtype == TF24_F16
+                 ? (results == GRAD_AS_OPERANDS ? launch_either<f16_t, f16_t> : results == GRAD_WIDENED ? launch_either<f16_t, float> : launch_either<f16_t, sum_t>)
+                 : (results == GRAD_AS_OPERANDS ? launch_either<bf16_t, bf16_t> : results == GRAD_WIDENED ? launch_either<bf16_t, float> : launch_either<bf16_t, sum_t>);
   return go(g, ldg, x, ldx, tokens, m, n, dw, db, workspace, workspace_bytes, s);
 }
-}  // namespace
+
 }  // namespace tf24
 
 extern "C" int tf24_grad_weight(const void* g, int64_t ldg, const void* x, int64_t ldx, int dtype, int64_t tokens, int64_t m, int64_t n,
                                 void* dw, void* db, void* workspace, int64_t workspace_bytes, void* stream) {
-  return tf24::run("tf24_grad_weight", false, g, ldg, x, ldx, dtype, tokens, m, n, dw, db, workspace, workspace_bytes, stream);
+  return tf24::dense_weight_grad("tf24_grad_weight", tf24::GRAD_AS_OPERANDS, g, ldg, x, ldx, dtype, tokens, m, n, dw, db, workspace, workspace_bytes, stream);
 }
 
 extern "C" int tf24_grad_weight_f32(const void* g, int64_t ldg, const void* x, int64_t ldx, int dtype, int64_t tokens, int64_t m, int64_t n,
                                     float* dw, float* db, void* workspace, int64_t workspace_bytes, void* stream) {
-  return tf24::run("tf24_grad_weight_f32", true, g, ldg, x, ldx, dtype, tokens, m, n, dw, db, workspace, workspace_bytes, stream);
+  return tf24::dense_weight_grad("tf24_grad_weight_f32", tf24::GRAD_WIDENED, g, ldg, x, ldx, dtype, tokens, m, n, dw, db, workspace, workspace_bytes, stream);
 }

@@ -2,16 +2,20 @@
 //
 //     dW[i, j] = sum_t G[t, i] * X[t, j]        db[i] = sum_t G[t, i]
 //
-// G [tokens, m] 16-bit as it lies, X [tokens, n] as blocks of e4m3 and their scales, which are widened to G's type (exactly: 4 bits of mantissa)
-// on their way through the registers into LDS; a pass that decodes X to memory first, and the product on it, read and write three times the bytes.
+// G [tokens, m] 16-bit as it lies, X [tokens, n] as blocks of e4m3 and their scales.  Two ways, by expected time (takes_decoded):
 //
-// The summed axis is the slow one of both operands: eight consecutive tokens of a column, which a lane of a matrix instruction takes, come from
-// transposing LDS reads (DS_READ_B64_TR_B16) of rows of a tile's columns.
+// - X is decoded to 16 bits in the workspace and multiplied by the kernels of tf24_grad_weight: large products, of which the pass over X is a few
+//   percent (12288 tokens, 4096 x 1024: 102 us, 99 of them the product; 8192 tokens, 11008 x 4096: 564 of 558).
+// - One kernel that widens X (exactly: 4 bits of mantissa) on its way through the registers into LDS; products that are small, where the
+//   launch of a pass more shows, and those that its smaller tiles divide better (1003 tokens, 2304 x 768: 12.7 us, 19.8 the other way; 4096 tokens, 2048 x
+//   2048 40.4 and 48.9).  Its loads and its writes to LDS are issued by the waves that multiply, in whose place: a stage of a tile takes 0.55 to
+//   0.65 us (1.0 PFLOP/s), on one card 0.65, without the writes 0.49, without the loads 0.55.  Tiles of 192 x 192 come to the same rate (8192 tokens,
+//   4096 x 4096 275 us, without writes 206, without loads 232), and writes in both halves of a stage are no better than all in one.
 //
-// A block of four waves (2 x 2) multiplies a tile of 192 x 192 or 128 x 128 over a piece of the token axis with V_MFMA_F32_16X16X32.  64
-// tokens are a stage; two stage buffers rotate in LDS, and the global loads of two more stages are in flight in registers: a stage's loads are
-// issued in the second half of the stage three ahead of it and written to LDS in the first half of the stage before it.  One barrier a stage, between its
-// halves: behind it lie the next stage's writes and this stage's reads.  The fragments of a half are read while the half before is multiplied.
+// The kernel.  The summed axis is the slow one of both operands: eight consecutive tokens of a column, which a lane of a matrix instruction takes,
+// come from transposing LDS reads (DS_READ_B64_TR_B16) of rows of a tile's columns.  A block of four waves (2 x 2) multiplies a tile of 128 x 128 over a
+// piece of the token axis with V_MFMA_F32_16X16X32.  64 tokens are a stage; two stage buffers rotate in LDS, and the global loads of two more
+// stages are in flight in registers.  One barrier a stage, between its halves; the fragments of a half are read while the half before is multiplied.
 // Tokens past the last one are read as zeros by the buffer loads' own bounds (both operands: a zero times whatever lies there would not do).
 // 16-byte chunks of a row are XOR-swizzled by token, so that the four tokens x 64 bytes that 32 lanes read touch every bank once.
 // Few tiles and a long token axis: the axis is cut into pieces, whose float32 partial tiles a second kernel adds in piece order.
@@ -26,18 +30,15 @@ typedef uint32_t uint4v __attribute__((ext_vector_type(4)));
 
 constexpr int kMaxPieces = 16;
 
-template <int F_>
 struct KeptTile {
-  static constexpr int F = F_;                                     // fragments of 16 rows and of 16 columns per wave
+  static constexpr int F = 4;                                      // fragments of 16 rows and of 16 columns per wave
   static constexpr int TILE = 32 * F, THREADS = 256, TOKENS = 64;
   static constexpr int ROW = TILE * 2, OPERAND = TOKENS * ROW, STAGE = 2 * OPERAND;
   static constexpr int G_CHUNKS = TILE / 8, G_LOADS = TOKENS * G_CHUNKS / THREADS;      // 16 bytes each: 8 columns of G, 16 of X
   static constexpr int X_CHUNKS = TILE / 16, X_LOADS = TOKENS * X_CHUNKS / THREADS;
   static constexpr int MMA = F * F, READS = 4 * F, SUMS = F / 2;   // of a half stage; row fragments whose column sums a wave forms
   static_assert(G_LOADS * THREADS == TOKENS * G_CHUNKS && X_LOADS * THREADS == TOKENS * X_CHUNKS && F % 2 == 0 && 2 * STAGE <= 160 * 1024, "a stage divides among the threads");
-  static __device__ __forceinline__ uint32_t swizzle(uint32_t token) {
-    return TILE == 128 ? ((token & 3) << 2) | (((token >> 3) & 1) << 1) : (((token >> 1) & 1) << 2) | (((token >> 3) & 1) << 1);
-  }
+  static __device__ __forceinline__ uint32_t swizzle(uint32_t token) { return ((token & 3) << 2) | (((token >> 3) & 1) << 1); }
   // rows of fragment f of a wave: the two waves that share rows hold them rotated, so that the first SUMS fragments of each are its own
   static __device__ __forceinline__ int fragment_row(int wave, int f) { return (wave >> 1) * (16 * F) + ((f + (wave & 1) * SUMS) % F) * 16; }
 };
@@ -68,9 +69,10 @@ struct KeptArgs {
   float *partial, *sums;                            // [pieces][tiles][TILE * TILE], [pieces][tiles_i * TILE]
 };
 
-template <typename T, typename OutT, typename C, bool SUMS>
-__global__ void __launch_bounds__(C::THREADS)
+template <typename T, typename OutT, bool SUMS>
+__global__ void __launch_bounds__(KeptTile::THREADS)
 grad_weight_kept(const KeptArgs a, OutT* __restrict__ dw, OutT* __restrict__ db) {
+  using C = KeptTile;
   __shared__ __attribute__((aligned(1024))) uint8_t smem[2 * C::STAGE];
   // workgroup ids are dealt to the 8 XCDs round-robin: each XCD takes a run of units, which share operand columns in its L2
   const int tiles = a.tiles_i * a.tiles_j, units = tiles * a.pieces, per_xcd = (units + 7) / 8;
@@ -90,6 +92,9 @@ grad_weight_kept(const KeptArgs a, OutT* __restrict__ dw, OutT* __restrict__ db)
 
   // ---- global loads: number q of a thread
   const int x_row = a.blocks * kKeptBlock;
+  // (a lane's 16 columns of X are two chunks of LDS: four lanes write the lower one first, the next four the upper one, so that eight of them
+  // touch 128 different bytes of banks either time)
+  const uint32_t upper_first = (tid >> 2) & 1;
   uint32_t g_from[C::G_LOADS], g_to[C::G_LOADS], x_from[C::X_LOADS], s_from[C::X_LOADS], x_to[C::X_LOADS];
 #pragma unroll
   for (int q = 0; q < C::G_LOADS; q++) {
@@ -102,48 +107,49 @@ grad_weight_kept(const KeptArgs a, OutT* __restrict__ dw, OutT* __restrict__ db)
     const uint32_t at = q * C::THREADS + tid, token = at / C::X_CHUNKS, chunk = at % C::X_CHUNKS;
     x_from[q] = token * x_row + chunk * 16;
     s_from[q] = token * a.blocks + chunk / 2;
-    x_to[q] = C::OPERAND + token * C::ROW + (((2 * chunk) ^ C::swizzle(token)) * 16);
+    x_to[q] = C::OPERAND + token * C::ROW + (((2 * chunk) ^ C::swizzle(token)) * 16) + upper_first * 16;
   }
   struct Loads { uint4v g[C::G_LOADS], x[C::X_LOADS]; uint8_t s[C::X_LOADS]; };
   Loads regs[2];
   // the rows of the stage to load next, as far as there are any
-  int rows_left = a.tokens - (int)first;
+  int rows_left = a.tokens - (int)first, rows = 0;
   const uint8_t* g_at = a.g + first * a.ldg + i0 * 2;
   const uint8_t* x_at = a.values + first * x_row + j0;
   const uint8_t* s_at = a.scales + first * a.blocks + j0 / kKeptBlock;
   const int g_end = (int)(a.m - i0) * 2, x_end = x_row - (int)j0, s_end = a.blocks - (int)(j0 / kKeptBlock);
   __amdgpu_buffer_rsrc_t g_window, x_window, s_window;
-  auto open_next = [&] {
-    const int rows = min(rows_left, C::TOKENS) - 1;
-    g_window = window(g_at, rows < 0 ? 0 : rows * a.ldg + g_end);
+  auto open_x = [&] {
+    rows = min(rows_left, C::TOKENS) - 1;
     x_window = window(x_at, rows < 0 ? 0 : rows * x_row + x_end);
     s_window = window(s_at, rows < 0 ? 0 : rows * a.blocks + s_end);
-    g_at += (int64_t)C::TOKENS * a.ldg;
     x_at += (int64_t)C::TOKENS * x_row;
     s_at += (int64_t)C::TOKENS * a.blocks;
     rows_left -= C::TOKENS;
   };
-  constexpr int LOADS = C::G_LOADS + 2 * C::X_LOADS, STORES = C::G_LOADS + C::X_LOADS;
-  auto load_one = [&](Loads& r, int k) {
+  auto open_g = [&] {                                             // of the same stage, behind open_x
+    g_window = window(g_at, rows < 0 ? 0 : rows * a.ldg + g_end);
+    g_at += (int64_t)C::TOKENS * a.ldg;
+  };
+  auto load_x = [&](Loads& r, int k) {                            // all scales, then all values
     if (k < C::X_LOADS) r.s[k] = __builtin_amdgcn_raw_buffer_load_b8(s_window, s_from[k], 0, 0);
-    else if (k < 2 * C::X_LOADS) r.x[k - C::X_LOADS] = __builtin_bit_cast(uint4v, __builtin_amdgcn_raw_buffer_load_b128(x_window, x_from[k - C::X_LOADS], 0, 0));
-    else r.g[k - 2 * C::X_LOADS] = __builtin_bit_cast(uint4v, __builtin_amdgcn_raw_buffer_load_b128(g_window, g_from[k - 2 * C::X_LOADS], 0, 0));
+    else r.x[k - C::X_LOADS] = __builtin_bit_cast(uint4v, __builtin_amdgcn_raw_buffer_load_b128(x_window, x_from[k - C::X_LOADS], 0, 0));
   };
-  auto store_one = [&](const Loads& r, int k, uint32_t buf) {
-    if (k < C::X_LOADS) {
-      const float scale = __builtin_bit_cast(float, (uint32_t)r.s[k] << 23);
-      const uint4v w = r.x[k];
-      const uint32_t w0 = w[0], w1 = w[1], w2 = w[2], w3 = w[3];
-      *reinterpret_cast<uint4v*>(smem + buf + x_to[k]) = uint4v{widen2<T, false>(w0, scale), widen2<T, true>(w0, scale), widen2<T, false>(w1, scale), widen2<T, true>(w1, scale)};
-      *reinterpret_cast<uint4v*>(smem + buf + x_to[k] + 16) = uint4v{widen2<T, false>(w2, scale), widen2<T, true>(w2, scale), widen2<T, false>(w3, scale), widen2<T, true>(w3, scale)};
-    } else {
-      *reinterpret_cast<uint4v*>(smem + buf + g_to[k - C::X_LOADS]) = r.g[k - C::X_LOADS];
-    }
+  auto load_g = [&](Loads& r, int k) { r.g[k] = __builtin_bit_cast(uint4v, __builtin_amdgcn_raw_buffer_load_b128(g_window, g_from[k], 0, 0)); };
+  auto store_x = [&](const Loads& r, int k, uint32_t buf) {
+    const float scale = __builtin_bit_cast(float, (uint32_t)r.s[k] << 23);
+    const uint4v w = r.x[k];
+    const uint32_t w0 = upper_first ? w[2] : w[0], w1 = upper_first ? w[3] : w[1], w2 = upper_first ? w[0] : w[2], w3 = upper_first ? w[1] : w[3];
+    *reinterpret_cast<uint4v*>(smem + buf + x_to[k]) = uint4v{widen2<T, false>(w0, scale), widen2<T, true>(w0, scale), widen2<T, false>(w1, scale), widen2<T, true>(w1, scale)};
+    *reinterpret_cast<uint4v*>(smem + buf + (x_to[k] ^ 16)) = uint4v{widen2<T, false>(w2, scale), widen2<T, true>(w2, scale), widen2<T, false>(w3, scale), widen2<T, true>(w3, scale)};
   };
+  auto store_g = [&](const Loads& r, int k, uint32_t buf) { *reinterpret_cast<uint4v*>(smem + buf + g_to[k]) = r.g[k]; };
   auto load_stage = [&](Loads& r) {
-    open_next();
+    open_x();
+    open_g();
 #pragma unroll
-    for (int k = 0; k < LOADS; k++) load_one(r, k);
+    for (int k = 0; k < 2 * C::X_LOADS; k++) load_x(r, k);
+#pragma unroll
+    for (int k = 0; k < C::G_LOADS; k++) load_g(r, k);
   };
 
   // ---- fragments: in a group of 16 lanes, lane i receives the halfwords i % 4 of the source lanes 4e + i / 4 (e = 0..3).
@@ -171,6 +177,7 @@ grad_weight_kept(const KeptArgs a, OutT* __restrict__ dw, OutT* __restrict__ db)
     if (f >= 1 && f <= C::F) bf[set][f - 1][q & 1] = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_short4_ptr)(lds_ptr_t)(base + b_off[f - 1]));
     else af[set][f ? f - C::F : 0][q & 1] = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_short4_ptr)(lds_ptr_t)(base + a_off[f ? f - C::F : 0]));
   };
+  constexpr int READ_SLOTS = C::MMA * 2 / 3;                      // (all of them are back by the barrier)
   constexpr int PER_MMA = (8 * C::SUMS + C::MMA - 1) / C::MMA;
   // The instructions of a half from one register set; among them the reads of the next half into the other set and, `work` saying which, the
   // stage's stores to LDS or global loads.
@@ -184,7 +191,7 @@ grad_weight_kept(const KeptArgs a, OutT* __restrict__ dw, OutT* __restrict__ db)
       acc[ti][tj] = mma<T>(x, y, acc[ti][tj]);
       __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
-      for (int q = i * C::READS / C::MMA; q < (i + 1) * C::READS / C::MMA; q++) read_one(set ^ 1, q, src, next_half);
+      for (int q = i * C::READS / READ_SLOTS; q < min((i + 1) * C::READS / READ_SLOTS, C::READS); q++) read_one(set ^ 1, q, src, next_half);
       work(i);
       if constexpr (SUMS) {
 #pragma unroll
@@ -196,23 +203,32 @@ grad_weight_kept(const KeptArgs a, OutT* __restrict__ dw, OutT* __restrict__ db)
       __builtin_amdgcn_sched_barrier(0);
     }
   };
-  // the halves of a stage in buffer P: stores of the next stage, loads of the third one after it into the registers that are free then
+  // The halves of stage s, in buffer P.  Buffer P is free from the barrier in the middle on, the other one holds stage s + 1 up to there: the first
+  // half stores G of stage s + 1 and loads X of stage s + 3 (into the registers that held X of stage s + 1), the second half stores X of stage
+  // s + 2 and loads G of stage s + 3.  Half of the writes to LDS in either half: all of them in the first one kept it busier than the matrix cores.
   auto first_half = [&](auto parity) {
     constexpr int P = decltype(parity)::value;
     half_stage(0, P * C::STAGE, 1, [&](int i) {
-      if (i == 0) open_next();
+      if (i == 0) open_x();
 #pragma unroll
-      for (int k = 0; k < STORES; k++)
-        if (i == C::MMA / 4 + k * (C::MMA / 2) / STORES) store_one(regs[1 - P], k, (1 - P) * C::STAGE);
+      for (int k = 0; k < C::G_LOADS; k++)
+        if (i == k * (C::MMA / 2) / C::G_LOADS + 1) store_g(regs[1 - P], k, (1 - P) * C::STAGE);
+#pragma unroll
+      for (int k = 0; k < 2 * C::X_LOADS; k++)
+        if (i == C::MMA / 4 + k * (C::MMA * 3 / 4) / (2 * C::X_LOADS)) load_x(regs[1 - P], k);
     });
   };
   auto second_half = [&](auto parity) {
     constexpr int P = decltype(parity)::value;
     wait_reads_and_barrier();
     half_stage(1, (1 - P) * C::STAGE, 0, [&](int i) {
+      if (i == 0) open_g();
 #pragma unroll
-      for (int k = 0; k < LOADS; k++)
-        if (i == k * C::MMA / LOADS) load_one(regs[1 - P], k);
+      for (int k = 0; k < C::X_LOADS; k++)
+        if (i == k * (C::MMA / 2) / C::X_LOADS + 1) store_x(regs[P], k, P * C::STAGE);
+#pragma unroll
+      for (int k = 0; k < C::G_LOADS; k++)
+        if (i == C::MMA / 4 + k * (C::MMA * 3 / 4) / C::G_LOADS) load_g(regs[1 - P], k);
     });
   };
   constexpr std::integral_constant<int, 0> even{};
@@ -221,8 +237,12 @@ grad_weight_kept(const KeptArgs a, OutT* __restrict__ dw, OutT* __restrict__ db)
   load_stage(regs[0]);
   load_stage(regs[1]);
 #pragma unroll
-  for (int k = 0; k < STORES; k++) store_one(regs[0], k, 0);
+  for (int k = 0; k < C::X_LOADS; k++) store_x(regs[0], k, 0);
+#pragma unroll
+  for (int k = 0; k < C::G_LOADS; k++) store_g(regs[0], k, 0);
   load_stage(regs[0]);
+#pragma unroll
+  for (int k = 0; k < C::X_LOADS; k++) store_x(regs[1], k, C::STAGE);
   wait_reads_and_barrier();
 #pragma unroll
   for (int q = 0; q < C::READS; q++) read_one(0, q, 0, 0);
@@ -268,9 +288,10 @@ grad_weight_kept(const KeptArgs a, OutT* __restrict__ dw, OutT* __restrict__ db)
 }
 
 // dW and db from the pieces: block (tile, fragment), and with blockIdx.x one past the tiles the column sums
-template <typename OutT, typename C>
-__global__ void __launch_bounds__(C::THREADS)
+template <typename OutT>
+__global__ void __launch_bounds__(KeptTile::THREADS)
 grad_weight_kept_reduce(const KeptArgs a, OutT* __restrict__ dw, OutT* __restrict__ db) {
+  using C = KeptTile;
   const int tiles = a.tiles_i * a.tiles_j, tid = threadIdx.x;
   if ((int)blockIdx.x == tiles) {
     for (int64_t i = (int64_t)blockIdx.y * C::THREADS + tid; i < a.m; i += (int64_t)gridDim.y * C::THREADS) {
@@ -299,52 +320,47 @@ grad_weight_kept_reduce(const KeptArgs a, OutT* __restrict__ dw, OutT* __restric
   for (int r = 0; r < 4; r++) dw[(row + r) * a.n + col] = from_float<OutT>(v[r]);
 }
 
-using Large = KeptTile<6>;
-using Small = KeptTile<4>;
-
-// The number of pieces with the least estimated time: rounds of the compute units x stages x time of a stage, and for the partial tiles 3 us and
-// 0.32 us a MB.
+// The number of pieces with the least estimated time: 4 us, 0.535 us a stage in each round of the compute units, and for the partial tiles 3 us and
+// 0.35 us a MB.  (Fitted to 120 products of 33 to 12288 tokens and 256 x 2048 to 11008 x 4096 outputs.)
 struct Cut { int pieces; double us; };
-template <typename C>
 Cut cut(int64_t tokens, int64_t m, int64_t n, int64_t workspace_bytes) {
-  constexpr double STAGE_US = C::F == 6 ? 0.72 : 0.36;
-  const int64_t tiles_i = (m + C::TILE - 1) / C::TILE, tiles = tiles_i * ((n + C::TILE - 1) / C::TILE), pairs = (tokens + 2 * C::TOKENS - 1) / (2 * C::TOKENS);
-  const int64_t bytes = (tiles * C::TILE + tiles_i) * C::TILE * 4;
-  Cut best{1, (double)(2 * pairs * ((tiles + 255) / 256)) * STAGE_US};
-  for (int64_t p = 2; p <= kMaxPieces && p <= pairs && p * tiles <= 512 && p * bytes <= workspace_bytes; p++) {
-    const double us = (double)((pairs + p - 1) / p * 2 * ((p * tiles + 255) / 256)) * STAGE_US + 3.0 + (double)(p * bytes) * 0.32e-6;
+  const int64_t tiles_i = (m + KeptTile::TILE - 1) / KeptTile::TILE, tiles = tiles_i * ((n + KeptTile::TILE - 1) / KeptTile::TILE);
+  const int64_t pairs = (tokens + 2 * KeptTile::TOKENS - 1) / (2 * KeptTile::TOKENS), bytes = (tiles + tiles_i) * KeptTile::TILE * KeptTile::TILE * 4;
+  Cut best{1, 4.0 + (double)(2 * pairs * ((tiles + 255) / 256)) * 0.535};
+  for (int64_t p = 2; p <= kMaxPieces && p <= pairs && p * tiles <= 1024 && p * bytes <= workspace_bytes; p++) {
+    const double us = 7.0 + (double)((pairs + p - 1) / p * 2 * ((p * tiles + 255) / 256)) * 0.535 + (double)(p * tiles) * (KeptTile::TILE * KeptTile::TILE * 4e-6 * 0.35);
     if (us < best.us) best = {(int)p, us};
   }
   return best;
 }
-bool takes_small(int64_t tokens, int64_t m, int64_t n, int64_t workspace_bytes) {
-  return cut<Small>(tokens, m, n, workspace_bytes).us < cut<Large>(tokens, m, n, workspace_bytes).us;
+int64_t pieces_bytes(int64_t tokens, int64_t m, int64_t n) {
+  const int pieces = cut(tokens, m, n, (int64_t)1 << 40).pieces;
+  const int64_t tiles_i = (m + KeptTile::TILE - 1) / KeptTile::TILE;
+  return pieces > 1 ? pieces * (tiles_i * ((n + KeptTile::TILE - 1) / KeptTile::TILE) + tiles_i) * KeptTile::TILE * KeptTile::TILE * 4 : 0;
 }
-template <typename C>
-int64_t workspace_of(int64_t tokens, int64_t m, int64_t n) {
-  const int pieces = cut<C>(tokens, m, n, (int64_t)1 << 40).pieces;
-  const int64_t tiles_i = (m + C::TILE - 1) / C::TILE;
-  return pieces > 1 ? pieces * (tiles_i * ((n + C::TILE - 1) / C::TILE) * C::TILE + tiles_i) * C::TILE * 4 : 0;
+// Decoded to the workspace first: 7.5 us for the launch and what the products' estimate leaves out, 0.41 us for a million elements.  (The kernel's
+// estimate on the same 120 products: the way taken is 2 % slower than the better one in the mean; 12288 tokens, 1024 x 4096 123 for 118, 2000
+// tokens, 2304 x 768 23.6 for 21.5.)
+bool takes_decoded(int64_t tokens, int64_t m, int64_t n) {
+  if (n % 8 || tokens > (int64_t)1 << 30) return false;
+  return 7.5 + dense_weight_grad_us(tokens, m, n) + (double)(tokens * n) * 0.41e-6 < cut(tokens, m, n, (int64_t)1 << 40).us;
 }
+int64_t decoded_bytes(int64_t tokens, int64_t n) { return (tokens * n * 2 + 255) / 256 * 256; }
 
-template <typename T, typename OutT, typename C>
+template <typename T, typename OutT>
 int launch(KeptArgs a, void* dw, void* db, void* workspace, int64_t workspace_bytes, hipStream_t s) {
+  using C = KeptTile;
   a.tiles_i = (int)((a.m + C::TILE - 1) / C::TILE);
   a.tiles_j = (int)((a.n + C::TILE - 1) / C::TILE);
-  a.pieces = cut<C>(a.tokens, a.m, a.n, workspace ? workspace_bytes : 0).pieces;
+  a.pieces = cut(a.tokens, a.m, a.n, workspace ? workspace_bytes : 0).pieces;
   a.partial = (float*)workspace;
   a.sums = a.pieces > 1 ? a.partial + (int64_t)a.pieces * a.tiles_i * a.tiles_j * C::TILE * C::TILE : nullptr;
   const int per_xcd = (a.tiles_i * a.tiles_j * a.pieces + 7) / 8;
-  auto* kernel = db ? grad_weight_kept<T, OutT, C, true> : grad_weight_kept<T, OutT, C, false>;
+  auto* kernel = db ? grad_weight_kept<T, OutT, true> : grad_weight_kept<T, OutT, false>;
   hipLaunchKernelGGL(kernel, dim3((unsigned)(per_xcd * 8)), dim3(C::THREADS), 0, s, a, (OutT*)dw, (OutT*)db);
   if (a.pieces > 1)
-    hipLaunchKernelGGL((grad_weight_kept_reduce<OutT, C>), dim3((unsigned)(a.tiles_i * a.tiles_j + (db ? 1 : 0)), C::MMA), dim3(C::THREADS), 0, s, a, (OutT*)dw, (OutT*)db);
+    hipLaunchKernelGGL(grad_weight_kept_reduce<OutT>, dim3((unsigned)(a.tiles_i * a.tiles_j + (db ? 1 : 0)), C::MMA), dim3(C::THREADS), 0, s, a, (OutT*)dw, (OutT*)db);
   return check_launch("tf24_checkpoint_weight_grad");
-}
-template <typename T, typename OutT>
-int launch_either(const KeptArgs& a, void* dw, void* db, void* workspace, int64_t workspace_bytes, hipStream_t s) {
-  return takes_small(a.tokens, a.m, a.n, workspace ? workspace_bytes : 0) ? launch<T, OutT, Small>(a, dw, db, workspace, workspace_bytes, s)
-                                                                          : launch<T, OutT, Large>(a, dw, db, workspace, workspace_bytes, s);
 }
 
 }  // namespace
@@ -353,7 +369,7 @@ int launch_either(const KeptArgs& a, void* dw, void* db, void* workspace, int64_
 extern "C" int64_t tf24_checkpoint_weight_grad_workspace_bytes(int64_t tokens, int64_t m, int64_t n) {
   using namespace tf24;
   if (tokens <= 0 || m <= 0 || n <= 0) return 0;
-  return takes_small(tokens, m, n, (int64_t)1 << 40) ? workspace_of<Small>(tokens, m, n) : workspace_of<Large>(tokens, m, n);
+  return takes_decoded(tokens, m, n) ? decoded_bytes(tokens, n) + dense_weight_grad_workspace_bytes(tokens, m, n) : pieces_bytes(tokens, m, n);
 }
 
 extern "C" int tf24_checkpoint_weight_grad(const void* g, int64_t ldg, int dtype, const void* values, const void* scales, int64_t tokens, int64_t m, int64_t n, void* dw,
@@ -371,11 +387,16 @@ extern "C" int tf24_checkpoint_weight_grad(const void* g, int64_t ldg, int dtype
   if (workspace_bytes < 0) return fail(TF24_ERR_ARG, "%s: negative workspace size", fn);
   if (int rc = check_aligned(fn, 16, {g, values, workspace})) return rc;
   if (int rc = check_aligned(fn, dtype_size(out_dtype), {dw, db})) return rc;
+  const bool wide = out_dtype == TF24_F32;
+  if (workspace && takes_decoded(tokens, m, n) && workspace_bytes >= decoded_bytes(tokens, n) + dense_weight_grad_workspace_bytes(tokens, m, n)) {
+    if (int rc = tf24_checkpoint_decode(values, scales, tokens, n, workspace, dtype, n, stream)) return rc;
+    const int64_t at = decoded_bytes(tokens, n);
+    return dense_weight_grad(fn, wide ? GRAD_SUMS : GRAD_AS_OPERANDS, g, ldg, workspace, n, dtype, tokens, m, n, dw, db, (uint8_t*)workspace + at, workspace_bytes - at, stream);
+  }
   KeptArgs a{};
   a.blocks = (int)kept_blocks(n);
   a.g = (const uint8_t*)g, a.values = (const uint8_t*)values, a.scales = (const uint8_t*)scales;
   a.ldg = (int)ldg * 2, a.m = m, a.n = n, a.tokens = (int)tokens;
-  const bool wide = out_dtype == TF24_F32;
-  auto* go = dtype == TF24_F16 ? (wide ? launch_either<f16_t, float> : launch_either<f16_t, f16_t>) : (wide ? launch_either<bf16_t, float> : launch_either<bf16_t, bf16_t>);
+  auto* go = dtype == TF24_F16 ? (wide ? launch<f16_t, float> : launch<f16_t, f16_t>) : (wide ? launch<bf16_t, float> : launch<bf16_t, bf16_t>);
   return go(a, dw, db, workspace, workspace_bytes, (hipStream_t)stream);
 }

@@ -564,4 +564,13 @@ int compress_with_partial_sums(const char* fn, const void* dense, int dtype, int
                                float* partial, hipStream_t stream);
 int finish_row_sums(const char* fn, const RowSums& sums, hipStream_t stream);
 
+// ---------------------------------------------------------------- weight gradients
+// The product of tf24_grad_weight (all of its checks) for calls that bring the second operand themselves: results of the operands' type, the same
+// widened to float32, or the float32 sums; and the time that its choice of tiles and pieces expects.
+enum GradResults { GRAD_AS_OPERANDS, GRAD_WIDENED, GRAD_SUMS };
+int dense_weight_grad(const char* fn, GradResults results, const void* g, int64_t ldg, const void* x, int64_t ldx, int dtype, int64_t tokens, int64_t m, int64_t n,
+                      void* dw, void* db, void* workspace, int64_t workspace_bytes, void* stream);
+int64_t dense_weight_grad_workspace_bytes(int64_t tokens, int64_t m, int64_t n);
+double dense_weight_grad_us(int64_t tokens, int64_t m, int64_t n);
+
 }  // namespace tf24

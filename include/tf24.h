@@ -455,8 +455,9 @@ int tf24_gelu_glu_backward_checkpoint(const void* grad_out, int64_t ld_grad_out,
  * g [tokens, m] row-major F16 or BF16 (leading dimension a multiple of 8, 16-byte aligned), which should hold the kept values: what was kept of
  * a float16 matrix for F16, of a bfloat16 one for BF16.  dw [m, n] and db [m] (NULL: not wanted) contiguous, of g's type or F32; sums in
  * float32, rounded once.  m a multiple of 8, any n, at most 2^20; tokens >= 1.
- *   workspace  16-byte aligned scratch; with tf24_checkpoint_weight_grad_workspace_bytes(tokens, m, n) bytes the token axis is cut into the
- *              number of pieces that suits the shape (0: one piece), with less or none into fewer.  Deterministic either way.
+ *   workspace  16-byte aligned scratch; with tf24_checkpoint_weight_grad_workspace_bytes(tokens, m, n) bytes (room for x in 16 bits, or
+ *              for partial sums of pieces of the token axis) the call takes the way that suits the shape, with less or none a slower one
+ *              (whose sums may differ in their last bits).  The same call with the same size gives the same bits.
  */
 int tf24_checkpoint_weight_grad(const void* g, int64_t ldg, int dtype, const void* values, const void* scales, int64_t tokens, int64_t m, int64_t n, void* dw,
                                 void* db, int out_dtype, void* workspace, int64_t workspace_bytes, void* stream);

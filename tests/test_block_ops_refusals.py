@@ -49,7 +49,7 @@ def test_weight_gradient_arguments(lib):
     assert call(g=None) == ARG and call(values=None) == ARG and call(scales=None) == ARG and call(dw=None) == ARG and call(ws_bytes=-1) == ARG
     assert call(g=A + 8) == STRIDE and call(values=B + 8) == STRIDE and call(ws=A + 8) == STRIDE and call(dw=A + 2, out=N.F32) == STRIDE
     need = lib.tf24_checkpoint_weight_grad_workspace_bytes
-    assert need(0, 64, 64) == 0 and need(64, 8192, 8192) == 0 and need(8192, 768, 768) > 0
+    assert need(0, 64, 64) == 0 and need(64, 256, 256) == 0 and need(8192, 768, 768) > 0
 
 
 def test_block_norm_arguments(lib):

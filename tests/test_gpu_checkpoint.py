@@ -200,7 +200,7 @@ def check_weight_gradient(cuda, tokens, m, n, dtype, wide=False, bias=True, lead
 
 @pytest.mark.parametrize("dtype", [F16, BF16])
 @pytest.mark.parametrize("tokens,m,n", [(1, 8, 1), (1, 8, 8), (2, 16, 33), (31, 200, 100), (63, 128, 128), (64, 192, 192), (65, 8, 257), (127, 264, 40), (128, 384, 193),
-                                        (129, 136, 384), (300, 512, 512), (1003, 768, 520), (2047, 256, 1000), (5000, 64, 96), (4096, 1024, 1536)])
+                                        (129, 136, 384), (300, 512, 512), (1003, 768, 520), (2047, 256, 1000), (5000, 64, 96), (4096, 1024, 1536), (1024, 4096, 4096), (1030, 4104, 4088)])
 def test_weight_gradient(cuda, tokens, m, n, dtype):
     check_weight_gradient(cuda, tokens, m, n, dtype)
     check_weight_gradient(cuda, tokens, m, n, dtype, wide=True, bias=False)
@@ -263,12 +263,12 @@ def test_weight_gradient_at_every_scale(cuda):
         assert torch.equal(dw[:len(x)], want), dtype
 
 
-def test_weight_gradient_without_a_workspace(cuda):
+@pytest.mark.parametrize("tokens,m,n", [(3000, 200, 160), (1000, 4096, 4096)])
+def test_weight_gradient_without_a_workspace(cuda, tokens, m, n):
     """Through the C ABI with less scratch than the cut into pieces asks for, and none: fewer pieces, the same sums (of integers)."""
     import sparse
     from sparse import _native as N
     gen = torch.Generator().manual_seed(4)
-    tokens, m, n = 3000, 200, 160
     x, g = (torch.randint(-4, 5, (tokens, c), generator=gen).to(F16).to(cuda) for c in (n, m))
     kept = sparse.checkpoint_activation(x)
     full = N.lib().tf24_checkpoint_weight_grad_workspace_bytes(tokens, m, n)
