@@ -83,6 +83,15 @@ def checkpoint_activation(x):
     return ActivationCheckpoint(values, scales, x.shape, x.dtype)
 
 
+def as_checkpoint(x, given):
+    """What a layer keeps of its input x: the checkpoint that came with it, or with given=True one made here."""
+    if given is True:
+        return checkpoint_activation(x)
+    if given.shape != x.shape or given.dtype != x.dtype or given.values.get_device() != x.get_device():
+        raise RuntimeError(f"the checkpoint of a tensor {tuple(given.shape)} {given.dtype} on {given.device} is not one of {tuple(x.shape)} {x.dtype} on {x.device}")
+    return given
+
+
 def checkpoint_weight_gradient(grad_output, checkpoint, bias=False, dtype=None):
     """(dW, db) of y = x W^T + b: dW = grad_output^T x with x as `checkpoint` keeps it, db the sum of grad_output's rows with bias=True, otherwise None.
     grad_output [..., out_features] is float16 or bfloat16, x of the same type and leading dimensions; dW [out_features, in_features] and db

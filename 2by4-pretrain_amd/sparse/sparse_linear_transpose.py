@@ -14,6 +14,7 @@ import torch
 import torch.nn.functional as F
 from torch import autograd, nn
 
+from .activation_checkpoint import ActivationCheckpoint, as_checkpoint
 from .semi_structured import (SparseSemiStructuredTensor, _dense_times_sparse_t, _mvue_weight_gradient, _spmm, to_sparse_semi_structured,
                               to_sparse_semi_structured_pair, to_sparse_semi_structured_with_row_sums)
 from .transposable_semi_structured import TransposableSparse, transposable_mask_
@@ -29,14 +30,16 @@ class sparse_linear_transpose(autograd.Function):
     matmul in the master weight's dtype instead of float16 followed by autograd's cast.  Neither pass
     enters an autocast context: every tensor operation in them is an explicit cast, a view or a call
     into the library, none of which autocast touches (three context managers per layer and step are
-    12 us of host time; the one reduction that autocast would promote keeps its own guard)."""
+    12 us of host time; the one reduction that autocast would promote keeps its own guard).
+    `kept` (True, or the ActivationCheckpoint of the input in the compressed copies' dtype): the input is kept in 8 bits, and
+    dW = MVUE24(dY^T) . x is formed from the kept values, decoded again for that product."""
 
     # True: a 3-d grad_output whose strides are all zero is replaced by ones, as the reference does
     # (README.md:186-187); False (default): its values are used
     ones_for_expanded_grad = False
 
     @staticmethod
-    def forward(ctx, input, weight, weight_sparse, weight_sparse_T, bias):
+    def forward(ctx, input, weight, weight_sparse, weight_sparse_T, bias, kept=None):
         compute = weight_sparse._dtype
         if input.dtype != compute:
             input = input.to(compute)
@@ -47,7 +50,13 @@ class sparse_linear_transpose(autograd.Function):
         ctx.bias_dtype = None if bias is None else bias.dtype
         if bias is not None and bias.dtype != compute and bias.dtype != torch.float32:
             bias = bias.to(compute)
-        ctx.save_for_backward(input, weight_sparse_T)
+        ctx.dtype = compute
+        ctx.kept = kept is not None and ctx.needs_input_grad[1]
+        if ctx.kept:
+            kept = as_checkpoint(input, kept)
+            ctx.save_for_backward(weight_sparse_T, kept.values, kept.scales)
+        else:
+            ctx.save_for_backward(weight_sparse_T, input)
         shape = ctx.shape = input.shape
         ctx.weight_dtype = weight.dtype
         if len(shape) != 2:
@@ -59,7 +68,7 @@ class sparse_linear_transpose(autograd.Function):
 
     @staticmethod
     def backward(ctx, grad_output):
-        input, weight_T = ctx.saved_tensors
+        weight_T, *saved = ctx.saved_tensors
         grad_input = grad_weight = grad_bias = None
         # An expanded scalar gradient (all strides 0: the layer's output fed straight into .sum()) is
         # materialised with its values.  The reference replaces a 3-d one by ones (README.md:186-187), which
@@ -74,14 +83,15 @@ class sparse_linear_transpose(autograd.Function):
             grad_output = grad_output.resolve_neg()
         if grad_output.stride(-1) != 1 or grad_output.stride(0) < grad_output.shape[-1]:
             grad_output = grad_output.contiguous()
-        if grad_output.dtype != input.dtype:
-            grad_output = grad_output.to(input.dtype)
+        if grad_output.dtype != ctx.dtype:
+            grad_output = grad_output.to(ctx.dtype)
         needs = ctx.needs_input_grad
         if needs[0]:
             grad_input = _dense_times_sparse_t(grad_output, weight_T)      # = torch.mm(grad_output, weight_T.t())
             if len(ctx.shape) != 2:
                 grad_input = grad_input.view(ctx.shape)
         if needs[1]:
+            input = ActivationCheckpoint(*saved, ctx.shape, ctx.dtype).decode() if ctx.kept else saved[0]
             if input.dim() != 2:
                 input = input.view(-1, input.shape[-1])
             both = None
@@ -101,12 +111,19 @@ class sparse_linear_transpose(autograd.Function):
         elif needs[4]:
             with torch.autocast(device_type="cuda", enabled=False):      # (autocast would promote the sum to float32)
                 grad_bias = grad_output.sum(0)
-        return grad_input, grad_weight, None, None, grad_bias
+        return grad_input, grad_weight, None, None, grad_bias, None
 
 
 class SparseLinearTranspose(nn.Linear):
-    def __init__(self, in_features: int, out_features: int, bias: bool = True, func=lambda step: 'dense', **kwargs):
+    """checkpoint=True: in mode 'sparse' the input is kept in 8 bits for the weight's gradient.  forward(x, checkpoint) takes the
+    ActivationCheckpoint of x in float16 that the operator in front made, whatever the layer's own setting."""
+
+    checkpoint = False
+
+    def __init__(self, in_features: int, out_features: int, bias: bool = True, func=lambda step: 'dense', checkpoint: bool = False, **kwargs):
         super().__init__(in_features, out_features, bias=bias, **kwargs)
+        if checkpoint:
+            self.checkpoint = True
         self.weight.freq = 40      # mask refresh period, in optimizer steps
         self.weight.cnt = 0        # forward passes since the last optimizer step
         self.weight.counter = 0    # optimizer steps
@@ -119,9 +136,12 @@ class SparseLinearTranspose(nn.Linear):
         self.transposable_sparse = TransposableSparse(abs=True)
         SparseSemiStructuredTensor._FORCE_CUTLASS = True
 
-    def forward(self, x):
+    def forward(self, x, checkpoint=None):
         w = self.weight
+        kept = True if checkpoint is None and self.checkpoint else checkpoint
         if w.mode == 'dense':
+            if checkpoint is not None:
+                raise RuntimeError("SparseLinearTranspose: a checkpoint of the input is taken in mode 'sparse' only")
             x = F.linear(x, w, self.bias)
         else:
             if w.mask.device != w.device:
@@ -143,7 +163,7 @@ class SparseLinearTranspose(nn.Linear):
                 w.weight_sparse, w.weight_sparse_T = to_sparse_semi_structured_pair(w, w.mask, dtype=torch.float16)
             # (the README wraps this call in torch.autocast(dtype=float16) for the function's custom_fwd to cast its
             # arguments; the function here casts them itself, to the compressed copies' dtype)
-            x = sparse_linear_transpose.apply(x, w, w.weight_sparse, w.weight_sparse_T, self.bias)
+            x = sparse_linear_transpose.apply(x, w, w.weight_sparse, w.weight_sparse_T, self.bias, *(() if kept is None else (kept,)))
         if self.training:
             if w.cnt == 0:
                 w.counter += 1

@@ -10,7 +10,8 @@
     Sparse24                     STE magnitude pruning of the STEP recipe       (README.md:286-295)
 
 The matrix products are torch's dense ones, as in the reference, except in SoftThresholdLinear under mixed precision: its weight and bias
-gradients (`_linear16`), and its forward product and input gradient where their tiles fill the compute units (`_product16`).
+gradients (`_linear16`), and its forward product and input gradient where their tiles fill the compute units (`_product16`).  There it
+may keep its input in 8 bits for the backward pass (checkpoint=True, or a checkpoint that the operator in front made).
 """
 from contextlib import nullcontext
 
@@ -20,6 +21,7 @@ from torch import autograd, nn
 from torch.amp import custom_bwd, custom_fwd
 
 from . import _native as N
+from .activation_checkpoint import ActivationCheckpoint, as_checkpoint, checkpoint_weight_gradient
 from .dense_ops import MVUE24_approx, soft_threshold24, sparse24
 
 __all__ = ["MyLinear", "my_linear", "SparseLinear", "sparse_linear", "SoftThreshold", "SoftThresholdLinear", "Sparse24"]
@@ -179,15 +181,33 @@ class _linear16(autograd.Function):
     MIN_TOKENS, MIN_TOKENS_NO_BIAS = 256, 4096
 
     @staticmethod
-    def forward(ctx, x, weight, bias):
+    def forward(ctx, x, weight, bias, kept=None):
         needs = ctx.needs_input_grad
-        ctx.save_for_backward(x if needs[1] else None, weight if needs[0] else None)
+        ctx.save_for_backward(*_keep(ctx, x, kept, needs[1]), weight if needs[0] else None)
         return _product16(x, weight, bias)
 
     @staticmethod
     def backward(ctx, grad_output):
-        x, weight = ctx.saved_tensors
-        return _linear16_backward(grad_output, x, weight, *ctx.needs_input_grad)
+        x, weight = _kept(ctx)
+        return *_linear16_backward(grad_output, x, weight, *ctx.needs_input_grad[:3]), None
+
+
+def _keep(ctx, x, kept, needed):
+    """The tensors that are saved of a layer's input x for its weight gradient: x, or what is kept of it in 8 bits (kept: True, or its checkpoint)."""
+    ctx.kept = None
+    if not needed or kept is None:
+        return (x if needed else None,)
+    kept = as_checkpoint(x, kept)
+    ctx.kept = kept.shape, kept.dtype
+    return kept.values, kept.scales
+
+
+def _kept(ctx):
+    """The saved tensors with the input as _keep took it in front: itself, its checkpoint or None."""
+    if ctx.kept is None:
+        return ctx.saved_tensors
+    values, scales, *others = ctx.saved_tensors
+    return ActivationCheckpoint(values, scales, *ctx.kept), *others
 
 
 def _linear16_backward(grad_output, x, weight, need_input, need_weight, need_bias, dtype=None):
@@ -197,7 +217,11 @@ def _linear16_backward(grad_output, x, weight, need_input, need_weight, need_bia
     # where a graph of the gradients is wanted (double backward), or a tangent, mode or transform has come up since the
     # forward pass: torch's operators, which those know
     kernels = not torch.is_grad_enabled() and N.plain_eager() and type(g) is torch.Tensor
-    if need_weight:
+    if need_weight and isinstance(x, ActivationCheckpoint):
+        if torch.is_grad_enabled():
+            raise RuntimeError("a graph of the gradients of a layer that keeps its input in 8 bits is not supported")
+        grad_weight, grad_bias = checkpoint_weight_gradient(grad_output, x, need_bias, dtype)
+    elif need_weight:
         x = x.reshape(-1, x.shape[-1])
         if (kernels and g.dtype == x.dtype and g.shape[0] == x.shape[0] and _on_current_gpu(g, x) and _rows_for_kernels(g) and _rows_for_kernels(x)
                 and g.shape[0] >= (_linear16.MIN_TOKENS if need_bias else _linear16.MIN_TOKENS_NO_BIAS)):
@@ -224,7 +248,7 @@ class _soft_threshold_linear16(autograd.Function):
     the values that 16-bit ones would be widened to: four casts of 3 to 5 us a layer less."""
 
     @staticmethod
-    def forward(ctx, x, weight, scale, bias, dtype):
+    def forward(ctx, x, weight, scale, bias, dtype, kept=None):
         rows, cols = weight.shape
         weight16 = torch.empty_like(weight, dtype=dtype)
         bias16 = None if bias is None else torch.empty_like(bias, dtype=dtype)
@@ -240,18 +264,18 @@ class _soft_threshold_linear16(autograd.Function):
         if needs[0] and needs[1] and weight.grad_fn is not None:
             with torch.enable_grad():
                 source = _place_of.apply(weight)
-        ctx.save_for_backward(x if needs[1] else None, weight16 if needs[0] else None, source)
+        ctx.save_for_backward(*_keep(ctx, x, kept, needs[1]), weight16 if needs[0] else None, source)
         return _product16(x, weight16, bias16)
 
     @staticmethod
     def backward(ctx, grad_output):
-        x, weight16, source = ctx.saved_tensors
+        x, weight16, source = _kept(ctx)
         needs = ctx.needs_input_grad
         if weight16 is not None and needs[1] and torch.is_grad_enabled():
             # a graph of the gradients leads on to the weight (a parameter is held by the graph itself)
             weight16 = _straight_through.apply(ctx.next_functions[1][0].variable if source is None else source, weight16)
         grad_input, grad_weight, grad_bias = _linear16_backward(grad_output, x, weight16, needs[0], needs[1], needs[3], torch.float32)
-        return grad_input, grad_weight, None, grad_bias, None
+        return grad_input, grad_weight, None, grad_bias, None, None
 
 
 def _grad_weight(g, x, with_bias, dtype=None):
@@ -278,8 +302,16 @@ def _takes_linear16(x, weight, bias):
 
 
 class SoftThresholdLinear(nn.Linear):
-    def __init__(self, in_features: int, out_features: int, bias: bool = True, device=None, dtype=None):
+    """checkpoint=True: where autocast makes the layer's products 16-bit ones, its input is kept in 8 bits for the weight's gradient
+    (which is the one at the kept values).  forward(x, checkpoint) takes the ActivationCheckpoint of x (as autocast casts it) that the operator
+    in front made, whatever the layer's own setting."""
+
+    checkpoint = False
+
+    def __init__(self, in_features: int, out_features: int, bias: bool = True, device=None, dtype=None, checkpoint: bool = False):
         super().__init__(in_features, out_features, bias=bias, device=device, dtype=dtype)
+        if checkpoint:
+            self.checkpoint = True
         self.register_buffer("scale", torch.tensor(0.0))
 
     def get_sparse_weights(self):
@@ -295,21 +327,24 @@ class SoftThresholdLinear(nn.Linear):
         self.scale.copy_(scale)
         self.weight.scale = self.scale
 
-    def forward(self, x):
+    def forward(self, x, checkpoint=None):
         weight, scale, bias = self.weight, self.scale, self.bias
         if not _takes_linear16(x, weight, bias):
+            if checkpoint is not None:
+                raise RuntimeError("SoftThresholdLinear: a checkpoint of the input is taken with contiguous GPU tensors under autocast to 16 bits only")
             return F.linear(x, self.get_sparse_weights(), bias)
+        kept = True if checkpoint is None and self.checkpoint else checkpoint
         dtype = torch.get_autocast_dtype("cuda")                   # (what autocast does to the arguments of F.linear)
         if (getattr(self.get_sparse_weights, "__func__", None) is SoftThresholdLinear.get_sparse_weights and weight.dtype == torch.float32
                 and weight.is_contiguous() and not weight.is_neg() and weight.shape[1] % 8 == 0 and weight.data_ptr() % 16 == 0
                 and type(scale) is torch.Tensor and scale.dtype == torch.float32 and scale.dim() == 0 and scale.device in (weight.device, torch.device("cpu"))
                 and not scale.requires_grad and not scale.is_neg()):
             if bias is None or (bias.dtype == torch.float32 and bias.is_contiguous() and not bias.is_neg() and bias.shape == weight.shape[:1]):
-                return _soft_threshold_linear16.apply(x.to(dtype), weight, scale, bias, dtype)
+                return _soft_threshold_linear16.apply(x.to(dtype), weight, scale, bias, dtype, *(() if kept is None else (kept,)))
             weight = _soft_threshold16.apply(weight, scale, dtype)
         else:
             weight = self.get_sparse_weights().to(dtype)
-        return _linear16.apply(x.to(dtype), weight, None if bias is None else bias.to(dtype))
+        return _linear16.apply(x.to(dtype), weight, None if bias is None else bias.to(dtype), *(() if kept is None else (kept,)))
 
 
 class Sparse24(autograd.Function):
