@@ -14,11 +14,11 @@
 // share a gate, dg = w_post A + b_post B, dw_post = sum over gates g A, db_post = sum g B; without a norm of y, A = sum d y and dg = A.
 //
 // Bound by memory: a row is read once and kept in registers while its means are taken (the variance from the centred values: a
-// second pass over registers, not over memory).  A row belongs to a wave (up to 1024 columns), or to 4 to 16 waves that
+// second pass over registers, not over memory).  A row belongs to a wave (up to 1024 columns), or to 2 to 16 waves that
 // exchange their sums through LDS; a lane holds one or two units of eight adjacent columns, so accesses are 16 bytes whatever the type
-// and the alignment, and four adjacent lanes hold a block of what is kept in 8 bits (checkpoint8.hpp).  Workgroups take runs of rows and keep the
-// parameters in registers.  In the backward pass a run ends in one partial sum per column, which a second launch adds in a
-// fixed order: no atomics, the same bits every time.
+// and the alignment, and four adjacent lanes hold a block of what is kept in 8 bits (checkpoint8.hpp).  Workgroups take runs of rows, keep the
+// parameters in registers, and load the next row while they compute on one.  In the backward pass a run ends in one partial sum per column, which a
+// second launch adds in a fixed order: no atomics, the same bits every time.
 #include "checkpoint8.hpp"
 
 namespace tf24 {
@@ -26,10 +26,10 @@ namespace {
 
 constexpr int kMaxCols = 16384;
 
-// GROUP threads share a row, each with UNITS units of 8 columns
-template <int GROUP_, int UNITS_>
+// GROUP threads share a row, each with UNITS units of 8 columns; a workgroup has at least THREADS threads, and works on ROWS rows at once
+template <int GROUP_, int UNITS_, int THREADS_>
 struct ShapeT {
-  static constexpr int GROUP = GROUP_, UNITS = UNITS_, THREADS = GROUP < 256 ? 256 : GROUP, ROWS = THREADS / GROUP, WAVES = GROUP / 64;
+  static constexpr int GROUP = GROUP_, UNITS = UNITS_, THREADS = GROUP > THREADS_ ? GROUP : THREADS_, ROWS = THREADS / GROUP, WAVES = GROUP / 64;
   static constexpr int MAX_COLS = GROUP * UNITS * 8;
 };
 
@@ -45,38 +45,77 @@ __device__ __forceinline__ float wave_sum(float v) {
 }
 
 // Sums over the threads of a row.  More than one wave: through LDS, in two buffers by turns, so that one barrier a sum is enough (who writes
-// a buffer again has passed the barrier that every reader of its last use arrived at afterwards).
+// a buffer again has passed the barrier that every reader of its last use arrived at afterwards).  All rows of a workgroup take their sums together.
 template <typename S>
 struct RowSum {
-  float (*lds)[S::WAVES][2];
+  float (*lds)[S::ROWS][S::WAVES][2];
   int turn = 0;
   __device__ __forceinline__ void operator()(float& a, float& b) {
     a = wave_sum(a);
     b = wave_sum(b);
     if constexpr (S::WAVES > 1) {
-      const int wave = threadIdx.x / 64;
-      if ((threadIdx.x & 63) == 0) { lds[turn][wave][0] = a; lds[turn][wave][1] = b; }
+      const int group = threadIdx.x / S::GROUP, wave = threadIdx.x % S::GROUP / 64;
+      if ((threadIdx.x & 63) == 0) { lds[turn][group][wave][0] = a; lds[turn][group][wave][1] = b; }
       __syncthreads();
       a = b = 0.0f;
 #pragma unroll
-      for (int w = 0; w < S::WAVES; w++) { a += lds[turn][w][0]; b += lds[turn][w][1]; }
+      for (int w = 0; w < S::WAVES; w++) { a += lds[turn][group][w][0]; b += lds[turn][group][w][1]; }
       turn ^= 1;
     }
   }
   __device__ __forceinline__ void operator()(float& a) {
-    float unused = 0.0f;
-    if constexpr (S::WAVES > 1) (*this)(a, unused);
-    else a = wave_sum(a);
+    a = wave_sum(a);
+    if constexpr (S::WAVES > 1) {
+      const int group = threadIdx.x / S::GROUP, wave = threadIdx.x % S::GROUP / 64;
+      if ((threadIdx.x & 63) == 0) lds[turn][group][wave][0] = a;
+      __syncthreads();
+      a = 0.0f;
+#pragma unroll
+      for (int w = 0; w < S::WAVES; w++) a += lds[turn][group][w][0];
+      turn ^= 1;
+    }
+  }
+};
+
+// A lane's part of a row as it lies in memory, zeros behind the last column
+template <typename T, int UNITS>
+struct Raw {
+  any4 w[UNITS][sizeof(T) / 2];
+  __device__ __forceinline__ void load(const T* row, const uint32_t (&col)[UNITS], const int (&n)[UNITS]) {
+#pragma unroll
+    for (int u = 0; u < UNITS; u++) {
+      const T* p = row + col[u];
+#pragma unroll
+      for (int q = 0; q < (int)sizeof(T) / 2; q++) w[u][q] = any4{0, 0, 0, 0};
+      if (n[u] == 8) {
+#pragma unroll
+        for (int q = 0; q < (int)sizeof(T) / 2; q++) w[u][q] = *(reinterpret_cast<const any4*>(p) + q);
+      } else if (n[u] > 0) {
+#pragma unroll
+        for (int e = 0; e < 8; e++)
+          if (e < n[u]) {
+            if constexpr (sizeof(T) == 2) w[u][0][e >> 1] |= (uint32_t)p[e].bits << (16 * (e & 1));
+            else w[u][e >> 2][e & 3] = __builtin_bit_cast(uint32_t, p[e]);
+          }
+      }
+    }
+  }
+  __device__ __forceinline__ float get(int u, int e) const {
+    if constexpr (sizeof(T) == 2) return to_float(T{(uint16_t)(w[u][0][e >> 1] >> (16 * (e & 1)))});
+    else {
+      const uint32_t bits = w[u][e >> 2][e & 3];
+      return __builtin_bit_cast(float, bits);
+    }
   }
 };
 
 template <int UNITS> struct Cells { float v[UNITS][8]; };
 
-// `n` <= 8 parameters from element `at` on, of a type known at the call; `otherwise` without any
+// `n` <= 8 parameters from element `at` on, of a type known at the call, zeros behind them; `otherwise` without any
 __device__ __forceinline__ void load_params(const void* p, int dtype, int64_t at, int n, float otherwise, float (&v)[8]) {
   if (!p) {
 #pragma unroll
-    for (int e = 0; e < 8; e++) v[e] = otherwise;
+    for (int e = 0; e < 8; e++) v[e] = e < n ? otherwise : 0.0f;
   } else if (dtype == TF24_F32) load_up_to_8((const float*)p + at, n, v);
   else if (dtype == TF24_F16) load_up_to_8((const f16_t*)p + at, n, v);
   else load_up_to_8((const bf16_t*)p + at, n, v);
@@ -116,7 +155,7 @@ __device__ __forceinline__ void statistics(Cells<S::UNITS>& c, const int (&n)[S:
 #pragma unroll
     for (int u = 0; u < S::UNITS; u++)
 #pragma unroll
-      for (int e = 0; e < 8; e++) c.v[u][e] -= left;
+      for (int e = 0; e < 8; e++) c.v[u][e] = e < n[u] ? c.v[u][e] - left : 0.0f;
   } else {
 #pragma unroll
     for (int u = 0; u < S::UNITS; u++)
@@ -143,17 +182,29 @@ template <typename R, typename T, bool RESIDUAL, typename S>
 __global__ void __launch_bounds__(S::THREADS)
 block_norm_forward(const ForwardArgs a) {
   constexpr int U = S::UNITS;
-  __shared__ float lds[2][S::WAVES][2];
+  static_assert(S::ROWS == 1 || S::WAVES == 1, "rows of a workgroup end at different times: no barriers then");
+  __shared__ float lds[2][S::ROWS][S::WAVES][2];
   RowSum<S> sum{lds};
   const int t = threadIdx.x % S::GROUP;
-  const uint32_t first = blockIdx.x * a.rows_per_block, last = min(a.rows, first + a.rows_per_block);
+  const uint32_t last = min(a.rows, (blockIdx.x + 1) * a.rows_per_block);
+  uint32_t row = blockIdx.x * a.rows_per_block + (S::ROWS > 1 ? __builtin_amdgcn_readfirstlane(threadIdx.x / S::GROUP) : 0);
   int n[U];
   uint32_t col[U];
-  Cells<U> post_w, post_b, pre_w, pre_b, gate;
 #pragma unroll
   for (int u = 0; u < U; u++) {
     col[u] = (uint32_t)(t + u * S::GROUP) * 8;
     n[u] = min(max(a.cols - (int)col[u], 0), 8);
+  }
+  struct Row { Raw<R, U> x; Raw<T, U> y; };
+  Row rows[2];
+  auto load = [&](Row& r, uint32_t at) {
+    r.x.load((const R*)a.x + (int64_t)at * a.ld_x, col, n);
+    if (RESIDUAL) r.y.load((const T*)a.y + (int64_t)at * a.ld_y, col, n);
+  };
+  if (row < last) load(rows[0], row);
+  Cells<U> post_w, post_b, pre_w, pre_b, gate;
+#pragma unroll
+  for (int u = 0; u < U; u++) {
     if (RESIDUAL) {
       load_params(a.post_weight, a.param_dtype, col[u], n[u], 1.0f, post_w.v[u]);
       load_params(a.post_bias, a.param_dtype, col[u], n[u], 0.0f, post_b.v[u]);
@@ -162,47 +213,48 @@ block_norm_forward(const ForwardArgs a) {
     load_params(a.pre_bias, a.param_dtype, col[u], n[u], 0.0f, pre_b.v[u]);
   }
   uint32_t gate_row = ~0u;
-  // (rows of a workgroup of several waves to a row: the same for all of them, as its barriers ask)
-  for (uint32_t row = first + (S::ROWS > 1 ? __builtin_amdgcn_readfirstlane(threadIdx.x / S::GROUP) : 0); row < last; row += S::ROWS) {
+  // (columns behind the last one hold zeros throughout: their weights and biases are zeros)
+  auto process = [&](const Row& r, uint32_t row) {
     Cells<U> h, v;
-#pragma unroll
-    for (int u = 0; u < U; u++) {
-      load_up_to_8((const R*)a.x + (int64_t)row * a.ld_x + col[u], n[u], h.v[u]);
-      if (RESIDUAL) load_up_to_8((const T*)a.y + (int64_t)row * a.ld_y + col[u], n[u], v.v[u]);
-    }
     if constexpr (RESIDUAL) {
       if (a.gate && row / a.rows_per_gate != gate_row) {
         gate_row = row / a.rows_per_gate;
 #pragma unroll
         for (int u = 0; u < U; u++) load_params(a.gate, a.gate_dtype, gate_row * a.ld_gate + col[u], n[u], 1.0f, gate.v[u]);
       }
+#pragma unroll
+      for (int u = 0; u < U; u++)
+#pragma unroll
+        for (int e = 0; e < 8; e++) v.v[u][e] = r.y.get(u, e);
       if (a.post_kind) {
-        float mean, r;
-        statistics<S>(v, n, a.post_kind, a.inv_cols, a.eps, sum, mean, r);
-        if (a.stats && t == 0) { a.stats[row] = mean; a.stats[a.rows + row] = r; }
+        float mean, scale;
+        statistics<S>(v, n, a.post_kind, a.inv_cols, a.eps, sum, mean, scale);
+        if (a.stats && t == 0) { a.stats[row] = mean; a.stats[a.rows + row] = scale; }
 #pragma unroll
         for (int u = 0; u < U; u++)
 #pragma unroll
-          for (int e = 0; e < 8; e++) v.v[u][e] = __builtin_fmaf(v.v[u][e] * r, post_w.v[u][e], post_b.v[u][e]);
+          for (int e = 0; e < 8; e++) v.v[u][e] = __builtin_fmaf(v.v[u][e] * scale, post_w.v[u][e], post_b.v[u][e]);
       }
 #pragma unroll
       for (int u = 0; u < U; u++) {
 #pragma unroll
-        for (int e = 0; e < 8; e++) {
-          const float z = a.gate ? gate.v[u][e] * v.v[u][e] : v.v[u][e];
-          h.v[u][e] = e < n[u] ? __builtin_fmaf(a.scale, h.v[u][e], z) : 0.0f;
-        }
+        for (int e = 0; e < 8; e++) h.v[u][e] = __builtin_fmaf(a.scale, r.x.get(u, e), a.gate ? gate.v[u][e] * v.v[u][e] : v.v[u][e]);
         store_up_to_8((R*)a.out + (int64_t)row * a.cols + col[u], n[u], h.v[u]);
       }
+    } else {
+#pragma unroll
+      for (int u = 0; u < U; u++)
+#pragma unroll
+        for (int e = 0; e < 8; e++) h.v[u][e] = r.x.get(u, e);
     }
     if (a.pre_kind) {
-      float mean, r;
-      statistics<S>(h, n, a.pre_kind, a.inv_cols, a.eps, sum, mean, r);
-      if (a.stats && t == 0) { a.stats[2 * (uint64_t)a.rows + row] = mean; a.stats[3 * (uint64_t)a.rows + row] = r; }
+      float mean, scale;
+      statistics<S>(h, n, a.pre_kind, a.inv_cols, a.eps, sum, mean, scale);
+      if (a.stats && t == 0) { a.stats[2 * (uint64_t)a.rows + row] = mean; a.stats[3 * (uint64_t)a.rows + row] = scale; }
 #pragma unroll
       for (int u = 0; u < U; u++) {
 #pragma unroll
-        for (int e = 0; e < 8; e++) h.v[u][e] = e < n[u] ? __builtin_fmaf(h.v[u][e] * r, pre_w.v[u][e], pre_b.v[u][e]) : 0.0f;
+        for (int e = 0; e < 8; e++) h.v[u][e] = __builtin_fmaf(h.v[u][e] * scale, pre_w.v[u][e], pre_b.v[u][e]);
         store_up_to_8((T*)a.n + (int64_t)row * a.cols + col[u], n[u], h.v[u]);
         if (a.values) {
           const Kept8 k = keep_8<T>(h.v[u]);
@@ -214,6 +266,15 @@ block_norm_forward(const ForwardArgs a) {
         }
       }
     }
+  };
+  while (row < last) {                                           // (by twos: a copy of a row's registers would wait for its loads)
+    const uint32_t second = row + S::ROWS, third = second + S::ROWS;
+    if (second < last) load(rows[1], second);
+    process(rows[0], row);
+    if (second >= last) break;
+    if (third < last) load(rows[0], third);
+    process(rows[1], second);
+    row = third;
   }
 }
 
@@ -239,70 +300,84 @@ template <typename R, typename T, bool RESIDUAL, typename S>
 __global__ void __launch_bounds__(S::THREADS)
 block_norm_backward(const BackwardArgs a) {
   constexpr int U = S::UNITS;
-  __shared__ float lds[2][S::WAVES][2];
+  __shared__ float lds[2][S::ROWS][S::WAVES][2];
   __shared__ __attribute__((aligned(16))) float column_sums[S::ROWS > 1 ? S::ROWS : 1][S::ROWS > 1 ? S::MAX_COLS : 4];
   RowSum<S> sum{lds};
   const int t = threadIdx.x % S::GROUP;
+  const uint32_t turn = S::ROWS > 1 ? __builtin_amdgcn_readfirstlane(threadIdx.x / S::GROUP) : 0;
   const uint32_t group = blockIdx.x / a.pieces.per_group, sub = blockIdx.x - group * a.pieces.per_group;
   const uint32_t start = group * a.pieces.rows_of_group;
   const uint32_t first = start + (uint32_t)((uint64_t)sub * a.pieces.rows_of_group / a.pieces.per_group);
   const uint32_t last = start + (uint32_t)((uint64_t)(sub + 1) * a.pieces.rows_of_group / a.pieces.per_group);
   int n[U];
   uint32_t col[U];
-  Cells<U> post_w, post_b, pre_w, gate, sum_dy, sum_d, sum_nh, sum_n;
 #pragma unroll
   for (int u = 0; u < U; u++) {
     col[u] = (uint32_t)(t + u * S::GROUP) * 8;
     n[u] = min(max(a.cols - (int)col[u], 0), 8);
+  }
+  struct Row { Raw<R, U> dout, h; Raw<T, U> dn, y; };
+  Row rows[2] = {};
+  auto load = [&](Row& r, uint32_t at) {
+    if (a.grad_out) r.dout.load((const R*)a.grad_out + (int64_t)at * a.ld_grad_out, col, n);
+    if (a.pre_kind) {
+      r.dn.load((const T*)a.grad_n + (int64_t)at * a.ld_grad_n, col, n);
+      r.h.load((const R*)a.h + (int64_t)at * a.ld_h, col, n);
+    }
+    if (RESIDUAL && a.y) r.y.load((const T*)a.y + (int64_t)at * a.ld_y, col, n);
+  };
+  if (first + turn < last) load(rows[0], first + turn);
+  // Columns behind the last one have zeros for weights and gradients, and what their other terms are (hat: minus the mean) meets a zero before a sum.
+  // `post_w` is the weight times the gate that the rows share.
+  Cells<U> post_w, pre_w, sum_dy, sum_d, sum_nh, sum_n;
+#pragma unroll
+  for (int u = 0; u < U; u++) {
     if (RESIDUAL) {
       load_params(a.post_weight, a.param_dtype, col[u], n[u], 1.0f, post_w.v[u]);
-      load_params(a.post_bias, a.param_dtype, col[u], n[u], 0.0f, post_b.v[u]);
-      if (!a.gate_per_row) load_params(a.gate, a.gate_dtype, group * a.ld_gate + col[u], n[u], 1.0f, gate.v[u]);
+      if (a.gate && !a.gate_per_row) {
+        float gate[8];
+        load_params(a.gate, a.gate_dtype, group * a.ld_gate + col[u], n[u], 1.0f, gate);
+#pragma unroll
+        for (int e = 0; e < 8; e++) post_w.v[u][e] *= gate[e];
+      }
     }
     load_params(a.pre_weight, a.param_dtype, col[u], n[u], 1.0f, pre_w.v[u]);
 #pragma unroll
     for (int e = 0; e < 8; e++) sum_dy.v[u][e] = sum_d.v[u][e] = sum_nh.v[u][e] = sum_n.v[u][e] = 0.0f;
   }
-  for (uint32_t row = first + (S::ROWS > 1 ? __builtin_amdgcn_readfirstlane(threadIdx.x / S::GROUP) : 0); row < last; row += S::ROWS) {
-    Cells<U> d, dn, h, y;
+  // One row of each of the workgroup's groups of threads; `here`: there is one (the others go along with zeros, for the barriers).
+  auto process = [&](const Row& r, uint32_t row, bool here) {
+    const uint32_t at = here ? row : first;
+    Cells<U> d;
 #pragma unroll
-    for (int u = 0; u < U; u++) {
-      if (a.grad_out) load_up_to_8((const R*)a.grad_out + (int64_t)row * a.ld_grad_out + col[u], n[u], d.v[u]);
-      else {
+    for (int u = 0; u < U; u++)
 #pragma unroll
-        for (int e = 0; e < 8; e++) d.v[u][e] = 0.0f;
-      }
-      if (a.pre_kind) {
-        load_up_to_8((const T*)a.grad_n + (int64_t)row * a.ld_grad_n + col[u], n[u], dn.v[u]);
-        load_up_to_8((const R*)a.h + (int64_t)row * a.ld_h + col[u], n[u], h.v[u]);
-      }
-      if (RESIDUAL && a.y) load_up_to_8((const T*)a.y + (int64_t)row * a.ld_y + col[u], n[u], y.v[u]);
-    }
+      for (int e = 0; e < 8; e++) d.v[u][e] = r.dout.get(u, e);
     if (a.pre_kind) {
-      const float mean = a.stats[2 * (uint64_t)a.rows + row], r = a.stats[3 * (uint64_t)a.rows + row];
+      const float mean = a.stats[2 * (uint64_t)a.rows + at], scale = a.stats[3 * (uint64_t)a.rows + at], shift = -mean * scale;
+      Cells<U> hat, q;
       float s1 = 0.0f, s2 = 0.0f;
 #pragma unroll
       for (int u = 0; u < U; u++)
 #pragma unroll
         for (int e = 0; e < 8; e++) {
-          const float hat = e < n[u] ? (h.v[u][e] - mean) * r : 0.0f, g = dn.v[u][e];
-          sum_nh.v[u][e] = __builtin_fmaf(g, hat, sum_nh.v[u][e]);
+          const float g = r.dn.get(u, e);
+          hat.v[u][e] = __builtin_fmaf(r.h.get(u, e), scale, shift);
+          sum_nh.v[u][e] = __builtin_fmaf(g, hat.v[u][e], sum_nh.v[u][e]);
           sum_n.v[u][e] += g;
-          const float q = e < n[u] ? g * pre_w.v[u][e] : 0.0f;
-          s1 += q;
-          s2 = __builtin_fmaf(q, hat, s2);
-          h.v[u][e] = hat;
-          dn.v[u][e] = q;
+          q.v[u][e] = g * pre_w.v[u][e];
+          s1 += q.v[u][e];
+          s2 = __builtin_fmaf(q.v[u][e], hat.v[u][e], s2);
         }
       sum(s1, s2);
       s1 = a.pre_kind == TF24_NORM_LAYER ? s1 * a.inv_cols : 0.0f;
-      s2 *= a.inv_cols;
+      s2 *= -a.inv_cols;
 #pragma unroll
       for (int u = 0; u < U; u++)
 #pragma unroll
-        for (int e = 0; e < 8; e++) d.v[u][e] = __builtin_fmaf(r, dn.v[u][e] - s1 - h.v[u][e] * s2, d.v[u][e]);
+        for (int e = 0; e < 8; e++) d.v[u][e] = __builtin_fmaf(scale, __builtin_fmaf(hat.v[u][e], s2, q.v[u][e] - s1), d.v[u][e]);
     }
-    if (a.grad_x) {
+    if (a.grad_x && here) {
 #pragma unroll
       for (int u = 0; u < U; u++) {
         float dx[8];
@@ -312,50 +387,62 @@ block_norm_backward(const BackwardArgs a) {
       }
     }
     if constexpr (RESIDUAL) {
-      const float mean = a.post_kind ? a.stats[row] : 0.0f, r = a.post_kind ? a.stats[a.rows + row] : 1.0f;
-      if (a.gate_per_row) {
+      const float mean = a.post_kind ? a.stats[at] : 0.0f, scale = a.post_kind ? a.stats[a.rows + at] : 1.0f, shift = -mean * scale;
+      if (a.gate_per_row) {                                      // d becomes that of z
 #pragma unroll
         for (int u = 0; u < U; u++) {
-          load_params(a.gate, a.gate_dtype, row * a.ld_gate + col[u], n[u], 1.0f, gate.v[u]);
-          if (a.grad_gate) {
-            float dg[8];
+          float gate[8];
+          load_params(a.gate, a.gate_dtype, at * a.ld_gate + col[u], n[u], 1.0f, gate);
+          if (a.grad_gate && here) {
+            float dg[8], b[8];
+            load_params(a.post_bias, a.param_dtype, col[u], n[u], 0.0f, b);
 #pragma unroll
-            for (int e = 0; e < 8; e++) dg[e] = d.v[u][e] * (a.post_kind ? __builtin_fmaf((y.v[u][e] - mean) * r, post_w.v[u][e], post_b.v[u][e]) : y.v[u][e]);
+            for (int e = 0; e < 8; e++) dg[e] = d.v[u][e] * (a.post_kind ? __builtin_fmaf(__builtin_fmaf(r.y.get(u, e), scale, shift), post_w.v[u][e], b[e]) : r.y.get(u, e));
             if (a.gate_dtype == TF24_F32) store_up_to_8((float*)a.grad_gate + (int64_t)row * a.cols + col[u], n[u], dg);
             else if (a.gate_dtype == TF24_F16) store_up_to_8((f16_t*)a.grad_gate + (int64_t)row * a.cols + col[u], n[u], dg);
             else store_up_to_8((bf16_t*)a.grad_gate + (int64_t)row * a.cols + col[u], n[u], dg);
           }
+#pragma unroll
+          for (int e = 0; e < 8; e++) d.v[u][e] *= gate[e];
         }
       }
+      Cells<U> hat;
       float s1 = 0.0f, s2 = 0.0f;
 #pragma unroll
       for (int u = 0; u < U; u++)
 #pragma unroll
         for (int e = 0; e < 8; e++) {
-          const float dz = a.gate ? d.v[u][e] * gate.v[u][e] : d.v[u][e];
-          const float hat = a.y && e < n[u] ? (y.v[u][e] - mean) * r : 0.0f, summed = a.gate_per_row ? dz : d.v[u][e];
-          sum_dy.v[u][e] = __builtin_fmaf(summed, hat, sum_dy.v[u][e]);
-          sum_d.v[u][e] += summed;
-          const float q = a.post_kind ? (e < n[u] ? dz * post_w.v[u][e] : 0.0f) : dz;
-          s1 += q;
-          s2 = __builtin_fmaf(q, hat, s2);
-          y.v[u][e] = hat;
-          d.v[u][e] = q;
+          hat.v[u][e] = __builtin_fmaf(r.y.get(u, e), scale, shift);
+          sum_dy.v[u][e] = __builtin_fmaf(d.v[u][e], hat.v[u][e], sum_dy.v[u][e]);
+          sum_d.v[u][e] += d.v[u][e];
+          d.v[u][e] *= post_w.v[u][e];
+          s1 += d.v[u][e];
+          s2 = __builtin_fmaf(d.v[u][e], hat.v[u][e], s2);
         }
       if (a.post_kind) {
         sum(s1, s2);
         s1 = a.post_kind == TF24_NORM_LAYER ? s1 * a.inv_cols : 0.0f;
-        s2 *= a.inv_cols;
+        s2 *= -a.inv_cols;
 #pragma unroll
         for (int u = 0; u < U; u++)
 #pragma unroll
-          for (int e = 0; e < 8; e++) d.v[u][e] = r * (d.v[u][e] - s1 - y.v[u][e] * s2);
+          for (int e = 0; e < 8; e++) d.v[u][e] = scale * __builtin_fmaf(hat.v[u][e], s2, d.v[u][e] - s1);
       }
-      if (a.grad_y) {
+      if (a.grad_y && here) {
 #pragma unroll
         for (int u = 0; u < U; u++) store_up_to_8((T*)a.grad_y + (int64_t)row * a.cols + col[u], n[u], d.v[u]);
       }
     }
+  };
+  for (uint32_t base = first; base < last; base += 2 * S::ROWS) {          // (by twos: a copy of a row's registers would wait for its loads)
+    const uint32_t row = base + turn, second = row + S::ROWS, third = second + S::ROWS;
+    if (second < last) load(rows[1], second);
+    else rows[1] = {};
+    process(rows[0], row, row < last);
+    if (base + S::ROWS >= last) break;
+    if (third < last) load(rows[0], third);
+    else rows[0] = {};
+    process(rows[1], second, second < last);
   }
   if (!a.partial) return;
   const uint32_t pieces = a.pieces.count();
@@ -391,7 +478,8 @@ block_norm_backward(const BackwardArgs a) {
 }
 
 // The gradients of the parameters from the pieces' sums.  Job 0: weight of the norm behind, 1: its bias, 2, 3: those of the norm before,
-// 4 + i: the gate that the rows of group i share; a workgroup takes 32 columns of a job, 32 strands of pieces side by side.
+// from 4 on: the gates that rows share; a workgroup takes 32 columns of a job, 32 strands of pieces side by side, or where a gate has few pieces
+// a gate for each strand.
 struct FinishArgs {
   const float* partial;
   const void *gate, *post_weight, *post_bias;
@@ -399,6 +487,7 @@ struct FinishArgs {
   int64_t ld_gate;
   Pieces pieces;
   int cols, column_blocks, gate_per_row, param_dtype, gate_dtype, post_kind;
+  __host__ __device__ bool strand_per_gate() const { return pieces.per_group < 16; }
 };
 
 constexpr int kStrands = 32;
@@ -410,7 +499,11 @@ block_norm_finish(const FinishArgs a) {
   if (!to) return;
   const int c = threadIdx.x & 31, strand = threadIdx.x >> 5;
   const int col = (int)(blockIdx.x - job * a.column_blocks) * 32 + c;
-  const uint32_t pieces = a.pieces.count(), begin = job < 4 ? 0 : (job - 4) * a.pieces.per_group, end = job < 4 ? pieces : begin + a.pieces.per_group;
+  const uint32_t pieces = a.pieces.count();
+  const bool alone = job >= 4 && a.strand_per_gate();
+  const uint32_t gate = job < 4 ? 0 : alone ? (job - 4) * kStrands + strand : job - 4;
+  const uint32_t begin = gate * a.pieces.per_group, end = job < 4 ? pieces : min(pieces, begin + a.pieces.per_group);
+  const uint32_t step = alone ? 1 : kStrands;
   float total = 0.0f;
   if (col < a.cols) {
     const uint64_t one = (uint64_t)pieces * a.cols;
@@ -421,13 +514,13 @@ block_norm_finish(const FinishArgs a) {
       load_params(a.post_weight, a.param_dtype, col, 1, 1.0f, w);
       load_params(a.post_bias, a.param_dtype, col, 1, 0.0f, b);
     }
-    for (uint32_t p0 = begin + strand; p0 < end; p0 += 8 * kStrands) {
+    for (uint32_t p0 = begin + (alone ? 0 : strand); p0 < end; p0 += 8 * step) {
       float v[8];
 #pragma unroll
-      for (int i = 0; i < 8; i++) v[i] = p0 + i * kStrands < end ? from[(uint64_t)(p0 + i * kStrands) * a.cols] : 0.0f;
+      for (int i = 0; i < 8; i++) v[i] = p0 + i * step < end ? from[(uint64_t)(p0 + i * step) * a.cols] : 0.0f;
 #pragma unroll
       for (int i = 0; i < 8; i++) {
-        const uint32_t p = p0 + i * kStrands;
+        const uint32_t p = p0 + i * step;
         if (p < end) {
           if (gated) {
             float g[8];
@@ -441,33 +534,33 @@ block_norm_finish(const FinishArgs a) {
       }
     }
   }
+  if (alone) {
+    if (gate < a.pieces.groups && col < a.cols) store_result(to, a.gate_dtype, (int64_t)gate * a.cols + col, total);
+    return;
+  }
   strands[strand][c] = total;
   __syncthreads();
   if (strand == 0 && col < a.cols) {
 #pragma unroll
     for (int s = 1; s < kStrands; s++) total += strands[s][c];
-    store_result(to, job < 4 ? a.param_dtype : a.gate_dtype, job < 4 ? col : (int64_t)(job - 4) * a.cols + col, total);
+    store_result(to, job < 4 ? a.param_dtype : a.gate_dtype, (int64_t)gate * a.cols + col, total);
   }
 }
 
 // ---------------------------------------------------------------- host
-using Wave1 = ShapeT<64, 1>;
-using Wave2 = ShapeT<64, 2>;
-using Four1 = ShapeT<256, 1>;
-using Four2 = ShapeT<256, 2>;
-using Eight2 = ShapeT<512, 2>;
-using Sixteen2 = ShapeT<1024, 2>;
-
-// the narrowest shape that holds a row
-template <typename F>
+// the narrowest shape that holds a row; THREADS: the least number of a workgroup
+template <int THREADS, typename F>
 auto with_shape(int64_t cols, F&& f) {
-  if (cols <= Wave1::MAX_COLS) return f(Wave1{});
-  if (cols <= Wave2::MAX_COLS) return f(Wave2{});
-  if (cols <= Four1::MAX_COLS) return f(Four1{});
-  if (cols <= Four2::MAX_COLS) return f(Four2{});
-  if (cols <= Eight2::MAX_COLS) return f(Eight2{});
-  return f(Sixteen2{});
+  if (cols <= 512) return f(ShapeT<64, 1, THREADS>{});
+  constexpr int WIDE = THREADS > 256 ? THREADS : 64;             // (forward: one row to a workgroup, whose barriers are its own)
+  if (cols <= 1024) return f(ShapeT<128, 1, WIDE>{});
+  if (cols <= 2048) return f(ShapeT<256, 1, WIDE>{});
+  if (cols <= 4096) return f(ShapeT<512, 1, WIDE>{});
+  if (cols <= 8192) return f(ShapeT<512, 2, WIDE>{});
+  return f(ShapeT<1024, 2, WIDE>{});
 }
+constexpr int kForwardThreads = 256, kBackwardThreads = 512;
+
 template <typename F>
 auto with_types(int stream_dtype, int block_dtype, F&& f) {
   if (stream_dtype == TF24_F32) {
@@ -479,13 +572,15 @@ auto with_types(int stream_dtype, int block_dtype, F&& f) {
   return f(bf16_t{}, bf16_t{});
 }
 
-constexpr uint32_t kForwardBlocks = 2048, kBackwardPieces = 512;
+// What 256 compute units hold at once, so that no part of a round runs by itself: forward four waves a SIMD, backward a workgroup of eight
+// waves a compute unit, two a SIMD (3003 rows of 1601 columns in 1502 workgroups and 259 pieces 56 us both passes, in 1001 and 252 40).
+constexpr uint32_t kForwardWaves = 4096, kBackwardPieces = 256;
 
 Pieces plan_pieces(int64_t rows, int64_t cols, int64_t rows_per_gate) {
   const uint32_t groups = rows_per_gate > 1 && rows_per_gate < rows ? (uint32_t)(rows / rows_per_gate) : 1;
   const uint32_t rows_of_group = (uint32_t)(rows / groups);
-  const uint32_t at_once = with_shape(cols, [](auto s) { return (uint32_t)decltype(s)::ROWS; });
-  const uint32_t wanted = (kBackwardPieces + groups - 1) / groups, most = (rows_of_group + at_once - 1) / at_once;
+  const uint32_t at_once = with_shape<kBackwardThreads>(cols, [](auto s) { return (uint32_t)decltype(s)::ROWS; });
+  const uint32_t wanted = groups < kBackwardPieces ? kBackwardPieces / groups : 1, most = (rows_of_group + at_once - 1) / at_once;
   return {groups, wanted < most ? wanted : most, rows_of_group};
 }
 
@@ -496,7 +591,7 @@ int check_norm(const char* fn, int stream_dtype, int block_dtype, int param_dtyp
   if (!is_float(stream_dtype) || !is_float(block_dtype) || (stream_dtype != TF24_F32 && block_dtype != stream_dtype))
     return fail(TF24_ERR_DTYPE, "%s: types %d (stream) and %d (block) are not supported together", fn, stream_dtype, block_dtype);
   if (!is_float(param_dtype) || (gate && !is_float(gate_dtype))) return fail(TF24_ERR_DTYPE, "%s: unsupported parameter or gate dtype %d, %d", fn, param_dtype, gate_dtype);
-  if (rows < 0 || rows > 0x7fffffffLL - kForwardBlocks * 64 || cols < 1 || cols > kMaxCols)
+  if (rows < 0 || rows > 0x7fffffffLL - kForwardWaves || cols < 1 || cols > kMaxCols)
     return fail(TF24_ERR_SHAPE, "%s: shape (%lld, %lld) is not supported: 1 to %d columns", fn, (long long)rows, (long long)cols, kMaxCols);
   if (post_kind < 0 || post_kind > TF24_NORM_LAYER || pre_kind < 0 || pre_kind > TF24_NORM_LAYER) return fail(TF24_ERR_ARG, "%s: bad kind of norm %d, %d", fn, post_kind, pre_kind);
   if (gate && rows && (rows_per_gate < 1 || rows % rows_per_gate))
@@ -524,9 +619,10 @@ extern "C" int tf24_block_norm_forward(const void* x, int64_t ld_x, const void* 
   if (int rc = check_aligned(fn, gate ? dtype_size(gate_dtype) : 1, {gate})) return rc;
   if (int rc = check_aligned(fn, 16, {values, stats})) return rc;
   return with_types(stream_dtype, block_dtype, [&](auto r, auto t) {
-    return with_shape(cols, [&](auto shape) {
+    return with_shape<kForwardThreads>(cols, [&](auto shape) {
       using S = decltype(shape);
-      const uint32_t each = (uint32_t)((rows + kForwardBlocks - 1) / kForwardBlocks);
+      constexpr uint32_t most = kForwardWaves / (S::THREADS / 64);
+      const uint32_t each = (uint32_t)((rows + most - 1) / most);
       const uint32_t per_block = (each + S::ROWS - 1) / S::ROWS * S::ROWS;
       ForwardArgs a{x, y, gate, post_weight, post_bias, pre_weight, pre_bias, out, n, stats, (uint8_t*)values, (uint8_t*)scales, ld_x, ld_y, ld_gate, (uint32_t)rows,
                     per_block, (uint32_t)(gate ? rows_per_gate : 1), (int)cols, (int)kept_blocks(cols), param_dtype, gate_dtype, post_kind, pre_kind, scale, eps,
@@ -571,10 +667,12 @@ extern "C" int tf24_block_norm_backward(const void* grad_out, int64_t ld_grad_ou
   if (sums && (!workspace || workspace_bytes < (int64_t)pieces.count() * cols * 16))
     return fail(TF24_ERR_ARG, "%s: a workspace of %lld bytes is needed", fn, (long long)pieces.count() * cols * 16);
   const int column_blocks = (int)((cols + 31) / 32);
-  const int64_t jobs = 4 + (wants_gate && !per_row ? (int64_t)pieces.groups : 0);
+  const FinishArgs f{(const float*)workspace, gate, post_weight, post_bias, grad_post_weight, grad_post_bias, grad_pre_weight, grad_pre_bias, per_row ? nullptr : grad_gate,
+                     ld_gate, pieces, (int)cols, column_blocks, per_row, param_dtype, gate_dtype, post_kind};
+  const int64_t gate_jobs = !f.grad_gate ? 0 : f.strand_per_gate() ? (pieces.groups + kStrands - 1) / kStrands : pieces.groups, jobs = 4 + gate_jobs;
   if (jobs * column_blocks > 0x7fffffffLL) return fail(TF24_ERR_SHAPE, "%s: too many gates (%lld)", fn, (long long)pieces.groups);
   const int rc = with_types(stream_dtype, block_dtype, [&](auto r, auto t) {
-    return with_shape(cols, [&](auto shape) {
+    return with_shape<kBackwardThreads>(cols, [&](auto shape) {
       using S = decltype(shape);
       BackwardArgs a{grad_out, grad_n, h, y, gate, post_weight, post_bias, pre_weight, stats, grad_x, grad_y, per_row ? grad_gate : nullptr,
                      sums ? (float*)workspace : nullptr, ld_grad_out, ld_grad_n, ld_h, ld_y, ld_gate, pieces, (uint32_t)rows, (int)cols, per_row, param_dtype,
@@ -585,8 +683,6 @@ extern "C" int tf24_block_norm_backward(const void* grad_out, int64_t ld_grad_ou
     });
   });
   if (rc || !sums) return rc;
-  FinishArgs f{(const float*)workspace, gate, post_weight, post_bias, grad_post_weight, grad_post_bias, grad_pre_weight, grad_pre_bias, per_row ? nullptr : grad_gate,
-               ld_gate, pieces, (int)cols, column_blocks, per_row, param_dtype, gate_dtype, post_kind};
   hipLaunchKernelGGL(block_norm_finish, dim3((uint32_t)(jobs * column_blocks)), dim3(32 * kStrands), 0, (hipStream_t)stream, f);
   return check_launch(fn);
 }
