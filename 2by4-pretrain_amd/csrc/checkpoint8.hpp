@@ -22,29 +22,47 @@ constexpr int kKeptLanes = kKeptBlock / kKeptUnit;
 
 __host__ __device__ inline int64_t kept_blocks(int64_t cols) { return (cols + kKeptBlock - 1) / kKeptBlock; }
 
-// 16-byte accesses at any element: global memory takes them unaligned, in the same instruction
+// 4-, 8- and 16-byte accesses at any element: global memory takes them unaligned, in the same instruction
+typedef unsigned int any1 __attribute__((aligned(2)));
+typedef unsigned int any2 __attribute__((ext_vector_type(2), aligned(2)));
 typedef unsigned int any4 __attribute__((ext_vector_type(4), aligned(2)));
 
-// The `n` <= 8 elements at p as float32, zeros behind them
+// The `n` <= 8 elements at p as float32, zeros behind them.  Fewer than eight are four, two and one, as far as there are.
 template <typename T>
 __device__ __forceinline__ void load_up_to_8(const T* p, int n, float (&v)[8]) {
-  if (n == 8) {
-    if constexpr (sizeof(T) == 2) {
-      const any4 w = *reinterpret_cast<const any4*>(p);
-#pragma unroll
-      for (int e = 0; e < 8; e++) v[e] = to_float(T{(uint16_t)(w[e >> 1] >> (16 * (e & 1)))});
-    } else {
-      const any4 a = *reinterpret_cast<const any4*>(p), b = *reinterpret_cast<const any4*>(p + 4);
-#pragma unroll
-      for (int e = 0; e < 4; e++) {
-        const uint32_t lo = a[e], hi = b[e];                     // (a bit cast of a vector's element itself takes the first one)
-        v[e] = __builtin_bit_cast(float, lo);
-        v[4 + e] = __builtin_bit_cast(float, hi);
-      }
+  if constexpr (sizeof(T) == 2) {
+    any4 w = {0, 0, 0, 0};
+    if (n == 8) w = *reinterpret_cast<const any4*>(p);
+    else if (n > 0) {
+      any2 four = {0, 0};
+      uint32_t two = 0, one = 0;
+      if (n & 4) four = *reinterpret_cast<const any2*>(p);
+      if (n & 2) two = *reinterpret_cast<const any1*>(p + (n & 4));
+      if (n & 1) one = p[n - 1].bits;
+      const uint32_t r0 = n & 2 ? two : one, r1 = n & 2 ? one : 0;
+      w = n & 4 ? any4{four.x, four.y, r0, r1} : any4{r0, r1, 0, 0};
     }
-  } else {
 #pragma unroll
-    for (int e = 0; e < 8; e++) v[e] = e < n ? to_float(p[e]) : 0.0f;
+    for (int e = 0; e < 8; e++) v[e] = to_float(T{(uint16_t)(w[e >> 1] >> (16 * (e & 1)))});
+  } else {
+    any4 a = {0, 0, 0, 0}, b = {0, 0, 0, 0};
+    if (n & 12) a = *reinterpret_cast<const any4*>(p);
+    if (n == 8) b = *reinterpret_cast<const any4*>(p + 4);
+    else if (n > 0) {
+      any2 two = {0, 0};
+      uint32_t one = 0;
+      if (n & 2) two = *reinterpret_cast<const any2*>(p + (n & 4));
+      if (n & 1) one = __builtin_bit_cast(uint32_t, p[n - 1]);
+      const any4 rest = n & 2 ? any4{two.x, two.y, one, 0} : any4{one, 0, 0, 0};
+      if (n & 4) b = rest;
+      else a = rest;
+    }
+#pragma unroll
+    for (int e = 0; e < 4; e++) {
+      const uint32_t lo = a[e], hi = b[e];                       // (a bit cast of a vector's element itself takes the first one)
+      v[e] = __builtin_bit_cast(float, lo);
+      v[4 + e] = __builtin_bit_cast(float, hi);
+    }
   }
 }
 // v rounded to T; the values as they are stored are left in v
@@ -71,10 +89,32 @@ __device__ __forceinline__ void store_up_to_8(T* p, int n, float (&v)[8]) {
   if (n == 8) {
     *reinterpret_cast<any4*>(p) = w[0];
     if constexpr (sizeof(T) == 4) *reinterpret_cast<any4*>(p + 4) = w[1];
-  } else {
-#pragma unroll
-    for (int e = 0; e < 8; e++)
-      if (e < n) p[e] = from_float<T>(v[e]);
+  } else if (n > 0) {                                            // four, two and one, as far as there are
+    if constexpr (sizeof(T) == 2) {
+      uint32_t r0 = w[0][0], r1 = w[0][1];
+      if (n & 4) {
+        *reinterpret_cast<any2*>(p) = any2{r0, r1};
+        r0 = w[0][2];
+        r1 = w[0][3];
+      }
+      if (n & 2) {
+        *reinterpret_cast<any1*>(p + (n & 4)) = r0;
+        r0 = r1;
+      }
+      if (n & 1) p[n - 1].bits = (uint16_t)r0;
+    } else {
+      any4 r = w[0];
+      if (n & 4) {
+        *reinterpret_cast<any4*>(p) = r;
+        r = w[1];
+      }
+      if (n & 2) {
+        *reinterpret_cast<any2*>(p + (n & 4)) = any2{r[0], r[1]};
+        r[0] = r[2];
+      }
+      const uint32_t one = r[0];
+      if (n & 1) p[n - 1] = __builtin_bit_cast(float, one);
+    }
   }
 }
 
