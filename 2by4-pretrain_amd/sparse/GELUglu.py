@@ -7,7 +7,6 @@ the column-major one and, like the reference, return an output stored the same w
 """
 import torch
 from torch import autograd
-from torch.autograd.function import once_differentiable
 
 from . import _native as N
 from .activation_checkpoint import ActivationCheckpoint, empty_checkpoint
@@ -104,8 +103,9 @@ class gelu_glu_checkpoint(autograd.Function):
         return out, out_values, out_scales
 
     @staticmethod
-    @once_differentiable
     def backward(ctx, grad_output, *_):
+        if torch.is_grad_enabled():
+            raise RuntimeError("a graph of the gradients of gelu_glu_checkpoint is not supported")
         if grad_output is None:
             return None, None
         values, scales = ctx.saved_tensors

@@ -11,7 +11,6 @@ The reference has no such operators; its recipe trains models that bring their o
 """
 import torch
 from torch import autograd, nn
-from torch.autograd.function import once_differentiable
 
 from . import _native as N
 from .activation_checkpoint import ActivationCheckpoint, empty_checkpoint
@@ -33,11 +32,11 @@ def _forward(x, y, gate, rows_per_gate, post_weight, post_bias, pre_weight, pre_
     param = post_weight if post_weight is not None else post_bias if post_bias is not None else pre_weight if pre_weight is not None else pre_bias
     if y is not None:
         y2, ld_y = N.as_rows(y)
-        out = torch.empty_like(x, memory_format=torch.contiguous_format)
+        out = torch.empty_like(x) if flat is x else torch.empty(shape, dtype=x.dtype, device=x.device)
     if gate is not None:
         gate, ld_gate = N.as_rows(gate)
     if pre_kind:
-        n = torch.empty_like(x if y is None else y, dtype=block_dtype, memory_format=torch.contiguous_format)
+        n = torch.empty_like(y) if y is not None and y2 is y else torch.empty(shape, dtype=block_dtype, device=x.device)
         if keep:
             values, scales = empty_checkpoint(rows, cols, x.device)
     if with_stats and (post_kind or pre_kind):
@@ -65,8 +64,9 @@ class _block_norm(autograd.Function):
         return out, n, values, scales
 
     @staticmethod
-    @once_differentiable
     def backward(ctx, grad_out, grad_n, _values, _scales):
+        if torch.is_grad_enabled():
+            raise RuntimeError("a graph of the gradients of block_norm and residual_norm is not supported")
         h, y, gate, post_weight, post_bias, pre_weight, stats = ctx.saved_tensors
         shape, stream_dtype, block_dtype, pre_bias_dtype, residual, rows_per_gate, scale, post_kind, pre_kind = ctx.call
         needs = ctx.needs_input_grad
@@ -79,11 +79,18 @@ class _block_norm(autograd.Function):
         param = post_weight if post_weight is not None else post_bias if post_bias is not None else pre_weight
         param_dtype = pre_bias_dtype if param is None else param.dtype
         make = torch.empty if rows else torch.zeros                # (sums over no rows)
-        grad_x = torch.empty(shape, dtype=stream_dtype, device=device) if needs[0] else None
-        grad_y = torch.empty(shape, dtype=block_dtype, device=device) if needs[1] else None
-        grad_gate = make(gate.shape, dtype=gate.dtype, device=device) if needs[2] else None
-        grads = [make(cols, dtype=param_dtype, device=device) if need and kind else None for need, kind in zip(needs[3:7], (post_kind, post_kind, pre_kind, pre_kind))]
-        sums = any(needs[2:7])
+        grad_x = grad_y = grad_gate = None
+        if needs[0]:
+            grad_x = torch.empty(shape, dtype=stream_dtype, device=device)
+        if needs[1]:
+            grad_y = torch.empty(shape, dtype=block_dtype, device=device)
+        if needs[2]:
+            grad_gate = make(gate.shape, dtype=gate.dtype, device=device)
+        grads = [None] * 4
+        for i, kind in enumerate((post_kind, post_kind, pre_kind, pre_kind)):
+            if needs[3 + i] and kind:
+                grads[i] = make(cols, dtype=param_dtype, device=device)
+        sums = needs[2] or needs[3] or needs[4] or needs[5] or needs[6]
         if rows:
             lib, code, ptr = N.lib(), N.dtype_codes, N.ptr
             dout = dn = h2 = y2 = gate2 = workspace = None
@@ -149,9 +156,15 @@ def _gate(fn, gate, y):
 
 def _call(x, y, gate, rows_per_gate, post_weight, post_bias, pre_weight, pre_bias, scale, post_kind, pre_kind, eps, block_dtype, keep):
     """(out, n, checkpoint of n)"""
-    tensors = (x, y, gate, post_weight, post_bias, pre_weight, pre_bias)
-    if (torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in tensors)) or not N.plain_eager():
-        out, n, values, scales = _block_norm.apply(*tensors, rows_per_gate, scale, post_kind, pre_kind, eps, block_dtype, keep)
+    graph = False
+    if torch.is_grad_enabled():
+        for t in (x, y, gate, post_weight, post_bias, pre_weight, pre_bias):
+            if t is not None and t.requires_grad:
+                graph = True
+                break
+    if graph or not N.plain_eager():
+        out, n, values, scales = _block_norm.apply(x, y, gate, post_weight, post_bias, pre_weight, pre_bias, rows_per_gate, scale, post_kind, pre_kind, eps, block_dtype,
+                                                   keep)
     else:
         out, n, _, values, scales = _forward(x, y, gate, rows_per_gate, post_weight, post_bias, pre_weight, pre_bias, scale, post_kind, pre_kind, eps, block_dtype,
                                              keep, False)
@@ -204,10 +217,9 @@ def residual_norm(residual, y, gate=None, residual_scale=1.0, *, post_kind=None,
     of n).  Gradients (once) for residual, y, gate, weights and biases."""
     fn = "residual_norm"
     _check_rows(fn, "residual", residual)
-    _check_rows(fn, "y", y)
-    if residual.shape != y.shape or residual.device != y.device:
+    if residual.shape != y.shape or residual.get_device() != y.get_device():
         raise RuntimeError(f"{fn}: residual {tuple(residual.shape)} on {residual.device} and y {tuple(y.shape)} on {y.device} differ")
-    if residual.dtype != torch.float32 and residual.dtype != y.dtype:
+    if y.dtype not in _TYPES or (residual.dtype != torch.float32 and residual.dtype != y.dtype):
         raise RuntimeError(f"{fn}: a stream of {residual.dtype} with a block of {y.dtype} is not supported")
     post, pre = _kind(fn, post_kind, post_weight, post_bias), _kind(fn, pre_kind, pre_weight, pre_bias)
     if checkpoint and not pre:

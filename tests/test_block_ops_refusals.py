@@ -109,3 +109,41 @@ def test_python_refuses_what_does_not_fit_together():
         sparse.GELUglu(output_checkpoint=True)
     assert sparse.ResidualNorm(8, post="rms", pre="layer", gate=0.1).gate.tolist() == [pytest.approx(0.1)] * 8
     assert {k for k, _ in sparse.ResidualNorm(8, post="rms", pre="layer").named_parameters()} == {"post_weight", "pre_weight", "pre_bias"}
+
+
+def test_calls_go_to_the_stream_of_the_tensors_device(monkeypatch):
+    from contextlib import contextmanager
+    from sparse import _native as N
+    current, streams = [0], []
+
+    class Tensor:
+        device = "device 1"
+
+        def get_device(self):
+            return 1
+
+    @contextmanager
+    def device(d):
+        assert d == "device 1"
+        current[0] = 1
+        yield
+        current[0] = 0
+
+    monkeypatch.setattr(torch.cuda, "current_device", lambda: current[0])
+    monkeypatch.setattr(torch.cuda, "device", device)
+    monkeypatch.setattr(N, "stream_ptr", lambda: 100 + current[0])
+    N.launch(Tensor(), lambda *a: (streams.append(a), 0)[1], 7)
+    current[0] = 1
+    N.launch(Tensor(), lambda *a: (streams.append(a), 0)[1], 8)
+    assert streams == [(7, 101), (8, 101)]
+
+
+def test_rows_of_any_tensor():
+    """as_rows: contiguous tensors as they are, others as a matrix of contiguous rows whose leading dimension may be 0."""
+    from sparse import _native as N
+    x = torch.arange(60.0).view(3, 4, 5)
+    assert N.as_rows(x)[0] is x and N.as_rows(x)[1] == 5
+    for view in (x[:, ::2], x[..., 1:4], x.transpose(0, 1), x.transpose(1, 2), x[:1, :1].expand(2, 3, 5), x[..., :1].expand(3, 4, 5), x[0, 0, ::2], torch._neg_view(x)):
+        rows, ld = N.as_rows(view)
+        flat = torch.as_strided(rows, (view.numel() // view.shape[-1], view.shape[-1]), (ld, 1))
+        assert torch.equal(flat, view.resolve_neg().reshape(-1, view.shape[-1]))

@@ -311,6 +311,59 @@ def test_refusals(cuda):
             call()
 
 
+def test_rows_beyond_32_bits_of_elements(cuda):
+    """More than 2^31 elements: the last rows are what they are by themselves, forward and backward, with a gate for every row and without."""
+    import sparse
+    rows, cols = 262400, 8200
+    tail = {k: draw(120 + i, 5, cols, dtype=BF16).to(cuda) for i, k in enumerate(("x", "y", "gate", "go", "gn"))}
+    w = draw(130, cols, mean=1.0, dtype=BF16).to(cuda)
+    whole = {}
+    for k, v in tail.items():
+        whole[k] = torch.zeros(rows, cols, dtype=BF16, device=cuda)
+        whole[k][-5:] = v
+    for gated in (False, True):
+        def step(t):
+            x, y, g = (t[k].detach().requires_grad_() for k in ("x", "y", "gate"))
+            out, n, kept = sparse.residual_norm(x, y, g if gated else None, post_kind="rms", post_weight=w, pre_kind="layer", pre_weight=w, checkpoint=True)
+            grads = torch.autograd.grad((out, n), (x, y, g) if gated else (x, y), (t["go"], t["gn"]))
+            return [v[-5:].clone() for v in (out.detach(), n.detach(), kept.values.view(torch.uint8), kept.scales, *grads)]
+        for a, b in zip(step(whole), step(tail)):
+            assert torch.equal(a, b)
+
+
+def test_two_threads_on_two_streams(cuda):
+    """Calls from two threads at once, each on a stream of its own."""
+    import threading
+    import sparse
+    data = [[draw(140 + 5 * i + j, 300, 1000, dtype=BF16).to(cuda) for j in range(4)] for i in range(2)]
+    w = draw(150, 1000, mean=1.0, dtype=BF16).to(cuda)
+
+    def step(x, y, go, gn):
+        leaves = [t.detach().requires_grad_() for t in (x, y, w)]
+        out, n = sparse.residual_norm(leaves[0], leaves[1], post_kind="layer", post_weight=leaves[2], pre_kind="rms", pre_weight=leaves[2])
+        return [out.detach(), n.detach(), *torch.autograd.grad((out, n), leaves, (go, gn))]
+
+    want = [step(*d) for d in data]
+    torch.cuda.synchronize()
+    wrong = []
+
+    def work(i):
+        stream = torch.cuda.Stream()
+        with torch.cuda.stream(stream):
+            for _ in range(20):
+                got = step(*data[i])
+                stream.synchronize()
+                if not all(torch.equal(a, b) for a, b in zip(got, want[i])):
+                    wrong.append(i)
+
+    threads = [threading.Thread(target=work, args=(i,)) for i in range(2)]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join(60)
+    assert not wrong and not any(t.is_alive() for t in threads)
+
+
 def test_other_streams_and_replayed_graphs(cuda):
     """On a side stream, and captured (both passes): every replay gives the bits of the eager call on the inputs of the moment, with eager work between."""
     import sparse
