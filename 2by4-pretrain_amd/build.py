@@ -3,7 +3,8 @@
     python 2by4-pretrain_amd/build.py [-j N] [--force]
 
 Objects go to 2by4-pretrain_amd/build/, the library next to the Python package that loads it
-(2by4-pretrain_amd/sparse/lib2by4_gfx950.so), beside it _fastcall.abi3.so, through which Python makes the frequent calls.
+(2by4-pretrain_amd/sparse/lib2by4_gfx950.so), beside it _fastcall.abi3.so, through which Python makes the frequent calls, and _torchcall, which
+makes the ordinary calls of some operators from torch's C++ side.
 """
 import argparse
 import concurrent.futures
@@ -65,6 +66,35 @@ def build_fastcall():
         raise RuntimeError(f"building the CPython module failed:\n{res.stdout}\n{res.stderr}")
 
 
+def torchcall_path():
+    return os.path.join(HERE, "sparse", "_torchcall" + sysconfig.get_config_var("EXT_SUFFIX"))
+
+
+def build_torchcall():
+    """The calls from torch's C++ side, for the torch that is installed; Python makes them where this is left out.  It finds the library beside itself
+    and torch's among what `import torch` has loaded."""
+    path = torchcall_path()
+    if os.path.exists(path):
+        os.remove(path)
+    try:
+        import torch
+    except ImportError:
+        print("no torch: _torchcall is left out", file=sys.stderr)
+        return
+    at = os.path.dirname(torch.__file__)
+    flags = ["-O2", "-std=c++17", "-shared", "-fPIC", "-D__HIP_PLATFORM_AMD__=1", "-DUSE_ROCM", f"-D_GLIBCXX_USE_CXX11_ABI={int(torch._C._GLIBCXX_USE_CXX11_ABI)}",
+             "-DTORCH_EXTENSION_NAME=_torchcall", f'-DTF24_TORCH_VERSION="{torch.__version__}"', "-I", os.path.join(ROOT, "include"), "-I", sysconfig.get_paths()["include"],
+             "-isystem", os.path.join(at, "include"), "-isystem", os.path.join(at, "include", "torch", "csrc", "api", "include"),
+             "-isystem", os.path.join(os.path.dirname(os.path.dirname(HIPCC)), "include")]
+    libraries = ["-L", os.path.dirname(LIB), "-l:" + os.path.basename(LIB), "-L", os.path.join(at, "lib"), "-lc10", "-lc10_hip", "-ltorch_cpu", "-ltorch", "-ltorch_python",
+                 "-Wl,--disable-new-dtags,-rpath,$ORIGIN", "-Wl,--allow-shlib-undefined"]
+    res = subprocess.run([CXX, *flags, os.path.join(CSRC, "torch_calls.cpp"), "-o", path, *libraries], capture_output=True, text=True)
+    if res.returncode:
+        print(f"_torchcall is left out, its calls will go through Python:\n{res.stderr[-2000:]}", file=sys.stderr)
+        if os.path.exists(path):
+            os.remove(path)
+
+
 def build_library(jobs=8, force=True, verbose=False):
     os.makedirs(OBJ, exist_ok=True)
     with concurrent.futures.ThreadPoolExecutor(max_workers=max(1, jobs)) as pool:
@@ -79,6 +109,7 @@ def build_library(jobs=8, force=True, verbose=False):
     if res.returncode:
         raise RuntimeError(f"link failed:\n{res.stdout}\n{res.stderr}")
     build_fastcall()
+    build_torchcall()
     return LIB
 
 

@@ -76,6 +76,15 @@ class gelu_glu_checkpoint(autograd.Function):
     output is the same.  apply(input) -> out; apply(input, True) -> (out, values, scales), the last two being out kept in 8 bits.  Any
     input with a last dimension of an even size; the output is row-major."""
 
+    @classmethod
+    def apply(cls, input, keep_output=False):
+        calls = N.torch_calls()
+        if calls is not None and cls is gelu_glu_checkpoint and N.plain_eager():
+            result = calls.gelu_glu_checkpoint(input, keep_output)
+            if result is not None:
+                return result
+        return super().apply(input, keep_output)
+
     @staticmethod
     def forward(ctx, input, keep_output=False):
         if not input.is_cuda:
@@ -136,4 +145,4 @@ class GELUglu(torch.nn.Module):
         if not self.output_checkpoint:
             return gelu_glu_checkpoint.apply(x)
         out, values, scales = gelu_glu_checkpoint.apply(x, True)
-        return out, ActivationCheckpoint(values, scales, out.shape, out.dtype)
+        return out, ActivationCheckpoint._of(values, scales, out.shape, out.dtype)

@@ -118,6 +118,23 @@ def lib():
     return _lib
 
 
+_calls = ...
+
+
+def torch_calls():
+    """The module _torchcall (csrc/torch_calls.cpp), which makes the ordinary calls of some operators from torch's C++ side, or None: not built, or for another
+    torch.  Its functions give None for a call that is Python's."""
+    global _calls
+    if _calls is ...:
+        lib()
+        try:
+            from . import _torchcall
+        except ImportError:
+            _torchcall = None
+        _calls = _torchcall if _torchcall is not None and _torchcall.built_for == torch.__version__ else None
+    return _calls
+
+
 def version():
     return lib().tf24_version().decode()
 

@@ -38,6 +38,13 @@ class ActivationCheckpoint:
                                f"do not hold a tensor {tuple(shape)} {dtype}")
         self.values, self.scales, self.shape, self.dtype = values, scales, shape, dtype
 
+    @classmethod
+    def _of(cls, values, scales, shape, dtype):
+        """One of tensors that were made for it."""
+        self = object.__new__(cls)
+        self.values, self.scales, self.shape, self.dtype = values, scales, shape, dtype
+        return self
+
     @property
     def device(self):
         return self.values.device
@@ -51,6 +58,11 @@ class ActivationCheckpoint:
         dtype = self.dtype if dtype is None else dtype
         if dtype not in _TYPES:
             raise RuntimeError(f"ActivationCheckpoint.decode: dtype {dtype} is not supported")
+        calls = N.torch_calls()
+        if calls is not None:
+            out = calls.checkpoint_decode(self.values, self.scales, self.shape, N.dtype_codes[dtype])
+            if out is not None:
+                return out
         out = torch.empty(self.shape, dtype=dtype, device=self.values.device)
         rows, cols = self.values.shape[0], self.shape[-1]
         N.launch(out, N.lib().tf24_checkpoint_decode, self.values.data_ptr(), self.scales.data_ptr(), rows, cols, out.data_ptr(), N.dtype_code(dtype), cols)
@@ -69,6 +81,11 @@ def empty_checkpoint(rows, cols, device):
 
 def checkpoint_activation(x):
     """x (float32, float16 or bfloat16, on a GPU, at least one dimension and one column) kept in 8 bits."""
+    calls = N.torch_calls()
+    if calls is not None and N.plain_eager():
+        kept = calls.checkpoint_encode(x)
+        if kept is not None:
+            return ActivationCheckpoint._of(*kept, x.shape, x.dtype)
     if not x.is_cuda:
         raise RuntimeError("checkpoint_activation: only CUDA tensors are supported")
     if x.dtype not in _TYPES:
@@ -80,7 +97,7 @@ def checkpoint_activation(x):
     rows = x.shape[:-1].numel()
     values, scales = empty_checkpoint(rows, cols, x.device)
     N.launch(x, N.lib().tf24_checkpoint_encode, flat.data_ptr(), N.dtype_code(x.dtype), ld, rows, cols, values.data_ptr(), scales.data_ptr())
-    return ActivationCheckpoint(values, scales, x.shape, x.dtype)
+    return ActivationCheckpoint._of(values, scales, x.shape, x.dtype)
 
 
 def as_checkpoint(x, given):
@@ -108,6 +125,11 @@ def checkpoint_weight_gradient(grad_output, checkpoint, bias=False, dtype=None):
     if g.dim() == 0 or g.shape[:-1] != shape[:-1] or g.shape[-1] == 0:
         raise RuntimeError(f"checkpoint_weight_gradient: grad_output {tuple(g.shape)} does not suit a checkpoint of {tuple(shape)}")
     tokens, m, n = checkpoint.values.shape[0], g.shape[-1], shape[-1]
+    calls = N.torch_calls()
+    if calls is not None and N.plain_eager():
+        grads = calls.checkpoint_weight_grad(g, checkpoint.values, checkpoint.scales, n, bias, N.dtype_codes[dtype])
+        if grads is not None:
+            return grads
     if tokens == 0:
         return torch.zeros((m, n), dtype=dtype, device=g.device), torch.zeros(m, dtype=dtype, device=g.device) if bias else None
     g, ld = N.as_rows(g)

@@ -168,7 +168,23 @@ def _call(x, y, gate, rows_per_gate, post_weight, post_bias, pre_weight, pre_bia
     else:
         out, n, _, values, scales = _forward(x, y, gate, rows_per_gate, post_weight, post_bias, pre_weight, pre_bias, scale, post_kind, pre_kind, eps, block_dtype,
                                              keep, False)
-    return out, n, ActivationCheckpoint(values, scales, n.shape, n.dtype) if keep else None
+    return out, n, ActivationCheckpoint._of(values, scales, n.shape, n.dtype) if keep else None
+
+
+def _ordinary(x, y, gate, post_weight, post_bias, pre_weight, pre_bias, scale, post_kind, pre_kind, eps, block_code, checkpoint):
+    """_call from torch's C++ side, or None: a call to be looked at more closely."""
+    calls = N.torch_calls()
+    if calls is None or not N.plain_eager():
+        return None
+    post, pre = _KINDS.get(post_kind), _KINDS.get(pre_kind)
+    if (post is None or pre is None or (not post and (post_weight is not None or post_bias is not None))
+            or (not pre and (checkpoint or pre_weight is not None or pre_bias is not None))):
+        return None
+    result = calls.block_norm(x, y, gate, post_weight, post_bias, pre_weight, pre_bias, scale, post, pre, eps, block_code, bool(checkpoint))
+    if result is None:
+        return None
+    out, n, values, scales = result
+    return out, n, ActivationCheckpoint._of(values, scales, n.shape, n.dtype) if checkpoint else None
 
 
 def _check_rows(fn, name, t):
@@ -193,6 +209,9 @@ def block_norm(x, weight=None, bias=None, kind="layer", eps=1e-5, out_dtype=None
     the last dimension (1 to 16384 columns), of type `out_dtype` (default: x's; a 16-bit x gives its own type only).  With checkpoint=True
     the result is (n, ActivationCheckpoint of n)."""
     fn = "block_norm"
+    done = None if kind is None else _ordinary(x, None, None, None, None, weight, bias, 1.0, None, kind, eps, N.dtype_codes.get(out_dtype or x.dtype, -1), checkpoint)
+    if done is not None:
+        return done[1:] if checkpoint else done[1]
     _check_rows(fn, "x", x)
     if kind is None:
         raise RuntimeError(f"{fn}: kind of norm None is not supported (rms, layer)")
@@ -216,6 +235,9 @@ def residual_norm(residual, y, gate=None, residual_scale=1.0, *, post_kind=None,
     a sequence's [B, 1, C], a token's [B, S, C].  Returns out, with a pre_kind (out, n), with checkpoint=True (out, n, ActivationCheckpoint
     of n).  Gradients (once) for residual, y, gate, weights and biases."""
     fn = "residual_norm"
+    done = _ordinary(residual, y, gate, post_weight, post_bias, pre_weight, pre_bias, residual_scale, post_kind, pre_kind, eps, 0, checkpoint)
+    if done is not None:
+        return done if checkpoint else done[:2] if pre_kind else done[0]
     _check_rows(fn, "residual", residual)
     if residual.shape != y.shape or residual.get_device() != y.get_device():
         raise RuntimeError(f"{fn}: residual {tuple(residual.shape)} on {residual.device} and y {tuple(y.shape)} on {y.device} differ")

@@ -12,6 +12,17 @@ pytestmark = pytest.mark.gpu
 F32, F16, BF16 = torch.float32, torch.float16, torch.bfloat16
 
 
+@pytest.fixture(autouse=True, params=["torchcall", "python"])
+def calls(request, monkeypatch):
+    """Everything twice: with the module that makes ordinary calls from torch's C++ side, and with Python making all of them."""
+    from sparse import _native as N
+    if request.param == "python":
+        monkeypatch.setattr(N, "_calls", None)
+    elif N.torch_calls() is None:
+        pytest.skip("_torchcall is not built for this torch")
+
+
+
 def draw(seed, *shape, dtype=F32, std=1.0):
     return (torch.randn(shape, generator=torch.Generator().manual_seed(seed)) * std).to(dtype)
 
@@ -82,6 +93,32 @@ def test_sparse_layer(cuda, lead, d_in, d_out, dtype):
     assert torch.equal(grads["weight"], of_kept["weight"]) and not torch.equal(grads["weight"], want["weight"])
     given = step(plain, x, dy, F16, checkpoint=kept)
     assert torch.equal(given[0], out) and all(torch.equal(given[1][k], grads[k]) for k in grads)
+
+
+def test_ordinary_calls_are_made_from_the_c_side(cuda, calls):
+    """With the module, and where it is built for this torch it is there: graphs of its nodes; what it does not take is Python's, with the same result."""
+    import sparse
+    from sparse import _native as N
+    module = N.torch_calls()
+    x, y, w = draw(1, 3, 4, 64).to(cuda).requires_grad_(), draw(2, 3, 4, 64, dtype=F16).to(cuda).requires_grad_(), torch.ones(64, device=cuda, requires_grad=True)
+    out, n = sparse.residual_norm(x, y, pre_kind="rms", pre_weight=w)
+    strided = sparse.residual_norm(x.transpose(0, 1).contiguous().transpose(0, 1), y, pre_kind="rms", pre_weight=w)
+    assert torch.equal(out, strided[0]) and torch.equal(n, strided[1])
+    names = [t.grad_fn.name() for t in (out, n, strided[0], sparse.block_norm(x), sparse.gelu_glu_checkpoint.apply(x), sparse.gelu_glu_checkpoint.apply(x[..., 1:63]))]
+    if module is None:
+        assert not any(name in ("BlockNormBackward", "GeluGluBackward") for name in names)
+    else:
+        assert names[0] == names[1] == names[3] == "BlockNormBackward" != names[2] and names[4] == "GeluGluBackward" != names[5]
+        assert module.checkpoint_encode(x.detach()[..., ::2]) is None and module.checkpoint_encode(x.detach()) is not None
+    first = torch.autograd.grad(n.float().sum(), w, retain_graph=True)[0]
+    assert torch.equal(first, torch.autograd.grad(n.float().sum(), w)[0])
+    with pytest.raises(RuntimeError):                              # its tensors are gone
+        torch.autograd.grad(n.float().sum(), w)
+    z = draw(3, 3, 4, 64).to(cuda).requires_grad_()
+    out, n = sparse.residual_norm(z, y, pre_kind="layer")
+    out.detach().add_(1)                                           # what the backward pass reads was changed
+    with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+        n.float().sum().backward()
 
 
 def test_what_is_held_between_the_passes(cuda):

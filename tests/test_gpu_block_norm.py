@@ -20,6 +20,17 @@ F32, F16, BF16 = torch.float32, torch.float16, torch.bfloat16
 U = 2.0 ** -24
 
 
+@pytest.fixture(autouse=True, params=["torchcall", "python"])
+def calls(request, monkeypatch):
+    """Everything twice: with the module that makes ordinary calls from torch's C++ side, and with Python making all of them."""
+    from sparse import _native as N
+    if request.param == "python":
+        monkeypatch.setattr(N, "_calls", None)
+    elif N.torch_calls() is None:
+        pytest.skip("_torchcall is not built for this torch")
+
+
+
 def draw(seed, *shape, dtype=F32, std=1.0, mean=0.0):
     return (torch.randn(shape, generator=torch.Generator().manual_seed(seed), dtype=torch.float64) * std + mean).to(dtype)
 
