@@ -61,7 +61,8 @@ __device__ __forceinline__ void statistics(Cells<S::UNITS>& c, const P& at, int 
       for (int e = 0; e < 8; e++) s = __builtin_fmaf(c.v[u][e], c.v[u][e], s);
     sum(s);
   }
-  r = rsqrtf(__builtin_fmaf(s, inv_cols, eps) - left * left);
+  const float variance = __builtin_fmaf(s, inv_cols, -left * left);
+  r = rsqrtf((variance < 0.0f ? 0.0f : variance) + eps);          // (of a row of one value rounding may leave less than nothing; a NaN stays)
 }
 
 struct ForwardArgs {

@@ -88,7 +88,7 @@ block_norm_backward(const BackwardArgs a) {
 #pragma unroll
       for (int e = 0; e < 8; e++) d.v[u][e] = r.dout.get(u, e);
     if (a.pre_kind) {
-      const float scale = r.pre_scale, shift = -r.pre_mean * scale;
+      const float scale = r.pre_scale, mean = r.pre_mean;
       Cells<U> hat, q;
       float s1 = 0.0f, s2 = 0.0f;
 #pragma unroll
@@ -96,7 +96,7 @@ block_norm_backward(const BackwardArgs a) {
 #pragma unroll
         for (int e = 0; e < 8; e++) {
           const float g = r.dn.get(u, e);
-          hat.v[u][e] = __builtin_fmaf(r.h.get(u, e), scale, shift);
+          hat.v[u][e] = (r.h.get(u, e) - mean) * scale;           // (-mean * scale would be rounded where the mean is large)
           sum_nh.v[u][e] = __builtin_fmaf(g, hat.v[u][e], sum_nh.v[u][e]);
           sum_n.v[u][e] += g;
           q.v[u][e] = g * pre_w.v[u][e];
@@ -121,7 +121,7 @@ block_norm_backward(const BackwardArgs a) {
       }
     }
     if constexpr (RESIDUAL) {
-      const float scale = a.post_kind ? r.post_scale : 1.0f, shift = a.post_kind ? -r.post_mean * scale : 0.0f;
+      const float scale = a.post_kind ? r.post_scale : 1.0f, mean = a.post_kind ? r.post_mean : 0.0f;
       if (MODE == ROW_GATES && here) {                              // d becomes that of z
         Cells<U> gate, bias;
         load_params(a.gate, a.gate_dtype, row * a.ld_gate, place, 1.0f, gate);
@@ -132,7 +132,7 @@ block_norm_backward(const BackwardArgs a) {
             float dg[8];
 #pragma unroll
             for (int e = 0; e < 8; e++)
-              dg[e] = d.v[u][e] * (a.post_kind ? __builtin_fmaf(__builtin_fmaf(r.y.get(u, e), scale, shift), post_w.v[u][e], bias.v[u][e]) : r.y.get(u, e));
+              dg[e] = d.v[u][e] * (a.post_kind ? __builtin_fmaf((r.y.get(u, e) - mean) * scale, post_w.v[u][e], bias.v[u][e]) : r.y.get(u, e));
             const int64_t to = (int64_t)row * a.cols;
             if (a.gate_dtype == TF24_F32) place.store((float*)a.grad_gate + to, u, dg);
             else if (a.gate_dtype == TF24_F16) place.store((f16_t*)a.grad_gate + to, u, dg);
@@ -150,7 +150,7 @@ block_norm_backward(const BackwardArgs a) {
       for (int u = 0; u < U; u++)
 #pragma unroll
         for (int e = 0; e < 8; e++) {
-          hat.v[u][e] = __builtin_fmaf(r.y.get(u, e), scale, shift);
+          hat.v[u][e] = (r.y.get(u, e) - mean) * scale;
           sum_dy.v[u][e] = __builtin_fmaf(d.v[u][e], hat.v[u][e], sum_dy.v[u][e]);
           sum_d.v[u][e] += d.v[u][e];
           d.v[u][e] *= post_w.v[u][e];

@@ -405,3 +405,20 @@ def test_other_streams_and_replayed_graphs(cuda):
         graph.replay()
         torch.cuda.synchronize()
         assert all(torch.equal(a, b) for a, b in zip(recorded, want)), replay
+
+
+def test_constant_rows_of_large_values(cuda):
+    """Rows of one value up to 1e12: their variance is zero, whatever rounding makes of it.  The first mean is off by 64 u |v| at most, the second one
+    by 64 u of that, which r = 1 / sqrt(eps) scales."""
+    import sparse
+    value = 10.0 ** torch.linspace(0, 12, 400, dtype=torch.float64).view(-1, 1)
+    for cols in (5, 96, 1000, 1601, 5000):
+        x = value.float().expand(-1, cols).contiguous()
+        x[::2] *= -1
+        w, b = draw(160, cols, mean=1.0), draw(161, cols)
+        leaf = x.to(cuda).requires_grad_()
+        n = sparse.block_norm(leaf, w.to(cuda), b.to(cuda), kind="layer", eps=1e-5)
+        assert n.isfinite().all(), cols
+        off = (n.detach().cpu().double() - b.double()).abs()
+        assert (off <= ((64 * U) ** 2 * value * 1e-5 ** -0.5 + 1e-6) * w.double().abs() + U * b.double().abs()).all(), cols
+        assert torch.autograd.grad(n, leaf, torch.ones_like(n))[0].isfinite().all()
