@@ -422,3 +422,69 @@ def test_constant_rows_of_large_values(cuda):
         off = (n.detach().cpu().double() - b.double()).abs()
         assert (off <= ((64 * U) ** 2 * value * 1e-5 ** -0.5 + 1e-6) * w.double().abs() + U * b.double().abs()).all(), cols
         assert torch.autograd.grad(n, leaf, torch.ones_like(n))[0].isfinite().all()
+
+
+def test_graphs_hooks_and_changes_in_place(cuda):
+    import sparse
+    from torch.utils.checkpoint import checkpoint
+    x, y, w = draw(170, 6, 96).to(cuda).requires_grad_(), draw(171, 6, 96).to(cuda).requires_grad_(), draw(172, 96, mean=1.0).to(cuda).requires_grad_()
+    go, gn = draw(173, 6, 96).to(cuda), draw(174, 6, 96).to(cuda)
+    call = lambda x, y, w: sparse.residual_norm(x, y, post_kind="rms", post_weight=w, pre_kind="layer", pre_weight=w)  # noqa: E731
+    out, n = call(x, y, w)
+    want = torch.autograd.grad((out, n), (x, y, w), (go, gn), retain_graph=True)
+    same = lambda got: all(torch.equal(a, b) for a, b in zip(got, want))  # noqa: E731
+    assert same(torch.autograd.grad((out, n), (x, y, w), (go, gn)))
+    with pytest.raises(RuntimeError, match="second time"):
+        torch.autograd.grad((out, n), (x, y, w), (go, gn))
+    # one output alone: as with zeros for the other one
+    for one in (0, 1):
+        zeros = [go, gn]
+        zeros[1 - one] = torch.zeros_like(go)
+        a = torch.autograd.grad(call(x, y, w)[one], (x, y, w), (go, gn)[one])
+        b = torch.autograd.grad(call(x, y, w), (x, y, w), zeros)
+        assert all(torch.allclose(s, t, rtol=1e-5, atol=1e-5) for s, t in zip(a, b))
+    # what the backward pass reads may not change
+    for i in (0, 1):
+        y2 = y.detach().clone().requires_grad_()
+        moved = y2 * 1
+        out, n = call(x, moved, w)
+        with torch.no_grad():
+            (out, moved)[i].add_(1)
+        with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+            torch.autograd.grad(n, w, gn)
+    out = sparse.residual_norm(x, y, residual_scale=0.5)           # (reads nothing)
+    out.add_(1)
+    assert all(torch.equal(a, b) for a, b in zip(torch.autograd.grad(out, (x, y), go), (0.5 * go, go)))
+    # hooks of the saved tensors, the forward pass made again, gradients of the outputs
+    with torch.autograd.graph.save_on_cpu():
+        out, n = call(x, y, w)
+    assert same(torch.autograd.grad((out, n), (x, y, w), (go, gn)))
+    for reentrant in (False, True):
+        out, n = checkpoint(call, x, y, w, use_reentrant=reentrant)
+        for t in (x, y, w):
+            t.grad = None
+        torch.autograd.backward((out, n), (go, gn))
+        assert same((x.grad, y.grad, w.grad))
+    out, n = call(x, y, w)
+    out.retain_grad()
+    n.register_hook(lambda g: 2 * g)
+    torch.autograd.backward((out, n), (go, gn / 2))
+    assert torch.equal(out.grad, go)
+    with torch.inference_mode():
+        assert all(torch.equal(a, b) for a, b in zip(call(x, y, w), call(x.detach(), y.detach(), w.detach())))
+    out, n = call(x, y, w)
+    with pytest.raises(RuntimeError, match="graph of the gradients"):
+        torch.autograd.grad(n, x, gn, create_graph=True)
+
+
+def test_refusals_of_what_is_no_tensor(cuda):
+    import sparse
+    x = torch.zeros(4, 64, device=cuda)
+    for y in (None, 1.0):
+        with pytest.raises(RuntimeError, match="residual_norm"):
+            sparse.residual_norm(x, y, pre_kind="rms")
+        with pytest.raises(RuntimeError, match="residual_norm"):
+            sparse.residual_norm(x, y, x, pre_kind="rms")
+    with pytest.raises(RuntimeError, match="residual_scale"):
+        sparse.residual_norm(x, x, residual_scale=torch.ones((), device=cuda, requires_grad=True))
+    assert torch.equal(sparse.residual_norm(x + 1, x, residual_scale=torch.tensor(0.5)), x + 0.5)
