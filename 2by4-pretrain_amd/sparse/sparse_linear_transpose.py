@@ -91,6 +91,8 @@ class sparse_linear_transpose(autograd.Function):
             if len(ctx.shape) != 2:
                 grad_input = grad_input.view(ctx.shape)
         if needs[1]:
+            if ctx.kept and torch.is_grad_enabled():
+                raise RuntimeError("a graph of the gradients of a layer that keeps its input in 8 bits is not supported")
             input = ActivationCheckpoint(*saved, ctx.shape, ctx.dtype).decode() if ctx.kept else saved[0]
             if input.dim() != 2:
                 input = input.view(-1, input.shape[-1])

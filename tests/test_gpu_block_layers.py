@@ -287,3 +287,9 @@ def test_block_captured_and_replayed(cuda):
         got = [t.clone() for t in recorded]
         for a, b in zip(got, one()):
             assert torch.equal(a, b), replay
+
+
+def test_no_graph_of_the_gradients_of_a_sparse_layer_that_keeps_its_input_in_8_bits(cuda):
+    layer, x = sparse_layer(cuda, 64, 64, 3), draw(4, 64, 64, dtype=F16).to(cuda).requires_grad_()
+    with pytest.raises(RuntimeError, match="graph of the gradients"):
+        torch.autograd.grad(layer(x, checkpoint=True).float().sum(), layer.weight, create_graph=True)
