@@ -133,11 +133,14 @@ class GELUglu(torch.nn.Module):
     """checkpoint=True: the input is kept in 8 bits for the backward pass (gelu_glu_checkpoint).  output_checkpoint=True as well: forward
     returns (out, ActivationCheckpoint of out), for a layer that takes its input with one."""
 
+    checkpoint = output_checkpoint = False
+
     def __init__(self, checkpoint=False, output_checkpoint=False):
         super().__init__()
         if output_checkpoint and not checkpoint:
             raise RuntimeError("GELUglu: output_checkpoint without checkpoint is not supported")
-        self.checkpoint, self.output_checkpoint = checkpoint, output_checkpoint
+        if checkpoint:
+            self.checkpoint, self.output_checkpoint = True, bool(output_checkpoint)
 
     def forward(self, x):
         if not self.checkpoint:

@@ -104,6 +104,8 @@ def as_checkpoint(x, given):
     """What a layer keeps of its input x: the checkpoint that came with it, or with given=True one made here."""
     if given is True:
         return checkpoint_activation(x)
+    if not isinstance(given, ActivationCheckpoint):
+        raise RuntimeError(f"{type(given).__name__} is not a checkpoint of the input")
     if given.shape != x.shape or given.dtype != x.dtype or given.values.get_device() != x.get_device():
         raise RuntimeError(f"the checkpoint of a tensor {tuple(given.shape)} {given.dtype} on {given.device} is not one of {tuple(x.shape)} {x.dtype} on {x.device}")
     return given

@@ -147,3 +147,19 @@ def test_rows_of_any_tensor():
         rows, ld = N.as_rows(view)
         flat = torch.as_strided(rows, (view.numel() // view.shape[-1], view.shape[-1]), (ld, 1))
         assert torch.equal(flat, view.resolve_neg().reshape(-1, view.shape[-1]))
+
+
+def test_layers_refuse_what_is_no_checkpoint():
+    from sparse.activation_checkpoint import as_checkpoint
+    for given in (False, torch.zeros(4, 64), 1):
+        with pytest.raises(RuntimeError, match="checkpoint"):
+            as_checkpoint(torch.zeros(4, 64), given)
+
+
+def test_a_gated_activation_from_before_it_could_keep_anything():
+    import sparse
+    old = sparse.GELUglu.__new__(sparse.GELUglu)
+    old.__setstate__({k: v for k, v in sparse.GELUglu().__dict__.items() if "checkpoint" not in k})
+    assert not old.checkpoint and not old.output_checkpoint
+    with pytest.raises(RuntimeError, match="CUDA"):
+        old(torch.zeros(1, 4, 64))
