@@ -488,3 +488,10 @@ def test_refusals_of_what_is_no_tensor(cuda):
     with pytest.raises(RuntimeError, match="residual_scale"):
         sparse.residual_norm(x, x, residual_scale=torch.ones((), device=cuda, requires_grad=True))
     assert torch.equal(sparse.residual_norm(x + 1, x, residual_scale=torch.tensor(0.5)), x + 0.5)
+
+
+@pytest.mark.parametrize("gates,seq", [(130, 48), (300, 31)])
+def test_gates_whose_rows_are_cut_into_pieces(cuda, gates, seq):
+    from sparse import _native as N
+    assert N.lib().tf24_block_norm_backward_workspace_bytes(gates * seq, 1152, seq) > gates * 1152 * 16
+    check(cuda, (gates, seq), 1152, BF16, BF16, None, "layer", "sequence", seed=13)
