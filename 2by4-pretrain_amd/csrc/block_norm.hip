@@ -14,11 +14,17 @@
 // share a gate, dg = w_post A + b_post B, dw_post = sum over gates g A, db_post = sum g B; without a norm of y, A = sum d y and dg = A.
 //
 // Bound by memory: a row is read once and kept in registers while its means are taken (the variance from the centred values: a
-// second pass over registers, not over memory).  A row belongs to a wave (up to 1024 columns), or to 2 to 16 waves that
+// second pass over registers, not over memory).  A row belongs to a wave (up to 512 columns), or to 2 to 16 waves that
 // exchange their sums through LDS; a lane holds one or two units of eight adjacent columns, so accesses are 16 bytes whatever the type
 // and the alignment, and four adjacent lanes hold a block of what is kept in 8 bits (checkpoint8.hpp).  Workgroups take runs of rows, keep the
 // parameters in registers, and load the next row while they compute on one.  In the backward pass a run ends in one partial sum per column, which a
 // second launch adds in a fixed order: no atomics, the same bits every time.
+//
+// Measured (kernel time, bytes that it cannot do without): 12288 rows of 768, float32 stream and float16 blocks, both norms and a gate: 26 us = 4.4 TB/s;
+// 8192 rows of 4096 bf16: 53 us = 5.0 TB/s, where a copy of such a size reaches 5.2.  Rows of 1601 bf16, which begin at any even address and end in the middle of a unit:
+// 14.2 us for 3003 of them = 2.7 TB/s: three rows to each of 1001 workgroups.  A row of 4096 by itself 3.4 us: the latency of one load, sums over eight
+// waves and a store.  A lane's parameters are 40 registers, a row as it is loaded 8 to 16; the next row's keep the memory busy while the sums of one
+// wait for each other (the first kernel, which loaded a row when its turn came, took 29.7 and 76.9 us).
 #include "block_norm_rows.hpp"
 
 namespace tf24 {
@@ -76,6 +82,20 @@ struct ForwardArgs {
   int param_dtype, gate_dtype, post_kind, pre_kind;
   float scale, eps, inv_cols;
 };
+
+// n, and what is kept of it in 8 bits
+template <typename T, typename P>
+__device__ __forceinline__ void store_normed(const ForwardArgs& a, const P& place, uint32_t row, int u, float (&n)[8]) {
+  place.store((T*)a.n + (int64_t)row * a.cols, u, n);
+  if (a.values) {
+    const Kept8 k = keep_8<T>(n);
+    if ((int)place.col[u] < a.blocks * kKeptBlock) {
+      const uint64_t unit = (uint64_t)row * a.blocks * kKeptLanes + place.col[u] / 8;
+      *reinterpret_cast<uint2*>(a.values + unit * 8) = k.values;
+      if ((unit & 3) == 0) a.scales[unit >> 2] = (uint8_t)k.scale;
+    }
+  }
+}
 
 template <typename R, typename T, bool RESIDUAL, bool RAGGED, typename S>
 __global__ void __launch_bounds__(S::THREADS)
@@ -146,15 +166,7 @@ block_norm_forward(const ForwardArgs a) {
       for (int u = 0; u < U; u++) {
 #pragma unroll
         for (int e = 0; e < 8; e++) h.v[u][e] = __builtin_fmaf(h.v[u][e] * scale, pre_w.v[u][e], pre_b.v[u][e]);
-        place.store((T*)a.n + (int64_t)row * a.cols, u, h.v[u]);
-        if (a.values) {
-          const Kept8 k = keep_8<T>(h.v[u]);
-          if ((int)place.col[u] < a.blocks * kKeptBlock) {
-            const uint64_t unit = (uint64_t)row * a.blocks * kKeptLanes + place.col[u] / 8;
-            *reinterpret_cast<uint2*>(a.values + unit * 8) = k.values;
-            if ((t & 3) == 0) a.scales[unit >> 2] = (uint8_t)k.scale;
-          }
-        }
+        store_normed<T>(a, place, row, u, h.v[u]);
       }
     }
   };
@@ -173,6 +185,90 @@ block_norm_forward(const ForwardArgs a) {
     if (third < last) load(rows[0], third);
     process(rows[1], second);
     row = third;
+  }
+}
+
+// Rows of more columns than the registers above hold: a row to a workgroup of 16 waves, 128 registers a lane.  Parameters and gates are loaded where they
+// are used (from the caches: up to five times four bytes a column beside the eight or twelve of the row itself), the next row's registers when this row's
+// have been used.  Both passes of 4000 x 12288 bf16 359 us and of 4000 x 16384 429 (2.2 and 2.4 TB/s); with everything in registers, most of it
+// spilled, 990 and 1090.
+template <typename R, typename T, bool RESIDUAL, bool RAGGED>
+__global__ void __launch_bounds__(kWideThreads)
+block_norm_forward_wide(const ForwardArgs a) {
+  using S = ShapeT<kWideThreads, 2, kWideThreads>;
+  constexpr int U = S::UNITS;
+  __shared__ float lds[2][1][S::WAVES][2];
+  RowSum<S> sum{lds};
+  const int t = threadIdx.x;
+  const uint32_t last = min(a.rows, (blockIdx.x + 1) * a.rows_per_block);
+  const Place<U, RAGGED> own(t, S::GROUP, a.cols);
+  Raw<R, U> x;
+  Raw<T, U> y;
+  auto load = [&](uint32_t row) {
+    x.load((const R*)a.x + (int64_t)row * a.ld_x, own);
+    if (RESIDUAL) y.load((const T*)a.y + (int64_t)row * a.ld_y, own);
+  };
+  const uint32_t first = blockIdx.x * a.rows_per_block;
+  if (first < last) load(first);
+  for (uint32_t row = first; row < last; row++) {
+    const auto place = own.another();
+    Cells<U> h;
+    x.settle(place);
+    if constexpr (RESIDUAL) {
+      y.settle(place);
+#pragma unroll
+      for (int u = 0; u < U; u++)
+#pragma unroll
+        for (int e = 0; e < 8; e++) h.v[u][e] = y.get(u, e);
+      if (a.post_kind) {
+        float mean, scale;
+        statistics<S>(h, place, a.post_kind, a.inv_cols, a.eps, sum, mean, scale);
+        if (a.stats && t == 0) { a.stats[row] = mean; a.stats[a.rows + row] = scale; }
+#pragma unroll
+        for (int u = 0; u < U; u++) {
+          in_turn();
+          float w[8], b[8];
+          load_unit(a.post_weight, a.param_dtype, 0, place, u, 1.0f, w);
+          load_unit(a.post_bias, a.param_dtype, 0, place, u, 0.0f, b);
+#pragma unroll
+          for (int e = 0; e < 8; e++) h.v[u][e] = __builtin_fmaf(h.v[u][e] * scale, w[e], b[e]);
+        }
+      }
+#pragma unroll
+      for (int u = 0; u < U; u++) {
+        in_turn();
+        if (a.gate) {
+          float g[8];
+          load_unit(a.gate, a.gate_dtype, row / a.rows_per_gate * a.ld_gate, place, u, 1.0f, g);
+#pragma unroll
+          for (int e = 0; e < 8; e++) h.v[u][e] *= g[e];
+        }
+#pragma unroll
+        for (int e = 0; e < 8; e++) h.v[u][e] = __builtin_fmaf(a.scale, x.get(u, e), h.v[u][e]);
+        place.store((R*)a.out + (int64_t)row * a.cols, u, h.v[u]);
+      }
+    } else {
+#pragma unroll
+      for (int u = 0; u < U; u++)
+#pragma unroll
+        for (int e = 0; e < 8; e++) h.v[u][e] = x.get(u, e);
+    }
+    if (row + 1 < last) load(row + 1);
+    if (a.pre_kind) {
+      float mean, scale;
+      statistics<S>(h, place, a.pre_kind, a.inv_cols, a.eps, sum, mean, scale);
+      if (a.stats && t == 0) { a.stats[2 * (uint64_t)a.rows + row] = mean; a.stats[3 * (uint64_t)a.rows + row] = scale; }
+#pragma unroll
+      for (int u = 0; u < U; u++) {
+        in_turn();
+        float w[8], b[8];
+        load_unit(a.pre_weight, a.param_dtype, 0, place, u, 1.0f, w);
+        load_unit(a.pre_bias, a.param_dtype, 0, place, u, 0.0f, b);
+#pragma unroll
+        for (int e = 0; e < 8; e++) h.v[u][e] = __builtin_fmaf(h.v[u][e] * scale, w[e], b[e]);
+        store_normed<T>(a, place, row, u, h.v[u]);
+      }
+    }
   }
 }
 
@@ -196,20 +292,24 @@ extern "C" int tf24_block_norm_forward(const void* x, int64_t ld_x, const void* 
   if (int rc = check_aligned(fn, gate ? dtype_size(gate_dtype) : 1, {gate})) return rc;
   if (int rc = check_aligned(fn, 16, {values, stats})) return rc;
   return with_types(stream_dtype, block_dtype, [&](auto r, auto t) {
+    using R = decltype(r);
+    using T = decltype(t);
+    const auto launch = [&](auto* kernel, int threads, int rows_at_once) {
+      const uint32_t most = kForwardWaves / (uint32_t)(threads / 64), each = (uint32_t)((rows + most - 1) / most);
+      const uint32_t per_block = (each + rows_at_once - 1) / rows_at_once * rows_at_once;
+      const ForwardArgs a{x, y, gate, post_weight, post_bias, pre_weight, pre_bias, out, n, stats, (uint8_t*)values, (uint8_t*)scales, ld_x, ld_y, ld_gate, (uint32_t)rows,
+                          per_block, (uint32_t)(gate ? rows_per_gate : 1), (int)cols, (int)kept_blocks(cols), param_dtype, gate_dtype, post_kind, pre_kind, scale, eps,
+                          1.0f / (float)cols};
+      hipLaunchKernelGGL(kernel, dim3(((uint32_t)rows + per_block - 1) / per_block), dim3(threads), 0, (hipStream_t)stream, a);
+      return check_launch("tf24_block_norm_forward");
+    };
+    if (cols > kNarrowCols)
+      return launch(cols % 8 ? (y ? block_norm_forward_wide<R, T, true, true> : block_norm_forward_wide<R, T, false, true>)
+                             : (y ? block_norm_forward_wide<R, T, true, false> : block_norm_forward_wide<R, T, false, false>), kWideThreads, 1);
     return with_shape<kForwardThreads>(cols, [&](auto shape) {
       using S = decltype(shape);
-      constexpr uint32_t most = kForwardWaves / (S::THREADS / 64);
-      const uint32_t each = (uint32_t)((rows + most - 1) / most);
-      const uint32_t per_block = (each + S::ROWS - 1) / S::ROWS * S::ROWS;
-      ForwardArgs a{x, y, gate, post_weight, post_bias, pre_weight, pre_bias, out, n, stats, (uint8_t*)values, (uint8_t*)scales, ld_x, ld_y, ld_gate, (uint32_t)rows,
-                    per_block, (uint32_t)(gate ? rows_per_gate : 1), (int)cols, (int)kept_blocks(cols), param_dtype, gate_dtype, post_kind, pre_kind, scale, eps,
-                    1.0f / (float)cols};
-      using R = decltype(r);
-      using T = decltype(t);
-      auto* kernel = cols % 8 ? (y ? block_norm_forward<R, T, true, true, S> : block_norm_forward<R, T, false, true, S>)
-                              : (y ? block_norm_forward<R, T, true, false, S> : block_norm_forward<R, T, false, false, S>);
-      hipLaunchKernelGGL(kernel, dim3(((uint32_t)rows + per_block - 1) / per_block), dim3(S::THREADS), 0, (hipStream_t)stream, a);
-      return check_launch("tf24_block_norm_forward");
+      return launch(cols % 8 ? (y ? block_norm_forward<R, T, true, true, S> : block_norm_forward<R, T, false, true, S>)
+                             : (y ? block_norm_forward<R, T, true, false, S> : block_norm_forward<R, T, false, false, S>), S::THREADS, S::ROWS);
     });
   });
 }

@@ -1,4 +1,10 @@
 // The backward pass of the block norms (block_norm.hip has the formulas).
+//
+// Four sums over the rows stay in registers (32 of a lane) while a workgroup goes through its piece of the rows: 256 pieces, a workgroup of eight waves on
+// each compute unit, whose next rows are loaded while it computes on these.  More pieces than are at work at once would be a second round, and their
+// partial sums (16 bytes a column and piece) more to write and to add.
+// Measured (kernel time, bytes that it cannot do without): 12288 rows of 768, float32 stream and float16 blocks: 36 us = 4.7 TB/s; 8192 rows of 4096
+// bf16: 84 us = 4.8 TB/s; block_norm_finish 5.0 and 7.0 us, of which the launch is 2.  The first kernels, without loads ahead: 47 and 146 us.
 #include "block_norm_rows.hpp"
 
 namespace tf24 {
@@ -25,6 +31,7 @@ struct BackwardArgs {
   Pieces pieces;
   uint32_t rows;
   int cols, param_dtype, gate_dtype, post_kind, pre_kind;
+  bool gate_per_row;
   float scale, inv_cols;
 };
 
@@ -223,6 +230,162 @@ block_norm_backward(const BackwardArgs a) {
   }
 }
 
+// Rows of more columns than the registers above hold: a row to a workgroup of 16 waves with 128 registers a lane.  Parameters and gates are loaded where they
+// are used (from the caches), centred values formed twice, and two of the four sums over the rows live in LDS, each lane's own 16 bytes at a time.  A row's
+// registers are loaded when its turn comes: the next row's beside them would be spilled.
+template <typename R, typename T, bool RESIDUAL, bool RAGGED>
+__global__ void __launch_bounds__(kWideThreads)
+block_norm_backward_wide(const BackwardArgs a, uint32_t rows_per_gate) {
+  using S = ShapeT<kWideThreads, 2, kWideThreads>;
+  constexpr int U = S::UNITS;
+  typedef float float4w __attribute__((ext_vector_type(4)));
+  __shared__ float lds[2][1][S::WAVES][2];
+  __shared__ float4w column_sums[RESIDUAL ? 2 : 1][RESIDUAL ? U * 2 : 1][RESIDUAL ? kWideThreads : 1];
+  RowSum<S> sum{lds};
+  const int t = threadIdx.x;
+  const uint32_t group = blockIdx.x / a.pieces.per_group, sub = blockIdx.x - group * a.pieces.per_group;
+  const uint32_t start = group * a.pieces.rows_of_group;
+  const uint32_t first = start + (uint32_t)((uint64_t)sub * a.pieces.rows_of_group / a.pieces.per_group);
+  const uint32_t last = start + (uint32_t)((uint64_t)(sub + 1) * a.pieces.rows_of_group / a.pieces.per_group);
+  const Place<U, RAGGED> own(t, S::GROUP, a.cols);
+  Cells<U> sum_nh = {}, sum_n = {};
+  if (RESIDUAL) {
+#pragma unroll
+    for (int k = 0; k < 2; k++)
+#pragma unroll
+      for (int q = 0; q < 2 * U; q++) column_sums[RESIDUAL ? k : 0][RESIDUAL ? q : 0][RESIDUAL ? t : 0] = float4w{0, 0, 0, 0};
+  }
+  for (uint32_t row = first; row < last; row++) {
+    const auto place = own.another();
+    Cells<U> d = {};
+    if (a.grad_out) {
+      Raw<R, U> dout;
+      dout.load_all((const R*)a.grad_out + (int64_t)row * a.ld_grad_out, place);
+#pragma unroll
+      for (int u = 0; u < U; u++)
+#pragma unroll
+        for (int e = 0; e < 8; e++) d.v[u][e] = dout.get(u, e);
+    }
+    if (a.pre_kind) {
+      const float mean = a.stats[2 * (uint64_t)a.rows + row], scale = a.stats[3 * (uint64_t)a.rows + row];
+      float s1 = 0.0f, s2 = 0.0f;
+      Raw<R, U> h;
+      Raw<T, U> dn;
+      h.load_all((const R*)a.h + (int64_t)row * a.ld_h, place);
+      dn.load_all((const T*)a.grad_n + (int64_t)row * a.ld_grad_n, place);
+#pragma unroll
+      for (int u = 0; u < U; u++) {
+        in_turn();
+        float w[8];
+        load_unit(a.pre_weight, a.param_dtype, 0, place, u, 1.0f, w);
+#pragma unroll
+        for (int e = 0; e < 8; e++) {
+          const float g = dn.get(u, e), hat = (h.get(u, e) - mean) * scale, q = g * w[e];
+          sum_nh.v[u][e] = __builtin_fmaf(g, hat, sum_nh.v[u][e]);
+          sum_n.v[u][e] += g;
+          s1 += q;
+          s2 = __builtin_fmaf(q, hat, s2);
+        }
+      }
+      sum(s1, s2);
+      s1 = a.pre_kind == TF24_NORM_LAYER ? s1 * a.inv_cols : 0.0f;
+      s2 *= -a.inv_cols;
+#pragma unroll
+      for (int u = 0; u < U; u++) {
+        in_turn();
+        float w[8];
+        load_unit(a.pre_weight, a.param_dtype, 0, place, u, 1.0f, w);
+#pragma unroll
+        for (int e = 0; e < 8; e++) {
+          const float hat = (h.get(u, e) - mean) * scale;
+          d.v[u][e] = __builtin_fmaf(scale, __builtin_fmaf(hat, s2, dn.get(u, e) * w[e] - s1), d.v[u][e]);
+        }
+      }
+    }
+    if (a.grad_x) {
+#pragma unroll
+      for (int u = 0; u < U; u++) {
+        in_turn();
+        float dx[8];
+#pragma unroll
+        for (int e = 0; e < 8; e++) dx[e] = a.scale * d.v[u][e];
+        place.store((R*)a.grad_x + (int64_t)row * a.cols, u, dx);
+      }
+    }
+    if constexpr (RESIDUAL) {
+      const float mean = a.post_kind ? a.stats[row] : 0.0f, scale = a.post_kind ? a.stats[a.rows + row] : 1.0f;
+      Raw<T, U> y = {};
+      if (a.y) y.load_all((const T*)a.y + (int64_t)row * a.ld_y, place);
+      float s1 = 0.0f, s2 = 0.0f;
+#pragma unroll
+      for (int u = 0; u < U; u++) {
+        in_turn();
+        float w[8], g[8];
+        load_unit(a.post_weight, a.param_dtype, 0, place, u, 1.0f, w);
+        load_unit(a.gate, a.gate_dtype, row / rows_per_gate * a.ld_gate, place, u, 1.0f, g);
+        if (a.grad_gate) {                                         // a gate for every row
+          float b[8], dg[8];
+          load_unit(a.post_bias, a.param_dtype, 0, place, u, 0.0f, b);
+#pragma unroll
+          for (int e = 0; e < 8; e++) dg[e] = d.v[u][e] * (a.post_kind ? __builtin_fmaf((y.get(u, e) - mean) * scale, w[e], b[e]) : y.get(u, e));
+          const int64_t to = (int64_t)row * a.cols;
+          if (a.gate_dtype == TF24_F32) place.store((float*)a.grad_gate + to, u, dg);
+          else if (a.gate_dtype == TF24_F16) place.store((f16_t*)a.grad_gate + to, u, dg);
+          else place.store((bf16_t*)a.grad_gate + to, u, dg);
+        }
+#pragma unroll
+        for (int half = 0; half < 2; half++) {
+          float4w dy = column_sums[0][2 * u + half][t], dd = column_sums[1][2 * u + half][t];
+#pragma unroll
+          for (int i = 0; i < 4; i++) {
+            const int e = 4 * half + i;
+            const float hat = (y.get(u, e) - mean) * scale;
+            float v = d.v[u][e];
+            if (a.gate_per_row) v *= g[e];                         // (the sums of gates that rows share are taken without them)
+            dy[i] = __builtin_fmaf(v, hat, dy[i]);
+            dd[i] += v;
+            v *= a.gate_per_row ? w[e] : w[e] * g[e];
+            s1 += v;
+            s2 = __builtin_fmaf(v, hat, s2);
+            d.v[u][e] = v;
+          }
+          column_sums[0][2 * u + half][t] = dy;
+          column_sums[1][2 * u + half][t] = dd;
+        }
+      }
+      if (a.post_kind) {
+        sum(s1, s2);
+        s1 = a.post_kind == TF24_NORM_LAYER ? s1 * a.inv_cols : 0.0f;
+        s2 *= -a.inv_cols;
+#pragma unroll
+        for (int u = 0; u < U; u++)
+#pragma unroll
+          for (int e = 0; e < 8; e++) d.v[u][e] = scale * __builtin_fmaf((y.get(u, e) - mean) * scale, s2, d.v[u][e] - s1);
+      }
+      if (a.grad_y) {
+#pragma unroll
+        for (int u = 0; u < U; u++) place.store((T*)a.grad_y + (int64_t)row * a.cols, u, d.v[u]);
+      }
+    }
+  }
+  if (!a.partial) return;
+#pragma unroll
+  for (int k = RESIDUAL ? 0 : 2; k < 4; k++) {
+    float* to = a.partial + ((uint64_t)k * a.pieces.count() + blockIdx.x) * a.cols;
+#pragma unroll
+    for (int u = 0; u < U; u++) {
+      in_turn();
+      float v[8];
+#pragma unroll
+      for (int e = 0; e < 8; e++) {
+        if (RESIDUAL && k < 2) v[e] = column_sums[RESIDUAL ? k : 0][RESIDUAL ? 2 * u + (e >> 2) : 0][RESIDUAL ? t : 0][e & 3];
+        else v[e] = k == 2 ? sum_nh.v[u][e] : sum_n.v[u][e];
+      }
+      own.store(to, u, v);
+    }
+  }
+}
+
 // The gradients of the parameters from the pieces' sums.  Job 0: weight of the norm behind, 1: its bias, 2, 3: those of the norm before,
 // from 4 on: the gates that rows share; a workgroup takes 32 columns of a job, 32 strands of pieces side by side, or where a gate has few pieces
 // a gate for each strand.
@@ -291,7 +454,7 @@ block_norm_finish(const FinishArgs a) {
 Pieces plan_pieces(int64_t rows, int64_t cols, int64_t rows_per_gate) {
   const uint32_t groups = rows_per_gate > 1 && rows_per_gate < rows ? (uint32_t)(rows / rows_per_gate) : 1;
   const uint32_t rows_of_group = (uint32_t)(rows / groups);
-  const uint32_t at_once = with_shape<kBackwardThreads>(cols, [](auto s) { return (uint32_t)decltype(s)::ROWS; });
+  const uint32_t at_once = cols > kNarrowCols ? 1 : with_shape<kBackwardThreads>(cols, [](auto s) { return (uint32_t)decltype(s)::ROWS; });
   const uint32_t most = (rows_of_group + at_once - 1) / at_once;
   if (groups < 16) return {groups, kBackwardPieces / groups < most ? kBackwardPieces / groups : most, rows_of_group};
   // The last round of workgroups should be a full one: with 4096 sequences or more it hardly counts, with 320 of them a piece each would leave three
@@ -348,14 +511,20 @@ extern "C" int tf24_block_norm_backward(const void* grad_out, int64_t ld_grad_ou
                      ld_gate, pieces, (int)cols, column_blocks, per_row, param_dtype, gate_dtype, post_kind};
   const int64_t gate_jobs = !f.grad_gate ? 0 : f.strand_per_gate() ? (pieces.groups + kStrands - 1) / kStrands : pieces.groups, jobs = 4 + gate_jobs;
   if (jobs * column_blocks > 0x7fffffffLL) return fail(TF24_ERR_SHAPE, "%s: too many gates (%lld)", fn, (long long)pieces.groups);
+  const BackwardArgs a{grad_out, grad_n, h, y, gate, post_weight, post_bias, pre_weight, stats, grad_x, grad_y, per_row ? grad_gate : nullptr,
+                       sums ? (float*)workspace : nullptr, ld_grad_out, ld_grad_n, ld_h, ld_y, ld_gate, pieces, (uint32_t)rows, (int)cols, param_dtype,
+                       gate_dtype, post_kind, pre_kind, per_row, scale, 1.0f / (float)cols};
   const int rc = with_types(stream_dtype, block_dtype, [&](auto r, auto t) {
+    using R = decltype(r);
+    using T = decltype(t);
+    if (cols > kNarrowCols) {
+      auto* kernel = cols % 8 ? (residual ? block_norm_backward_wide<R, T, true, true> : block_norm_backward_wide<R, T, false, true>)
+                              : (residual ? block_norm_backward_wide<R, T, true, false> : block_norm_backward_wide<R, T, false, false>);
+      hipLaunchKernelGGL(kernel, dim3(pieces.count()), dim3(kWideThreads), 0, (hipStream_t)stream, a, gate ? (uint32_t)rows_per_gate : (uint32_t)rows);
+      return check_launch("tf24_block_norm_backward");
+    }
     return with_shape<kBackwardThreads>(cols, [&](auto shape) {
       using S = decltype(shape);
-      BackwardArgs a{grad_out, grad_n, h, y, gate, post_weight, post_bias, pre_weight, stats, grad_x, grad_y, per_row ? grad_gate : nullptr,
-                     sums ? (float*)workspace : nullptr, ld_grad_out, ld_grad_n, ld_h, ld_y, ld_gate, pieces, (uint32_t)rows, (int)cols, param_dtype,
-                     gate_dtype, post_kind, pre_kind, scale, 1.0f / (float)cols};
-      using R = decltype(r);
-      using T = decltype(t);
       auto* kernel = per_row ? block_norm_backward<R, T, true, ROW_GATES, S>
                              : cols % 8 ? (residual ? block_norm_backward<R, T, true, ANY, S> : block_norm_backward<R, T, false, ANY, S>)
                                         : (residual ? block_norm_backward<R, T, true, WHOLE, S> : block_norm_backward<R, T, false, WHOLE, S>);

@@ -6,6 +6,7 @@ namespace tf24 {
 namespace {
 
 constexpr int kMaxCols = 16384;
+constexpr int kNarrowCols = 8192, kWideThreads = 1024;           // wider rows have kernels of their own
 
 // GROUP threads share a row, each with UNITS units of 8 columns; a workgroup has at least THREADS threads, and works on ROWS rows at once
 template <int GROUP_, int UNITS_, int THREADS_>
@@ -58,6 +59,13 @@ struct RowSum {
   }
 };
 
+// p + i, as an address that all lanes share and 32 bits of a lane's own (i elements are less than 2^32 bytes)
+template <typename T>
+__device__ __forceinline__ T* lane_at(T* p, uint32_t i) {
+  using Byte = std::conditional_t<std::is_const<T>::value, const char, char>;
+  return reinterpret_cast<T*>(reinterpret_cast<Byte*>(p) + i * (uint32_t)sizeof(T));
+}
+
 template <int UNITS> struct Cells { float v[UNITS][8]; };
 
 // Where a lane's units lie in a row: unit u is `count[u]` columns (8, fewer in the row's last unit, or none) from `col[u]` on.  RAGGED: the last
@@ -77,11 +85,18 @@ struct Place {
       from[u] = (uint32_t)max(min((int)col[u], cols - 8), 0);
     }
   }
+  // The same, as if it were another: addresses formed with it are not kept in registers from row to row.
+  __device__ __forceinline__ Place another() const {
+    Place p = *this;
+#pragma unroll
+    for (int u = 0; u < UNITS; u++) asm volatile("" : "+v"(p.col[u]), "+v"(p.from[u]), "+v"(p.count[u]));
+    return p;
+  }
   // v, rounded to T, to unit u of a row; the values as they are stored are left in v
   template <typename T>
   __device__ __forceinline__ void store(T* row, int u, float (&v)[8]) const {
-    if (RAGGED) store_up_to_8(row + col[u], count[u], v);
-    else if (count[u] > 0) store_up_to_8(row + col[u], 8, v);
+    if (RAGGED) store_up_to_8(lane_at(row, col[u]), count[u], v);
+    else if (count[u] > 0) store_up_to_8(lane_at(row, col[u]), 8, v);
     else {
       any4 unused[sizeof(T) / 2];
       round_8<T>(v, unused);
@@ -104,7 +119,7 @@ struct Raw {
       if (!P::RAGGED || at.cols >= 8) {
         if (at.count[u] > 0) {
 #pragma unroll
-          for (int q = 0; q < WORDS / 4; q++) w[u][q] = *(reinterpret_cast<const any4*>(row + at.from[u]) + q);
+          for (int q = 0; q < WORDS / 4; q++) w[u][q] = *(reinterpret_cast<const any4*>(lane_at(row, at.from[u])) + q);
         }
       } else {                                                   // rows shorter than a load
 #pragma unroll 1
@@ -117,6 +132,19 @@ struct Raw {
         }
       }
     }
+  }
+  // A row of eight columns or more, without branches: lanes that have no columns load the last ones and drop them.
+  template <typename P>
+  __device__ __forceinline__ void load_all(const T* row, const P& at) {
+#pragma unroll
+    for (int u = 0; u < UNITS; u++)
+#pragma unroll
+      for (int q = 0; q < WORDS / 4; q++) w[u][q] = *(reinterpret_cast<const any4*>(lane_at(row, at.from[u])) + q);
+    settle(at);
+#pragma unroll
+    for (int u = 0; u < UNITS; u++)
+#pragma unroll
+      for (int q = 0; q < WORDS; q++) w[u][q >> 2][q & 3] = at.count[u] > 0 ? w[u][q >> 2][q & 3] : 0;
   }
   // the columns of a unit that is not whole to its front, zeros behind them
   template <typename P>
@@ -151,6 +179,12 @@ struct Raw {
   }
 };
 
+// Nothing is moved across: units one after the other, with the registers of one.
+__device__ __forceinline__ void in_turn() {
+  asm volatile("" ::: "memory");
+  __builtin_amdgcn_sched_barrier(0);
+}
+
 // A lane's parameters, of a type known at the call, from element `first` on; without any `otherwise`.  Zeros where it has no columns.
 template <typename T, typename P>
 __device__ __forceinline__ void load_typed(const void* p, int64_t first, const P& at, Cells<P::UNITS>& c) {
@@ -175,6 +209,24 @@ __device__ __forceinline__ void load_params(const void* p, int dtype, int64_t fi
   else if (dtype == TF24_F16) load_typed<f16_t>(p, first, at, c);
   else load_typed<bf16_t>(p, first, at, c);
 }
+// unit u of them alone
+template <typename P>
+__device__ __forceinline__ void load_unit(const void* p, int dtype, int64_t first, const P& at, int u, float otherwise, float (&v)[8]) {
+  if (!p) {
+#pragma unroll
+    for (int e = 0; e < 8; e++) v[e] = (P::RAGGED ? e < at.count[u] : at.count[u] > 0) ? otherwise : 0.0f;
+    return;
+  }
+  if (!P::RAGGED && at.count[u] <= 0) {
+#pragma unroll
+    for (int e = 0; e < 8; e++) v[e] = 0.0f;
+    return;
+  }
+  const int n = P::RAGGED ? at.count[u] : 8;
+  if (dtype == TF24_F32) load_up_to_8(lane_at((const float*)p + first, at.col[u]), n, v);
+  else if (dtype == TF24_F16) load_up_to_8(lane_at((const f16_t*)p + first, at.col[u]), n, v);
+  else load_up_to_8(lane_at((const bf16_t*)p + first, at.col[u]), n, v);
+}
 __device__ __forceinline__ float load_param(const void* p, int dtype, int64_t at, float otherwise) {
   if (!p) return otherwise;
   if (dtype == TF24_F32) return ((const float*)p)[at];
@@ -182,7 +234,7 @@ __device__ __forceinline__ float load_param(const void* p, int dtype, int64_t at
 }
 
 // ---------------------------------------------------------------- host
-// the narrowest shape that holds a row; THREADS: the least number of a workgroup
+// the narrowest shape that holds a row of up to kNarrowCols; THREADS: the least number of a workgroup
 template <int THREADS, typename F>
 auto with_shape(int64_t cols, F&& f) {
   if (cols <= 512) return f(ShapeT<64, 1, THREADS>{});
@@ -190,8 +242,7 @@ auto with_shape(int64_t cols, F&& f) {
   if (cols <= 1024) return f(ShapeT<128, 1, WIDE>{});
   if (cols <= 2048) return f(ShapeT<256, 1, WIDE>{});
   if (cols <= 4096) return f(ShapeT<512, 1, WIDE>{});
-  if (cols <= 8192) return f(ShapeT<512, 2, WIDE>{});
-  return f(ShapeT<1024, 2, WIDE>{});
+  return f(ShapeT<512, 2, WIDE>{});
 }
 constexpr int kForwardThreads = 256, kBackwardThreads = 512;
 // What 256 compute units hold at once, so that no part of a round runs by itself: forward four waves a SIMD, backward a workgroup of eight

@@ -495,3 +495,11 @@ def test_gates_whose_rows_are_cut_into_pieces(cuda, gates, seq):
     from sparse import _native as N
     assert N.lib().tf24_block_norm_backward_workspace_bytes(gates * seq, 1152, seq) > gates * 1152 * 16
     check(cuda, (gates, seq), 1152, BF16, BF16, None, "layer", "sequence", seed=13)
+
+
+@pytest.mark.parametrize("cols", [8193, 12288, 16383])
+@pytest.mark.parametrize("gate", ["channel", "sequence", "token"])
+def test_wide_rows(cuda, cols, gate):
+    """Rows that have kernels of their own, more of them than workgroups."""
+    check(cuda, (3, 171), cols, BF16, BF16, "layer", "rms", gate, seed=14)
+    check(cuda, (2, 3), cols, F32, F16, "rms" if gate == "channel" else None, "layer", gate, bias=False, strided=True, seed=15)
