@@ -240,8 +240,19 @@ py::object checkpoint_encode(const Tensor& x) {
   return py::make_tuple(values, scales);
 }
 
+// what is kept of `rows` rows of `cols` columns, as it was made
+bool holds(const Tensor& values, const Tensor& scales, int64_t rows, int64_t cols) {
+  return values.dim() == 2 && scales.dim() == 2 && values.size(0) == rows && scales.size(0) == rows && values.size(1) == 32 * blocks_of(cols) &&
+         scales.size(1) == blocks_of(cols) && values.is_contiguous() && scales.is_contiguous() && values.scalar_type() == at::kFloat8_e4m3fn &&
+         scales.scalar_type() == at::kByte && values.is_cuda() && scales.is_cuda() && values.get_device() == scales.get_device() &&
+         values.get_device() == c10::hip::current_device();
+}
+
 py::object checkpoint_decode(const Tensor& values, const Tensor& scales, const std::vector<int64_t>& shape, int code) {
-  if (!values.is_cuda() || values.get_device() != c10::hip::current_device()) return py::none();
+  if (shape.empty() || shape.back() < 1) return py::none();
+  int64_t rows = 1;
+  for (size_t i = 0; i + 1 < shape.size(); i++) rows *= shape[i];
+  if (!holds(values, scales, rows, shape.back())) return py::none();
   const Tensor out = make(shape, type_of(code), values);
   check(tf24_checkpoint_decode(pointer(values), pointer(scales), values.size(0), shape.back(), pointer(out), code, shape.back(), stream_of(values)));
   return py::cast(out);
@@ -249,8 +260,9 @@ py::object checkpoint_decode(const Tensor& values, const Tensor& scales, const s
 
 // (dW, db or None), of arguments that checkpoint_weight_gradient has looked at; None for a call that is Python's
 py::object checkpoint_weight_grad(const Tensor& g, const Tensor& values, const Tensor& scales, int64_t n, bool bias, int out_code) {
-  if (!plain(g) || g.size(-1) % 8 || (uintptr_t)g.data_ptr() % 16 || values.size(0) == 0) return py::none();
-  const int64_t m = g.size(-1), tokens = values.size(0);
+  if (!plain(g) || g.size(-1) == 0 || g.size(-1) % 8 || (uintptr_t)g.data_ptr() % 16) return py::none();
+  const int64_t m = g.size(-1), tokens = g.numel() / m;
+  if (tokens == 0 || !holds(values, scales, tokens, n)) return py::none();
   Tensor dw = make({m, n}, type_of(out_code), g), db, workspace;
   if (bias) db = make({m}, type_of(out_code), g);
   const int64_t bytes = tf24_checkpoint_weight_grad_workspace_bytes(tokens, m, n);

@@ -29,14 +29,17 @@ class ActivationCheckpoint:
     __slots__ = ("values", "scales", "shape", "dtype")
 
     def __init__(self, values, scales, shape, dtype):
-        shape = torch.Size(shape)
-        rows, blocks = shape[:-1].numel(), (shape[-1] + _BLOCK - 1) // _BLOCK
-        if (values.shape != (rows, _BLOCK * blocks) or scales.shape != (rows, blocks) or values.dtype != torch.float8_e4m3fn
+        self.values, self.scales, self.shape, self.dtype = values, scales, torch.Size(shape), dtype
+        self._check()
+
+    def _check(self):
+        values, scales, shape, dtype = self.values, self.scales, self.shape, self.dtype
+        rows, blocks = shape[:-1].numel(), (shape[-1] + _BLOCK - 1) // _BLOCK if len(shape) else 0
+        if (not blocks or values.shape != (rows, _BLOCK * blocks) or scales.shape != (rows, blocks) or values.dtype != torch.float8_e4m3fn
                 or scales.dtype != torch.uint8 or values.device != scales.device or not values.is_contiguous() or not scales.is_contiguous()
                 or dtype not in _TYPES):
             raise RuntimeError(f"ActivationCheckpoint: values {tuple(values.shape)} {values.dtype} and scales {tuple(scales.shape)} {scales.dtype} "
                                f"do not hold a tensor {tuple(shape)} {dtype}")
-        self.values, self.scales, self.shape, self.dtype = values, scales, shape, dtype
 
     @classmethod
     def _of(cls, values, scales, shape, dtype):
@@ -63,6 +66,7 @@ class ActivationCheckpoint:
             out = calls.checkpoint_decode(self.values, self.scales, self.shape, N.dtype_codes[dtype])
             if out is not None:
                 return out
+        self._check()
         out = torch.empty(self.shape, dtype=dtype, device=self.values.device)
         rows, cols = self.values.shape[0], self.shape[-1]
         N.launch(out, N.lib().tf24_checkpoint_decode, self.values.data_ptr(), self.scales.data_ptr(), rows, cols, out.data_ptr(), N.dtype_code(dtype), cols)
@@ -132,6 +136,7 @@ def checkpoint_weight_gradient(grad_output, checkpoint, bias=False, dtype=None):
         grads = calls.checkpoint_weight_grad(g, checkpoint.values, checkpoint.scales, n, bias, N.dtype_codes[dtype])
         if grads is not None:
             return grads
+    checkpoint._check()
     if tokens == 0:
         return torch.zeros((m, n), dtype=dtype, device=g.device), torch.zeros(m, dtype=dtype, device=g.device) if bias else None
     g, ld = N.as_rows(g)

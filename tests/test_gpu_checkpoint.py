@@ -338,3 +338,17 @@ def test_captured_and_on_another_stream(cuda):
         graph.replay()
         torch.cuda.synchronize()
         assert all(torch.equal(a, b) for a, b in zip(recorded, want)), replay
+
+
+def test_a_checkpoint_that_was_changed_is_refused(cuda):
+    """Before anything reads past what is kept."""
+    import sparse
+    x, g = draw(90, 6, 64).half().to(cuda), draw(91, 6, 32).half().to(cuda)
+    for name, value in (("shape", torch.Size((7, 64))), ("shape", torch.Size((6, 96))), ("shape", torch.Size(())), ("scales", torch.zeros(6, 1, dtype=torch.uint8, device=cuda)),
+                        ("values", torch.zeros(5, 64, device=cuda).to(torch.float8_e4m3fn)), ("values", torch.zeros(6, 64, device=cuda)), ("scales", torch.zeros(6, 2, dtype=torch.uint8))):
+        kept = sparse.checkpoint_activation(x)
+        setattr(kept, name, value)
+        with pytest.raises(RuntimeError):
+            kept.decode()
+        with pytest.raises(RuntimeError):
+            sparse.checkpoint_weight_gradient(g, kept)
