@@ -510,7 +510,8 @@ extern "C" int tf24_block_norm_backward(const void* grad_out, int64_t ld_grad_ou
   const FinishArgs f{(const float*)workspace, gate, post_weight, post_bias, grad_post_weight, grad_post_bias, grad_pre_weight, grad_pre_bias, per_row ? nullptr : grad_gate,
                      ld_gate, pieces, (int)cols, column_blocks, per_row, param_dtype, gate_dtype, post_kind};
   const int64_t gate_jobs = !f.grad_gate ? 0 : f.strand_per_gate() ? (pieces.groups + kStrands - 1) / kStrands : pieces.groups, jobs = 4 + gate_jobs;
-  if (jobs * column_blocks > 0x7fffffffLL) return fail(TF24_ERR_SHAPE, "%s: too many gates (%lld)", fn, (long long)pieces.groups);
+  if ((int64_t)pieces.count() * kWideThreads > 0xffffffffLL || (sums && jobs * column_blocks * (32 * kStrands) > 0xffffffffLL))      // (threads of a launch)
+    return fail(TF24_ERR_SHAPE, "%s: too many gates (%lld)", fn, (long long)pieces.groups);
   const BackwardArgs a{grad_out, grad_n, h, y, gate, post_weight, post_bias, pre_weight, stats, grad_x, grad_y, per_row ? grad_gate : nullptr,
                        sums ? (float*)workspace : nullptr, ld_grad_out, ld_grad_n, ld_h, ld_y, ld_gate, pieces, (uint32_t)rows, (int)cols, param_dtype,
                        gate_dtype, post_kind, pre_kind, per_row, scale, 1.0f / (float)cols};

@@ -163,3 +163,14 @@ def test_a_gated_activation_from_before_it_could_keep_anything():
     assert not old.checkpoint and not old.output_checkpoint
     with pytest.raises(RuntimeError, match="CUDA"):
         old(torch.zeros(1, 4, 64))
+
+
+def test_more_gates_than_a_launch_has_workgroups(lib):
+    from sparse import _native as N
+
+    def backward(rows, cols, per_gate, grad_gate, ws_bytes):
+        return lib.tf24_block_norm_backward(A, cols, None, 0, None, 0, A, cols, N.F16, N.F16, rows, cols, A, N.F16, cols, per_gate, None, None, None, N.F32, 0, 0, 1, 1.0,
+                                            None, B, C, grad_gate, None, None, None, None, A if ws_bytes else None, ws_bytes, None)
+
+    assert backward(1 << 24, 64, 2, None, 0) == SHAPE and b"gates" in lib.tf24_last_error()
+    assert backward(1 << 22, 16384, 2, C, 1 << 62) == SHAPE and b"gates" in lib.tf24_last_error()
