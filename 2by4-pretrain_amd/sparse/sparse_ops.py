@@ -331,7 +331,8 @@ class SoftThresholdLinear(nn.Linear):
         weight, scale, bias = self.weight, self.scale, self.bias
         if not _takes_linear16(x, weight, bias):
             if checkpoint is not None:
-                raise RuntimeError("SoftThresholdLinear: a checkpoint of the input is taken with contiguous GPU tensors under autocast to 16 bits only")
+                raise RuntimeError("SoftThresholdLinear: a checkpoint of the input is taken with contiguous GPU tensors under autocast to 16 bits only, and where no "
+                                   "mode or transform stands around the call (torch.set_default_device is one)")
             return F.linear(x, self.get_sparse_weights(), bias)
         kept = True if checkpoint is None and self.checkpoint else checkpoint
         dtype = torch.get_autocast_dtype("cuda")                   # (what autocast does to the arguments of F.linear)
