@@ -186,10 +186,14 @@ def stream_ptr():
     return torch.cuda.current_stream().cuda_stream
 
 
+# (found once: the names alone are 1 us of a call)
+_transforms, _tracing, _compiling = torch._C._are_functorch_transforms_active, torch._C._is_tracing, torch.compiler.is_compiling
+_dispatch_modes, _function_modes, _forward_ad = torch._C._len_torch_dispatch_stack, torch._C._len_torch_function_stack, torch.autograd.forward_ad
+
+
 def plain_eager():
     """No transform, mode or tracer stands between a call and its kernels."""
-    return not (torch._C._are_functorch_transforms_active() or torch.autograd.forward_ad._current_level >= 0 or torch.compiler.is_compiling()
-                or torch.jit.is_tracing() or torch._C._len_torch_dispatch_stack() or torch._C._len_torch_function_stack())
+    return not (_transforms() or _forward_ad._current_level >= 0 or _compiling() or _tracing() or _dispatch_modes() or _function_modes())
 
 
 _PLAIN_KEYS = set()
