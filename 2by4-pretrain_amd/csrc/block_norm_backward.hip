@@ -51,7 +51,7 @@ block_norm_backward(const BackwardArgs a) {
   const uint32_t first = start + (uint32_t)((uint64_t)sub * a.pieces.rows_of_group / a.pieces.per_group);
   const uint32_t last = start + (uint32_t)((uint64_t)(sub + 1) * a.pieces.rows_of_group / a.pieces.per_group);
   const Place<U, MODE != WHOLE> place(t, S::GROUP, a.cols);
-  struct Row { Raw<R, U> dout, h; Raw<T, U> dn, y; float pre_mean, pre_scale, post_mean, post_scale; };
+  struct Row { Raw<R, U> dout; Raw<R, U, true> h; Raw<T, U> dn; Raw<T, U, true> y; float pre_mean, pre_scale, post_mean, post_scale; };
   Row rows[2] = {};
   auto load = [&](Row& r, uint32_t at) {
     if (a.grad_out) r.dout.load((const R*)a.grad_out + (int64_t)at * a.ld_grad_out, place);
@@ -68,7 +68,8 @@ block_norm_backward(const BackwardArgs a) {
     }
   };
   if (first + turn < last) load(rows[0], first + turn);
-  // Columns behind the last one have zeros for weights and gradients, and what their other terms are (hat: minus the mean) meets a zero before a sum.
+  // Columns behind the last one have zeros for weights and gradients and another column's normed value, so that every term of theirs in a sum is a zero
+  // (with zeros for h, its normed value would be minus the mean times r: an infinity in a row of one very large value, and NaN in the sums).
   // `post_w` is the weight times the gate that the rows share.
   Cells<U> post_w, pre_w, sum_dy = {}, sum_d = {}, sum_nh = {}, sum_n = {};
   if (RESIDUAL) {
@@ -116,7 +117,10 @@ block_norm_backward(const BackwardArgs a) {
 #pragma unroll
       for (int u = 0; u < U; u++)
 #pragma unroll
-        for (int e = 0; e < 8; e++) d.v[u][e] = __builtin_fmaf(scale, __builtin_fmaf(hat.v[u][e], s2, q.v[u][e] - s1), d.v[u][e]);
+        for (int e = 0; e < 8; e++) {
+          d.v[u][e] = __builtin_fmaf(scale, __builtin_fmaf(hat.v[u][e], s2, q.v[u][e] - s1), d.v[u][e]);
+          if (RESIDUAL && !place.has(u, e)) d.v[u][e] = 0.0f;
+        }
     }
     if (a.grad_x && here) {
 #pragma unroll
@@ -269,7 +273,7 @@ block_norm_backward_wide(const BackwardArgs a, uint32_t rows_per_gate) {
     if (a.pre_kind) {
       const float mean = a.stats[2 * (uint64_t)a.rows + row], scale = a.stats[3 * (uint64_t)a.rows + row];
       float s1 = 0.0f, s2 = 0.0f;
-      Raw<R, U> h;
+      Raw<R, U, true> h;
       Raw<T, U> dn;
       h.load_all((const R*)a.h + (int64_t)row * a.ld_h, place);
       dn.load_all((const T*)a.grad_n + (int64_t)row * a.ld_grad_n, place);
@@ -299,6 +303,7 @@ block_norm_backward_wide(const BackwardArgs a, uint32_t rows_per_gate) {
         for (int e = 0; e < 8; e++) {
           const float hat = (h.get(u, e) - mean) * scale;
           d.v[u][e] = __builtin_fmaf(scale, __builtin_fmaf(hat, s2, dn.get(u, e) * w[e] - s1), d.v[u][e]);
+          if (RESIDUAL && !place.has(u, e)) d.v[u][e] = 0.0f;
         }
       }
     }
@@ -314,7 +319,7 @@ block_norm_backward_wide(const BackwardArgs a, uint32_t rows_per_gate) {
     }
     if constexpr (RESIDUAL) {
       const float mean = a.post_kind ? a.stats[row] : 0.0f, scale = a.post_kind ? a.stats[a.rows + row] : 1.0f;
-      Raw<T, U> y = {};
+      Raw<T, U, true> y = {};
       if (a.y) y.load_all((const T*)a.y + (int64_t)row * a.ld_y, place);
       float s1 = 0.0f, s2 = 0.0f;
 #pragma unroll

@@ -85,6 +85,7 @@ struct Place {
       from[u] = (uint32_t)max(min((int)col[u], cols - 8), 0);
     }
   }
+  __device__ __forceinline__ bool has(int u, int e) const { return RAGGED ? e < count[u] : count[u] > 0; }
   // The same, as if it were another: addresses formed with it are not kept in registers from row to row.
   __device__ __forceinline__ Place another() const {
     Place p = *this;
@@ -104,9 +105,10 @@ struct Place {
   }
 };
 
-// A lane's part of a row as it lies in memory, zeros where it has no columns.  The last unit of a row, if it is not a whole one, is loaded with the
-// columns in front of it (settle moves them out): one load whatever the size, which nothing waits for before the row's turn.
-template <typename T, int UNITS>
+// A lane's part of a row as it lies in memory, where it has no columns zeros, or with OTHERS values of other columns of the row.  The last unit of a row, if it is
+// not a whole one, is loaded with the columns in front of it (settle moves them out, with OTHERS behind the unit's own): one load whatever the
+// size, which nothing waits for before the row's turn.
+template <typename T, int UNITS, bool OTHERS = false>
 struct Raw {
   static constexpr int WORDS = (int)sizeof(T) * 2;               // of 32 bits in a unit
   any4 w[UNITS][WORDS / 4];
@@ -117,23 +119,23 @@ struct Raw {
 #pragma unroll
       for (int q = 0; q < WORDS / 4; q++) w[u][q] = any4{0, 0, 0, 0};
       if (!P::RAGGED || at.cols >= 8) {
-        if (at.count[u] > 0) {
+        if (OTHERS || at.count[u] > 0) {
 #pragma unroll
           for (int q = 0; q < WORDS / 4; q++) w[u][q] = *(reinterpret_cast<const any4*>(lane_at(row, at.from[u])) + q);
         }
       } else {                                                   // rows shorter than a load
 #pragma unroll 1
-        for (int e = 0; e < at.count[u]; e++) {
+        for (int e = 0; e < (OTHERS ? 8 : at.count[u]); e++) {
           uint32_t bits;
-          if constexpr (sizeof(T) == 2) bits = (uint32_t)row[e].bits << (16 * (e & 1));
-          else bits = __builtin_bit_cast(uint32_t, row[e]);
+          if constexpr (sizeof(T) == 2) bits = (uint32_t)row[OTHERS ? min(e, at.cols - 1) : e].bits << (16 * (e & 1));
+          else bits = __builtin_bit_cast(uint32_t, row[OTHERS ? min(e, at.cols - 1) : e]);
 #pragma unroll
           for (int q = 0; q < WORDS; q++) w[u][q >> 2][q & 3] |= q == (sizeof(T) == 2 ? e >> 1 : e) ? bits : 0;
         }
       }
     }
   }
-  // A row of eight columns or more, without branches: lanes that have no columns load the last ones and drop them.
+  // A row of eight columns or more, without branches: lanes that have no columns load the last ones, and without OTHERS drop them.
   template <typename P>
   __device__ __forceinline__ void load_all(const T* row, const P& at) {
 #pragma unroll
@@ -141,30 +143,37 @@ struct Raw {
 #pragma unroll
       for (int q = 0; q < WORDS / 4; q++) w[u][q] = *(reinterpret_cast<const any4*>(lane_at(row, at.from[u])) + q);
     settle(at);
+    if (OTHERS) return;
 #pragma unroll
     for (int u = 0; u < UNITS; u++)
 #pragma unroll
       for (int q = 0; q < WORDS; q++) w[u][q >> 2][q & 3] = at.count[u] > 0 ? w[u][q >> 2][q & 3] : 0;
   }
-  // the columns of a unit that is not whole to its front, zeros behind them
+  // the columns of a unit that is not whole to its front, zeros (OTHERS: those in front of them) behind them
   template <typename P>
   __device__ __forceinline__ void settle(const P& at) {
     if (!P::RAGGED || (at.cols & 7) == 0 || at.cols < 8) return;
 #pragma unroll
     for (int u = 0; u < UNITS; u++) {
       const int by = at.count[u] > 0 ? 8 - at.count[u] : 0;      // columns in front
-      uint32_t v[WORDS];
+      uint32_t v[2 * WORDS];                                     // the unit, and what moves in behind it
+      const auto behind = [&] {
+#pragma unroll
+        for (int q = 0; q < WORDS; q++) v[WORDS + q] = OTHERS ? v[q] : 0;
+      };
 #pragma unroll
       for (int q = 0; q < WORDS; q++) v[q] = w[u][q >> 2][q & 3];
       if constexpr (sizeof(T) == 2) {
+        behind();
 #pragma unroll
-        for (int q = 0; q < WORDS; q++) v[q] = by & 1 ? __builtin_amdgcn_alignbit(q + 1 < WORDS ? v[q + 1] : 0, v[q], 16) : v[q];
+        for (int q = 0; q < WORDS; q++) v[q] = by & 1 ? __builtin_amdgcn_alignbit(v[q + 1], v[q], 16) : v[q];
       }
 #pragma unroll
       for (int step = 1; step < WORDS; step *= 2) {
         const bool move = by & (sizeof(T) == 2 ? 2 * step : step);
+        behind();
 #pragma unroll
-        for (int q = 0; q < WORDS; q++) v[q] = move ? (q + step < WORDS ? v[q + step] : 0) : v[q];
+        for (int q = 0; q < WORDS; q++) v[q] = move ? v[q + step] : v[q];
       }
 #pragma unroll
       for (int q = 0; q < WORDS; q++) w[u][q >> 2][q & 3] = v[q];

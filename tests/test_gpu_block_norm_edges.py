@@ -1,0 +1,78 @@
+"""residual_norm / block_norm and their gradients at the ends of what they take: rows of one very large value, gates of 16 bits that broadcast, very many gates."""
+import pytest
+import torch
+
+import oracle
+from test_gpu_block_norm import check
+
+pytestmark = pytest.mark.gpu
+
+F32, F16, BF16 = torch.float32, torch.float16, torch.bfloat16
+U = 2.0 ** -24
+
+
+@pytest.fixture(autouse=True, params=["torchcall", "python"])
+def calls(request, monkeypatch):
+    """Everything twice: with the module that makes ordinary calls from torch's C++ side, and with Python making all of them."""
+    from sparse import _native as N
+    if request.param == "python":
+        monkeypatch.setattr(N, "_calls", None)
+    elif N.torch_calls() is None:
+        pytest.skip("_torchcall is not built for this torch")
+
+
+def draw(seed, *shape, dtype=F32, std=1.0, mean=0.0):
+    return (torch.randn(shape, generator=torch.Generator().manual_seed(seed), dtype=torch.float64) * std + mean).to(dtype)
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16])
+@pytest.mark.parametrize("cols", [8, 36, 50, 768, 1601, 5000, 8193, 12288])
+def test_gradients_of_rows_of_one_very_large_value(cuda, cols, dtype):
+    """2^110 in every column, eps 1e-12: the mean is exact (partial sums are small integers times 2^110, and cols times the float32 1 / cols rounds to 1), the
+    variance 0, r = 1e6, and |mean| r is over float32's largest number.  With q = dn w the gradient is dout + r (q - mean q), nothing of which comes near that.
+    The mean of q is off by 40 u of its terms' mean magnitude, q, r, the difference and the last addition by a few u each: 64 u of all of them, and
+    one rounding to the type.  Weight gradients are 0: every normed value is."""
+    import sparse
+    eps, rows = 1e-12, 3
+    large = torch.full((rows, cols), 2.0 ** 110, dtype=dtype)
+    large[1] *= -1
+    w, b = draw(1, cols, mean=1.0, dtype=dtype), draw(2, cols, dtype=dtype)
+    dout, dn = draw(3, rows, cols, dtype=dtype), draw(4, rows, cols, dtype=dtype)
+    r = eps ** -0.5
+
+    def expected(dn, w, add):
+        q = dn.double() * w.double()
+        return r * (q - q.mean(-1, keepdim=True)) + add, r * (q.abs() + q.abs().mean(-1, keepdim=True)) + abs(add)
+
+    def close(name, got, want, magnitude):
+        tolerance = 64 * U * magnitude + torch.finfo(got.dtype).eps / 2 * want.abs() * 1.01
+        off = (got.cpu().double() - want).abs()
+        assert (off <= tolerance).all(), (name, cols, got.isnan().sum().item(), (off / tolerance).max().item())
+
+    def leaves(*ts):
+        return [t.to(cuda).requires_grad_() for t in ts]
+
+    # before a block: by itself, and behind the addition
+    x, w1, b1 = leaves(large, w, b)
+    n = sparse.block_norm(x, w1, b1, eps=eps)
+    assert torch.equal(n.detach().cpu(), b.expand(rows, cols))
+    dx, dw, db = torch.autograd.grad(n, (x, w1, b1), dn.to(cuda))
+    close("x", dx, *expected(dn, w, 0.0))
+    close("bias", db, dn.double().sum(0), dn.double().abs().sum(0))
+    assert not dw.any()
+    x, y, w1, b1 = leaves(large, torch.zeros_like(large), w, b)
+    out, n = sparse.residual_norm(x, y, pre_kind="layer", pre_weight=w1, pre_bias=b1, eps=eps)
+    assert torch.equal(out.detach().cpu(), large)
+    dx, dy, dw = torch.autograd.grad((out, n), (x, y, w1), (dout.to(cuda), dn.to(cuda)))
+    close("residual", dx, *expected(dn, w, dout.double()))
+    assert torch.equal(dx, dy) and not dw.any()
+    # behind a block
+    for gate in (None, torch.full((cols,), 0.5, dtype=dtype), torch.full((rows, cols), 0.5, dtype=dtype)):
+        x, y, w1, b1 = leaves(draw(5, rows, cols, dtype=dtype), large, w, b)
+        g = None if gate is None else gate.to(cuda)
+        out = sparse.residual_norm(x, y, g, post_kind="layer", post_weight=w1, post_bias=b1, eps=eps)
+        dx, dy, dw, db = torch.autograd.grad(out, (x, y, w1, b1), dout.to(cuda))
+        of_z = dout.double() * (1.0 if gate is None else 0.5)
+        assert torch.equal(dx.cpu(), dout) and not dw.any()
+        close("y", dy, *expected(of_z, w, 0.0))
+        close("post_bias", db, of_z.sum(0), of_z.abs().sum(0))
