@@ -133,6 +133,11 @@ def _parameters(fn, x, *params):
     return [None if p is None else (p.float() if mixed else p).resolve_neg().contiguous() for p in params]
 
 
+def _wide(gate):
+    """A gate that is spelled out, in float32 where it gets a gradient: that of every element is added up behind the kernel, and rounded to the gate's type then."""
+    return gate.float() if gate.requires_grad and torch.is_grad_enabled() else gate
+
+
 def _gate(fn, gate, y):
     """(gate as rows of columns, the number of adjacent rows of y that each is for)"""
     cols, lead = y.shape[-1], y.shape[:-1]
@@ -143,14 +148,14 @@ def _gate(fn, gate, y):
     if gate.dim() > y.dim() or any(g not in (1, s) for g, s in zip(gate.shape[::-1], y.shape[::-1])):
         raise RuntimeError(f"{fn}: a gate {tuple(gate.shape)} does not broadcast to {tuple(y.shape)}")
     if gate.dim() == 0 or gate.shape[-1] != cols:
-        gate = gate.expand(*gate.shape[:-1], cols)
+        gate = _wide(gate).expand(*gate.shape[:-1], cols)
     own = (1,) * (y.dim() - gate.dim()) + gate.shape[:-1]
     # dimensions that the gate follows, then dimensions that share it; any other order is spelled out row by row
     shared = len(lead)
     while shared and own[shared - 1] == 1:
         shared -= 1
     if own[:shared] != lead[:shared]:
-        gate, shared = gate.expand(y.shape), len(lead)
+        gate, shared = _wide(gate).expand(y.shape), len(lead)
     return gate, lead[shared:].numel()
 
 

@@ -76,3 +76,12 @@ def test_gradients_of_rows_of_one_very_large_value(cuda, cols, dtype):
         assert torch.equal(dx.cpu(), dout) and not dw.any()
         close("y", dy, *expected(of_z, w, 0.0))
         close("post_bias", db, of_z.sum(0), of_z.abs().sum(0))
+
+
+@pytest.mark.parametrize("stream", [F16, BF16])
+@pytest.mark.parametrize("shape", [(), (1,), (1, 1, 1), (6, 1, 1), (1, 40, 512), (6, 40, 1), (40, 512), (1, 512), (6, 1, 512)])
+def test_gates_of_16_bits_that_broadcast(cuda, shape, stream):
+    """The gradient of a gate is rounded once, whatever rows and columns share it: 256 u of the sum of the magnitudes and one rounding to its type, as
+    for a gate of float32."""
+    check(cuda, (6, 40), 512, stream, stream, "rms", "rms", "given", gate_shape=shape, seed=9)
+    check(cuda, (6, 40), 512, stream, stream, None, "layer", "given", gate_shape=shape, seed=19)
