@@ -34,11 +34,13 @@ Tensor make(at::IntArrayRef shape, at::ScalarType type, const Tensor& like) { re
 void* pointer(const Tensor& t) { return t.defined() ? t.data_ptr() : nullptr; }
 Tensor or_none(const Maybe& t) { return t ? *t : Tensor(); }
 
-// a contiguous tensor of floating-point numbers on the current device, with nothing between a call and its storage
-bool plain(const Tensor& t) {
+// a strided tensor on a GPU, with nothing between a call and its storage
+bool stored(const Tensor& t) {
   static const auto allowed = c10::DispatchKeySet({c10::DispatchKey::CUDA, c10::DispatchKey::AutogradCUDA, c10::DispatchKey::ADInplaceOrView, c10::DispatchKey::AutocastCUDA});
-  return t.is_cuda() && (t.key_set() | allowed) == allowed && t.is_contiguous() && code_of(t.scalar_type()) >= 0 && t.get_device() == c10::hip::current_device();
+  return t.is_cuda() && (t.key_set() | allowed) == allowed;
 }
+// one of floating-point numbers, contiguous and on the current device
+bool plain(const Tensor& t) { return stored(t) && t.is_contiguous() && code_of(t.scalar_type()) >= 0 && t.get_device() == c10::hip::current_device(); }
 bool wants_graph(std::initializer_list<const Tensor*> inputs) {
   if (!at::GradMode::is_enabled()) return false;
   for (const Tensor* t : inputs)
@@ -46,10 +48,18 @@ bool wants_graph(std::initializer_list<const Tensor*> inputs) {
   return false;
 }
 [[noreturn]] void no_second_derivative(const char* what) { throw std::runtime_error(std::string("a graph of the gradients of ") + what + " is not supported"); }
-// a gradient as the kernels take it (undefined: zero)
-Tensor settled(const Tensor& g, at::ScalarType type) {
+// A gradient, or a saved tensor, as the kernels take it (undefined: zero, or none).  The engine looks at gradients, but not where a node is called by itself; a
+// saved tensor is whatever its hook hands back.
+Tensor as_it_was(const char* what, const Tensor& t, at::IntArrayRef shape, at::ScalarType type, c10::DeviceIndex device) {
+  if (!t.defined()) return t;
+  const Tensor plain = t.resolve_neg();
+  if (!stored(plain) || plain.get_device() != device || plain.scalar_type() != type || plain.sizes() != shape)
+    throw std::runtime_error(std::string(what) + " is not the one that was saved, or of its output: another shape, type or device");
+  return plain.contiguous();
+}
+Tensor settled(const char* fn, const Tensor& g, at::IntArrayRef shape, at::ScalarType type, c10::DeviceIndex device) {
   if (!g.defined()) return g;
-  return (g.scalar_type() == type ? g : g.to(type)).resolve_neg().contiguous();
+  return as_it_was(fn, g.scalar_type() == type ? g : g.to(type), shape, type, device);
 }
 int64_t blocks_of(int64_t cols) { return tf24_checkpoint_blocks(cols); }
 std::pair<Tensor, Tensor> empty_checkpoint(int64_t rows, int64_t cols, const Tensor& like) {
@@ -58,9 +68,10 @@ std::pair<Tensor, Tensor> empty_checkpoint(int64_t rows, int64_t cols, const Ten
 
 // ---------------------------------------------------------------- block norms
 struct NormCall {
-  std::vector<int64_t> shape;
+  std::vector<int64_t> shape, gate_shape;
   int64_t rows, cols, rows_per_gate;
-  at::ScalarType stream, block, param;
+  at::ScalarType stream, block, param, gate;
+  c10::DeviceIndex device;
   double scale;
   int post_kind, pre_kind;
   bool residual, has_n;
@@ -73,16 +84,20 @@ struct BlockNormBackward : public torch::autograd::Node {
   variable_list apply(variable_list&& grads) override {
     if (at::GradMode::is_enabled()) no_second_derivative("block_norm and residual_norm");
     std::lock_guard<std::mutex> lock(mutex_);
+    const char* fn = "block_norm and residual_norm: a gradient or saved tensor";
     // of out (a call with y has one) and of n
     Tensor dout = call.residual ? grads[0] : Tensor(), dn = call.has_n ? grads[call.residual ? 1 : 0] : Tensor();
     variable_list result(7);
     if (!dout.defined() && !dn.defined()) return result;
+    dout = settled(fn, dout, call.shape, call.stream, call.device);
+    dn = settled(fn, dn, call.shape, call.block, call.device);
     const Tensor like = dn.defined() ? dn : dout;
     const int pre_kind = dn.defined() ? call.pre_kind : 0, post_kind = call.post_kind;
-    const Tensor h_ = h.unpack(call.residual ? shared_from_this() : nullptr), y_ = y.unpack(), gate_ = gate.unpack(), post_weight_ = post_weight.unpack(),
-                 post_bias_ = post_bias.unpack(), pre_weight_ = pre_weight.unpack(), stats_ = stats.unpack();
-    dout = settled(dout, call.stream);
-    dn = settled(dn, call.block);
+    auto saved = [&](const Tensor& t, at::IntArrayRef shape, at::ScalarType type) { return as_it_was(fn, t, shape, type, call.device); };
+    const Tensor h_ = saved(h.unpack(call.residual ? shared_from_this() : nullptr), call.shape, call.stream), y_ = saved(y.unpack(), call.shape, call.block),
+                 gate_ = saved(gate.unpack(), call.gate_shape, call.gate), post_weight_ = saved(post_weight.unpack(), {call.cols}, call.param),
+                 post_bias_ = saved(post_bias.unpack(), {call.cols}, call.param), pre_weight_ = saved(pre_weight.unpack(), {call.cols}, call.param),
+                 stats_ = saved(stats.unpack(), {4, call.rows}, at::kFloat);
     auto wanted = [&](int i) { return task_should_compute_output(i); };
     auto zeros_of = [&](at::IntArrayRef shape, at::ScalarType type) { return call.rows ? make(shape, type, like) : at::zeros(shape, like.options().dtype(type)); };
     if (wanted(0)) result[0] = make(call.shape, call.stream, like);
@@ -148,6 +163,11 @@ py::object block_norm(const Tensor& x, const Maybe& y_in, const Maybe& gate_in, 
         if (gate.size(i) != y.size(i)) return py::none();
     }
   }
+  if (gate.defined()) {
+    call.gate_shape = gate.sizes().vec();
+    call.gate = gate.scalar_type();
+  }
+  call.device = x.get_device();
   call.scale = scale;
   call.post_kind = post_kind;
   call.pre_kind = pre_kind;
@@ -187,14 +207,19 @@ py::object block_norm(const Tensor& x, const Maybe& y_in, const Maybe& gate_in, 
 struct GeluGluBackward : public torch::autograd::Node {
   std::vector<int64_t> shape;
   at::ScalarType type;
+  c10::DeviceIndex device;
   SavedVariable values, scales;
 
   variable_list apply(variable_list&& grads) override {
     if (at::GradMode::is_enabled()) no_second_derivative("gelu_glu_checkpoint");
     std::lock_guard<std::mutex> lock(mutex_);
     if (!grads[0].defined()) return {Tensor()};
-    const Tensor go = settled(grads[0], type), v = values.unpack(), s = scales.unpack();
-    const int64_t cols = shape.back(), rows = go.numel() / (cols / 2);
+    const char* fn = "gelu_glu_checkpoint: a gradient or saved tensor";
+    const int64_t cols = shape.back(), rows = c10::multiply_integers(shape) / cols, blocks = blocks_of(cols / 2);
+    auto out_shape = shape;
+    out_shape.back() = cols / 2;
+    const Tensor go = settled(fn, grads[0], out_shape, type, device), v = as_it_was(fn, values.unpack(), {2 * rows, 32 * blocks}, at::kFloat8_e4m3fn, device),
+                 s = as_it_was(fn, scales.unpack(), {2 * rows, blocks}, at::kByte, device);
     const Tensor result = make(shape, type, go);
     check(tf24_gelu_glu_backward_checkpoint(pointer(go), cols / 2, pointer(v), pointer(s), code_of(type), rows, cols, pointer(result), cols, stream_of(go)));
     return {result};
@@ -226,6 +251,7 @@ py::object gelu_glu_checkpoint(const Tensor& x, bool keep_output) {
     node->scales = SavedVariable(scales, false);
     node->shape = x.sizes().vec();
     node->type = x.scalar_type();
+    node->device = x.get_device();
   }
   if (!keep_output) return py::cast(out);
   return py::make_tuple(out, out_values, out_scales);

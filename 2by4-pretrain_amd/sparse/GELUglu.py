@@ -104,7 +104,7 @@ class gelu_glu_checkpoint(autograd.Function):
         N.launch(input, N.lib().tf24_gelu_glu_forward_checkpoint, x2.data_ptr(), N.dtype_code(input.dtype), ld, rows, cols, out.data_ptr(), half,
                  values.data_ptr(), scales.data_ptr(), N.ptr(out_values), N.ptr(out_scales))
         ctx.save_for_backward(values, scales)
-        ctx.shape, ctx.dtype = input.shape, input.dtype
+        ctx.shape, ctx.dtype, ctx.device = input.shape, input.dtype, input.device
         if not keep_output:
             return out
         ctx.mark_non_differentiable(out_values, out_scales)
@@ -119,8 +119,15 @@ class gelu_glu_checkpoint(autograd.Function):
             return None, None
         values, scales = ctx.saved_tensors
         cols = ctx.shape[-1]
-        go, ld = N.as_rows(grad_output if grad_output.dtype == ctx.dtype else grad_output.to(ctx.dtype))
         rows, half = ctx.shape[:-1].numel(), cols // 2
+        blocks = N.lib().tf24_checkpoint_blocks(half)
+
+        def as_it_was(t, shape, dtype):
+            return N.as_it_was("gelu_glu_checkpoint", t, shape, dtype, ctx.device)
+
+        values = as_it_was(values, (2 * rows, 32 * blocks), torch.float8_e4m3fn).contiguous()
+        scales = as_it_was(scales, (2 * rows, blocks), torch.uint8).contiguous()
+        go, ld = N.as_rows(as_it_was(grad_output if grad_output.dtype == ctx.dtype else grad_output.to(ctx.dtype), (*ctx.shape[:-1], half), ctx.dtype))
         if rows > 1 and ld < half:
             go, ld = go.contiguous(), half
         grad_in = torch.empty(ctx.shape, dtype=ctx.dtype, device=values.device)

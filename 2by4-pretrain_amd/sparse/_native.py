@@ -267,6 +267,13 @@ def as_rows(t):
     return flat, flat.stride(0)
 
 
+def as_it_was(what, t, shape, dtype, device):
+    """t, a tensor or None, if it has this shape, type and place: what a saved-tensor hook hands back may be anything."""
+    if t is not None and (not torch._C._has_storage(t) or t.layout != torch.strided or t.shape != shape or t.dtype != dtype or t.device != device):
+        raise RuntimeError(f"{what}: a gradient or saved tensor is not the one that was saved, or of its output: another shape, type or device")
+    return t
+
+
 def ptr(t):
     return None if t is None else t.data_ptr()
 

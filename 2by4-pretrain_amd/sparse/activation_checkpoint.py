@@ -67,6 +67,8 @@ class ActivationCheckpoint:
             if out is not None:
                 return out
         self._check()
+        if not self.values.is_cuda:
+            raise RuntimeError("ActivationCheckpoint.decode: only CUDA tensors are supported")
         out = torch.empty(self.shape, dtype=dtype, device=self.values.device)
         rows, cols = self.values.shape[0], self.shape[-1]
         N.launch(out, N.lib().tf24_checkpoint_decode, self.values.data_ptr(), self.scales.data_ptr(), rows, cols, out.data_ptr(), N.dtype_code(dtype), cols)

@@ -58,7 +58,9 @@ class _block_norm(autograd.Function):
         residual = y is not None
         ctx.save_for_backward((out if residual else x) if pre_kind else None, y if post_kind or (gate is not None and ctx.needs_input_grad[2]) else None, gate,
                               post_weight, post_bias, pre_weight, stats)
-        ctx.call = x.shape, x.dtype, block_dtype, None if pre_bias is None else pre_bias.dtype, residual, rows_per_gate, scale, post_kind, pre_kind
+        param = next((p for p in (post_weight, post_bias, pre_weight, pre_bias) if p is not None), None)
+        ctx.call = (x.shape, x.dtype, x.device, block_dtype, None if param is None else param.dtype, None if gate is None else (gate.shape, gate.dtype), residual,
+                    rows_per_gate, scale, post_kind, pre_kind)
         if values is not None:
             ctx.mark_non_differentiable(values, scales)
         return out, n, values, scales
@@ -68,16 +70,23 @@ class _block_norm(autograd.Function):
         if torch.is_grad_enabled():
             raise RuntimeError("a graph of the gradients of block_norm and residual_norm is not supported")
         h, y, gate, post_weight, post_bias, pre_weight, stats = ctx.saved_tensors
-        shape, stream_dtype, block_dtype, pre_bias_dtype, residual, rows_per_gate, scale, post_kind, pre_kind = ctx.call
+        shape, stream_dtype, device, block_dtype, param_dtype, gate_as, residual, rows_per_gate, scale, post_kind, pre_kind = ctx.call
         needs = ctx.needs_input_grad
         if grad_n is None:
             pre_kind = N.NORM_NONE                                 # only the stream goes on
             if grad_out is None:
                 return (None,) * 14
-        device = (grad_out if grad_n is None else grad_n).device
         rows, cols = shape[:-1].numel(), shape[-1]
-        param = post_weight if post_weight is not None else post_bias if post_bias is not None else pre_weight
-        param_dtype = pre_bias_dtype if param is None else param.dtype
+
+        def as_it_was(t, shape, dtype):
+            return N.as_it_was("block_norm and residual_norm", t, shape, dtype, device)
+
+        grad_out = None if grad_out is None else as_it_was(grad_out if grad_out.dtype == stream_dtype else grad_out.to(stream_dtype), shape, stream_dtype)
+        grad_n = None if grad_n is None else as_it_was(grad_n if grad_n.dtype == block_dtype else grad_n.to(block_dtype), shape, block_dtype)
+        h, y = as_it_was(h, shape, stream_dtype), as_it_was(y, shape, block_dtype)
+        gate = None if gate is None else as_it_was(gate, *gate_as)
+        post_weight, post_bias, pre_weight = (None if t is None else as_it_was(t, (cols,), param_dtype).resolve_neg().contiguous() for t in (post_weight, post_bias, pre_weight))
+        stats = None if stats is None else as_it_was(stats, (4, rows), torch.float32).contiguous()
         make = torch.empty if rows else torch.zeros                # (sums over no rows)
         grad_x = grad_y = grad_gate = None
         if needs[0]:
@@ -96,9 +105,9 @@ class _block_norm(autograd.Function):
             dout = dn = h2 = y2 = gate2 = workspace = None
             ld_dout = ld_dn = ld_h = ld_y = ld_gate = nbytes = 0
             if grad_out is not None:
-                dout, ld_dout = N.as_rows(grad_out if grad_out.dtype == stream_dtype else grad_out.to(stream_dtype))
+                dout, ld_dout = N.as_rows(grad_out)
             if pre_kind:
-                dn, ld_dn = N.as_rows(grad_n if grad_n.dtype == block_dtype else grad_n.to(block_dtype))
+                dn, ld_dn = N.as_rows(grad_n)
                 h2, ld_h = N.as_rows(h)
             if y is not None:
                 y2, ld_y = N.as_rows(y)

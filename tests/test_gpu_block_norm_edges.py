@@ -85,3 +85,73 @@ def test_gates_of_16_bits_that_broadcast(cuda, shape, stream):
     for a gate of float32."""
     check(cuda, (6, 40), 512, stream, stream, "rms", "rms", "given", gate_shape=shape, seed=9)
     check(cuda, (6, 40), 512, stream, stream, None, "layer", "given", gate_shape=shape, seed=19)
+
+
+class Given:
+    """Saved-tensor hooks that hand back something else than they were given: change(tensor) for tensors of `numel` elements."""
+
+    def __init__(self, change, numel):
+        self.hooks = torch.autograd.graph.saved_tensors_hooks(lambda t: t, lambda t: change(t) if t.numel() == numel else t)
+
+    def __enter__(self):
+        return self.hooks.__enter__()
+
+    def __exit__(self, *args):
+        return self.hooks.__exit__(*args)
+
+
+def apart(t):
+    """The same values, a row not next to the one before it."""
+    wide = torch.full((*t.shape[:-1], t.shape[-1] + 7), 3, device=t.device).to(t.dtype)
+    wide[..., :t.shape[-1]] = t
+    return wide[..., :t.shape[-1]]
+
+
+CHANGES = [lambda t: t.cpu(), lambda t: t[:1], lambda t: t.to(torch.float64), lambda t: t.flatten()[:1].expand(1)]
+
+
+def test_saved_tensors_that_hooks_hand_back(cuda):
+    """Values that lie elsewhere are taken; another shape, type or place is refused, before a kernel reads it."""
+    import sparse
+    rows, cols = 6, 96
+    x, y, gate = (draw(i, rows, cols).to(cuda).requires_grad_() for i in (20, 21, 22))
+    w = draw(23, cols, mean=1.0).to(cuda).requires_grad_()
+    go, gn = draw(24, rows, cols).to(cuda), draw(25, rows, cols).to(cuda)
+
+    def call():
+        return sparse.residual_norm(x, y, gate, post_kind="rms", post_weight=w, pre_kind="layer", pre_weight=w)
+
+    want = torch.autograd.grad(call(), (x, y, gate, w), (go, gn))
+    for numel in (rows * cols, cols, 4 * rows):                    # rows; weights; statistics
+        with Given(apart, numel):
+            outputs = call()
+        assert all(torch.equal(a, b) for a, b in zip(torch.autograd.grad(outputs, (x, y, gate, w), (go, gn)), want))
+        for change in CHANGES:
+            with Given(change, numel):
+                outputs = call()
+            with pytest.raises(RuntimeError, match="saved"):
+                torch.autograd.grad(outputs, (x, y, gate, w), (go, gn))
+    from sparse import _native as N
+    if N.torch_calls() is not None:                                # nodes that are called by themselves, past the engine's checks
+        node = call()[1].grad_fn
+        with torch.no_grad():
+            for grads in ((go[:1], gn), (go, gn[:, :32]), (go.cpu(), gn.cpu()), (go,), ()):
+                with pytest.raises((RuntimeError, TypeError), match="gradient|arguments"):       # (torch counts them)
+                    node(*grads)
+            assert all(torch.equal(a, b) for a, b in zip(node(go, gn), want[:3]))
+
+
+def test_saved_tensors_of_the_gated_activation_that_hooks_hand_back(cuda):
+    import sparse
+    rows, half = 6, 96
+    x, dy = draw(26, rows, 2 * half).to(cuda).requires_grad_(), draw(27, rows, half).to(cuda)
+    (want,) = torch.autograd.grad(sparse.gelu_glu_checkpoint.apply(x), x, dy)
+    for numel in (2 * rows * half, 2 * rows * half // 32):         # values; scales
+        with Given(lambda t: apart(t.view(torch.uint8)).view(t.dtype), numel):
+            out = sparse.gelu_glu_checkpoint.apply(x)
+        assert torch.equal(torch.autograd.grad(out, x, dy)[0], want)
+        for change in CHANGES[:2] + [lambda t: t.view(torch.int8)]:
+            with Given(change, numel):
+                out = sparse.gelu_glu_checkpoint.apply(x)
+            with pytest.raises(RuntimeError, match="saved"):
+                torch.autograd.grad(out, x, dy)
