@@ -393,7 +393,8 @@ block_norm_backward_wide(const BackwardArgs a, uint32_t rows_per_gate) {
 
 // The gradients of the parameters from the pieces' sums.  Job 0: weight of the norm behind, 1: its bias, 2, 3: those of the norm before,
 // from 4 on: the gates that rows share; a workgroup takes 32 columns of a job, 32 strands of pieces side by side, or where a gate has few pieces
-// a gate for each strand.
+// a gate for each strand.  The pieces are added in float64: with millions of gates a strand has 10^5 of them, and float32 sums of so many are off by thousands of
+// units (2^20 gates of two rows, equal terms: 4341), where everything else is off by a few.
 struct FinishArgs {
   const float* partial;
   const void *gate, *post_weight, *post_bias;
@@ -407,7 +408,7 @@ struct FinishArgs {
 constexpr int kStrands = 32;
 __global__ void __launch_bounds__(32 * kStrands)
 block_norm_finish(const FinishArgs a) {
-  __shared__ float strands[kStrands][33];
+  __shared__ double strands[kStrands][33];
   const uint32_t job = blockIdx.x / a.column_blocks;
   void* to = job == 0 ? a.grad_post_weight : job == 1 ? a.grad_post_bias : job == 2 ? a.grad_pre_weight : job == 3 ? a.grad_pre_bias : a.grad_gate;
   if (!to) return;
@@ -418,7 +419,7 @@ block_norm_finish(const FinishArgs a) {
   const uint32_t gate = job < 4 ? 0 : alone ? (job - 4) * kStrands + strand : job - 4;
   const uint32_t begin = gate * a.pieces.per_group, end = job < 4 ? pieces : min(pieces, begin + a.pieces.per_group);
   const uint32_t step = alone ? 1 : kStrands;
-  float total = 0.0f;
+  double total = 0.0;
   if (col < a.cols) {
     const uint64_t one = (uint64_t)pieces * a.cols;
     const float* from = a.partial + (job < 4 ? job * one : 0) + col;
@@ -443,7 +444,7 @@ block_norm_finish(const FinishArgs a) {
     }
   }
   if (alone) {
-    if (gate < a.pieces.groups && col < a.cols) store_result(to, a.gate_dtype, (int64_t)gate * a.cols + col, total);
+    if (gate < a.pieces.groups && col < a.cols) store_result(to, a.gate_dtype, (int64_t)gate * a.cols + col, (float)total);
     return;
   }
   strands[strand][c] = total;
@@ -451,7 +452,7 @@ block_norm_finish(const FinishArgs a) {
   if (strand == 0 && col < a.cols) {
 #pragma unroll
     for (int s = 1; s < kStrands; s++) total += strands[s][c];
-    store_result(to, job < 4 ? a.param_dtype : a.gate_dtype, (int64_t)gate * a.cols + col, total);
+    store_result(to, job < 4 ? a.param_dtype : a.gate_dtype, (int64_t)gate * a.cols + col, (float)total);
   }
 }
 

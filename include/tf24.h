@@ -488,8 +488,8 @@ int tf24_block_norm_forward(const void* x, int64_t ld_x, const void* y, int64_t 
  * the stats of the forward pass.  Every result may be NULL: grad_x, grad_y (contiguous), the gradients of weights and biases (of param_dtype),
  * grad_gate (of gate_dtype, contiguous).  y is read where there is a norm of it or grad_gate is wanted, h where pre_kind is not NONE.
  *   workspace  for the gradients of parameters and of gates that rows share: tf24_block_norm_backward_workspace_bytes(rows, cols, rows_per_gate or rows)
- * Sums over rows are float32 in a fixed order, rounded once.  rows >= 1; up to 2^22 gates that rows share (their gradients: a launch of one workgroup for
- * 32 columns of a gate, or of 32 gates with few rows, has to hold them).
+ * Sums over rows are float32 in a piece of the rows and float64 over the pieces, in a fixed order, rounded once.  rows >= 1; up to 2^22 gates that rows
+ * share (their gradients: a launch of one workgroup for 32 columns of a gate, or of 32 gates with few rows, has to hold them).
  */
 int tf24_block_norm_backward(const void* grad_out, int64_t ld_grad_out, const void* grad_n, int64_t ld_grad_n, const void* h, int64_t ld_h, const void* y,
                              int64_t ld_y, int stream_dtype, int block_dtype, int64_t rows, int64_t cols, const void* gate, int gate_dtype, int64_t ld_gate,

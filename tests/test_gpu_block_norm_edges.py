@@ -155,3 +155,21 @@ def test_saved_tensors_of_the_gated_activation_that_hooks_hand_back(cuda):
                 out = sparse.gelu_glu_checkpoint.apply(x)
             with pytest.raises(RuntimeError, match="saved"):
                 torch.autograd.grad(out, x, dy)
+
+
+def test_sums_over_very_many_gates(cuda):
+    """2^20 gates of two rows: the sums over the gates' pieces are as exact as those over few.  A sum of `count` equal terms c is count c to 256 u; in float32 in sequence
+    2^15 of them in each of 32 strands would be off by 4341 u for c = 0.2."""
+    import sparse
+    gates, cols = 1 << 20, 8
+    x, y = torch.zeros(gates, 2, cols, device=cuda, requires_grad=True), torch.ones(gates, 2, cols, device=cuda, requires_grad=True)
+    gate = torch.full((gates, 1, cols), 0.1, device=cuda, requires_grad=True)
+    w, b, pw, pb = (torch.full((cols,), v, device=cuda, requires_grad=True) for v in (1.0, 0.0, 1.0, 0.0))
+    out, n = sparse.residual_norm(x, y, gate, post_kind="rms", post_weight=pw, post_bias=pb, pre_kind="rms", pre_weight=w, pre_bias=b, eps=0.0)
+    go, gn = torch.full_like(out, 0.3), torch.full_like(n, 0.1)
+    dg, dw, db, dpw, dpb = torch.autograd.grad((out, n), (gate, w, b, pw, pb), (go, gn))
+    # y = 1, normed 1; out = 0.1, normed 1: no gradient passes the second norm, d = go
+    c, g, s, count = (torch.tensor(v, dtype=F32).double().item() for v in (0.1, 0.1, 0.3, 2.0 * gates))
+    for got, want in ((dw, count * c), (db, count * c), (dpw, count * g * s), (dpb, count * g * s)):
+        assert (got.cpu().double() - want).abs().max() <= 256 * U * want, ((got.cpu().double() - want).abs().max() / want / U).item()
+    assert (dg.cpu().double() - 2 * s).abs().max() <= 64 * U * 2 * s
