@@ -84,8 +84,9 @@ gelu_glu_bwd(const T* __restrict__ grad_out, int64_t ld_go, const T* __restrict_
 }
 
 // Row-major input, `half` columns of x and as many of gate in each row; a lane owns a unit of the output's columns.  What is kept of the
-// input has units and blocks of 2 * rows rows, that of the output of `rows` rows (numbered as the lanes are).
-template <typename T, bool KEEP_OUT>
+// input (KEEP: nothing where no backward pass will read it) has units and blocks of 2 * rows rows, that of the output of `rows` rows (numbered as
+// the lanes are).
+template <typename T, bool KEEP, bool KEEP_OUT>
 __global__ void __launch_bounds__(kThreads)
 gelu_glu_fwd_keep(const T* __restrict__ in, int64_t ld_in, int half, UnitRows by, uint32_t total, T* __restrict__ out, int64_t ld_out, uint8_t* __restrict__ values,
                   uint8_t* __restrict__ scales, uint8_t* __restrict__ out_values, uint8_t* __restrict__ out_scales) {
@@ -99,13 +100,15 @@ gelu_glu_fwd_keep(const T* __restrict__ in, int64_t ld_in, int half, UnitRows by
 #pragma unroll
   for (int e = 0; e < 8; e++) o[e] = glu_terms<false>(g[e]).gelu * x[e];
   store_up_to_8(out + (int64_t)row * ld_out + col, n, o);
-  const Kept8 kx = keep_8<T>(x), kg = keep_8<T>(g);
-  const uint64_t ux = (uint64_t)u + first, ug = ux + by.units;  // rows 2 row and 2 row + 1
-  *reinterpret_cast<uint2*>(values + ux * 8) = kx.values;
-  *reinterpret_cast<uint2*>(values + ug * 8) = kg.values;
-  if ((u & 3) == 0) {
-    scales[ux >> 2] = (uint8_t)kx.scale;
-    scales[ug >> 2] = (uint8_t)kg.scale;
+  if constexpr (KEEP) {
+    const Kept8 kx = keep_8<T>(x), kg = keep_8<T>(g);
+    const uint64_t ux = (uint64_t)u + first, ug = ux + by.units;  // rows 2 row and 2 row + 1
+    *reinterpret_cast<uint2*>(values + ux * 8) = kx.values;
+    *reinterpret_cast<uint2*>(values + ug * 8) = kg.values;
+    if ((u & 3) == 0) {
+      scales[ux >> 2] = (uint8_t)kx.scale;
+      scales[ug >> 2] = (uint8_t)kg.scale;
+    }
   }
   if constexpr (KEEP_OUT) {
     const Kept8 ko = keep_8<T>(o);
@@ -249,7 +252,8 @@ int forward_keep(const void* in, int64_t ld_in, int64_t rows, int64_t cols, void
                  hipStream_t s) {
   const UnitRows by = unit_rows(cols / 2);
   const uint32_t total = (uint32_t)rows * by.units;
-  auto* kernel = out_values ? gelu_glu_fwd_keep<T, true> : gelu_glu_fwd_keep<T, false>;
+  auto* kernel = values ? (out_values ? gelu_glu_fwd_keep<T, true, true> : gelu_glu_fwd_keep<T, true, false>)
+                        : (out_values ? gelu_glu_fwd_keep<T, false, true> : gelu_glu_fwd_keep<T, false, false>);
   hipLaunchKernelGGL(kernel, dim3((total + kThreads - 1) / kThreads), dim3(kThreads), 0, s, (const T*)in, ld_in, (int)(cols / 2), by, total, (T*)out, ld_out,
                      (uint8_t*)values, (uint8_t*)scales, (uint8_t*)out_values, (uint8_t*)out_scales);
   return check_launch("tf24_gelu_glu_forward_checkpoint");
@@ -273,7 +277,7 @@ extern "C" int tf24_gelu_glu_forward_checkpoint(const void* in, int dtype, int64
   const char* fn = "tf24_gelu_glu_forward_checkpoint";
   if (int rc = check_kept(fn, dtype, rows, cols, ld_in, ld_out)) return rc;
   if (!rows) return TF24_OK;
-  if (!in || !out || !values || !scales || !out_values != !out_scales) return fail(TF24_ERR_ARG, "%s: null pointer", fn);
+  if (!in || !out || !values != !scales || !out_values != !out_scales) return fail(TF24_ERR_ARG, "%s: null pointer", fn);
   if (int rc = check_aligned(fn, dtype_size(dtype), {in, out})) return rc;
   if (int rc = check_aligned(fn, 16, {values, out_values})) return rc;
   auto* go = dtype == TF24_F32 ? forward_keep<float> : dtype == TF24_F16 ? forward_keep<f16_t> : forward_keep<bf16_t>;

@@ -238,12 +238,13 @@ py::object gelu_glu_checkpoint(const Tensor& x, bool keep_output) {
   const int64_t cols = x.size(-1), half = cols / 2, rows = x.numel() / cols;
   auto shape = x.sizes().vec();
   shape.back() = half;
-  Tensor out = make(shape, x.scalar_type(), x), out_values, out_scales;
-  const auto [values, scales] = empty_checkpoint(2 * rows, half, x);
+  Tensor out = make(shape, x.scalar_type(), x), values, scales, out_values, out_scales;
+  const bool graph = wants_graph({&x});
+  if (graph) std::tie(values, scales) = empty_checkpoint(2 * rows, half, x);
   if (keep_output) std::tie(out_values, out_scales) = empty_checkpoint(rows, half, x);
   check(tf24_gelu_glu_forward_checkpoint(pointer(x), code_of(x.scalar_type()), cols, rows, cols, pointer(out), half, pointer(values), pointer(scales), pointer(out_values),
                                          pointer(out_scales), stream_of(x)));
-  if (wants_graph({&x})) {
+  if (graph) {
     auto node = std::shared_ptr<GeluGluBackward>(new GeluGluBackward(), torch::autograd::deleteNode);
     node->set_next_edges(torch::autograd::collect_next_edges(x));
     torch::autograd::set_history(out, node);

@@ -74,7 +74,7 @@ class gelu_glu_checkpoint(autograd.Function):
     """gelu_glu that keeps its input in 8 bits for the backward pass (as in ActivationCheckpoint, x and gate of a row one after the
     other) and gives the gradient at the kept values: 1.03 bytes an element in place of 2, for an input that nothing else holds.  The
     output is the same.  apply(input) -> out; apply(input, True) -> (out, values, scales), the last two being out kept in 8 bits.  Any
-    input with a last dimension of an even size; the output is row-major."""
+    input with a last dimension of an even size; the output is row-major.  Where no graph is recorded nothing is kept of the input."""
 
     @classmethod
     def apply(cls, input, keep_output=False):
@@ -83,10 +83,10 @@ class gelu_glu_checkpoint(autograd.Function):
             result = calls.gelu_glu_checkpoint(input, keep_output)
             if result is not None:
                 return result
-        return super().apply(input, keep_output)
+        return super().apply(input, keep_output, torch.is_grad_enabled() and input.requires_grad)
 
     @staticmethod
-    def forward(ctx, input, keep_output=False):
+    def forward(ctx, input, keep_output=False, keep_input=True):
         if not input.is_cuda:
             raise RuntimeError("gelu_glu_checkpoint: only CUDA tensors are supported")
         if input.dim() == 0 or input.shape[-1] == 0 or input.shape[-1] % 2:
@@ -97,13 +97,14 @@ class gelu_glu_checkpoint(autograd.Function):
         rows, cols = input.shape[:-1].numel(), input.shape[-1]
         half = cols // 2
         out = torch.empty((*input.shape[:-1], half), dtype=input.dtype, device=input.device)
-        values, scales = empty_checkpoint(2 * rows, half, input.device)
+        values, scales = empty_checkpoint(2 * rows, half, input.device) if keep_input else (None, None)
         out_values, out_scales = empty_checkpoint(rows, half, input.device) if keep_output else (None, None)
         if rows > 1 and ld < cols:                                 # rows that overlap
             x2, ld = x2.contiguous(), cols
         N.launch(input, N.lib().tf24_gelu_glu_forward_checkpoint, x2.data_ptr(), N.dtype_code(input.dtype), ld, rows, cols, out.data_ptr(), half,
-                 values.data_ptr(), scales.data_ptr(), N.ptr(out_values), N.ptr(out_scales))
-        ctx.save_for_backward(values, scales)
+                 N.ptr(values), N.ptr(scales), N.ptr(out_values), N.ptr(out_scales))
+        if keep_input:
+            ctx.save_for_backward(values, scales)
         ctx.shape, ctx.dtype, ctx.device = input.shape, input.dtype, input.device
         if not keep_output:
             return out
@@ -116,7 +117,7 @@ class gelu_glu_checkpoint(autograd.Function):
         if torch.is_grad_enabled():
             raise RuntimeError("a graph of the gradients of gelu_glu_checkpoint is not supported")
         if grad_output is None:
-            return None, None
+            return None, None, None
         values, scales = ctx.saved_tensors
         cols = ctx.shape[-1]
         rows, half = ctx.shape[:-1].numel(), cols // 2
@@ -133,7 +134,7 @@ class gelu_glu_checkpoint(autograd.Function):
         grad_in = torch.empty(ctx.shape, dtype=ctx.dtype, device=values.device)
         N.launch(values, N.lib().tf24_gelu_glu_backward_checkpoint, go.data_ptr(), ld, values.data_ptr(), scales.data_ptr(), N.dtype_code(ctx.dtype), rows, cols,
                  grad_in.data_ptr(), cols)
-        return grad_in, None
+        return grad_in, None, None
 
 
 class GELUglu(torch.nn.Module):

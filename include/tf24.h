@@ -440,9 +440,9 @@ int tf24_checkpoint_encode(const void* x, int dtype, int64_t ld, int64_t rows, i
 int tf24_checkpoint_decode(const void* values, const void* scales, int64_t rows, int64_t cols, void* out, int dtype, int64_t ld, void* stream);
 
 /*
- * GELU-GLU (row-major) whose backward pass reads its input from 8 bits: `forward` writes, besides out, `in` [rows, cols] as a kept matrix of
- * 2 * rows rows and cols / 2 columns (x and gate of a row one after the other), and with out_values and out_scales (both or neither) `out`
- * [rows, cols / 2] as another; `backward` gives the gradient at the kept values.
+ * GELU-GLU (row-major) whose backward pass reads its input from 8 bits: `forward` writes, besides out, with values and scales (both or neither:
+ * no backward pass will follow) `in` [rows, cols] as a kept matrix of 2 * rows rows and cols / 2 columns (x and gate of a row one after the
+ * other), and with out_values and out_scales (both or neither) `out` [rows, cols / 2] as another; `backward` gives the gradient at the kept values.
  */
 int tf24_gelu_glu_forward_checkpoint(const void* in, int dtype, int64_t ld_in, int64_t rows, int64_t cols, void* out, int64_t ld_out, void* values,
                                      void* scales, void* out_values, void* out_scales, void* stream);
