@@ -106,6 +106,13 @@ def checkpoint_activation(x):
     return ActivationCheckpoint._of(values, scales, x.shape, x.dtype)
 
 
+def kept_of_input(given, setting):
+    """What a layer is to keep of its input: the checkpoint that was given to the call, with a setting of its own (or given=True) one to be made where a
+    graph is recorded, or None: the input as it is."""
+    kept = (True if setting else None) if given is None else given
+    return None if kept is True and not torch.is_grad_enabled() else kept
+
+
 def as_checkpoint(x, given):
     """What a layer keeps of its input x: the checkpoint that came with it, or with given=True one made here."""
     if given is True:

@@ -14,7 +14,7 @@ import torch
 import torch.nn.functional as F
 from torch import autograd, nn
 
-from .activation_checkpoint import ActivationCheckpoint, as_checkpoint
+from .activation_checkpoint import ActivationCheckpoint, as_checkpoint, kept_of_input
 from .semi_structured import (SparseSemiStructuredTensor, _dense_times_sparse_t, _mvue_weight_gradient, _spmm, to_sparse_semi_structured,
                               to_sparse_semi_structured_pair, to_sparse_semi_structured_with_row_sums)
 from .transposable_semi_structured import TransposableSparse, transposable_mask_
@@ -140,7 +140,7 @@ class SparseLinearTranspose(nn.Linear):
 
     def forward(self, x, checkpoint=None):
         w = self.weight
-        kept = True if checkpoint is None and self.checkpoint else checkpoint
+        kept = kept_of_input(checkpoint, self.checkpoint)
         if w.mode == 'dense':
             if checkpoint is not None:
                 raise RuntimeError("SparseLinearTranspose: a checkpoint of the input is taken in mode 'sparse' only")

@@ -21,7 +21,7 @@ from torch import autograd, nn
 from torch.amp import custom_bwd, custom_fwd
 
 from . import _native as N
-from .activation_checkpoint import ActivationCheckpoint, as_checkpoint, checkpoint_weight_gradient
+from .activation_checkpoint import ActivationCheckpoint, as_checkpoint, checkpoint_weight_gradient, kept_of_input
 from .dense_ops import MVUE24_approx, soft_threshold24, sparse24
 
 __all__ = ["MyLinear", "my_linear", "SparseLinear", "sparse_linear", "SoftThreshold", "SoftThresholdLinear", "Sparse24"]
@@ -334,7 +334,7 @@ class SoftThresholdLinear(nn.Linear):
                 raise RuntimeError("SoftThresholdLinear: a checkpoint of the input is taken with contiguous GPU tensors under autocast to 16 bits only, and where no "
                                    "mode or transform stands around the call (torch.set_default_device is one)")
             return F.linear(x, self.get_sparse_weights(), bias)
-        kept = True if checkpoint is None and self.checkpoint else checkpoint
+        kept = kept_of_input(checkpoint, self.checkpoint)
         dtype = torch.get_autocast_dtype("cuda")                   # (what autocast does to the arguments of F.linear)
         if (getattr(self.get_sparse_weights, "__func__", None) is SoftThresholdLinear.get_sparse_weights and weight.dtype == torch.float32
                 and weight.is_contiguous() and not weight.is_neg() and weight.shape[1] % 8 == 0 and weight.data_ptr() % 16 == 0

@@ -55,3 +55,30 @@ def test_gated_activation_without_a_graph_keeps_no_input(cuda, rows, half, dtype
     strided[:, 1:-2] = x
     with torch.no_grad():
         assert torch.equal(sparse.gelu_glu_checkpoint.apply(strided[:, 1:-2]), out)
+
+
+@pytest.mark.parametrize("make", ["soft threshold", "2:4"])
+def test_layers_without_a_graph_keep_no_input(cuda, make):
+    """As many allocations as the layer that keeps its input as it is, and the same output."""
+    import sparse
+    if make == "2:4":
+        layer = sparse.SparseLinearTranspose(128, 256, device=cuda, checkpoint=True)
+    else:
+        layer = sparse.SoftThresholdLinear(128, 256, device=cuda, checkpoint=True)
+        layer.init_scale()
+    layer.eval()
+    x = draw(3, 64, 128).to(cuda)
+    with torch.autocast("cuda", dtype=F16):
+        want = layer(x).detach()
+        for mode in (torch.no_grad(), torch.inference_mode()):
+            with mode:
+                layer.checkpoint = False
+                same, fewest = allocations(lambda: layer(x))
+                layer.checkpoint = True
+                out, count = allocations(lambda: layer(x))
+                assert torch.equal(out, want) and torch.equal(same, want) and count == fewest, (mode, count, fewest)
+    # with a graph it is kept
+    saved = []
+    with torch.autograd.graph.saved_tensors_hooks(lambda t: (saved.append(t.dtype), t)[1], lambda t: t), torch.autocast("cuda", dtype=F16):
+        layer(x)
+    assert torch.float8_e4m3fn in saved
