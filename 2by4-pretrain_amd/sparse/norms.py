@@ -274,7 +274,7 @@ def residual_norm(residual, y, gate=None, residual_scale=1.0, *, post_kind=None,
 
 
 def _make(module, name, wanted, cols, value, factory):
-    module.register_parameter(name, nn.Parameter(torch.full((cols,), value, **factory)) if wanted else None)
+    module.register_parameter(name, nn.Parameter(torch.full((cols,), float(value), **factory)) if wanted else None)
 
 
 class BlockNorm(nn.Module):

@@ -8,3 +8,12 @@ def test_a_checkpoint_off_the_gpu_is_not_decoded():
     kept = sparse.ActivationCheckpoint(torch.zeros(4, 64).to(torch.float8_e4m3fn), torch.zeros(4, 2, dtype=torch.uint8), (4, 64), torch.float16)
     with pytest.raises(RuntimeError, match="CUDA"):
         kept.decode()
+
+
+@pytest.mark.parametrize("first", [0, 1, 0.25, torch.tensor(2)])
+@pytest.mark.parametrize("dtype", [None, torch.bfloat16])
+def test_first_values_of_a_learned_gate(first, dtype):
+    """Whole numbers are numbers: zero and one are the usual first values."""
+    import sparse
+    gate = sparse.ResidualNorm(8, gate=first, dtype=dtype).gate
+    assert gate.requires_grad and gate.dtype == (dtype or torch.float32) and gate.tolist() == [float(first)] * 8
