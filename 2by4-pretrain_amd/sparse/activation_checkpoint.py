@@ -108,9 +108,9 @@ def checkpoint_activation(x):
 
 def kept_of_input(given, setting):
     """What a layer is to keep of its input: the checkpoint that was given to the call, with a setting of its own (or given=True) one to be made where a
-    graph is recorded, or None: the input as it is."""
-    kept = (True if setting else None) if given is None else given
-    return None if kept is True and not torch.is_grad_enabled() else kept
+    graph is recorded, or None (given=False, whatever the setting): the input as it is."""
+    kept = bool(setting) if given is None else given
+    return None if kept is False or (kept is True and not torch.is_grad_enabled()) else kept
 
 
 def as_checkpoint(x, given):

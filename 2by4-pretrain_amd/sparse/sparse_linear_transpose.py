@@ -118,7 +118,7 @@ class sparse_linear_transpose(autograd.Function):
 
 class SparseLinearTranspose(nn.Linear):
     """checkpoint=True: in mode 'sparse' the input is kept in 8 bits for the weight's gradient.  forward(x, checkpoint) takes the
-    ActivationCheckpoint of x in float16 that the operator in front made, whatever the layer's own setting."""
+    ActivationCheckpoint of x in float16 that the operator in front made, True or False for this call, whatever the layer's own setting."""
 
     checkpoint = False
 
@@ -142,7 +142,7 @@ class SparseLinearTranspose(nn.Linear):
         w = self.weight
         kept = kept_of_input(checkpoint, self.checkpoint)
         if w.mode == 'dense':
-            if checkpoint is not None:
+            if checkpoint is not None and checkpoint is not False:
                 raise RuntimeError("SparseLinearTranspose: a checkpoint of the input is taken in mode 'sparse' only")
             x = F.linear(x, w, self.bias)
         else:

@@ -304,7 +304,7 @@ def _takes_linear16(x, weight, bias):
 class SoftThresholdLinear(nn.Linear):
     """checkpoint=True: where autocast makes the layer's products 16-bit ones, its input is kept in 8 bits for the weight's gradient
     (which is the one at the kept values).  forward(x, checkpoint) takes the ActivationCheckpoint of x (as autocast casts it) that the operator
-    in front made, whatever the layer's own setting."""
+    in front made, True or False for this call, whatever the layer's own setting."""
 
     checkpoint = False
 
@@ -330,7 +330,7 @@ class SoftThresholdLinear(nn.Linear):
     def forward(self, x, checkpoint=None):
         weight, scale, bias = self.weight, self.scale, self.bias
         if not _takes_linear16(x, weight, bias):
-            if checkpoint is not None:
+            if checkpoint is not None and checkpoint is not False:
                 raise RuntimeError("SoftThresholdLinear: a checkpoint of the input is taken with contiguous GPU tensors under autocast to 16 bits only, and where no "
                                    "mode or transform stands around the call (torch.set_default_device is one)")
             return F.linear(x, self.get_sparse_weights(), bias)

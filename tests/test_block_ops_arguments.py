@@ -17,3 +17,14 @@ def test_first_values_of_a_learned_gate(first, dtype):
     import sparse
     gate = sparse.ResidualNorm(8, gate=first, dtype=dtype).gate
     assert gate.requires_grad and gate.dtype == (dtype or torch.float32) and gate.tolist() == [float(first)] * 8
+
+
+def test_no_checkpoint_of_a_dense_call():
+    """False is no, in mode 'dense' too; True and a checkpoint are refused there."""
+    import sparse
+    layer = sparse.SparseLinearTranspose(16, 8, checkpoint=True)
+    layer.weight.mode = "dense"
+    x = torch.randn(4, 16)
+    assert torch.equal(layer(x, checkpoint=False), torch.nn.functional.linear(x, layer.weight, layer.bias))
+    with pytest.raises(RuntimeError, match="mode 'sparse'"):
+        layer(x, checkpoint=True)

@@ -82,3 +82,26 @@ def test_layers_without_a_graph_keep_no_input(cuda, make):
     with torch.autograd.graph.saved_tensors_hooks(lambda t: (saved.append(t.dtype), t)[1], lambda t: t), torch.autocast("cuda", dtype=F16):
         layer(x)
     assert torch.float8_e4m3fn in saved
+
+
+@pytest.mark.parametrize("make", ["soft threshold", "2:4"])
+def test_no_for_one_call(cuda, make):
+    """checkpoint=False keeps the input of this call as it is, whatever the layer's own setting, True keeps it in 8 bits."""
+    import sparse
+    if make == "2:4":
+        layer = sparse.SparseLinearTranspose(128, 256, device=cuda, checkpoint=True)
+    else:
+        layer = sparse.SoftThresholdLinear(128, 256, device=cuda, checkpoint=True)
+        layer.init_scale()
+    layer.eval()
+    x = draw(4, 64, 128).to(cuda)
+
+    def kept(**kw):
+        saved = []
+        with torch.autograd.graph.saved_tensors_hooks(lambda t: (saved.append(t.dtype), t)[1], lambda t: t), torch.autocast("cuda", dtype=F16):
+            layer(x, **kw)
+        return torch.float8_e4m3fn in saved
+
+    assert [kept(), kept(checkpoint=False), kept(checkpoint=True)] == [True, False, True]
+    layer.checkpoint = False
+    assert [kept(), kept(checkpoint=False), kept(checkpoint=True)] == [False, False, True]
