@@ -11,6 +11,8 @@ SoftThresholdLinear, GELUglu with checkpoint=True); the operators in front of a 
 (block_norm, residual_norm, GELUglu), which saves the pass that reads the input again.  The reference keeps its activations
 as they are.
 """
+import warnings
+
 import torch
 
 from . import _native as N
@@ -111,6 +113,16 @@ def kept_of_input(given, setting):
     graph is recorded, or None (given=False, whatever the setting): the input as it is."""
     kept = bool(setting) if given is None else given
     return None if kept is False or (kept is True and not torch.is_grad_enabled()) else kept
+
+
+def says_that_nothing_is_kept(layer, given, why):
+    """A layer that was asked for it (setting, True or a checkpoint for one call) cannot keep its input in 8 bits: what was asked for this call is
+    refused; what its setting asks for is left out with a warning, where there will be a backward pass."""
+    name = type(layer).__name__
+    if given is not None and given is not False:
+        raise RuntimeError(f"{name}: a checkpoint of the input is taken {why}")
+    if given is None and layer.checkpoint and torch.is_grad_enabled() and layer.weight.requires_grad:
+        warnings.warn(f"{name}: checkpoint=True has no effect on this call, the input is kept as it is: in 8 bits it is kept {why}", stacklevel=3)
 
 
 def as_checkpoint(x, given):

@@ -14,7 +14,7 @@ import torch
 import torch.nn.functional as F
 from torch import autograd, nn
 
-from .activation_checkpoint import ActivationCheckpoint, as_checkpoint, kept_of_input
+from .activation_checkpoint import ActivationCheckpoint, as_checkpoint, kept_of_input, says_that_nothing_is_kept
 from .semi_structured import (SparseSemiStructuredTensor, _dense_times_sparse_t, _mvue_weight_gradient, _spmm, to_sparse_semi_structured,
                               to_sparse_semi_structured_pair, to_sparse_semi_structured_with_row_sums)
 from .transposable_semi_structured import TransposableSparse, transposable_mask_
@@ -142,8 +142,7 @@ class SparseLinearTranspose(nn.Linear):
         w = self.weight
         kept = kept_of_input(checkpoint, self.checkpoint)
         if w.mode == 'dense':
-            if checkpoint is not None and checkpoint is not False:
-                raise RuntimeError("SparseLinearTranspose: a checkpoint of the input is taken in mode 'sparse' only")
+            says_that_nothing_is_kept(self, checkpoint, "in mode 'sparse' only")
             x = F.linear(x, w, self.bias)
         else:
             if w.mask.device != w.device:

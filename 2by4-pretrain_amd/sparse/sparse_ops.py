@@ -21,7 +21,7 @@ from torch import autograd, nn
 from torch.amp import custom_bwd, custom_fwd
 
 from . import _native as N
-from .activation_checkpoint import ActivationCheckpoint, as_checkpoint, checkpoint_weight_gradient, kept_of_input
+from .activation_checkpoint import ActivationCheckpoint, as_checkpoint, checkpoint_weight_gradient, kept_of_input, says_that_nothing_is_kept
 from .dense_ops import MVUE24_approx, soft_threshold24, sparse24
 
 __all__ = ["MyLinear", "my_linear", "SparseLinear", "sparse_linear", "SoftThreshold", "SoftThresholdLinear", "Sparse24"]
@@ -330,9 +330,8 @@ class SoftThresholdLinear(nn.Linear):
     def forward(self, x, checkpoint=None):
         weight, scale, bias = self.weight, self.scale, self.bias
         if not _takes_linear16(x, weight, bias):
-            if checkpoint is not None and checkpoint is not False:
-                raise RuntimeError("SoftThresholdLinear: a checkpoint of the input is taken with contiguous GPU tensors under autocast to 16 bits only, and where no "
-                                   "mode or transform stands around the call (torch.set_default_device is one)")
+            says_that_nothing_is_kept(self, checkpoint, "with contiguous GPU tensors under autocast to 16 bits only, and where no mode or transform stands around "
+                                      "the call (torch.set_default_device is one)")
             return F.linear(x, self.get_sparse_weights(), bias)
         kept = kept_of_input(checkpoint, self.checkpoint)
         dtype = torch.get_autocast_dtype("cuda")                   # (what autocast does to the arguments of F.linear)

@@ -1,4 +1,6 @@
 """What the modules around the layers take and refuse, as far as it needs no GPU."""
+import warnings
+
 import pytest
 import torch
 
@@ -28,3 +30,19 @@ def test_no_checkpoint_of_a_dense_call():
     assert torch.equal(layer(x, checkpoint=False), torch.nn.functional.linear(x, layer.weight, layer.bias))
     with pytest.raises(RuntimeError, match="mode 'sparse'"):
         layer(x, checkpoint=True)
+
+
+def test_a_layer_says_that_its_setting_has_no_effect():
+    import sparse
+    layer = sparse.SparseLinearTranspose(16, 8, checkpoint=True)
+    layer.weight.mode = "dense"
+    x = torch.randn(4, 16)
+    with pytest.warns(UserWarning, match="no effect.*mode 'sparse'"):
+        layer(x)
+    with warnings.catch_warnings():
+        warnings.simplefilter("error")
+        layer(x, checkpoint=False)
+        with torch.no_grad():
+            layer(x)
+        layer.checkpoint = False
+        layer(x)

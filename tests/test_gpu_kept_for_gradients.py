@@ -1,4 +1,6 @@
 """What the operators keep in 8 bits is kept for a backward pass, and only where there will be one."""
+import warnings
+
 import pytest
 import torch
 
@@ -105,3 +107,24 @@ def test_no_for_one_call(cuda, make):
     assert [kept(), kept(checkpoint=False), kept(checkpoint=True)] == [True, False, True]
     layer.checkpoint = False
     assert [kept(), kept(checkpoint=False), kept(checkpoint=True)] == [False, False, True]
+
+
+def test_a_layer_says_that_its_setting_has_no_effect(cuda):
+    """Outside autocast, and for a transposed input, the soft-threshold layer keeps its input as it is, and says so where there will be a backward pass."""
+    import sparse
+    layer = sparse.SoftThresholdLinear(128, 256, device=cuda, checkpoint=True)
+    layer.init_scale()
+    x = draw(5, 64, 128).to(cuda)
+    with pytest.warns(UserWarning, match="no effect.*autocast"):
+        layer(x)
+    with torch.autocast("cuda", dtype=F16), pytest.warns(UserWarning, match="no effect.*contiguous"):
+        layer(draw(6, 128, 64).to(cuda).t())
+    with warnings.catch_warnings():
+        warnings.simplefilter("error")
+        with torch.autocast("cuda", dtype=F16):
+            layer(x)
+        layer(x, checkpoint=False)
+        with torch.no_grad():
+            layer(x)
+    with pytest.raises(RuntimeError, match="autocast"):
+        layer(x, checkpoint=True)
