@@ -285,6 +285,7 @@ extern "C" int tf24_block_norm_forward(const void* x, int64_t ld_x, const void* 
   if (!rows) return TF24_OK;
   if (!x || (y && !out) || (pre_kind && !n) || (!y && (!pre_kind || post_kind || gate || out)) || !values != !scales || (values && !pre_kind))
     return fail(TF24_ERR_ARG, "%s: null pointer, or one that nothing is read from or written to", fn);
+  if (values && too_many_units(rows, cols)) return fail(TF24_ERR_SHAPE, "%s: matrix too large to be kept (%lld x %lld)", fn, (long long)rows, (long long)cols);
   if (ld_x < 0 || ld_y < 0 || ld_gate < 0) return fail(TF24_ERR_STRIDE, "%s: negative leading dimension", fn);
   if (int rc = check_aligned(fn, dtype_size(stream_dtype), {x, out})) return rc;
   if (int rc = check_aligned(fn, dtype_size(block_dtype), {y, n})) return rc;

@@ -40,7 +40,7 @@ checkpoint_decode(const uint8_t* __restrict__ values, const uint8_t* __restrict_
 int check_matrix(const char* fn, int dtype, int64_t ld, int64_t rows, int64_t cols) {
   if (dtype != TF24_F32 && dtype != TF24_F16 && dtype != TF24_BF16) return fail(TF24_ERR_DTYPE, "%s: unsupported dtype %d", fn, dtype);
   if (rows < 0 || cols < 1 || cols > (int64_t)1 << 30) return fail(TF24_ERR_SHAPE, "%s: shape (%lld, %lld) is not supported", fn, (long long)rows, (long long)cols);
-  if (rows > 0x7fffffffLL / (kept_blocks(cols) * kKeptLanes)) return fail(TF24_ERR_SHAPE, "%s: matrix too large (%lld x %lld)", fn, (long long)rows, (long long)cols);
+  if (too_many_units(rows, cols)) return fail(TF24_ERR_SHAPE, "%s: matrix too large (%lld x %lld)", fn, (long long)rows, (long long)cols);
   if (ld < 0) return fail(TF24_ERR_STRIDE, "%s: negative leading dimension", fn);
   return TF24_OK;
 }

@@ -183,6 +183,7 @@ inline UnitRows unit_rows(int64_t cols) {
   while (((uint64_t)1 << l) < d) l++;
   return {d, (uint32_t)((((uint64_t)1 << (31 + l)) / d) + 1), l - 1};         // (d >= 4, so l >= 2)
 }
+inline bool too_many_units(int64_t rows, int64_t cols) { return rows > 0x7fffffffLL / (kept_blocks(cols) * kKeptLanes); }
 __device__ __forceinline__ uint32_t row_of_unit(const UnitRows& r, uint32_t u) { return __umulhi(u, r.multiplier) >> r.shift; }
 
 }  // namespace

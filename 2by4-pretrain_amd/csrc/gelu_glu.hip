@@ -241,7 +241,7 @@ int check_kept(const char* fn, int dtype, int64_t rows, int64_t cols, int64_t ld
   if (dtype != TF24_F32 && dtype != TF24_F16 && dtype != TF24_BF16) return fail(TF24_ERR_DTYPE, "%s: unsupported dtype %d", fn, dtype);
   if (rows < 0 || cols < 2 || cols % 2 || cols > (int64_t)1 << 30)
     return fail(TF24_ERR_SHAPE, "%s: shape (%lld, %lld) is not supported: the last dimension must be even", fn, (long long)rows, (long long)cols);
-  if (rows > 0x7fffffffLL / (kept_blocks(cols / 2) * kKeptLanes)) return fail(TF24_ERR_SHAPE, "%s: tensor too large", fn);
+  if (too_many_units(rows, cols / 2)) return fail(TF24_ERR_SHAPE, "%s: tensor too large", fn);
   if (rows > 1 && (ld_full < cols || ld_half < cols / 2))
     return fail(TF24_ERR_STRIDE, "%s: leading dimensions %lld, %lld too small", fn, (long long)ld_full, (long long)ld_half);
   return TF24_OK;

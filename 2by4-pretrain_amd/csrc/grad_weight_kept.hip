@@ -342,7 +342,7 @@ int64_t pieces_bytes(int64_t tokens, int64_t m, int64_t n) {
 // estimate on the same 120 products: the way taken is 2 % slower than the better one in the mean; 12288 tokens, 1024 x 4096 123 for 118, 2000
 // tokens, 2304 x 768 23.6 for 21.5.)
 bool takes_decoded(int64_t tokens, int64_t m, int64_t n) {
-  if (n % 8 || tokens > (int64_t)1 << 30) return false;
+  if (n % 8 || too_many_units(tokens, n)) return false;
   return 7.5 + dense_weight_grad_us(tokens, m, n) + (double)(tokens * n) * 0.41e-6 < cut(tokens, m, n, (int64_t)1 << 40).us;
 }
 int64_t decoded_bytes(int64_t tokens, int64_t n) { return (tokens * n * 2 + 255) / 256 * 256; }

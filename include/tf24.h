@@ -433,6 +433,7 @@ int tf24_gelu_glu_backward(const void* grad_out, int64_t ld_grad_out, const void
  * finite magnitude of the block lies in (224, 448] scales, and at least 2^-117; values are rounded to nearest even.  Magnitudes over
  * 1.875 * 2^Emax (of `dtype`) are held there, so that the decoded matrix is finite; infinities and NaNs become NaNs.
  * decode writes the values in any of the three types (exact in the type that was encoded, and in F32).
+ * A kept matrix has fewer than 2^31 units of 8 columns (rows * blocks * 4); every call that writes one refuses more.
  * The reference keeps activations as they are; these calls have no counterpart in it.
  */
 int64_t tf24_checkpoint_blocks(int64_t cols);

@@ -46,3 +46,28 @@ def test_a_layer_says_that_its_setting_has_no_effect():
             layer(x)
         layer.checkpoint = False
         layer(x)
+
+
+def test_n_that_could_not_be_read_again_is_not_kept():
+    """A kept matrix has at most 2^31 units of eight columns: what decode refuses, the norm that would write it does too.  (The addresses are made up.)"""
+    from sparse import _native as N
+    lib, at = N.lib(), 0x7f0000001000
+
+    def forward(rows, cols):
+        return lib.tf24_block_norm_forward(at, cols, None, 0, N.BF16, N.BF16, rows, cols, None, N.F32, 0, 1, None, None, None, None, N.F32, 0, N.NORM_RMS, 1.0, 1e-5, None,
+                                           at, None, at, at, None)
+
+    def decode(rows, cols):
+        return lib.tf24_checkpoint_decode(at, at, rows, cols, at, N.BF16, cols, None)
+
+    for rows, cols in ((1 << 20, 16384), (1 << 29, 32), (1 << 29, 1)):
+        assert forward(rows, cols) == decode(rows, cols) == -1 and b"too large" in lib.tf24_last_error()
+
+
+def test_weight_gradient_of_a_kept_matrix_that_is_not_decoded():
+    """A product whose decoded operand would be too large for that pass has the other way, and asks for room for its pieces at most."""
+    from sparse import _native as N
+    need = N.lib().tf24_checkpoint_weight_grad_workspace_bytes
+    tokens = 1 << 21
+    assert need(tokens // 4, 4096, 8192) >= tokens // 4 * 8192 * 2
+    assert need(tokens, 4096, 8192) < tokens * 8192 * 2
