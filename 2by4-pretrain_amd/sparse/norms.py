@@ -245,12 +245,14 @@ def residual_norm(residual, y, gate=None, residual_scale=1.0, *, post_kind=None,
         out = residual_scale * residual + gate * N_post(y)      n = N_pre(out)
 
     residual and y have the same shape (last dimension 1 to 16384); residual is float32, or of y's type; residual_scale is a number.  A kind is None (post: y as it is;
-    pre: no n is formed), "rms" or "layer"; weights and biases [columns].  `gate` is anything that broadcasts to y: a scalar, a channel's [C],
+    pre: no n is formed), "rms" or "layer"; weights and biases [columns].  `gate` is a tensor that broadcasts to y: of one element, a channel's [C],
     a sequence's [B, 1, C], a token's [B, S, C].  Returns out, with a pre_kind (out, n), with checkpoint=True (out, n, ActivationCheckpoint
     of n).  Gradients (once) for residual, y, gate, weights and biases."""
     fn = "residual_norm"
     if not isinstance(y, torch.Tensor):
         raise RuntimeError(f"{fn}: y is {type(y).__name__}, not a tensor")
+    if gate is not None and not isinstance(gate, torch.Tensor):
+        raise RuntimeError(f"{fn}: gate is {type(gate).__name__}, not a tensor")
     if isinstance(residual_scale, torch.Tensor) and residual_scale.requires_grad:
         raise RuntimeError(f"{fn}: residual_scale is a number, no gradient goes to it")
     done = _ordinary(residual, y, gate, post_weight, post_bias, pre_weight, pre_bias, residual_scale, post_kind, pre_kind, eps, 0, checkpoint)

@@ -71,3 +71,11 @@ def test_weight_gradient_of_a_kept_matrix_that_is_not_decoded():
     tokens = 1 << 21
     assert need(tokens // 4, 4096, 8192) >= tokens // 4 * 8192 * 2
     assert need(tokens, 4096, 8192) < tokens * 8192 * 2
+
+
+def test_a_gate_is_a_tensor():
+    import sparse
+    x = torch.zeros(4, 64)
+    for gate in (0.5, 1, [1.0] * 64):
+        with pytest.raises(RuntimeError, match="residual_norm: gate is"):
+            sparse.residual_norm(x, x, gate, pre_kind="rms")
