@@ -22,7 +22,7 @@
 //
 // Measured (kernel time, bytes that it cannot do without): 12288 rows of 768, float32 stream and float16 blocks, both norms and a gate: 26 us = 4.4 TB/s;
 // 8192 rows of 4096 bf16: 53 us = 5.0 TB/s, where a copy of such a size reaches 5.2.  Rows of 1601 bf16, which begin at any even address and end in the middle of a unit:
-// 14.2 us for 3003 of them = 2.7 TB/s: three rows to each of 1001 workgroups.  A row of 4096 by itself 3.4 us: the latency of one load, sums over eight
+// 14.4 us for 3003 of them = 2.7 TB/s: three rows to each of 1001 workgroups.  A row of 4096 by itself 3.4 us: the latency of one load, sums over eight
 // waves and a store.  A lane's parameters are 40 registers, a row as it is loaded 8 to 16; the next row's keep the memory busy while the sums of one
 // wait for each other (the first kernel, which loaded a row when its turn came, took 29.7 and 76.9 us).
 #include "block_norm_rows.hpp"

@@ -3,8 +3,8 @@
 // Four sums over the rows stay in registers (32 of a lane) while a workgroup goes through its piece of the rows: 256 pieces, a workgroup of eight waves on
 // each compute unit, whose next rows are loaded while it computes on these.  More pieces than are at work at once would be a second round, and their
 // partial sums (16 bytes a column and piece) more to write and to add.
-// Measured (kernel time, bytes that it cannot do without): 12288 rows of 768, float32 stream and float16 blocks: 36 us = 4.7 TB/s; 8192 rows of 4096
-// bf16: 84 us = 4.8 TB/s; block_norm_finish 5.0 and 7.0 us, of which the launch is 2.  The first kernels, without loads ahead: 47 and 146 us.
+// Measured (kernel time, bytes that it cannot do without): 12288 rows of 768, float32 stream and float16 blocks: 37 us = 4.6 TB/s; 8192 rows of 4096
+// bf16: 85 us = 4.7 TB/s; block_norm_finish 5.0 and 7.2 us, of which the launch is 2.  The first kernels, without loads ahead: 47 and 146 us.
 #include "block_norm_rows.hpp"
 
 namespace tf24 {

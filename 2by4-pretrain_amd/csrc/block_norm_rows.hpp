@@ -255,7 +255,7 @@ auto with_shape(int64_t cols, F&& f) {
 }
 constexpr int kForwardThreads = 256, kBackwardThreads = 512;
 // What 256 compute units hold at once, so that no part of a round runs by itself: forward four waves a SIMD, backward a workgroup of eight
-// waves a compute unit, two a SIMD (3003 rows of 1601 columns in 1502 workgroups and 259 pieces 56 us both passes, in 1001 and 252 42).
+// waves a compute unit, two a SIMD (3003 rows of 1601 columns in 1502 workgroups and 259 pieces 56 us both passes, in 1001 and 252 43).
 constexpr uint32_t kForwardWaves = 4096, kBackwardPieces = 256;
 
 template <typename F>

@@ -9,7 +9,7 @@
 //
 // The second pair of kernels keeps the input in 8 bits only (checkpoint8.hpp: as a matrix of 2 * rows rows, x and gate of a row one after the
 // other): the forward pass encodes what it reads, and on request what it writes, the backward pass decodes it.  Bound by memory: 12288 x 2 * 4096 float16,
-// 405 MB in each pass, 68 us forward and 70 backward = 5.8 TB/s.
+// 405 MB in each pass, 68 us forward and 70 backward = 5.8 TB/s; forward where nothing is kept 302 MB in 49 us = 6.1 TB/s.
 #include "checkpoint8.hpp"
 
 namespace tf24 {

@@ -5,10 +5,10 @@
 // G [tokens, m] 16-bit as it lies, X [tokens, n] as blocks of e4m3 and their scales.  Two ways, by expected time (takes_decoded):
 //
 // - X is decoded to 16 bits in the workspace and multiplied by the kernels of tf24_grad_weight: large products, of which the pass over X is a few
-//   percent (12288 tokens, 4096 x 1024: 102 us, 99 of them the product; 8192 tokens, 11008 x 4096: 564 of 558).
+//   percent (total, product with the sum of its pieces, decoding: 12288 tokens, 4096 x 1024 106, 98, 7 us; 8192 tokens, 11008 x 4096 594, 576, 16).
 // - One kernel that widens X (exactly: 4 bits of mantissa) on its way through the registers into LDS; products that are small, where the
-//   launch of a pass more shows, and those that its smaller tiles divide better (1003 tokens, 2304 x 768: 12.7 us, 19.8 the other way; 4096 tokens, 2048 x
-//   2048 40.4 and 48.9).  Its loads and its writes to LDS are issued by the waves that multiply, in whose place: a stage of a tile takes 0.55 to
+//   launch of a pass more shows, and those that its smaller tiles divide better (1003 tokens, 2304 x 768: 15.2 us, 23.8 the other way; 4096 tokens, 2048 x
+//   2048 46 and 51).  Its loads and its writes to LDS are issued by the waves that multiply, in whose place: a stage of a tile takes 0.55 to
 //   0.65 us (1.0 PFLOP/s), on one card 0.65, without the writes 0.49, without the loads 0.55.  Tiles of 192 x 192 come to the same rate (8192 tokens,
 //   4096 x 4096 275 us, without writes 206, without loads 232), and writes in both halves of a stage are no better than all in one.
 //
@@ -339,8 +339,7 @@ int64_t pieces_bytes(int64_t tokens, int64_t m, int64_t n) {
   return pieces > 1 ? pieces * (tiles_i * ((n + KeptTile::TILE - 1) / KeptTile::TILE) + tiles_i) * KeptTile::TILE * KeptTile::TILE * 4 : 0;
 }
 // Decoded to the workspace first: 7.5 us for the launch and what the products' estimate leaves out, 0.41 us for a million elements.  (The kernel's
-// estimate on the same 120 products: the way taken is 2 % slower than the better one in the mean; 12288 tokens, 1024 x 4096 123 for 118, 2000
-// tokens, 2304 x 768 23.6 for 21.5.)
+// estimate on the same 120 products: the way taken is 2 % slower than the better one in the mean; 12288 tokens, 1024 x 4096 126 for 121.)
 bool takes_decoded(int64_t tokens, int64_t m, int64_t n) {
   if (n % 8 || too_many_units(tokens, n)) return false;
   return 7.5 + dense_weight_grad_us(tokens, m, n) + (double)(tokens * n) * 0.41e-6 < cut(tokens, m, n, (int64_t)1 << 40).us;

@@ -247,7 +247,8 @@ def residual_norm(residual, y, gate=None, residual_scale=1.0, *, post_kind=None,
     residual and y have the same shape (last dimension 1 to 16384); residual is float32, or of y's type; residual_scale is a number.  A kind is None (post: y as it is;
     pre: no n is formed), "rms" or "layer"; weights and biases [columns].  `gate` is a tensor that broadcasts to y: of one element, a channel's [C],
     a sequence's [B, 1, C], a token's [B, S, C].  Returns out, with a pre_kind (out, n), with checkpoint=True (out, n, ActivationCheckpoint
-    of n).  Gradients (once) for residual, y, gate, weights and biases."""
+    of n).  Gradients (once) for residual, y, gate, weights and biases, where no more than 2^22 gates are shared by rows; their sums take 16 bytes of
+    scratch memory for each column of every such gate."""
     fn = "residual_norm"
     if not isinstance(y, torch.Tensor):
         raise RuntimeError(f"{fn}: y is {type(y).__name__}, not a tensor")

@@ -488,7 +488,8 @@ int tf24_block_norm_forward(const void* x, int64_t ld_x, const void* y, int64_t 
  * Its backward pass: from the gradients of out (NULL: zero) and n, with h = out (residual 0: the x of a call without y) and y as they were and
  * the stats of the forward pass.  Every result may be NULL: grad_x, grad_y (contiguous), the gradients of weights and biases (of param_dtype),
  * grad_gate (of gate_dtype, contiguous).  y is read where there is a norm of it or grad_gate is wanted, h where pre_kind is not NONE.
- *   workspace  for the gradients of parameters and of gates that rows share: tf24_block_norm_backward_workspace_bytes(rows, cols, rows_per_gate or rows)
+ *   workspace  for the gradients of parameters and of gates that rows share: tf24_block_norm_backward_workspace_bytes(rows, cols, rows_per_gate or rows),
+ *              16 bytes for each column of every piece of the rows: 256 pieces, or one and more for each of many gates (of two rows each: 8 bytes an element)
  * Sums over rows are float32 in a piece of the rows and float64 over the pieces, in a fixed order, rounded once.  rows >= 1; up to 2^22 gates that rows
  * share (their gradients: a launch of one workgroup for 32 columns of a gate, or of 32 gates with few rows, has to hold them).
  */
