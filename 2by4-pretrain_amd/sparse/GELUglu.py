@@ -70,23 +70,9 @@ class gelu_glu(autograd.Function):
         return grad_in.view(ctx.shape)
 
 
-class gelu_glu_checkpoint(autograd.Function):
-    """gelu_glu that keeps its input in 8 bits for the backward pass (as in ActivationCheckpoint, x and gate of a row one after the
-    other) and gives the gradient at the kept values: 1.03 bytes an element in place of 2, for an input that nothing else holds.  The
-    output is the same.  apply(input) -> out; apply(input, True) -> (out, values, scales), the last two being out kept in 8 bits.  Any
-    input with a last dimension of an even size; the output is row-major.  Where no graph is recorded nothing is kept of the input."""
-
-    @classmethod
-    def apply(cls, input, keep_output=False):
-        calls = N.torch_calls()
-        if calls is not None and cls is gelu_glu_checkpoint and N.plain_eager():
-            result = calls.gelu_glu_checkpoint(input, keep_output)
-            if result is not None:
-                return result
-        return super().apply(input, keep_output, torch.is_grad_enabled() and input.requires_grad)
-
+class _gelu_glu_checkpoint(autograd.Function):
     @staticmethod
-    def forward(ctx, input, keep_output=False, keep_input=True):
+    def forward(ctx, input, keep_output, keep_input):
         if not input.is_cuda:
             raise RuntimeError("gelu_glu_checkpoint: only CUDA tensors are supported")
         if input.dim() == 0 or input.shape[-1] == 0 or input.shape[-1] % 2:
@@ -135,6 +121,22 @@ class gelu_glu_checkpoint(autograd.Function):
         N.launch(values, N.lib().tf24_gelu_glu_backward_checkpoint, go.data_ptr(), ld, values.data_ptr(), scales.data_ptr(), N.dtype_code(ctx.dtype), rows, cols,
                  grad_in.data_ptr(), cols)
         return grad_in, None, None
+
+
+class gelu_glu_checkpoint:
+    """gelu_glu that keeps its input in 8 bits for the backward pass (as in ActivationCheckpoint, x and gate of a row one after the
+    other) and gives the gradient at the kept values: 1.03 bytes an element in place of 2, for an input that nothing else holds.  The
+    output is the same.  apply(input) -> out; apply(input, True) -> (out, values, scales), the last two being out kept in 8 bits.  Any
+    input with a last dimension of an even size; the output is row-major.  Where no graph is recorded nothing is kept of the input."""
+
+    @staticmethod
+    def apply(input, keep_output=False):
+        calls = N.torch_calls()
+        if calls is not None and N.plain_eager():
+            result = calls.gelu_glu_checkpoint(input, keep_output)
+            if result is not None:
+                return result
+        return _gelu_glu_checkpoint.apply(input, keep_output, torch.is_grad_enabled() and input.requires_grad)
 
 
 class GELUglu(torch.nn.Module):

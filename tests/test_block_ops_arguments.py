@@ -79,3 +79,15 @@ def test_a_gate_is_a_tensor():
     for gate in (0.5, 1, [1.0] * 64):
         with pytest.raises(RuntimeError, match="residual_norm: gate is"):
             sparse.residual_norm(x, x, gate, pre_kind="rms")
+
+
+def test_the_gated_activation_is_called_from_compiled_code(monkeypatch):
+    """Without the module of torch's C++ side as well: what the compiler cannot trace it leaves to Python, whose call says here that there is no GPU."""
+    import sparse
+    from sparse import _native as N
+    for calls in (N.torch_calls(), None):
+        monkeypatch.setattr(N, "_calls", calls)
+        torch._dynamo.reset()
+        with pytest.raises(Exception) as raised:
+            torch.compile(lambda x: sparse.gelu_glu_checkpoint.apply(x), backend="eager")(torch.zeros(2, 8))
+        assert "only CUDA tensors" in str(raised.value), raised.value
