@@ -90,7 +90,8 @@ PyMethodDef methods[] = {
     TF24_METHOD(tf24_mvue_weight_grad), TF24_METHOD(tf24_mvue_weight_grad_workspace_bytes),
     TF24_METHOD(tf24_checkpoint_encode), TF24_METHOD(tf24_checkpoint_decode), TF24_METHOD(tf24_gelu_glu_forward_checkpoint),
     TF24_METHOD(tf24_gelu_glu_backward_checkpoint), TF24_METHOD(tf24_block_norm_forward), TF24_METHOD(tf24_block_norm_backward),
-    TF24_METHOD(tf24_block_norm_backward_workspace_bytes), TF24_METHOD(tf24_checkpoint_weight_grad), TF24_METHOD(tf24_checkpoint_weight_grad_workspace_bytes),
+    TF24_METHOD(tf24_linear_loss_forward), TF24_METHOD(tf24_linear_loss_state_bytes), TF24_METHOD(tf24_linear_loss_forward_workspace_bytes),
+    TF24_METHOD(tf24_linear_loss_backward), TF24_METHOD(tf24_linear_loss_backward_workspace_bytes), TF24_METHOD(tf24_block_norm_backward_workspace_bytes), TF24_METHOD(tf24_checkpoint_weight_grad), TF24_METHOD(tf24_checkpoint_weight_grad_workspace_bytes),
     {nullptr, nullptr, 0, nullptr}};
 PyModuleDef module = {PyModuleDef_HEAD_INIT, "_fastcall", nullptr, -1, methods, nullptr, nullptr, nullptr, nullptr};
 

@@ -1,0 +1,794 @@
+// The loss of a vocabulary head, logits z = x W^T + b of `words` words, without keeping them:
+//
+//   cross entropy   lse - (1 - s) z[target] - s mean(z) + c lse^2             u = z, lse = log sum exp u
+//   distillation    sum_k q_k (log q_k - u[i_k] + lse)                        u = z / temperature, q the teacher's probabilities of its listed words
+//
+// Forward: one product whose tiles leave a maximum and a sum of exponentials per token and 96 words behind, and the logits of the listed
+// words; a small kernel joins them.  Backward: the product once more, P = dloss/dz in 16 bits for a piece of the vocabulary at a time (at most
+// 1 GiB of it), the listed words put right in it, then  dx += P W  and  dW = P^T x.  The product that is formed again is a quarter of the
+// arithmetic of a training step; kept, the logits would be the largest tensor of it.
+//
+// Tokens that do not count (their target is to be ignored, or no word of the teacher's is listed) are left out from the start: the others are
+// brought together, and the products run over those alone, whose number stays on the device.  Nothing of a token that does not count is read.
+//
+// P is rounded to the operands' type as the operand of a matrix instruction: relative to each of its elements, which is what a
+// 16-bit gradient of the logits is rounded to as well.  The gradients of the losses are scaled by a power of two that brings the largest to 2^14
+// (float16) or 1 (bfloat16) and taken back behind the products, so that the small probabilities of a large batch do not vanish in float16.
+// All sums are float32 (the loss over tokens: float64), in an order that the sizes alone decide.
+#include "linear_loss.hpp"
+#include "head_tiles.hpp"
+#include <algorithm>
+#include <cmath>
+
+namespace tf24 {
+namespace {
+
+constexpr float kLog2e = 1.44269504088896340736f, kLn2 = 0.69314718055994530942f;
+constexpr int kMaxEntries = 1024;
+constexpr int64_t kSlopeBytes = (int64_t)1 << 30, kPartialBytes = (int64_t)1 << 29;
+constexpr int kMaxSplits = 64;
+
+// ---------------------------------------------------------------- which tokens count
+// A token's place among those that count, and back; the target of each, -2 one that no word has.
+__global__ void __launch_bounds__(1024)
+count_tokens(const int64_t* __restrict__ targets, int64_t ignore, const int* __restrict__ flags, int tokens, int filled, int64_t words, int* __restrict__ count,
+             int* __restrict__ row_of, int* __restrict__ place_of, int* __restrict__ target, float* __restrict__ loss) {
+  __shared__ int sums[16];
+  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, each = (tokens + 1023) / 1024;
+  const int begin = min(tid * each, tokens), end = min(begin + each, tokens);
+  auto counts = [&](int t) { return targets ? targets[t] != ignore : flags[t] != 0; };
+  int own = 0;
+  for (int t = begin; t < end; t++) own += counts(t);
+  int upto = own;
+#pragma unroll
+  for (int d = 1; d < 64; d *= 2) {
+    const int v = __shfl_up(upto, d);
+    if (lane >= d) upto += v;
+  }
+  if (lane == 63) sums[wave] = upto;
+  __syncthreads();
+  int before = 0, total = 0;
+  for (int w = 0; w < 16; w++) {
+    if (w < wave) before += sums[w];
+    total += sums[w];
+  }
+  int at = before + upto - own;
+  for (int t = begin; t < end; t++) {
+    const bool yes = counts(t);
+    place_of[t] = yes ? at : -1;
+    if (!yes && loss) loss[t] = 0.0f;
+    if (yes) {
+      row_of[at] = t;
+      if (targets) target[at] = targets[t] >= 0 && targets[t] < words ? (int)targets[t] : -2;
+      at++;
+    }
+  }
+  for (int c = total + tid; c < filled; c += 1024) {
+    row_of[c] = -1;
+    if (targets) target[c] = -1;
+  }
+  if (tid == 0) *count = total;
+}
+
+// ---------------------------------------------------------------- the teacher's entries
+// A token counts if one of its entries is used (its word is not negative) and has a logit above -infinity (or NaN).
+template <typename L>
+__global__ void __launch_bounds__(256)
+flag_tokens(const int64_t* __restrict__ indices, int64_t ld_indices, const L* __restrict__ logits, int64_t ld_logits, int tokens, int entries, int* __restrict__ flags) {
+  const int t = blockIdx.x * 4 + (threadIdx.x >> 6), lane = threadIdx.x & 63;
+  if (t >= tokens) return;
+  bool any = false;
+  for (int k = lane; k < entries; k += 64) any = any || (indices[t * ld_indices + k] >= 0 && to_float(logits[t * ld_logits + k]) != -__builtin_inff());
+  any = __any(any);
+  if (lane == 0) flags[t] = any;
+}
+
+// The entries of a token in ascending order of their words (one word listed twice: in the order of the list), the logarithm of the teacher's
+// probability of each, their sum, and where in the list the entries of 96 words begin.  A workgroup of one wave per token.
+template <typename L>
+__global__ void __launch_bounds__(64)
+list_entries(const int64_t* __restrict__ indices, int64_t ld_indices, const L* __restrict__ logits, int64_t ld_logits, const float* __restrict__ teacher_lse,
+             float inv_temperature, int entries, int padded, int64_t words, const int* __restrict__ count, const int* __restrict__ row_of,
+             int* __restrict__ entry_words, float* __restrict__ logq, float* __restrict__ mass, uint32_t* __restrict__ slab_entries, int64_t filled) {
+  __shared__ uint64_t key[kMaxEntries];
+  __shared__ float value[kMaxEntries];
+  const int c = blockIdx.x, lane = threadIdx.x;
+  if (c >= *count) return;
+  const int64_t row = row_of[c];
+  float top = -__builtin_inff();
+  bool bad = false;
+  for (int k = lane; k < padded; k += 64) {
+    uint64_t at = ~0ull;
+    if (k < entries) {
+      const int64_t w = indices[row * ld_indices + k];
+      const float v = to_float(logits[row * ld_logits + k]) * inv_temperature;
+      value[k] = v;
+      if (w >= words) bad = true;
+      else if (w >= 0) {
+        at = (uint64_t)w << 32 | (uint32_t)k;
+        top = fmaxf(top, v);
+      }
+    }
+    key[k] = at;
+  }
+  __syncthreads();
+  for (int size = 2; size <= padded; size *= 2)
+    for (int step = size / 2; step > 0; step /= 2) {
+      for (int n = lane; n < padded / 2; n += 64) {
+        const int i = (n / step) * step * 2 + n % step, j = i + step;
+        const uint64_t a = key[i], b = key[j];
+        if ((a > b) == ((i & size) == 0)) { key[i] = b; key[j] = a; }
+      }
+      __syncthreads();
+    }
+#pragma unroll
+  for (int d = 1; d < 64; d *= 2) top = fmaxf(top, __shfl_xor(top, d));
+  bad = __any(bad);
+  const float from = top == -__builtin_inff() ? 0.0f : top;
+  float lse;
+  if (teacher_lse) lse = teacher_lse[row];
+  else {
+    float s = 0.0f;
+    for (int k = lane; k < entries; k += 64)
+      if (key[k] != ~0ull) s += expf(value[(uint32_t)key[k]] - from);
+#pragma unroll
+    for (int d = 1; d < 64; d *= 2) s += __shfl_xor(s, d);
+    lse = from + logf(s);
+  }
+  float q = 0.0f;
+  for (int k = lane; k < entries; k += 64) {
+    const uint64_t at = key[k];
+    const int64_t to = (int64_t)c * entries + k;
+    const int w = at == ~0ull ? -1 : (int)(at >> 32);
+    entry_words[to] = w;
+    if (w < 0) continue;
+    const float l = value[(uint32_t)at] - lse;
+    logq[to] = l;
+    q += expf(l);
+    const int slab = w / kSlab;
+    if (k == 0 || (int)(key[k - 1] >> 32) / kSlab != slab) {     // the first of its 96 words
+      int low = k, high = entries;                               // low: one of them, high: the first behind them
+      while (high - low > 1) {
+        const int mid = (low + high) / 2;
+        if (key[mid] != ~0ull && (int)(key[mid] >> 32) / kSlab == slab) low = mid;
+        else high = mid;
+      }
+      slab_entries[(int64_t)slab * filled + c] = (uint32_t)k | (uint32_t)(high - k) << 11 | (uint32_t)(w - slab * kSlab) << 22;
+    }
+  }
+#pragma unroll
+  for (int d = 1; d < 64; d *= 2) q += __shfl_xor(q, d);
+  if (lane == 0) mass[c] = bad ? __builtin_nanf("") : q;
+}
+
+// ---------------------------------------------------------------- operands as the products read them
+// Rows of `cols` 16-bit elements, filled up with zeros to `ld_out` (a multiple of 8): row c of the result is row row_of[c] of the source (null: row c),
+// or zeros behind the last of *count, up to a whole tile.
+__global__ void __launch_bounds__(256)
+pack_rows(const uint16_t* __restrict__ in, int64_t ld, int64_t rows, int64_t cols, bool aligned, const int* __restrict__ count, const int* __restrict__ row_of,
+          uint16_t* __restrict__ out, int64_t ld_out) {
+  const int64_t units = ld_out / 8;
+  if (count) rows = (int64_t)token_tiles(*count) * kTile;
+  for (int64_t u = (int64_t)blockIdx.x * 256 + threadIdx.x; u < rows * units; u += (int64_t)gridDim.x * 256) {
+    const int64_t c = u / units, col = (u - c * units) * 8, row = row_of ? row_of[c] : c;
+    int4v v = {0, 0, 0, 0};
+    if (row >= 0 && col < cols) {
+      const uint16_t* at = in + row * ld + col;
+      if (aligned && col + 8 <= cols) v = *reinterpret_cast<const int4v*>(at);
+      else {
+#pragma unroll
+        for (int e = 0; e < 8; e++)
+          if (col + e < cols) v[e >> 1] |= (int)((uint32_t)at[e] << (e & 1) * 16);
+      }
+    }
+    *reinterpret_cast<int4v*>(out + c * ld_out + col) = v;
+  }
+}
+
+// bias in units of log 2, -inf behind the last word; and zeros where the teacher's entries will be listed
+__global__ void __launch_bounds__(256)
+prepare_words(const void* __restrict__ bias, int dtype, int64_t words, int64_t filled, float scale, float* __restrict__ out, uint32_t* __restrict__ clear, int64_t cleared) {
+  const int64_t first = (int64_t)blockIdx.x * 256 + threadIdx.x, step = (int64_t)gridDim.x * 256;
+  for (int64_t i = first; out && i < filled; i += step) {
+    float v = 0.0f;
+    if (i >= words) v = -__builtin_inff();
+    else if (bias) v = (dtype == TF24_F32 ? ((const float*)bias)[i] : dtype == TF24_F16 ? to_float(((const f16_t*)bias)[i]) : to_float(((const bf16_t*)bias)[i])) * scale;
+    out[i] = v;
+  }
+  for (int64_t i = first; i < cleared; i += step) reinterpret_cast<uint4*>(clear)[i] = uint4{0, 0, 0, 0};
+}
+
+// ---------------------------------------------------------------- losses of the tokens
+struct LossTerms { float smoothing, z_loss; int64_t words; int slabs, entries; };
+
+// 2^by tokens of a workgroup, the slabs of each shared out to 256 / 2^by threads
+__global__ void __launch_bounds__(256)
+token_losses(const float2* __restrict__ stats, const float* __restrict__ sums, int64_t filled, LossTerms how, const int* __restrict__ count, const int* __restrict__ row_of,
+             const int* __restrict__ target, const float* __restrict__ picked, const int* __restrict__ entry_words, const float* __restrict__ logq,
+             const float* __restrict__ mass, float* __restrict__ lse2, float* __restrict__ by_place, float* __restrict__ by_token, int by) {
+  __shared__ float ms[256], ss[256], zs[256];
+  const int tid = threadIdx.x, per = 1 << by, share = tid >> by, shares = 256 >> by;
+  const int64_t c = (int64_t)blockIdx.x * per + (tid & (per - 1));
+  const int n = *count;
+  const bool counts = c < n;
+  if ((int64_t)blockIdx.x * per >= (int64_t)token_tiles(n) * kTile) return;
+  float m = -__builtin_inff(), s = 0.0f, z = 0.0f;
+  auto join = [](float& m, float& s, float m2, float s2) {
+    const float top = fmaxf(m, m2), from = top == -__builtin_inff() ? 0.0f : top;
+    s = s * exp2f(m - from) + s2 * exp2f(m2 - from);
+    m = top;
+  };
+  if (counts)
+    for (int i = share; i < how.slabs; i += shares) {
+      const float2 v = stats[(int64_t)i * filled + c];
+      join(m, s, v.x, v.y);
+      if (sums) z += sums[(int64_t)i * filled + c];
+    }
+  ms[tid] = m; ss[tid] = s; zs[tid] = z;
+  __syncthreads();
+  for (int d = shares / 2; d > 0; d /= 2) {
+    if (share < d) {
+      const int other = tid + (d << by);
+      join(ms[tid], ss[tid], ms[other], ss[other]);
+      zs[tid] += zs[other];
+    }
+    __syncthreads();
+  }
+  const float lse = ms[tid & (per - 1)] + log2f(ss[tid & (per - 1)]);
+  const float sum = zs[tid & (per - 1)];
+  __syncthreads();
+  float loss = 0.0f;
+  if (entry_words && counts) {
+    for (int k = share; k < how.entries; k += shares) {
+      const int64_t at = c * how.entries + k;
+      if (entry_words[at] < 0) break;                            // (used ones first)
+      const float l = logq[at], q = expf(l);
+      if (q != 0.0f) loss += q * (l - (picked[at] - lse) * kLn2);
+    }
+  }
+  zs[tid] = loss;
+  __syncthreads();
+  for (int d = shares / 2; d > 0; d /= 2) {
+    if (share < d) zs[tid] += zs[tid + (d << by)];
+    __syncthreads();
+  }
+  if (share) return;
+  lse2[c] = counts ? lse : __builtin_inff();
+  if (!counts) return;
+  if (entry_words) loss = mass[c] != mass[c] ? mass[c] : zs[tid];
+  else {
+    const float y = target[c] < 0 ? __builtin_nanf("") : picked[c], natural = lse * kLn2;
+    loss = (1.0f - how.smoothing) * ((lse - y) * kLn2) + how.z_loss * natural * natural;
+    if (how.smoothing != 0.0f) loss += how.smoothing * ((lse - sum / (float)how.words) * kLn2);
+  }
+  by_place[c] = loss;
+  if (by_token) by_token[row_of[c]] = loss;
+}
+
+__global__ void __launch_bounds__(1024)
+total_loss(const float* __restrict__ by_place, const int* __restrict__ count, bool mean, float* __restrict__ loss) {
+  __shared__ double sums[1024];
+  const int tid = threadIdx.x, n = *count;
+  double v = 0.0;
+  for (int c = tid; c < n; c += 1024) v += (double)by_place[c];
+  sums[tid] = v;
+  __syncthreads();
+  for (int d = 512; d > 0; d /= 2) {
+    if (tid < d) sums[tid] += sums[tid + d];
+    __syncthreads();
+  }
+  if (tid == 0) *loss = (float)(mean ? sums[0] / (double)max(n, 1) : sums[0]);
+}
+
+// ---------------------------------------------------------------- gradient of the logits
+// Per token that counts: P = factor exp2(y - lse2) - level everywhere, less `pull` times the listed probabilities.  All of it is scaled by a power of two.
+// By one workgroup; tokens behind the last get a factor of zero.
+__global__ void __launch_bounds__(1024)
+slope_terms(const float* __restrict__ grad, int reduction, LossTerms how, float inv_temperature, int to_exponent, const int* __restrict__ count,
+            const int* __restrict__ row_of, const int* __restrict__ target, const float* __restrict__ mass, const float* __restrict__ lse2,
+            float2* __restrict__ coef, float* __restrict__ level, float* __restrict__ pull, float* __restrict__ out_scale) {
+  __shared__ float largest[1024];
+  const int tid = threadIdx.x, n = *count, filled = token_tiles(n) * kTile;
+  auto upstream = [&](int c) {
+    const float g = reduction == TF24_REDUCE_NONE ? grad[row_of[c]] : reduction == TF24_REDUCE_MEAN ? grad[0] / (float)n : grad[0];
+    return g * inv_temperature;
+  };
+  auto widened = [&](int c) { return mass ? mass[c] : 1.0f + 2.0f * how.z_loss * (lse2[c] * kLn2); };
+  float top = 0.0f;
+  for (int c = tid; c < n; c += 1024) {
+    const float v = fabsf(upstream(c)) * fmaxf(1.0f, fabsf(widened(c)));
+    if (v < __builtin_inff()) top = fmaxf(top, v);               // (what is not finite is that anyhow)
+  }
+  largest[tid] = top;
+  __syncthreads();
+  for (int d = 512; d > 0; d /= 2) {
+    if (tid < d) largest[tid] = fmaxf(largest[tid], largest[tid + d]);
+    __syncthreads();
+  }
+  int exponent = 0;
+  if (largest[0] > 0.0f) exponent = max(-126, min(126, ilogbf(largest[0]) - to_exponent));
+  const float down = ldexpf(1.0f, -exponent);
+  if (tid == 0) *out_scale = ldexpf(1.0f, exponent);
+  for (int c = tid; c < filled; c += 1024) {
+    float2 v = {__builtin_inff(), 0.0f};
+    float l = 0.0f, p = 0.0f;
+    if (c < n) {
+      const float g = upstream(c) * down;
+      v = float2{lse2[c], g * widened(c)};
+      if (target && target[c] < 0) v.y = __builtin_nanf("");
+      l = g * (how.smoothing / (float)how.words);
+      p = g * (1.0f - how.smoothing);
+    }
+    coef[c] = v; pull[c] = p;
+    if (level) level[c] = l;
+  }
+}
+
+// The listed words of a piece of the vocabulary in P: one thread per token, or per entry of one; of a word listed twice the first does both.
+template <typename T>
+__global__ void __launch_bounds__(256)
+pull_listed(const int* __restrict__ count, const int* __restrict__ listed, const float* __restrict__ picked, const float* __restrict__ logq, int entries,
+            const float2* __restrict__ coef, const float* __restrict__ level, const float* __restrict__ pull, int64_t first_word, int64_t words, T* __restrict__ slope,
+            int64_t ld) {
+  const int64_t at = (int64_t)blockIdx.x * 256 + threadIdx.x, c = at / entries;
+  if (c >= *count) return;
+  const int w = listed[at];
+  if (w < first_word || w >= first_word + words) return;
+  float q = 1.0f;
+  if (logq) {
+    const int k = (int)(at - c * entries);
+    if (k && listed[at - 1] == w) return;
+    q = expf(logq[at]);
+    for (int j = 1; k + j < entries && listed[at + j] == w; j++) q += expf(logq[at + j]);
+  }
+  float v = coef[c].y * exp2f(picked[at] - coef[c].x) - pull[c] * q;
+  if (level) v -= level[c];
+  slope[c * ld + (w - first_word)] = from_float<T>(v);
+}
+
+// dx from the pieces: row by row of x, rows that do not count are zero.  `sum`: where the pieces of the vocabulary before this one were added up (null: there is
+// none), or, out null, where they go on.
+template <typename T>
+__global__ void __launch_bounds__(256)
+join_input(const float* __restrict__ partial, int splits, int64_t filled, int64_t ld, float* __restrict__ sum, bool first, const int* __restrict__ count,
+           const int* __restrict__ place_of, int64_t tokens, int64_t cols, const float* __restrict__ scale, T* __restrict__ out) {
+  const int64_t units = ld / 4, rows = out ? tokens : (int64_t)*count;
+  const float factor = *scale;
+  for (int64_t u = (int64_t)blockIdx.x * 256 + threadIdx.x; u < rows * units; u += (int64_t)gridDim.x * 256) {
+    const int64_t row = u / units, col = (u - row * units) * 4, c = out ? place_of[row] : row;
+    float4v v = {0, 0, 0, 0};
+    if (c >= 0) {
+      for (int s = 0; s < splits; s++) v += *reinterpret_cast<const float4v*>(partial + ((int64_t)s * filled + c) * ld + col);
+      if (!first) v += *reinterpret_cast<const float4v*>(sum + c * ld + col);
+    }
+    if (!out) {
+      *reinterpret_cast<float4v*>(sum + c * ld + col) = v;
+      continue;
+    }
+    T* at = out + row * cols + col;
+    T o[4];
+#pragma unroll
+    for (int e = 0; e < 4; e++) o[e] = from_float<T>(v[e] * factor);
+    if (cols % 4 == 0 && ((uintptr_t)out & 7) == 0) {
+      if (col < cols) *reinterpret_cast<Pack<T, 4>*>(at) = *reinterpret_cast<Pack<T, 4>*>(o);
+    } else {
+#pragma unroll
+      for (int e = 0; e < 4; e++)
+        if (col + e < cols) at[e] = o[e];
+    }
+  }
+}
+
+// dW of a piece of the vocabulary from the pieces of the tokens
+template <typename OutT>
+__global__ void __launch_bounds__(256)
+join_weight(const float* __restrict__ partial, int splits, const int* __restrict__ count, int64_t rows, int64_t ld, int64_t cols, const float* __restrict__ scale,
+            OutT* __restrict__ out) {
+  const int64_t units = ld / 4;
+  const float factor = *scale;
+  const int pieces = min(splits, token_stages(*count));
+  for (int64_t u = (int64_t)blockIdx.x * 256 + threadIdx.x; u < rows * units; u += (int64_t)gridDim.x * 256) {
+    const int64_t row = u / units, col = (u - row * units) * 4;
+    float4v v = {0, 0, 0, 0};
+    for (int s = 0; s < pieces; s++) v += *reinterpret_cast<const float4v*>(partial + ((int64_t)s * rows + row) * ld + col);
+#pragma unroll
+    for (int e = 0; e < 4; e++)
+      if (col + e < cols) out[row * cols + col + e] = from_float<OutT>(v[e] * factor);
+  }
+}
+
+// db: columns of P, in `pieces` of the tokens, then over the pieces
+constexpr int kBiasPieces = 16;
+template <typename T>
+__global__ void __launch_bounds__(256)
+sum_columns(const T* __restrict__ slope, int64_t ld, const int* __restrict__ count, float* __restrict__ sums) {
+  __shared__ float part[8][256];
+  const int n = *count, tid = threadIdx.x, chunk = tid & 31, group = tid >> 5;
+  const int64_t col = (int64_t)blockIdx.x * 256 + chunk * 8;
+  const int begin = (int)((int64_t)blockIdx.y * n / kBiasPieces), end = (int)((int64_t)(blockIdx.y + 1) * n / kBiasPieces);
+  float v[8] = {};
+  if (col < ld)
+    for (int c = begin + group; c < end; c += 8) {
+      Pack<T, 8> p;
+      p.load(slope + c * ld + col);
+#pragma unroll
+      for (int e = 0; e < 8; e++) v[e] += to_float(p.v[e]);
+    }
+#pragma unroll
+  for (int e = 0; e < 8; e++) part[group][chunk * 8 + e] = v[e];
+  __syncthreads();
+  float s = 0.0f;
+#pragma unroll
+  for (int g = 0; g < 8; g++) s += part[g][tid];
+  if ((int64_t)blockIdx.x * 256 + tid < ld) sums[blockIdx.y * ld + (int64_t)blockIdx.x * 256 + tid] = s;
+}
+__global__ void __launch_bounds__(256)
+join_bias(const float* __restrict__ sums, int64_t ld, int64_t words, const float* __restrict__ scale, void* __restrict__ out, int dtype) {
+  const int64_t w = (int64_t)blockIdx.x * 256 + threadIdx.x;
+  if (w >= words) return;
+  float v = 0.0f;
+  for (int p = 0; p < kBiasPieces; p++) v += sums[p * ld + w];
+  v *= *scale;
+  if (dtype == TF24_F32) ((float*)out)[w] = v;
+  else if (dtype == TF24_F16) ((f16_t*)out)[w] = from_float<f16_t>(v);
+  else ((bf16_t*)out)[w] = from_float<bf16_t>(v);
+}
+
+// ---------------------------------------------------------------- buffers
+int64_t up(int64_t v, int64_t to) { return (v + to - 1) / to * to; }
+
+struct Carve {                                                   // parts of a buffer, or (no buffer) how long it has to be
+  uint8_t* base;
+  int64_t used = 0;
+  template <typename P>
+  void operator()(P*& p, int64_t bytes) {
+    p = base ? (P*)(base + used) : nullptr;
+    used += up(bytes, 256);
+  }
+};
+
+// what the forward pass leaves for the backward pass
+struct State {
+  int *count, *row_of, *place_of, *listed;
+  float *lse2, *picked, *logq = nullptr, *mass = nullptr;
+  int64_t bytes;
+};
+State state_of(void* base, int64_t tokens, int64_t entries) {
+  State s;
+  Carve part{(uint8_t*)base};
+  const int64_t filled = up(tokens, kTile), many = filled * std::max<int64_t>(entries, 1);
+  part(s.count, 4);
+  part(s.row_of, filled * 4);
+  part(s.place_of, filled * 4);
+  part(s.lse2, filled * 4);
+  part(s.listed, many * 4);
+  part(s.picked, many * 4);
+  if (entries) {
+    part(s.logq, many * 4);
+    part(s.mass, filled * 4);
+  }
+  s.bytes = part.used;
+  return s;
+}
+
+struct Sizes {
+  int64_t tokens, width, words, entries;                         // entries: of a token, 0: a target
+  int64_t filled, k, slabs, word_tiles;
+  bool pack_weight, smooth;
+};
+Sizes sizes_of(int64_t tokens, int64_t width, int64_t words, int64_t entries, bool smooth, const void* w, int64_t ldw) {
+  Sizes z{tokens, width, words, entries, up(tokens, kTile), up(width, kStageK), 0, (words + kTile - 1) / kTile, false, smooth};
+  z.slabs = z.word_tiles * 2;
+  // rows of whole stages, 16-byte aligned, within reach of 32-bit offsets in a tile
+  z.pack_weight = width % kStageK || ldw % 8 || ldw > (1 << 22) || (uintptr_t)w % 16;
+  return z;
+}
+
+struct Forward {
+  uint16_t *x, *w = nullptr;
+  float *bias, *sums = nullptr, *losses;
+  float2* stats;
+  int* flags = nullptr;
+  uint32_t* slab_entries = nullptr;
+  int64_t bytes;
+};
+Forward forward_of(void* base, const Sizes& z) {
+  Forward f;
+  Carve part{(uint8_t*)base};
+  part(f.x, z.filled * z.k * 2);
+  if (z.pack_weight) part(f.w, z.words * z.k * 2);
+  part(f.bias, z.word_tiles * kTile * 4);
+  part(f.stats, z.slabs * z.filled * 8);
+  if (z.smooth) part(f.sums, z.slabs * z.filled * 4);
+  part(f.losses, z.filled * 4);
+  if (z.entries) {
+    part(f.flags, z.filled * 4);
+    part(f.slab_entries, z.slabs * z.filled * 4);
+  }
+  f.bytes = part.used;
+  return f;
+}
+
+// Pieces of a product's k: the number with the least rounds of the compute units x stages of a piece x 0.87 us + 0.32 us per MB of float32 results
+// (as measured on the dense weight gradient's pieces).
+int splits_of(int64_t tiles, int64_t stages, int64_t result_bytes, bool always_partial, int cus) {
+  int best = 1;
+  double least = 1e30;
+  for (int64_t s = 1; s <= std::min<int64_t>(kMaxSplits, stages); s++) {
+    if (s > 1 && s * result_bytes > kPartialBytes) break;
+    const double us = (double)((tiles * s + cus - 1) / cus) * (double)((stages + s - 1) / s) * 0.87 + (s > 1 || always_partial ? (double)(s * result_bytes) * 0.32e-6 : 0.0);
+    if (us < least) { least = us; best = (int)s; }
+  }
+  return best;
+}
+
+struct Backward {
+  uint16_t *x, *w = nullptr;
+  float *bias, *level = nullptr, *pull, *out_scale, *partial_x = nullptr, *sum_x = nullptr, *partial_w = nullptr, *bias_sums = nullptr;
+  float2* coef;
+  uint8_t* slope;
+  int64_t piece_tiles, pieces, ld, bytes;
+  int splits_x, splits_w;
+};
+Backward backward_of(void* base, const Sizes& z, bool input, bool weight, bool bias) {
+  Backward b;
+  Carve part{(uint8_t*)base};
+  const int cus = compute_units();
+  const int64_t most = std::max<int64_t>(1, kSlopeBytes / (z.filled * 2 * kTile));
+  b.pieces = (z.word_tiles + most - 1) / most;
+  b.piece_tiles = (z.word_tiles + b.pieces - 1) / b.pieces;
+  b.pieces = (z.word_tiles + b.piece_tiles - 1) / b.piece_tiles;
+  b.ld = b.piece_tiles * kTile;
+  const int64_t width_tiles = (z.k + kTile - 1) / kTile;
+  b.splits_x = splits_of(width_tiles * (z.filled / kTile), b.ld / kStageK, z.filled * z.k * 4, true, cus);
+  b.splits_w = splits_of(width_tiles * b.piece_tiles, z.filled / kStageK, b.ld * z.k * 4, false, cus);
+  part(b.x, z.filled * z.k * 2);
+  if (z.pack_weight) part(b.w, z.words * z.k * 2);
+  part(b.bias, z.word_tiles * kTile * 4);
+  part(b.coef, z.filled * 8);
+  if (z.smooth) part(b.level, z.filled * 4);
+  part(b.pull, z.filled * 4);
+  part(b.out_scale, 4);
+  part(b.slope, z.filled * b.ld * 2);
+  if (input) {
+    part(b.partial_x, b.splits_x * z.filled * z.k * 4);
+    if (b.pieces > 1) part(b.sum_x, z.filled * z.k * 4);
+  }
+  if (weight && b.splits_w > 1) part(b.partial_w, b.splits_w * b.ld * z.k * 4);
+  if (bias) part(b.bias_sums, kBiasPieces * b.ld * 4);
+  b.bytes = part.used;
+  return b;
+}
+
+unsigned blocks_for(int64_t items) { return (unsigned)std::max<int64_t>(1, std::min<int64_t>((items + 255) / 256, 4096)); }
+
+int check_head(const char* fn, const void* x, int64_t ldx, const void* w, int64_t ldw, const void* bias, int bias_dtype, int dtype, int64_t tokens, int64_t width,
+               int64_t words, int64_t entries, float smoothing, float z_loss, float inv_temperature, int reduction) {
+  if (dtype != TF24_F16 && dtype != TF24_BF16) return fail(TF24_ERR_DTYPE, "%s: unsupported dtype %d", fn, dtype);
+  if (bias && bias_dtype != TF24_F32 && bias_dtype != TF24_F16 && bias_dtype != TF24_BF16) return fail(TF24_ERR_DTYPE, "%s: unsupported dtype %d of the bias", fn, bias_dtype);
+  if (tokens < 1 || tokens > (1 << 22) || width < 1 || width > (1 << 16) || words < 1 || words > (1 << 22))
+    return fail(TF24_ERR_SHAPE, "%s: %lld tokens of %lld columns against %lld words: 1 to 2^22, 2^16 and 2^22 are supported", fn, (long long)tokens, (long long)width,
+                (long long)words);
+  if (up(tokens, kTile) / kTile * ((words + kTile - 1) / kTile) > (1 << 26))
+    return fail(TF24_ERR_SHAPE, "%s: %lld tokens against %lld words are more than one launch takes", fn, (long long)tokens, (long long)words);
+  if (entries < 0 || entries > kMaxEntries) return fail(TF24_ERR_SHAPE, "%s: %lld entries of a token, at most %d are supported", fn, (long long)entries, kMaxEntries);
+  if (ldx < 0 || ldw < 0) return fail(TF24_ERR_STRIDE, "%s: negative leading dimension", fn);
+  if (!(smoothing >= 0.0f && smoothing <= 1.0f) || !std::isfinite(z_loss) || !(inv_temperature > 0.0f) || !std::isfinite(inv_temperature))
+    return fail(TF24_ERR_ARG, "%s: smoothing %g, z_loss %g or 1 / temperature %g is out of range", fn, smoothing, z_loss, inv_temperature);
+  if (entries && (smoothing != 0.0f || z_loss != 0.0f)) return fail(TF24_ERR_ARG, "%s: smoothing and z_loss go with targets", fn);
+  if (reduction != TF24_REDUCE_MEAN && reduction != TF24_REDUCE_SUM && reduction != TF24_REDUCE_NONE) return fail(TF24_ERR_ARG, "%s: bad reduction %d", fn, reduction);
+  if (!x || !w) return fail(TF24_ERR_ARG, "%s: null pointer", fn);
+  if (int rc = check_aligned(fn, 2, {x, w})) return rc;
+  return bias ? check_aligned(fn, dtype_size(bias_dtype), {bias}) : TF24_OK;
+}
+
+void pack(const void* in, int64_t ld, int64_t rows, int64_t cols, const int* count, const int* row_of, uint16_t* out, int64_t ld_out, hipStream_t s) {
+  hipLaunchKernelGGL(pack_rows, dim3(blocks_for(rows * (ld_out / 8))), dim3(256), 0, s, (const uint16_t*)in, ld, rows, cols, ld % 8 == 0 && (uintptr_t)in % 16 == 0, count, row_of,
+                     out, ld_out);
+}
+
+}  // namespace
+}  // namespace tf24
+
+extern "C" int64_t tf24_linear_loss_state_bytes(int64_t tokens, int64_t entries) {
+  if (tokens < 1 || tokens > (1 << 22) || entries < 0 || entries > tf24::kMaxEntries) return 0;
+  return tf24::state_of(nullptr, tokens, entries).bytes;
+}
+
+extern "C" int64_t tf24_linear_loss_forward_workspace_bytes(int64_t tokens, int64_t width, int64_t words, int64_t entries, int smooth, const void* w, int64_t ldw) {
+  using namespace tf24;
+  if (tokens < 1 || width < 1 || words < 1 || entries < 0) return 0;
+  return forward_of(nullptr, sizes_of(tokens, width, words, entries, smooth != 0, w, ldw)).bytes;
+}
+
+extern "C" int64_t tf24_linear_loss_backward_workspace_bytes(int64_t tokens, int64_t width, int64_t words, int64_t entries, int smooth, const void* w, int64_t ldw, int input,
+                                                             int weight, int bias) {
+  using namespace tf24;
+  if (tokens < 1 || width < 1 || words < 1 || entries < 0) return 0;
+  return backward_of(nullptr, sizes_of(tokens, width, words, entries, smooth != 0, w, ldw), input != 0, weight != 0, bias != 0).bytes;
+}
+
+extern "C" int tf24_linear_loss_forward(const void* x, int64_t ldx, const void* w, int64_t ldw, const void* bias, int bias_dtype, int dtype, int64_t tokens, int64_t width,
+                                        int64_t words, const int64_t* targets, int64_t ignore, const int64_t* indices, int64_t ld_indices, const void* teacher_logits,
+                                        int64_t ld_teacher, int teacher_dtype, const float* teacher_lse, int64_t entries, float smoothing, float z_loss,
+                                        float inv_temperature, int reduction, float* loss, void* state, int64_t state_bytes, void* workspace, int64_t workspace_bytes,
+                                        void* stream) {
+  using namespace tf24;
+  const char* fn = "tf24_linear_loss_forward";
+  if (int rc = check_head(fn, x, ldx, w, ldw, bias, bias_dtype, dtype, tokens, width, words, entries, smoothing, z_loss, inv_temperature, reduction)) return rc;
+  if (entries ? !indices || !teacher_logits || targets : !targets || indices) return fail(TF24_ERR_ARG, "%s: either targets, or entries of a teacher", fn);
+  if (entries && teacher_dtype != TF24_F32 && teacher_dtype != TF24_F16 && teacher_dtype != TF24_BF16)
+    return fail(TF24_ERR_DTYPE, "%s: unsupported dtype %d of the teacher's logits", fn, teacher_dtype);
+  if (entries && (ld_indices < 0 || ld_teacher < 0)) return fail(TF24_ERR_STRIDE, "%s: negative leading dimension", fn);
+  if (!loss || !state || !workspace) return fail(TF24_ERR_ARG, "%s: null pointer", fn);
+  if (int rc = check_aligned(fn, 16, {state, workspace})) return rc;
+  if (int rc = check_aligned(fn, 8, {targets, indices})) return rc;
+  if (int rc = check_aligned(fn, 4, {loss, teacher_lse})) return rc;
+  if (entries) {
+    if (int rc = check_aligned(fn, dtype_size(teacher_dtype), {teacher_logits})) return rc;
+  }
+  const Sizes z = sizes_of(tokens, width, words, entries, smoothing != 0.0f, w, ldw);
+  const State st = state_of(state, tokens, entries);
+  const Forward f = forward_of(workspace, z);
+  if (state_bytes < st.bytes || workspace_bytes < f.bytes)
+    return fail(TF24_ERR_ARG, "%s: %lld and %lld bytes of state and workspace, %lld and %lld are needed", fn, (long long)state_bytes, (long long)workspace_bytes,
+                (long long)st.bytes, (long long)f.bytes);
+  hipStream_t s = (hipStream_t)stream;
+  const float scale = kLog2e * inv_temperature;
+  auto teacher = [&](auto go) {
+    if (teacher_dtype == TF24_F32) go((const float*)teacher_logits);
+    else if (teacher_dtype == TF24_F16) go((const f16_t*)teacher_logits);
+    else go((const bf16_t*)teacher_logits);
+  };
+  if (entries)
+    teacher([&](auto* logits) {
+      hipLaunchKernelGGL(flag_tokens, dim3((unsigned)((tokens + 3) / 4)), dim3(256), 0, s, indices, ld_indices, logits, ld_teacher, (int)tokens, (int)entries, f.flags);
+    });
+  hipLaunchKernelGGL(count_tokens, dim3(1), dim3(1024), 0, s, targets, ignore, f.flags, (int)tokens, (int)z.filled, words, st.count, st.row_of, st.place_of, st.listed,
+                     reduction == TF24_REDUCE_NONE ? loss : nullptr);
+  const bool with_bias = bias || words % kTile;
+  const int64_t cleared = entries ? z.slabs * z.filled / 4 : 0;
+  if (with_bias || entries)
+    hipLaunchKernelGGL(prepare_words, dim3(blocks_for(std::max(with_bias ? z.word_tiles * kTile : 0, cleared))), dim3(256), 0, s, bias, bias_dtype, words, z.word_tiles * kTile, scale,
+                       with_bias ? f.bias : nullptr, f.slab_entries, cleared);
+  if (entries) {
+    int padded = 2;
+    while (padded < entries) padded *= 2;
+    teacher([&](auto* logits) {
+      hipLaunchKernelGGL(list_entries, dim3((unsigned)tokens), dim3(64), 0, s, indices, ld_indices, logits, ld_teacher, teacher_lse, inv_temperature, (int)entries, padded,
+                         words, st.count, st.row_of, st.listed, st.logq, st.mass, f.slab_entries, z.filled);
+    });
+  }
+  pack(x, ldx, z.filled, width, st.count, st.row_of, f.x, z.k, s);
+  if (f.w) pack(w, ldw, words, width, nullptr, nullptr, f.w, z.k, s);
+  HeadProduct p{};
+  p.a = (const uint8_t*)(f.w ? f.w : w); p.lda = (f.w ? z.k : ldw) * 2;
+  p.b = (const uint8_t*)f.x; p.ldb = z.k * 2;
+  p.count = st.count;
+  p.rows_i = words;
+  p.stages = (int)(z.k / kStageK); p.tiles_i = (int)z.word_tiles; p.tiles_j = (int)(z.filled / kTile); p.splits = 1;
+  HeadResult r{};
+  r.scale = scale; r.bias = with_bias ? f.bias : nullptr; r.tokens_ld = z.filled;
+  r.stats = f.stats; r.sums = f.sums; r.picked = st.picked; r.words = words;
+  if (entries) { r.slab_entries = f.slab_entries; r.entry_words = st.listed; r.entries = (int)entries; }
+  else r.target = st.listed;
+  if (int rc = launch_head_product(HEAD_STATS, dtype, z.smooth, false, p, r, stream)) return rc;
+  const int by = tokens <= 64 ? 0 : 4;
+  hipLaunchKernelGGL(token_losses, dim3((unsigned)(z.filled >> by)), dim3(256), 0, s, f.stats, f.sums, z.filled, LossTerms{smoothing, z_loss, words, (int)z.slabs, (int)entries},
+                     st.count, st.row_of, st.listed, st.picked, entries ? st.listed : nullptr, st.logq, st.mass, st.lse2, f.losses,
+                     reduction == TF24_REDUCE_NONE ? loss : nullptr, by);
+  if (reduction != TF24_REDUCE_NONE) hipLaunchKernelGGL(total_loss, dim3(1), dim3(1024), 0, s, f.losses, st.count, reduction == TF24_REDUCE_MEAN, loss);
+  return check_launch(fn);
+}
+
+extern "C" int tf24_linear_loss_backward(const float* grad_loss, const void* x, int64_t ldx, const void* w, int64_t ldw, const void* bias, int bias_dtype, int dtype,
+                                         int64_t tokens, int64_t width, int64_t words, int64_t entries, float smoothing, float z_loss, float inv_temperature,
+                                         int reduction, const void* state, int64_t state_bytes, void* dx, void* dw, int dw_dtype, void* dbias, void* workspace,
+                                         int64_t workspace_bytes, void* stream) {
+  using namespace tf24;
+  const char* fn = "tf24_linear_loss_backward";
+  if (int rc = check_head(fn, x, ldx, w, ldw, bias, bias_dtype, dtype, tokens, width, words, entries, smoothing, z_loss, inv_temperature, reduction)) return rc;
+  if (dw && dw_dtype != dtype && dw_dtype != TF24_F32) return fail(TF24_ERR_DTYPE, "%s: a weight gradient of dtype %d from dtype %d", fn, dw_dtype, dtype);
+  if (!grad_loss || !state || !workspace) return fail(TF24_ERR_ARG, "%s: null pointer", fn);
+  if (dbias && !bias) return fail(TF24_ERR_ARG, "%s: the gradient of a bias that is none", fn);
+  if (int rc = check_aligned(fn, 16, {state, workspace})) return rc;
+  if (int rc = check_aligned(fn, 4, {grad_loss})) return rc;
+  if (int rc = check_aligned(fn, 2, {dx})) return rc;
+  if (dw) {
+    if (int rc = check_aligned(fn, dtype_size(dw_dtype), {dw})) return rc;
+  }
+  if (dbias) {
+    if (int rc = check_aligned(fn, dtype_size(bias_dtype), {dbias})) return rc;
+  }
+  const Sizes z = sizes_of(tokens, width, words, entries, smoothing != 0.0f, w, ldw);
+  const State st = state_of(const_cast<void*>(state), tokens, entries);
+  const Backward b = backward_of(workspace, z, dx != nullptr, dw != nullptr, dbias != nullptr);
+  if (state_bytes < st.bytes || workspace_bytes < b.bytes)
+    return fail(TF24_ERR_ARG, "%s: %lld and %lld bytes of state and workspace, %lld and %lld are needed", fn, (long long)state_bytes, (long long)workspace_bytes,
+                (long long)st.bytes, (long long)b.bytes);
+  if (!dx && !dw && !dbias) return TF24_OK;
+  hipStream_t s = (hipStream_t)stream;
+  const float scale = kLog2e * inv_temperature;
+  const LossTerms how{smoothing, z_loss, words, (int)z.slabs, (int)entries};
+  hipLaunchKernelGGL(slope_terms, dim3(1), dim3(1024), 0, s, grad_loss, reduction, how, inv_temperature, dtype == TF24_F16 ? 14 : 0, st.count, st.row_of,
+                     entries ? nullptr : st.listed, st.mass, st.lse2, b.coef, b.level, b.pull, b.out_scale);
+  const bool with_bias = bias || words % kTile;
+  if (with_bias)
+    hipLaunchKernelGGL(prepare_words, dim3(blocks_for(z.word_tiles * kTile)), dim3(256), 0, s, bias, bias_dtype, words, z.word_tiles * kTile, scale, b.bias, (uint32_t*)nullptr,
+                       (int64_t)0);
+  pack(x, ldx, z.filled, width, st.count, st.row_of, b.x, z.k, s);
+  if (b.w) pack(w, ldw, words, width, nullptr, nullptr, b.w, z.k, s);
+  const uint8_t* w_at = (const uint8_t*)(b.w ? b.w : w);
+  const int64_t w_ld = (b.w ? z.k : ldw) * 2;
+  const int token_tiles_most = (int)(z.filled / kTile), width_tiles = (int)((z.k + kTile - 1) / kTile);
+  for (int64_t piece = 0; piece < b.pieces; piece++) {
+    const int64_t first_tile = piece * b.piece_tiles, tiles = std::min(b.piece_tiles, z.word_tiles - first_tile);
+    const int64_t first = first_tile * kTile, here = std::min(tiles * kTile, words - first);
+    HeadProduct p{};
+    p.a = w_at + first * w_ld; p.lda = w_ld;
+    p.b = (const uint8_t*)b.x; p.ldb = z.k * 2;
+    p.count = st.count;
+    p.rows_i = here;
+    p.stages = (int)(z.k / kStageK); p.tiles_i = (int)tiles; p.tiles_j = token_tiles_most; p.splits = 1;
+    HeadResult r{};
+    r.scale = scale; r.bias = with_bias ? b.bias + first : nullptr; r.tokens_ld = z.filled;
+    r.coef = b.coef; r.level = b.level; r.slope = b.slope; r.ld_slope = b.ld; r.words = here;
+    if (int rc = launch_head_product(HEAD_SLOPE, dtype, z.smooth, false, p, r, stream)) return rc;
+    const int64_t many = std::max<int64_t>(entries, 1);
+    auto put_right = [&](auto* slope) {
+      hipLaunchKernelGGL(pull_listed, dim3((unsigned)((tokens * many + 255) / 256)), dim3(256), 0, s, st.count, st.listed, st.picked, st.logq, (int)many, b.coef,
+                         b.level, b.pull, first, here, slope, b.ld);
+    };
+    if (dtype == TF24_F16) put_right((f16_t*)b.slope);
+    else put_right((bf16_t*)b.slope);
+    if (dx) {
+      HeadProduct q{};
+      q.a = w_at + first * w_ld; q.lda = w_ld;
+      q.b = b.slope; q.ldb = b.ld * 2;
+      q.count = st.count;
+      q.rows_i = z.k; q.rows_k = here;
+      q.stages = (int)((here + kStageK - 1) / kStageK); q.tiles_i = width_tiles; q.tiles_j = token_tiles_most; q.splits = std::min(b.splits_x, q.stages);
+      HeadResult o{};
+      o.partial = b.partial_x; o.rows_j = z.filled; o.ld_out = z.k;
+      if (int rc = launch_head_product(HEAD_INPUT, dtype, false, false, q, o, stream)) return rc;
+      const bool last = piece == b.pieces - 1;
+      auto join = [&](auto* out) {
+        hipLaunchKernelGGL(join_input, dim3(blocks_for(z.filled * z.k / 4)), dim3(256), 0, s, b.partial_x, q.splits, z.filled, z.k, b.sum_x, piece == 0, st.count, st.place_of,
+                           tokens, width, b.out_scale, last ? out : nullptr);
+      };
+      if (dtype == TF24_F16) join((f16_t*)dx);
+      else join((bf16_t*)dx);
+    }
+    if (dw) {
+      HeadProduct q{};
+      q.a = (const uint8_t*)b.x; q.lda = z.k * 2;
+      q.b = b.slope; q.ldb = b.ld * 2;
+      q.count = st.count;
+      q.rows_i = z.k;
+      q.stages = (int)(z.filled / kStageK); q.tiles_i = width_tiles; q.tiles_j = (int)tiles; q.splits = b.splits_w;
+      HeadResult o{};
+      o.out = (uint8_t*)dw + first * width * dtype_size(dw_dtype); o.out_scale = b.out_scale;
+      o.rows_j = here; o.cols_out = width; o.ld_out = width;
+      if (b.partial_w) { o.partial = b.partial_w; o.ld_out = z.k; }
+      if (int rc = launch_head_product(HEAD_WEIGHT, dtype, false, dw_dtype == TF24_F32, q, o, stream)) return rc;
+      if (b.partial_w) {
+        auto join = [&](auto* out) {
+          hipLaunchKernelGGL(join_weight, dim3(blocks_for(here * z.k / 4)), dim3(256), 0, s, b.partial_w, b.splits_w, st.count, here, z.k, width, b.out_scale, out);
+        };
+        if (dw_dtype == TF24_F32) join((float*)o.out);
+        else if (dtype == TF24_F16) join((f16_t*)o.out);
+        else join((bf16_t*)o.out);
+      }
+    }
+    if (dbias) {
+      auto sum = [&](auto* slope) {
+        hipLaunchKernelGGL(sum_columns, dim3((unsigned)((b.ld + 255) / 256), kBiasPieces), dim3(256), 0, s, slope, b.ld, st.count, b.bias_sums);
+      };
+      if (dtype == TF24_F16) sum((const f16_t*)b.slope);
+      else sum((const bf16_t*)b.slope);
+      hipLaunchKernelGGL(join_bias, dim3((unsigned)((here + 255) / 256)), dim3(256), 0, s, b.bias_sums, b.ld, here, b.out_scale,
+                         (void*)((uint8_t*)dbias + first * dtype_size(bias_dtype)), bias_dtype);
+    }
+  }
+  return check_launch(fn);
+}

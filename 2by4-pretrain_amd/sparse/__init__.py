@@ -18,6 +18,7 @@ from .sparse_semi_structured_linear import sparse_semi_structured_linear
 from .GELUglu import GELUglu, gelu_glu, gelu_glu_checkpoint
 from .activation_checkpoint import ActivationCheckpoint, checkpoint_activation, checkpoint_weight_gradient
 from .norms import BlockNorm, ResidualNorm, block_norm, residual_norm
+from .linear_loss import VocabularyLinear, linear_cross_entropy, linear_distillation
 from .sparse_ops import MyLinear, SparseLinear, SoftThreshold, SoftThresholdLinear, Sparse24
 
 __all__ = [
@@ -33,5 +34,6 @@ __all__ = [
     "GELUglu", "gelu_glu", "gelu_glu_checkpoint",
     "ActivationCheckpoint", "checkpoint_activation", "checkpoint_weight_gradient",
     "BlockNorm", "ResidualNorm", "block_norm", "residual_norm",
+    "VocabularyLinear", "linear_cross_entropy", "linear_distillation",
     "MyLinear", "SparseLinear", "SoftThreshold", "SoftThresholdLinear", "Sparse24",
 ]

@@ -20,6 +20,7 @@ PRUNE_MAGNITUDE, PRUNE_MASK, PRUNE_MVUE, PRUNE_MVUE_PACKED, PRUNE_MVUE_SEEDED, P
 ACT_NONE, ACT_RELU, ACT_SILU, ACT_GELU = 0, 1, 2, 3
 BIAS_F32 = 0x100                                   # or-ed to the activation of a product
 NORM_NONE, NORM_RMS, NORM_LAYER = 0, 1, 2
+REDUCE_MEAN, REDUCE_SUM, REDUCE_NONE = 0, 1, 2
 COMPRESSED_CANONICAL, COMPRESSED_PANEL, COMPRESSED_CUTLASS = 0, 1, 2
 
 _DTYPES = {
@@ -84,6 +85,11 @@ _SIGNATURES = {
     "tf24_grad_weight_workspace_bytes": (_i64, [_i64, _i64, _i64]),
     "tf24_linear16_suits": (_i, [_i64, _i64, _i64]),
     "tf24_linear16": (_i, [_p, _i64, _i, _p, _i64, _i, _i64, _i64, _i64, _p, _i64, _p, _p]),
+    "tf24_linear_loss_forward": (_i, [_p, _i64, _p, _i64, _p, _i, _i, _i64, _i64, _i64, _p, _i64, _p, _i64, _p, _i64, _i, _p, _i64, _f, _f, _f, _i, _p, _p, _i64, _p, _i64, _p]),
+    "tf24_linear_loss_state_bytes": (_i64, [_i64, _i64]),
+    "tf24_linear_loss_forward_workspace_bytes": (_i64, [_i64, _i64, _i64, _i64, _i, _p, _i64]),
+    "tf24_linear_loss_backward": (_i, [_p, _p, _i64, _p, _i64, _p, _i, _i, _i64, _i64, _i64, _i64, _f, _f, _f, _i, _p, _i64, _p, _p, _i, _p, _p, _i64, _p]),
+    "tf24_linear_loss_backward_workspace_bytes": (_i64, [_i64, _i64, _i64, _i64, _i, _p, _i64, _i, _i, _i]),
     "tf24_transpose": (_i, [_p, _i, _i64, _i64, _i64, _p, _i64, _p]),
     "tf24_spmm_validate": (_i, [_i, _i64, _i64, _i, _i64, _i64, _i, _i, _i64, _i]),
 }

@@ -533,6 +533,41 @@ int tf24_linear16(const void* w, int64_t ldw, int w_strided, const void* x, int6
 int tf24_linear16_suits(int64_t rows, int64_t k, int64_t tokens);
 
 /*
+ * The loss of a vocabulary head, without keeping its logits: with z = x W^T + b, u = z * inv_temperature and lse = log(sum(exp(u))) of a token
+ *     targets   (1 - smoothing) (lse - z[target]) + smoothing (lse - mean(z)) + z_loss lse^2         (inv_temperature 1)
+ *     entries   sum_k q_k (log q_k - u[index_k] + lse),  q_k = exp(logit_k * inv_temperature - teacher_lse), or the softmax of those listed (teacher_lse NULL)
+ * x [tokens, width] and W [words, width] F16 or BF16, rows contiguous, of any leading dimension; b [words] of any floating type or NULL.
+ *   targets    int64 [tokens]; tokens whose target is `ignore` do not count, one without such a word has a loss of NaN and gives gradients of NaN
+ *   indices    int64 [tokens, entries] with leading dimension ld_indices, teacher_logits likewise (F32, F16 or BF16), teacher_lse float [tokens]; entries 1 to 1024.  An
+ *              entry of a negative word is unused; a token without a used entry above -inf does not count; a word listed twice has both probabilities
+ *   reduction  tf24_reduction: loss float, one number (the mean over tokens that count; of none: 0) or [tokens] (0 for those that do not count)
+ *   state      what the backward pass needs besides the operands: tf24_linear_loss_state_bytes(tokens, entries or 0), 16-byte aligned
+ *   workspace  16-byte aligned, as many bytes as the function below says for the same sizes, `smooth` (smoothing is not 0), w and ldw
+ * Nothing of the rows of x that do not count is read.  Sums in float32, in an order that the sizes alone decide.  The reference has no such
+ * operator: the model that its recipe trains (README.md:56-118) brings its own head and loss.
+ */
+typedef enum { TF24_REDUCE_MEAN = 0, TF24_REDUCE_SUM = 1, TF24_REDUCE_NONE = 2 } tf24_reduction;
+int tf24_linear_loss_forward(const void* x, int64_t ldx, const void* w, int64_t ldw, const void* bias, int bias_dtype, int dtype, int64_t tokens, int64_t width,
+                             int64_t words, const int64_t* targets, int64_t ignore, const int64_t* indices, int64_t ld_indices, const void* teacher_logits,
+                             int64_t ld_teacher, int teacher_dtype, const float* teacher_lse, int64_t entries, float smoothing, float z_loss,
+                             float inv_temperature, int reduction, float* loss, void* state, int64_t state_bytes, void* workspace, int64_t workspace_bytes,
+                             void* stream);
+int64_t tf24_linear_loss_state_bytes(int64_t tokens, int64_t entries);
+int64_t tf24_linear_loss_forward_workspace_bytes(int64_t tokens, int64_t width, int64_t words, int64_t entries, int smooth, const void* w, int64_t ldw);
+/*
+ * Its backward pass, from the gradient of the loss (one float, or [tokens]), the operands as they were and the state.  dx [tokens, width] of the operands' type
+ * (zero rows for tokens that do not count), dw [words, width] of that type or F32, dbias [words] of the bias's; contiguous, each may be NULL.
+ *   workspace  as many bytes as the function below says for the results that are wanted: at most 1 GiB of it for the gradient of the logits, 16-bit, of a piece
+ *              of the vocabulary
+ */
+int tf24_linear_loss_backward(const float* grad_loss, const void* x, int64_t ldx, const void* w, int64_t ldw, const void* bias, int bias_dtype, int dtype,
+                              int64_t tokens, int64_t width, int64_t words, int64_t entries, float smoothing, float z_loss, float inv_temperature,
+                              int reduction, const void* state, int64_t state_bytes, void* dx, void* dw, int dw_dtype, void* dbias, void* workspace,
+                              int64_t workspace_bytes, void* stream);
+int64_t tf24_linear_loss_backward_workspace_bytes(int64_t tokens, int64_t width, int64_t words, int64_t entries, int smooth, const void* w, int64_t ldw, int input,
+                                                  int weight, int bias);
+
+/*
  * out[c, r] = in[r, c] for 2-byte (F16|BF16) and 1-byte (E4M3|E5M2|U8) elements; in [rows, cols] with
  * leading dimension ld_in, out [cols, rows] with ld_out.  No counterpart in the reference (CUTLASS
  * reads either operand layout): it feeds tf24_spmm's fast kernel, which wants an 8-bit dense operand
