@@ -12,8 +12,8 @@
 // brought together, and the products run over those alone, whose number stays on the device.  Nothing of a token that does not count is read.
 //
 // P is rounded to the operands' type as the operand of a matrix instruction: relative to each of its elements, which is what a
-// 16-bit gradient of the logits is rounded to as well.  The gradients of the losses are scaled by a power of two that brings the largest to 2^14
-// (float16) or 1 (bfloat16) and taken back behind the products, so that the small probabilities of a large batch do not vanish in float16.
+// 16-bit gradient of the logits is rounded to as well.  It is formed in units of the largest gradient of a token's loss (float16: of 2^-14 of it), which come
+// back behind the products, so that the small probabilities of a large batch do not vanish in float16.
 // All sums are float32 (the loss over tokens: float64), in an order that the sizes alone decide.
 #include "linear_loss.hpp"
 #include "head_tiles.hpp"
@@ -281,8 +281,9 @@ total_loss(const float* __restrict__ by_place, const int* __restrict__ count, bo
 }
 
 // ---------------------------------------------------------------- gradient of the logits
-// Per token that counts: P = factor exp2(y - lse2) - level everywhere, less `pull` times the listed probabilities.  All of it is scaled by a power of two.
-// By one workgroup; tokens behind the last get a factor of zero.
+// Per token that counts: P = factor exp2(y - lse2) - level everywhere, less `pull` times the listed probabilities, all of it in units of the largest gradient of
+// a token's loss: of a mean P is 1 - p at the target, which rounding to 8 bits moves by 2^-9 where 4/3 of it (1 / 12288 less its power of
+// two) is moved by 2^-8.  By one workgroup; tokens behind the last get a factor of zero.
 __global__ void __launch_bounds__(1024)
 slope_terms(const float* __restrict__ grad, int reduction, LossTerms how, float inv_temperature, int to_exponent, const int* __restrict__ count,
             const int* __restrict__ row_of, const int* __restrict__ target, const float* __restrict__ mass, const float* __restrict__ lse2,
@@ -294,26 +295,32 @@ slope_terms(const float* __restrict__ grad, int reduction, LossTerms how, float 
     return g * inv_temperature;
   };
   auto widened = [&](int c) { return mass ? mass[c] : 1.0f + 2.0f * how.z_loss * (lse2[c] * kLn2); };
-  float top = 0.0f;
-  for (int c = tid; c < n; c += 1024) {
-    const float v = fabsf(upstream(c)) * fmaxf(1.0f, fabsf(widened(c)));
-    if (v < __builtin_inff()) top = fmaxf(top, v);               // (what is not finite is that anyhow)
-  }
-  largest[tid] = top;
-  __syncthreads();
-  for (int d = 512; d > 0; d /= 2) {
-    if (tid < d) largest[tid] = fmaxf(largest[tid], largest[tid + d]);
+  // the largest gradient of a token's loss, and the largest factor of one relative to it (what is not finite is that anyhow)
+  auto most = [&](float v) {
+    largest[tid] = v < __builtin_inff() ? v : 0.0f;
     __syncthreads();
-  }
-  int exponent = 0;
-  if (largest[0] > 0.0f) exponent = max(-126, min(126, ilogbf(largest[0]) - to_exponent));
-  const float down = ldexpf(1.0f, -exponent);
-  if (tid == 0) *out_scale = ldexpf(1.0f, exponent);
+    for (int d = 512; d > 0; d /= 2) {
+      if (tid < d) largest[tid] = fmaxf(largest[tid], largest[tid + d]);
+      __syncthreads();
+    }
+    const float top = largest[0];
+    __syncthreads();
+    return top;
+  };
+  float v = 0.0f;
+  for (int c = tid; c < n; c += 1024) v = fmaxf(v, fabsf(upstream(c)));
+  float unit = most(v);
+  if (unit == 0.0f) unit = 1.0f;
+  v = 0.0f;
+  for (int c = tid; c < n; c += 1024) v = fmaxf(v, fabsf(upstream(c) / unit * widened(c)));
+  v = most(v);
+  unit = ldexpf(unit, (v > 1.0f ? ilogbf(v) + 1 : 0) - to_exponent);
+  if (tid == 0) *out_scale = unit;
   for (int c = tid; c < filled; c += 1024) {
     float2 v = {__builtin_inff(), 0.0f};
     float l = 0.0f, p = 0.0f;
     if (c < n) {
-      const float g = upstream(c) * down;
+      const float g = upstream(c) / unit;
       v = float2{lse2[c], g * widened(c)};
       if (target && target[c] < 0) v.y = __builtin_nanf("");
       l = g * (how.smoothing / (float)how.words);
