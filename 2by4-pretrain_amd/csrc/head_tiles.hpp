@@ -71,6 +71,13 @@ namespace {
 __device__ __forceinline__ int token_stages(int count) { return max(1, (count + kStageK - 1) / kStageK); }
 __device__ __forceinline__ int token_tiles(int count) { return max(1, (count + kTile - 1) / kTile); }
 
+// v * scale as the float32 that it is (one instruction would take it to float16 unrounded, and the float32 result of the same sum another value)
+__device__ __forceinline__ float scaled(float v, float scale) {
+  v *= scale;
+  asm volatile("" : "+v"(v));
+  return v;
+}
+
 typedef short short8v __attribute__((ext_vector_type(8)));
 
 __device__ __forceinline__ float4v mma(f16_t, int4v a, int4v b, float4v c) {
@@ -279,23 +286,23 @@ head_product(const HeadProduct p, const HeadResult r) {
       for (int q = 0; q < 2; q++)
         if (q * 64 + lane < kSlab) bias_lds[q * 64 + lane] = bias_at[q];
       wave_lds_fence();
-#pragma unroll
-      for (int ti = 0; ti < kFrags; ti++) {
-        const float4v add = *reinterpret_cast<const float4v*>(bias_lds + ti * 16 + lq * 4);
-#pragma unroll
-        for (int tj = 0; tj < kFrags; tj++)
-#pragma unroll
-          for (int e = 0; e < 4; e++) acc[ti][tj][e] = __builtin_fmaf(acc[ti][tj][e], r.scale, add[e]);
-      }
     }
+    auto bias_of = [&](int ti) { return *reinterpret_cast<const float4v*>(bias_lds + ti * 16 + lq * 4); };
     if constexpr (KIND == HEAD_STATS) {
       const int64_t slab = now.i0 / kSlab + wi;
       const int base = (int)(slab * kSlab);
 #pragma unroll
       for (int tj = 0; tj < kFrags; tj++) {
+        // (the accumulators are read once: vector instructions reach them through copies alone)
+        float4v y[kFrags];
         float m = -__builtin_inff(), s = 0.0f, sum = 0.0f;
 #pragma unroll
-        for (int ti = 0; ti < kFrags; ti++) m = fmaxf(m, fmaxf(fmaxf(acc[ti][tj][0], acc[ti][tj][1]), fmaxf(acc[ti][tj][2], acc[ti][tj][3])));
+        for (int ti = 0; ti < kFrags; ti++) {
+          const float4v add = bias_of(ti);
+#pragma unroll
+          for (int e = 0; e < 4; e++) y[ti][e] = __builtin_fmaf(acc[ti][tj][e], r.scale, add[e]);
+          m = fmaxf(m, fmaxf(fmaxf(y[ti][0], y[ti][1]), fmaxf(y[ti][2], y[ti][3])));
+        }
         m = fmaxf(m, __shfl_xor(m, 16));
         m = fmaxf(m, __shfl_xor(m, 32));
         const float from = m == -__builtin_inff() ? 0.0f : m;
@@ -303,8 +310,8 @@ head_product(const HeadProduct p, const HeadResult r) {
         for (int ti = 0; ti < kFrags; ti++)
 #pragma unroll
           for (int e = 0; e < 4; e++) {
-            s += __builtin_amdgcn_exp2f(acc[ti][tj][e] - from);
-            if constexpr (SMOOTH) sum += base + ti * 16 + lq * 4 + e < r.words ? acc[ti][tj][e] : 0.0f;
+            s += __builtin_amdgcn_exp2f(y[ti][e] - from);
+            if constexpr (SMOOTH) sum += base + ti * 16 + lq * 4 + e < r.words ? y[ti][e] : 0.0f;
           }
         s += __shfl_xor(s, 16);
         s += __shfl_xor(s, 32);
@@ -324,7 +331,7 @@ head_product(const HeadProduct p, const HeadResult r) {
             for (int ti = 0; ti < kFrags; ti++)
 #pragma unroll
               for (int e = 0; e < 4; e++)
-                if (at == ti * 16 + lq * 4 + e) r.picked[token] = acc[ti][tj][e];
+                if (at == ti * 16 + lq * 4 + e) r.picked[token] = y[ti][e];
           }
         } else {
           // the teacher's entries of these 96 words, four of a token at a time, from the token's row in LDS
@@ -333,7 +340,7 @@ head_product(const HeadProduct p, const HeadResult r) {
             wave_lds_fence();
 #pragma unroll
             for (int ti = 0; ti < kFrags; ti++)
-              *reinterpret_cast<float4v*>(slice + l16 * 384 + ((ti * 4 + lq) ^ ((l16 >> 1) & 7)) * 16) = acc[ti][tj];
+              *reinterpret_cast<float4v*>(slice + l16 * 384 + ((ti * 4 + lq) ^ ((l16 >> 1) & 7)) * 16) = y[ti];
             wave_lds_fence();
             for (int n = lq; n < many; n += 4) {
               const int64_t entry = token * r.entries + first + n;
@@ -349,19 +356,21 @@ head_product(const HeadProduct p, const HeadResult r) {
       for (int tp = 0; tp < kFrags / 2; tp++) {
         if (tp > 0) wave_lds_fence();
 #pragma unroll
-        for (int ti = 0; ti < kFrags; ti++)
+        for (int ti = 0; ti < kFrags; ti++) {
+          const float4v add = bias_of(ti);
 #pragma unroll
           for (int t2 = 0; t2 < 2; t2++) {
             const int tj = tp * 2 + t2;
             T o[4];
 #pragma unroll
             for (int e = 0; e < 4; e++) {
-              float v = coef[tj].y * __builtin_amdgcn_exp2f(acc[ti][tj][e] - coef[tj].x);
+              float v = coef[tj].y * __builtin_amdgcn_exp2f(__builtin_fmaf(acc[ti][tj][e], r.scale, add[e]) - coef[tj].x);
               if constexpr (SMOOTH) v = now.i0 + wi * kSlab + ti * 16 + lq * 4 + e < r.words ? v - level[tj] : 0.0f;
               o[e] = from_float<T>(v);
             }
             *reinterpret_cast<Pack<T, 4>*>(slice + chunk_at(t2 * 16 + l16, ti * 2 + (lq >> 1)) + (lq & 1) * 8) = *reinterpret_cast<Pack<T, 4>*>(o);
           }
+        }
         wave_lds_fence();
 #pragma unroll
         for (int it = 0; it < 6; it++) {
@@ -417,7 +426,7 @@ head_product(const HeadProduct p, const HeadResult r) {
             for (int t2 = 0; t2 < 2; t2++) {
               T o[4];
 #pragma unroll
-              for (int e = 0; e < 4; e++) o[e] = from_float<T>(acc[ti][tp * 2 + t2][e] * scale);
+              for (int e = 0; e < 4; e++) o[e] = from_float<T>(scaled(acc[ti][tp * 2 + t2][e], scale));
               *reinterpret_cast<Pack<T, 4>*>(slice + chunk_at(t2 * 16 + l16, ti * 2 + (lq >> 1)) + (lq & 1) * 8) = *reinterpret_cast<Pack<T, 4>*>(o);
             }
           wave_lds_fence();

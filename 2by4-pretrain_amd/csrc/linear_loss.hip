@@ -400,7 +400,7 @@ join_weight(const float* __restrict__ partial, int splits, const int* __restrict
     for (int s = 0; s < pieces; s++) v += *reinterpret_cast<const float4v*>(partial + ((int64_t)s * rows + row) * ld + col);
 #pragma unroll
     for (int e = 0; e < 4; e++)
-      if (col + e < cols) out[row * cols + col + e] = from_float<OutT>(v[e] * factor);
+      if (col + e < cols) out[row * cols + col + e] = from_float<OutT>(scaled(v[e], factor));
   }
 }
 
