@@ -87,6 +87,16 @@ __device__ __forceinline__ float4v mma(bf16_t, int4v a, int4v b, float4v c) {
   return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, a), __builtin_bit_cast(bf16x8, b), c, 0, 0, 0);
 }
 
+// op over the four lanes l, l + 16, l + 32, l + 48, in each of them: swaps of rows of lanes, where a shuffle would wait for the LDS
+template <typename Op>
+__device__ __forceinline__ float over_quarters(float v, Op op) {
+  const uint32_t bits = __builtin_bit_cast(uint32_t, v);
+  const auto a = __builtin_amdgcn_permlane16_swap(bits, bits, false, false);
+  const uint32_t half = __builtin_bit_cast(uint32_t, op(__builtin_bit_cast(float, (uint32_t)a[0]), __builtin_bit_cast(float, (uint32_t)a[1])));
+  const auto b = __builtin_amdgcn_permlane32_swap(half, half, false, false);
+  return op(__builtin_bit_cast(float, (uint32_t)b[0]), __builtin_bit_cast(float, (uint32_t)b[1]));
+}
+
 template <typename T, typename OutT, int KIND, bool SMOOTH>
 __global__ void __launch_bounds__(kThreads)
 head_product(const HeadProduct p, const HeadResult r) {
@@ -105,70 +115,88 @@ head_product(const HeadProduct p, const HeadResult r) {
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int wi = wave >> 1, wj = wave & 1, l16 = lane & 15, lq = lane >> 4;
 
-  struct Unit { int64_t i0, j0; int split, begin, stages; };
-  auto unit_at = [&](int u) {
-    Unit at;
-    at.split = __builtin_amdgcn_readfirstlane((unsigned)u / (unsigned)ntiles);
-    const int tile = u - at.split * ntiles, group = __builtin_amdgcn_readfirstlane((unsigned)tile / (unsigned)(kRaster * tiles_j)), in_group = tile - group * (kRaster * tiles_j);
-    const int gh = min(kRaster, tiles_i - group * kRaster), col = __builtin_amdgcn_readfirstlane((unsigned)in_group / (unsigned)gh);
-    at.i0 = (int64_t)(group * kRaster + (in_group - col * gh)) * kTile;
-    at.j0 = (int64_t)col * kTile;
-    at.begin = __builtin_amdgcn_readfirstlane((unsigned)(at.split * stages_all) / (unsigned)splits);
-    at.stages = __builtin_amdgcn_readfirstlane((unsigned)((at.split + 1) * stages_all) / (unsigned)splits) - at.begin;
-    return at;
+  // a unit, its place among those of its piece of k, and (few instructions, which nothing covers) the way to the workgroup's next one
+  struct Unit { int number, split, group, in_group; int64_t i0, j0; int begin, stages; };
+  auto locate = [&](Unit& u) {
+    const int gh = min(kRaster, tiles_i - u.group * kRaster);
+    int col = (unsigned)u.in_group / kRaster;
+    if (gh != kRaster) col = __builtin_amdgcn_readfirstlane((unsigned)u.in_group / (unsigned)gh);
+    u.i0 = (int64_t)(u.group * kRaster + (u.in_group - col * gh)) * kTile;
+    u.j0 = (int64_t)col * kTile;
   };
+  auto unit_at = [&](int number) {
+    Unit u;
+    u.number = number;
+    u.split = __builtin_amdgcn_readfirstlane((unsigned)number / (unsigned)ntiles);
+    const int tile = number - u.split * ntiles;
+    u.group = __builtin_amdgcn_readfirstlane((unsigned)tile / (unsigned)(kRaster * tiles_j));
+    u.in_group = tile - u.group * (kRaster * tiles_j);
+    u.begin = __builtin_amdgcn_readfirstlane((unsigned)(u.split * stages_all) / (unsigned)splits);
+    u.stages = __builtin_amdgcn_readfirstlane((unsigned)((u.split + 1) * stages_all) / (unsigned)splits) - u.begin;
+    locate(u);
+    return u;
+  };
+  auto advance = [&](Unit& u) {
+    u.in_group += slots;
+    u.number += slots;
+    if (u.in_group < min(kRaster, tiles_i - u.group * kRaster) * tiles_j) locate(u);
+    else u = unit_at(u.number);
+  };
+  Unit now = unit_at(first_unit);
+  const int units_here = (xcd_end - first_unit + slots - 1) / slots;
 
   // ---- copies: number q of a wave brings 1 KB of an operand's stage, 8 rows of 128 bytes with their 16-byte chunks XOR-swizzled by row,
   // or (k slow) 1 KB of 64 rows of 384, swizzled for the transposing reads below.  Rows and columns past A's last re-read it.
   auto slow_swizzle = [](uint32_t krow) { return (((krow >> 1) & 1) << 2) | (((krow >> 3) & 1) << 1); };
   uint32_t oa[kCopies], ob[kCopies];
-  auto offset_of = [&](bool slow, int q, int64_t ld, int64_t last, int64_t last_k) {        // last: of the tile's 192 (k slow: its last whole chunk of eight)
+  auto offset_of = [&](bool slow, int q, uint32_t ld, uint32_t last, uint32_t last_k) {     // last: of the tile's 192 (k slow: its last whole chunk of eight)
     if (slow) {
       const uint32_t piece = (uint32_t)((wave * kCopies + q) * 64 + lane), krow = piece / (kTile / 8);
-      const int64_t col = min((int64_t)((piece % (kTile / 8)) ^ slow_swizzle(krow)) * 8, last);
-      return (uint32_t)(min((int64_t)krow, last_k) * ld + col * 2);
+      return min(krow, last_k) * ld + min(((piece % (kTile / 8)) ^ slow_swizzle(krow)) * 8, last) * 2;
     }
-    const int row = (wave * kCopies + q) * 8 + (lane >> 3), chunk = (lane & 7) ^ ((row >> 1) & 7);
-    return (uint32_t)(min((int64_t)row, last) * ld + chunk * 16);
+    const uint32_t row = (uint32_t)((wave * kCopies + q) * 8 + (lane >> 3)), chunk = (uint32_t)(lane & 7) ^ ((row >> 1) & 7);
+    return min(row, last) * ld + chunk * 16;
   };
   const uint8_t *a_at, *b_at;
   const int64_t a_step = A_SLOW ? kStageK * p.lda : kRowBytes, b_step = B_SLOW ? kStageK * p.ldb : kRowBytes;
-  int next_unit = first_unit, next_left = 0;
-  bool idle = false;                                             // all copies are made
-  int64_t next_i0 = 0, next_k = 0;
+  Unit next = now;                                               // whose stages are being copied
+  int next_left = 0, units_left = units_here;                    // of its stages, of the units
+  int64_t next_k = 0;
   auto point_a = [&]() {
-    const int64_t last = A_SLOW ? min((int64_t)kTile, p.rows_i - next_i0) - 8 : min((int64_t)kTile, p.rows_i - next_i0) - 1;
-    const int64_t last_k = KIND == HEAD_INPUT ? min((int64_t)kStageK, p.rows_k - next_k) - 1 : kStageK - 1;
+    asm volatile("");                                            // (rarely come by: not to be worked out ahead)
+    const uint32_t last = (uint32_t)min((int64_t)kTile, p.rows_i - next.i0) - (A_SLOW ? 8 : 1);
+    const uint32_t last_k = KIND == HEAD_INPUT ? (uint32_t)min((int64_t)kStageK, p.rows_k - next_k) - 1 : kStageK - 1;
 #pragma unroll
-    for (int q = 0; q < kCopies; q++) oa[q] = offset_of(A_SLOW, q, p.lda, last, last_k);
+    for (int q = 0; q < kCopies; q++) oa[q] = offset_of(A_SLOW, q, (uint32_t)p.lda, last, last_k);
   };
-  auto point_at = [&](int u) {
-    const Unit at = unit_at(u);
-    next_i0 = at.i0; next_k = (int64_t)at.begin * kStageK; next_left = at.stages;
-    a_at = p.a + (A_SLOW ? at.i0 * 2 : at.i0 * p.lda) + at.begin * a_step;
-    b_at = p.b + (B_SLOW ? at.j0 * 2 : at.j0 * p.ldb) + at.begin * b_step;
-    point_a();
+  bool whole = false;                                            // the offsets in A are those of any tile that lies in it
+  auto point_at = [&]() {
+    next_k = (int64_t)next.begin * kStageK; next_left = next.stages;
+    a_at = p.a + (A_SLOW ? next.i0 * 2 : next.i0 * p.lda) + next.begin * a_step;
+    b_at = p.b + (B_SLOW ? next.j0 * 2 : next.j0 * p.ldb) + next.begin * b_step;
+    const bool inside = next.i0 + kTile <= p.rows_i && (KIND != HEAD_INPUT || next_k + kStageK <= p.rows_k);
+    if (!(inside && whole)) point_a();
+    whole = inside;
   };
 #pragma unroll
-  for (int q = 0; q < kCopies; q++) ob[q] = offset_of(B_SLOW, q, p.ldb, kTile, kStageK - 1);
-  point_at(first_unit);
+  for (int q = 0; q < kCopies; q++) ob[q] = offset_of(B_SLOW, q, (uint32_t)p.ldb, kTile, kStageK - 1);
+  point_at();
   const uint32_t smem_at = lds_offset(smem);
   auto copy_one = [&](int q, uint32_t buf) {                     // the wave's copies of B, then those of A
     if (q < kCopies) g2l16(b_at, ob[q], smem_at + buf + kOperand + (uint32_t)(wave * kCopies + q) * 1024);
     else g2l16(a_at, oa[q - kCopies], smem_at + buf + (uint32_t)(wave * kCopies + q - kCopies) * 1024);
   };
   auto copied = [&]() {                                          // to the next stage, of this unit or of the next
-    if (idle) return;
+    if (!units_left) return;
     if (--next_left) {
       a_at += a_step; b_at += b_step;
       if constexpr (KIND == HEAD_INPUT) {
         next_k += kStageK;
-        if (next_k + kStageK > p.rows_k) point_a();              // the last words
+        if (next_k + kStageK > p.rows_k) { point_a(); whole = false; }       // the last words
       }
-    } else {
-      next_unit += slots;
-      if (next_unit < xcd_end) point_at(next_unit);
-      else idle = true;
+    } else if (--units_left) {
+      advance(next);
+      point_at();
     }
   };
   auto copy_stage = [&](uint32_t buf) {
@@ -178,13 +206,6 @@ head_product(const HeadProduct p, const HeadResult r) {
   };
 
   float4v acc[kFrags][kFrags];
-  auto clear = [&]() {
-#pragma unroll
-    for (int ti = 0; ti < kFrags; ti++)
-#pragma unroll
-      for (int tj = 0; tj < kFrags; tj++) acc[ti][tj] = float4v{0, 0, 0, 0};
-  };
-  clear();
 
   // ---- fragments of a step (32 elements of k): lane l takes row l % 16, elements 8 * (l / 16) .. + 7.  k slow: in a group of 16 lanes,
   // lane i receives the halfwords i % 4 of the source lanes 4e + i / 4 (e = 0..3), so source lane s addresses k-row s / 4 (of
@@ -251,7 +272,6 @@ head_product(const HeadProduct p, const HeadResult r) {
   using CA = std::integral_constant<int, 2 * kCopies>;
 
   // ---- what is done with a unit's accumulators.  The buffer `fre` is nobody's then; a wave keeps to the two slices of it that its own next copies go to.
-  Unit now = unit_at(first_unit);
   float bias_at[2] = {0, 0};
   float2 coef[kFrags];
   float level[kFrags];
@@ -278,6 +298,11 @@ head_product(const HeadProduct p, const HeadResult r) {
   };
   auto chunk_at = [](int row, int ch) { return row * 192 + (ch ^ ((row >> 2) & 3)) * 16; };
   auto finish = [&](uint32_t fre) {
+    // (numbers of their own: what is worked out from them, addresses above all, would be kept in registers through the loop over the stages otherwise)
+    int lane = (int)threadIdx.x & 63;
+    asm volatile("" : "+v"(lane));
+    const int l16 = lane & 15, lq = lane >> 4;
+    auto token_of = [&](int tj) { return now.j0 + wj * kSlab + tj * 16 + l16; };
     asm volatile("s_waitcnt vmcnt(0)" ::: "memory");             // the copies in flight: from here on stores count as well
     uint8_t* slice = smem + fre + wave * kSlice;
     float* bias_lds = reinterpret_cast<float*>(smem + fre + kOperand + wave * kSlice);
@@ -291,59 +316,71 @@ head_product(const HeadProduct p, const HeadResult r) {
     if constexpr (KIND == HEAD_STATS) {
       const int64_t slab = now.i0 / kSlab + wi;
       const int base = (int)(slab * kSlab);
+      // (the accumulators are read once: vector instructions reach them through copies alone)
+      float4v y[kFrags][kFrags];
+      float m[kFrags], t[kFrags], s[kFrags], sum[kFrags];
 #pragma unroll
-      for (int tj = 0; tj < kFrags; tj++) {
-        // (the accumulators are read once: vector instructions reach them through copies alone)
-        float4v y[kFrags];
-        float m = -__builtin_inff(), s = 0.0f, sum = 0.0f;
+      for (int tj = 0; tj < kFrags; tj++) { m[tj] = -__builtin_inff(); s[tj] = 0.0f; sum[tj] = 0.0f; }
 #pragma unroll
-        for (int ti = 0; ti < kFrags; ti++) {
-          const float4v add = bias_of(ti);
+      for (int ti = 0; ti < kFrags; ti++) {
+        const float4v add = bias_of(ti);
 #pragma unroll
-          for (int e = 0; e < 4; e++) y[ti][e] = __builtin_fmaf(acc[ti][tj][e], r.scale, add[e]);
-          m = fmaxf(m, fmaxf(fmaxf(y[ti][0], y[ti][1]), fmaxf(y[ti][2], y[ti][3])));
-        }
-        m = fmaxf(m, __shfl_xor(m, 16));
-        m = fmaxf(m, __shfl_xor(m, 32));
-        const float from = m == -__builtin_inff() ? 0.0f : m;
-#pragma unroll
-        for (int ti = 0; ti < kFrags; ti++)
+        for (int tj = 0; tj < kFrags; tj++) {
 #pragma unroll
           for (int e = 0; e < 4; e++) {
-            s += __builtin_amdgcn_exp2f(y[ti][e] - from);
-            if constexpr (SMOOTH) sum += base + ti * 16 + lq * 4 + e < r.words ? y[ti][e] : 0.0f;
+            y[ti][tj][e] = __builtin_fmaf(acc[ti][tj][e], r.scale, add[e]);
+            if constexpr (SMOOTH) sum[tj] += base + ti * 16 + lq * 4 + e < r.words ? y[ti][tj][e] : 0.0f;
           }
-        s += __shfl_xor(s, 16);
-        s += __shfl_xor(s, 32);
-        if constexpr (SMOOTH) {
-          sum += __shfl_xor(sum, 16);
-          sum += __shfl_xor(sum, 32);
+          m[tj] = fmaxf(fmaxf(m[tj], y[ti][tj][0]), y[ti][tj][1]);
+          m[tj] = fmaxf(fmaxf(m[tj], y[ti][tj][2]), y[ti][tj][3]);
         }
+      }
+#pragma unroll
+      for (int tj = 0; tj < kFrags; tj++) {
+        m[tj] = over_quarters(m[tj], [](float a, float b) { return fmaxf(a, b); });
+        t[tj] = m[tj] == -__builtin_inff() ? 0.0f : m[tj];
+      }
+#pragma unroll
+      for (int ti = 0; ti < kFrags; ti++)
+#pragma unroll
+        for (int e = 0; e < 4; e++)
+#pragma unroll
+          for (int tj = 0; tj < kFrags; tj++) s[tj] += __builtin_amdgcn_exp2f(y[ti][tj][e] - t[tj]);
+#pragma unroll
+      for (int tj = 0; tj < kFrags; tj++) {
+        s[tj] = over_quarters(s[tj], [](float a, float b) { return a + b; });
+        if constexpr (SMOOTH) sum[tj] = over_quarters(sum[tj], [](float a, float b) { return a + b; });
         const int64_t token = token_of(tj);
         if (lq == 0) {
-          r.stats[slab * r.tokens_ld + token] = float2{m, s};
-          if constexpr (SMOOTH) r.sums[slab * r.tokens_ld + token] = sum;
+          r.stats[slab * r.tokens_ld + token] = float2{m[tj], s[tj]};
+          if constexpr (SMOOTH) r.sums[slab * r.tokens_ld + token] = sum[tj];
         }
-        if (r.target) {
+      }
+      if (r.target) {
+#pragma unroll
+        for (int tj = 0; tj < kFrags; tj++) {
           const int at = target[tj] - base;
           if (__any(at >= 0 && at < kSlab)) {
 #pragma unroll
             for (int ti = 0; ti < kFrags; ti++)
 #pragma unroll
               for (int e = 0; e < 4; e++)
-                if (at == ti * 16 + lq * 4 + e) r.picked[token] = y[ti][e];
+                if (at == ti * 16 + lq * 4 + e) r.picked[token_of(tj)] = y[ti][tj][e];
           }
-        } else {
-          // the teacher's entries of these 96 words, four of a token at a time, from the token's row in LDS
+        }
+      } else {
+        // the teacher's entries of these 96 words, four of a token at a time, from the token's row in LDS
+#pragma unroll
+        for (int tj = 0; tj < kFrags; tj++) {
           const int many = (int)(listed[tj] >> 11 & 0x7ff), first = (int)(listed[tj] & 0x7ff);
           if (__any(many > 0)) {
             wave_lds_fence();
 #pragma unroll
             for (int ti = 0; ti < kFrags; ti++)
-              *reinterpret_cast<float4v*>(slice + l16 * 384 + ((ti * 4 + lq) ^ ((l16 >> 1) & 7)) * 16) = y[ti];
+              *reinterpret_cast<float4v*>(slice + l16 * 384 + ((ti * 4 + lq) ^ ((l16 >> 1) & 7)) * 16) = y[ti][tj];
             wave_lds_fence();
             for (int n = lq; n < many; n += 4) {
-              const int64_t entry = token * r.entries + first + n;
+              const int64_t entry = token_of(tj) * r.entries + first + n;
               const int at = n ? r.entry_words[entry] - base : (int)(listed[tj] >> 22);
               r.picked[entry] = *reinterpret_cast<const float*>(slice + l16 * 384 + ((at >> 2) ^ ((l16 >> 1) & 7)) * 16 + (at & 3) * 4);
             }
@@ -462,8 +499,12 @@ head_product(const HeadProduct p, const HeadResult r) {
 #pragma unroll
   for (int n = 0; n < READS; n++) read_one(0, n, cur, 0);
   bool landed = false;                                           // the next stage has arrived already
-  for (int unit = first_unit;;) {
+  for (int units = units_here;;) {
     fetch();
+#pragma unroll
+    for (int ti = 0; ti < kFrags; ti++)
+#pragma unroll
+      for (int tj = 0; tj < kFrags; tj++) acc[ti][tj] = float4v{0, 0, 0, 0};
     int left = now.stages;
     do {
       mma_step(0, CA{}, fre, cur, 1);                            // with the copies of the stage behind the next one
@@ -475,11 +516,9 @@ head_product(const HeadProduct p, const HeadResult r) {
       mma_step(1, C0{}, 0, cur, 0);
     } while (--left);
     finish(fre);
-    unit += slots;
-    if (unit >= xcd_end) break;
+    if (!--units) break;
     landed = true;
-    clear();
-    now = unit_at(unit);
+    advance(now);
   }
 }
 
