@@ -2,29 +2,41 @@
 //
 //     C[j, i] = sum_k A(i, k) * B(j, k)
 //
-//   HEAD_STATS  i: words, j: tokens, k: width      A = W, B = x     per token and slab of 96 words: maximum and sum of exponentials of the logits
+//   HEAD_STATS  i: words, j: tokens, k: width      A = W, B = x     per token and slab of words (half a tile): maximum and sum of exponentials of the logits
 //   HEAD_SLOPE  the same product once more, and from it the gradient of the logits, 16-bit, token by token
 //   HEAD_INPUT  i: width, j: tokens, k: words      A = W (k is its slow axis), B = the gradient of the logits
 //   HEAD_WEIGHT i: width, j: words,  k: tokens     A = x, B = the gradient of the logits (k is the slow axis of both)
 //
-// A workgroup of four waves (2 x 2, one per SIMD) computes 192(i) x 192(j) tiles, wave tile 96 x 96 = 6 x 6 V_MFMA_F32_16X16X32 with 144 accumulators.
-// 64 elements of k of both operands are a stage of 48 KB, three of which rotate through the LDS: while one is multiplied the copies of
-// the two behind it are in flight, memory to LDS directly.  A workgroup walks its units (a tile, or a piece of its k) as ONE sequence of stages, so
-// that the copies of the next unit run under the end of this one and under what is done with its accumulators.
+// A workgroup of four waves (2 x 2, one per SIMD) computes 256 x 256 tiles, a wave a quarter of it: 8 x 8 V_MFMA_F32_16X16X32 with 256
+// accumulators.  32 elements of k of both operands are a stage of 32 KB, four of which rotate through the LDS: while one is
+// multiplied, from registers, its successor is read and the copies of the ones behind are in flight, memory to LDS directly.  A workgroup walks its units (a
+// tile, or a piece of its k) as ONE sequence of stages, so that the copies of the next unit run under the end of this one and under what is done
+// with its accumulators; for that there is an LDS area apart, to which what a tile needs of its tokens and words is copied as well.
 // The number of tokens that count lies in device memory: no call waits for it.
 #pragma once
 #include "lds_copies.hpp"
+#include <algorithm>
 #include <type_traits>
 
 namespace tf24 {
 namespace {
 
-constexpr int kTile = 192, kThreads = 256, kWaves = 4, kFrags = 6, kSlab = kTile / 2;
-constexpr int kStageK = 64, kRowBytes = kStageK * 2, kStridedRowBytes = kTile * 2;
-constexpr int kOperand = kTile * kRowBytes, kStage = 2 * kOperand;          // [A | B]
+constexpr int kThreads = 256, kWaves = 4;
+constexpr int F = 8, kTile = 32 * F, kSlab = kTile / 2;                      // fragments of 16 along a side of a wave's quarter, a tile's side, the quarter's
+constexpr int kUnitK = 64, kStageK = 32;                                    // k is a multiple of kUnitK: two stages
+constexpr int kRowBytes = kStageK * 2, kSlowRowBytes = kTile * 2, kOperand = kTile * kRowBytes, kStage = 2 * kOperand, kRing = 4;
 constexpr int kCopies = kOperand / 1024 / kWaves;                           // 1 KB copies per wave and operand of a stage
+constexpr int kOverread = 1024;                                             // what is copied for a tile's tokens or words is 1 KB of each kind
 constexpr int kRaster = 8;                                                  // tiles along i of a group
-constexpr int kSlice = kOperand / kWaves;                                   // a wave's part of a stage's operand: where its own copies go
+// a wave's own LDS: 4 KB of results, then 1 KB each of the words' bias and what the tokens bring
+constexpr int kLds = 160 * 1024, kScratch = (kLds - kRing * kStage) / kWaves, kBiasAt = 4096, kTokensAt = 5120, kLevelAt = 6144;
+static_assert(kCopies * 1024 * kWaves == kOperand && kScratch >= kLevelAt + 1024, "a stage's copies divide among the waves");
+
+// 16-byte chunks of a row of 64 bytes are XOR-swizzled for reads of 16 bytes a lane, which go by lanes 0-3, 12-15, 20-23 and 24-27, then the
+// other 16 of the first 32, and so on: each such group touches every bank once ((row >> 2) & 3, which suits 16 lanes in a row, took twice the cycles)
+__device__ __forceinline__ uint32_t swizzle(uint32_t row) { return (0u - (row >> 2)) & 3; }
+// those of a k-row so that transposing reads do
+__device__ __forceinline__ uint32_t slow_swizzle(uint32_t krow) { return ((krow & 3) << 2) | (((krow >> 3) & 1) << 1); }
 
 enum { HEAD_STATS, HEAD_SLOPE, HEAD_INPUT, HEAD_WEIGHT };
 
@@ -35,15 +47,17 @@ struct HeadProduct {
   int64_t lda, ldb;                  // bytes; B's rows (and, k slow, columns) are filled up to whole tiles
   const int* count;                  // tokens that count
   int64_t rows_i, rows_k;            // rows of A; HEAD_INPUT: words, A has none beyond (B holds zeros there)
-  int stages, tiles_i, tiles_j, splits;    // upper bounds where the tokens that count decide
+  int stages, tiles_i, tiles_j;      // stages of kUnitK; upper bounds where the tokens that count decide
+  int groups, most;                  // HEAD_INPUT, HEAD_WEIGHT: workgroups, and tiles' pieces that there is room for
 };
 
 // What becomes of a tile
 struct HeadResult {
   // logits: y = acc * scale + bias (in units of log 2)
   float scale;
-  const float* bias;                 // [words, filled up with -inf to whole tiles] or null: none, and whole tiles
+  const float* bias;                 // [words, filled up with -inf to whole tiles] or null: none
   int64_t tokens_ld;                 // tokens, filled up to whole tiles
+  int64_t words;                     // of the vocabulary, or this piece of it
   // HEAD_STATS
   float2* stats;                     // [slab][token] maximum, sum
   float* sums;                       // SMOOTH: [slab][token] sum of y
@@ -57,19 +71,35 @@ struct HeadResult {
   const float* level;                // SMOOTH: [token] what is subtracted everywhere
   void* slope;
   int64_t ld_slope;
-  int64_t words;                     // of this piece of the vocabulary
   // HEAD_INPUT, HEAD_WEIGHT
-  float* partial;                    // [split][j][ld_out] or null
+  float* partial;                    // [piece][tile of the rest][kTile^2], as the accumulators lie
+  float* sum;                        // [tile][kTile^2]: what the pieces of the vocabulary before this one gave (add), and where it goes on (not last)
+  bool add, last;
   const float* out_scale;            // one number
-  void* out;                         // [j][ld_out]
-  int64_t rows_j, cols_out, ld_out;  // rows and columns that are stored
+  void* out;                         // [row][cols_out]: row row_of[j], or j
+  const int* row_of;
+  int64_t rows_j, cols_out;          // WEIGHT: rows; columns that are stored
 };
 
 namespace {
 
-// tokens in stages, of a product summed over tokens, and pieces that it is cut into
-__device__ __forceinline__ int token_stages(int count) { return max(1, (count + kStageK - 1) / kStageK); }
+__device__ __forceinline__ int token_stages(int count) { return max(1, (count + kUnitK - 1) / kUnitK); }
 __device__ __forceinline__ int token_tiles(int count) { return max(1, (count + kTile - 1) / kTile); }
+
+// How the tiles of a product with a long k go to `groups` workgroups: as many as fill whole rounds each in one piece, the rest cut along k into as many pieces as
+// cost least, in stages of kUnitK: rounds x stages of a piece, and for each piece of a tile 0.09 of one (256 KB written and read again), 4 for the pass that joins
+// them.  12288 tokens, 50304 x 768 bf16: see linear_loss.hip.
+struct Share { int whole, rest, pieces; };
+__host__ __device__ inline Share share_out(int tiles, int stages, int groups, int most) {
+  Share s{tiles / groups * groups, tiles % groups, 1};
+  int least = stages * 256;
+  for (int rounds = 1; rounds <= 4 && s.rest; rounds++) {        // (of the numbers of pieces that fit into so many rounds the largest)
+    const int p = min(min(rounds * groups / s.rest, stages), most / s.rest);
+    const int cost = p > 1 ? (rounds * ((stages + p - 1) / p) + 4) * 256 + s.rest * p * 23 : least;
+    if (cost < least) { least = cost; s.pieces = p; }
+  }
+  return s;
+}
 
 // v * scale as the float32 that it is (one instruction would take it to float16 unrounded, and the float32 result of the same sum another value)
 __device__ __forceinline__ float scaled(float v, float scale) {
@@ -77,8 +107,6 @@ __device__ __forceinline__ float scaled(float v, float scale) {
   asm volatile("" : "+v"(v));
   return v;
 }
-
-typedef short short8v __attribute__((ext_vector_type(8)));
 
 __device__ __forceinline__ float4v mma(f16_t, int4v a, int4v b, float4v c) {
   return __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(half8, a), __builtin_bit_cast(half8, b), c, 0, 0, 0);
@@ -101,22 +129,25 @@ template <typename T, typename OutT, int KIND, bool SMOOTH>
 __global__ void __launch_bounds__(kThreads)
 head_product(const HeadProduct p, const HeadResult r) {
   constexpr bool A_SLOW = KIND >= HEAD_INPUT, B_SLOW = KIND == HEAD_WEIGHT, LOGITS = KIND <= HEAD_SLOPE;
-  __shared__ __attribute__((aligned(1024))) uint8_t smem[3 * kStage];
+  __shared__ __attribute__((aligned(1024))) uint8_t smem[kLds];
   const int count = __builtin_amdgcn_readfirstlane(*p.count);
-  const int tiles_i = p.tiles_i, tiles_j = B_SLOW ? p.tiles_j : token_tiles(count);
-  const int stages_all = B_SLOW ? token_stages(count) : p.stages, splits = min(p.splits, stages_all);
-  const int ntiles = tiles_i * tiles_j, nunits = ntiles * splits;
-  // workgroup ids are dealt to the 8 XCDs round-robin: each XCD takes a run of units in a raster of groups of kRaster rows of tiles,
+  const int tiles_i = p.tiles_i, tiles_j = B_SLOW ? p.tiles_j : token_tiles(count), ntiles = tiles_i * tiles_j;
+  const int stages_all = B_SLOW ? token_stages(count) : p.stages;
+  // units: whole tiles (LOGITS: none, all of them are the rest, in one piece), then the pieces of the rest
+  const Share share = LOGITS ? Share{0, ntiles, 1} : share_out(ntiles, stages_all, p.groups, p.most);
+  const int whole = __builtin_amdgcn_readfirstlane(share.whole), rest = __builtin_amdgcn_readfirstlane(share.rest), pieces = __builtin_amdgcn_readfirstlane(share.pieces);
+  // workgroup ids are dealt to the 8 XCDs round-robin: each XCD takes a run of either kind of units, in a raster of groups of kRaster rows of tiles,
   // its workgroup number s the s-th of them and every `slots`-th after it
-  const int per_xcd = (nunits + 7) / 8, slots = (int)(gridDim.x >> 3);
-  const int xcd = (int)(blockIdx.x & 7), xcd_end = min((xcd + 1) * per_xcd, nunits);
-  const int first_unit = xcd * per_xcd + (int)(blockIdx.x >> 3);
-  if (first_unit >= xcd_end) return;
+  const int slots = (int)(gridDim.x >> 3), xcd = (int)(blockIdx.x & 7), slot = (int)(blockIdx.x >> 3);
+  const int rounds = LOGITS ? 0 : __builtin_amdgcn_readfirstlane((unsigned)whole / (unsigned)(8 * slots));
+  const int run = (rest * pieces + 7) / 8, first = xcd * run + slot, end = min((xcd + 1) * run, rest * pieces);
+  const int units_here = rounds + (first < end ? (end - first + slots - 1) / slots : 0);
+  if (!units_here) return;
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int wi = wave >> 1, wj = wave & 1, l16 = lane & 15, lq = lane >> 4;
 
-  // a unit, its place among those of its piece of k, and (few instructions, which nothing covers) the way to the workgroup's next one
-  struct Unit { int number, split, group, in_group; int64_t i0, j0; int begin, stages; };
+  // The workgroup's m-th unit, its place in its group, and (few instructions, which nothing covers) the way to the next one
+  struct Unit { int m, tile, piece, group, in_group; int64_t i0, j0; int begin, stages; };
   auto locate = [&](Unit& u) {
     const int gh = min(kRaster, tiles_i - u.group * kRaster);
     int col = (unsigned)u.in_group / kRaster;
@@ -124,37 +155,43 @@ head_product(const HeadProduct p, const HeadResult r) {
     u.i0 = (int64_t)(u.group * kRaster + (u.in_group - col * gh)) * kTile;
     u.j0 = (int64_t)col * kTile;
   };
-  auto unit_at = [&](int number) {
+  auto unit_at = [&](int m) {
     Unit u;
-    u.number = number;
-    u.split = __builtin_amdgcn_readfirstlane((unsigned)number / (unsigned)ntiles);
-    const int tile = number - u.split * ntiles;
-    u.group = __builtin_amdgcn_readfirstlane((unsigned)tile / (unsigned)(kRaster * tiles_j));
-    u.in_group = tile - u.group * (kRaster * tiles_j);
-    u.begin = __builtin_amdgcn_readfirstlane((unsigned)(u.split * stages_all) / (unsigned)splits);
-    u.stages = __builtin_amdgcn_readfirstlane((unsigned)((u.split + 1) * stages_all) / (unsigned)splits) - u.begin;
+    u.m = m; u.piece = 0; u.begin = 0; u.stages = stages_all;
+    if (m < rounds) u.tile = xcd * (whole >> 3) + slot + m * slots;
+    else {
+      const int number = first + (m - rounds) * slots;
+      u.tile = whole + number;
+      if (!LOGITS && pieces > 1) {
+        u.piece = __builtin_amdgcn_readfirstlane((unsigned)number / (unsigned)rest);
+        u.tile = whole + number - u.piece * rest;
+        u.begin = __builtin_amdgcn_readfirstlane((unsigned)(u.piece * stages_all) / (unsigned)pieces);
+        u.stages = __builtin_amdgcn_readfirstlane((unsigned)((u.piece + 1) * stages_all) / (unsigned)pieces) - u.begin;
+      }
+    }
+    u.group = __builtin_amdgcn_readfirstlane((unsigned)u.tile / (unsigned)(kRaster * tiles_j));
+    u.in_group = u.tile - u.group * (kRaster * tiles_j);
     locate(u);
     return u;
   };
   auto advance = [&](Unit& u) {
-    u.in_group += slots;
-    u.number += slots;
-    if (u.in_group < min(kRaster, tiles_i - u.group * kRaster) * tiles_j) locate(u);
-    else u = unit_at(u.number);
+    if (LOGITS && u.in_group + slots < min(kRaster, tiles_i - u.group * kRaster) * tiles_j) {
+      u.m++;
+      u.in_group += slots;
+      locate(u);
+    } else u = unit_at(u.m + 1);
   };
-  Unit now = unit_at(first_unit);
-  const int units_here = (xcd_end - first_unit + slots - 1) / slots;
+  Unit now = unit_at(0);
 
-  // ---- copies: number q of a wave brings 1 KB of an operand's stage, 8 rows of 128 bytes with their 16-byte chunks XOR-swizzled by row,
-  // or (k slow) 1 KB of 64 rows of 384, swizzled for the transposing reads below.  Rows and columns past A's last re-read it.
-  auto slow_swizzle = [](uint32_t krow) { return (((krow >> 1) & 1) << 2) | (((krow >> 3) & 1) << 1); };
+  // ---- copies: number q of a wave brings 1 KB of an operand's stage, 16 rows of 64 bytes with their 16-byte chunks XOR-swizzled by row,
+  // or (k slow) 1 KB of 32 rows of the tile's columns, swizzled for the transposing reads below.  Rows and columns past A's last re-read it.
   uint32_t oa[kCopies], ob[kCopies];
-  auto offset_of = [&](bool slow, int q, uint32_t ld, uint32_t last, uint32_t last_k) {     // last: of the tile's 192 (k slow: its last whole chunk of eight)
+  auto offset_of = [&](bool slow, int q, uint32_t ld, uint32_t last, uint32_t last_k) {     // last: of the tile's (k slow: its last whole chunk of eight)
     if (slow) {
       const uint32_t piece = (uint32_t)((wave * kCopies + q) * 64 + lane), krow = piece / (kTile / 8);
       return min(krow, last_k) * ld + min(((piece % (kTile / 8)) ^ slow_swizzle(krow)) * 8, last) * 2;
     }
-    const uint32_t row = (uint32_t)((wave * kCopies + q) * 8 + (lane >> 3)), chunk = (uint32_t)(lane & 7) ^ ((row >> 1) & 7);
+    const uint32_t row = (uint32_t)((wave * kCopies + q) * 16 + (lane >> 2)), chunk = (uint32_t)(lane & 3) ^ swizzle(row);
     return min(row, last) * ld + chunk * 16;
   };
   const uint8_t *a_at, *b_at;
@@ -169,14 +206,14 @@ head_product(const HeadProduct p, const HeadResult r) {
 #pragma unroll
     for (int q = 0; q < kCopies; q++) oa[q] = offset_of(A_SLOW, q, (uint32_t)p.lda, last, last_k);
   };
-  bool whole = false;                                            // the offsets in A are those of any tile that lies in it
+  bool inner = false;                                            // the offsets in A are those of any tile that lies in it
   auto point_at = [&]() {
-    next_k = (int64_t)next.begin * kStageK; next_left = next.stages;
-    a_at = p.a + (A_SLOW ? next.i0 * 2 : next.i0 * p.lda) + next.begin * a_step;
-    b_at = p.b + (B_SLOW ? next.j0 * 2 : next.j0 * p.ldb) + next.begin * b_step;
+    next_k = (int64_t)next.begin * kUnitK; next_left = next.stages * 2;
+    a_at = p.a + (A_SLOW ? next.i0 * 2 : next.i0 * p.lda) + next.begin * 2 * a_step;
+    b_at = p.b + (B_SLOW ? next.j0 * 2 : next.j0 * p.ldb) + next.begin * 2 * b_step;
     const bool inside = next.i0 + kTile <= p.rows_i && (KIND != HEAD_INPUT || next_k + kStageK <= p.rows_k);
-    if (!(inside && whole)) point_a();
-    whole = inside;
+    if (!(inside && inner)) point_a();
+    inner = inside;
   };
 #pragma unroll
   for (int q = 0; q < kCopies; q++) ob[q] = offset_of(B_SLOW, q, (uint32_t)p.ldb, kTile, kStageK - 1);
@@ -189,297 +226,284 @@ head_product(const HeadProduct p, const HeadResult r) {
   auto copied = [&]() {                                          // to the next stage, of this unit or of the next
     if (!units_left) return;
     if (--next_left) {
-      a_at += a_step; b_at += b_step;
+      b_at += b_step;
       if constexpr (KIND == HEAD_INPUT) {
         next_k += kStageK;
-        if (next_k + kStageK > p.rows_k) { point_a(); whole = false; }       // the last words
-      }
+        if (next_k < p.rows_k) {                                 // (behind the last word B holds zeros, whatever they meet)
+          a_at += a_step;
+          if (next_k + kStageK > p.rows_k) { point_a(); inner = false; }     // the last words
+        }
+      } else a_at += a_step;
     } else if (--units_left) {
       advance(next);
       point_at();
     }
   };
-  auto copy_stage = [&](uint32_t buf) {
-#pragma unroll
-    for (int q = 0; q < 2 * kCopies; q++) copy_one(q, buf);
-    copied();
-  };
 
-  float4v acc[kFrags][kFrags];
-
-  // ---- fragments of a step (32 elements of k): lane l takes row l % 16, elements 8 * (l / 16) .. + 7.  k slow: in a group of 16 lanes,
+  // ---- fragments of a stage: lane l takes row l % 16, elements 8 * (l / 16) .. + 7.  k slow: in a group of 16 lanes,
   // lane i receives the halfwords i % 4 of the source lanes 4e + i / 4 (e = 0..3), so source lane s addresses k-row s / 4 (of
   // four), columns 4 * (s % 4).. of the group's 16; two such reads make eight elements of k.
-  uint32_t a_off[A_SLOW ? kFrags : 2], b_off[B_SLOW ? kFrags : 2];
+  uint32_t a_off[A_SLOW ? F : 1], b_off[B_SLOW ? F : 1];
   auto fragment_offsets = [&](auto is_slow, uint32_t* off, int half) {
     if constexpr (decltype(is_slow)::value) {
       const uint32_t krow = lq * 8 + (l16 >> 2);
 #pragma unroll
-      for (int f = 0; f < kFrags; f++) {
+      for (int f = 0; f < F; f++) {
         const uint32_t col = (uint32_t)(half * kSlab + f * 16) + (l16 & 3) * 4;
-        off[f] = krow * kStridedRowBytes + (((col >> 3) ^ slow_swizzle(krow)) * 16) + ((col >> 2) & 1) * 8;
+        off[f] = krow * kSlowRowBytes + (((col >> 3) ^ slow_swizzle(krow)) * 16) + ((col >> 2) & 1) * 8;
       }
     } else {
-#pragma unroll
-      for (int step = 0; step < 2; step++) off[step] = (uint32_t)(half * kSlab + l16) * kRowBytes + (uint32_t)((step * 4 + lq) ^ ((l16 >> 1) & 7)) * 16;
+      off[0] = (uint32_t)(half * kSlab + l16) * kRowBytes + ((uint32_t)lq ^ swizzle(l16)) * 16;
     }
   };
   fragment_offsets(std::bool_constant<A_SLOW>{}, a_off, wi);
   fragment_offsets(std::bool_constant<B_SLOW>{}, b_off, wj);
-  int4v af[2][kFrags], bf[2][kFrags];                            // [register set][fragment]
-  short4v aq[2][kFrags][2], bq[2][kFrags][2];                    // k slow: the halves of a fragment
-  constexpr int A_READS = A_SLOW ? 2 * kFrags : kFrags, B_READS = B_SLOW ? 2 * kFrags : kFrags, READS = A_READS + B_READS, MMAS = kFrags * kFrags;
-  auto read_slow = [&](const uint8_t* base, uint32_t off, int q, int step) {
-    return __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_short4_ptr)(lds_ptr_t)(base + off + (step * 32 + (q & 1) * 4) * kStridedRowBytes));
+  int4v af[2][F], bf[2][F];                                      // [register set][fragment]
+  short4v aq[2][F][2], bq[2][F][2];                              // k slow: the halves of a fragment
+  constexpr int A_READS = A_SLOW ? 2 * F : F, B_READS = B_SLOW ? 2 * F : F, READS = A_READS + B_READS, MMAS = F * F;
+  auto read_slow = [&](const uint8_t* base, uint32_t off, int q) {
+    return __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_short4_ptr)(lds_ptr_t)(base + off + (q & 1) * 4 * kSlowRowBytes));
   };
-  auto read_a = [&](int set, int q, uint32_t buf, int step) {
-    if constexpr (A_SLOW) aq[set][q >> 1][q & 1] = read_slow(smem + buf, a_off[q >> 1], q, step);
-    else af[set][q] = *reinterpret_cast<const int4v*>(smem + buf + a_off[step] + q * 16 * kRowBytes);
+  auto read_a = [&](int set, int q, uint32_t buf) {
+    if constexpr (A_SLOW) aq[set][q >> 1][q & 1] = read_slow(smem + buf, a_off[q >> 1], q);
+    else af[set][q] = *reinterpret_cast<const int4v*>(smem + buf + a_off[0] + q * 16 * kRowBytes);
   };
-  auto read_b = [&](int set, int q, uint32_t buf, int step) {
-    if constexpr (B_SLOW) bq[set][q >> 1][q & 1] = read_slow(smem + buf + kOperand, b_off[q >> 1], q, step);
-    else bf[set][q] = *reinterpret_cast<const int4v*>(smem + buf + kOperand + b_off[step] + q * 16 * kRowBytes);
+  auto read_b = [&](int set, int q, uint32_t buf) {
+    if constexpr (B_SLOW) bq[set][q >> 1][q & 1] = read_slow(smem + buf + kOperand, b_off[q >> 1], q);
+    else bf[set][q] = *reinterpret_cast<const int4v*>(smem + buf + kOperand + b_off[0] + q * 16 * kRowBytes);
   };
-  // the reads of a step in the order the next step's instructions need them: A's first fragment, B's, A's others
-  auto read_one = [&](int set, int n, uint32_t buf, int step) {
-    constexpr int FIRST = A_READS / kFrags;
-    if (n >= FIRST && n < FIRST + B_READS) read_b(set, n - FIRST, buf, step);
-    else read_a(set, n < FIRST ? n : n - B_READS, buf, step);
+  // the reads of a stage in the order its instructions need them: A's first fragment, B's, A's others
+  auto read_one = [&](int set, int n, uint32_t buf) {
+    constexpr int FIRST = A_READS / F;
+    if (n >= FIRST && n < FIRST + B_READS) read_b(set, n - FIRST, buf);
+    else read_a(set, n < FIRST ? n : n - B_READS, buf);
   };
-  auto fragment = [&](auto is_slow, int4v& whole, short4v (&halves)[2]) {
+  auto fragment = [&](auto is_slow, int4v& whole_one, short4v (&halves)[2]) {
     if constexpr (decltype(is_slow)::value) return __builtin_bit_cast(int4v, __builtin_shufflevector(halves[0], halves[1], 0, 1, 2, 3, 4, 5, 6, 7));
-    else return whole;
+    else return whole_one;
   };
-  // The instructions of a step from one register set; behind them, one by one, the next step's reads into the other set and N copies
-  // of a stage.
-  auto mma_step = [&](int set, auto copies, uint32_t dst, uint32_t src, int rstep) {
-    constexpr int N = decltype(copies)::value;
+  float4v acc[F][F];
+  // The instructions of a stage from one register set; behind them, one by one, the next stage's reads into the other set and the copies of the stage that
+  // takes this one's buffer.
+  auto mma_stage = [&](auto which, auto is_first, uint32_t dst, uint32_t src) __attribute__((always_inline)) {
+    constexpr int set = decltype(which)::value;
     __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
     for (int n = 0; n < MMAS; n++) {
-      const int ti = n / kFrags, tj = n % kFrags;
-      acc[ti][tj] = mma(T{}, fragment(std::bool_constant<A_SLOW>{}, af[set][ti], aq[set][ti]), fragment(std::bool_constant<B_SLOW>{}, bf[set][tj], bq[set][tj]), acc[ti][tj]);
+      const int ti = n / F, tj = n % F;
+      acc[ti][tj] = mma(T{}, fragment(std::bool_constant<A_SLOW>{}, af[set][ti], aq[set][ti]), fragment(std::bool_constant<B_SLOW>{}, bf[set][tj], bq[set][tj]), decltype(is_first)::value ? float4v{0, 0, 0, 0} : acc[ti][tj]);
       __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
-      for (int q = n * READS / MMAS; q < (n + 1) * READS / MMAS; q++) read_one(set ^ 1, q, src, rstep);
-#pragma unroll
-      for (int q = 0; q < N; q++)
-        if (q * MMAS / (N ? N : 1) == n) copy_one(q, dst);
+      for (int q = n * READS / MMAS; q < (n + 1) * READS / MMAS; q++) read_one(set ^ 1, q, src);
+      if (n * 2 * kCopies % MMAS < 2 * kCopies) copy_one(n * 2 * kCopies / MMAS, dst);
       __builtin_amdgcn_sched_barrier(0);
     }
   };
-  using C0 = std::integral_constant<int, 0>;
-  using CA = std::integral_constant<int, 2 * kCopies>;
 
-  // ---- what is done with a unit's accumulators.  The buffer `fre` is nobody's then; a wave keeps to the two slices of it that its own next copies go to.
-  float bias_at[2] = {0, 0};
-  float2 coef[kFrags];
-  float level[kFrags];
-  int target[kFrags];
-  uint32_t listed[kFrags];
-  auto token_of = [&](int tj) { return now.j0 + wj * kSlab + tj * 16 + l16; };
-  auto fetch = [&]() {
+  // ---- what is done with a unit's accumulators, in the wave's own part of the LDS
+  constexpr uint32_t scratch_at = kRing * kStage;
+  auto fetch = [&]() {                                           // what the tile needs of its words and tokens
+    const uint32_t to = smem_at + scratch_at + wave * kScratch, off = (uint32_t)lane * 16;
+    const int64_t token = now.j0 + wj * kSlab;
+    if constexpr (KIND == HEAD_INPUT) g2l16((const uint8_t*)(r.row_of + token), off, to + kTokensAt);
     if constexpr (LOGITS) {
-      if (r.bias) {
-#pragma unroll
-        for (int q = 0; q < 2; q++) bias_at[q] = r.bias[now.i0 + wi * kSlab + min(q * 64 + lane, kSlab - 1)];
-      }
-#pragma unroll
-      for (int tj = 0; tj < kFrags; tj++) {
-        if constexpr (KIND == HEAD_STATS) {
-          if (r.target) target[tj] = r.target[token_of(tj)];
-          else listed[tj] = r.slab_entries[(now.i0 / kSlab + wi) * r.tokens_ld + token_of(tj)];
-        } else {
-          coef[tj] = r.coef[token_of(tj)];
-          if constexpr (SMOOTH) level[tj] = r.level[token_of(tj)];
-        }
+      if (r.bias) g2l16((const uint8_t*)(r.bias + now.i0 + wi * kSlab), off, to + kBiasAt);
+      if constexpr (KIND == HEAD_STATS) {
+        const uint8_t* from = r.target ? (const uint8_t*)(r.target + token) : (const uint8_t*)(r.slab_entries + (now.i0 / kSlab + wi) * r.tokens_ld + token);
+        g2l16(from, off, to + kTokensAt);
+      } else {
+        g2l16((const uint8_t*)(r.coef + token), off, to + kTokensAt);
+        if constexpr (SMOOTH) g2l16((const uint8_t*)(r.level + token), off, to + kLevelAt);
       }
     }
   };
-  auto chunk_at = [](int row, int ch) { return row * 192 + (ch ^ ((row >> 2) & 3)) * 16; };
-  auto finish = [&](uint32_t fre) {
+  constexpr int ROW16 = kSlab * 2, CHUNKS = kSlab / 8;             // 16-bit results go out by 16 rows, through the wave's 4 KB
+  auto chunk_at = [](int row, int ch) { return row * ROW16 + (ch ^ row) * 16; };
+  auto pieces_of = [&](const Unit& u) { return u.m < rounds ? 1 : pieces; };
+  auto finish = [&]() __attribute__((always_inline)) {
     // (numbers of their own: what is worked out from them, addresses above all, would be kept in registers through the loop over the stages otherwise)
     int lane = (int)threadIdx.x & 63;
     asm volatile("" : "+v"(lane));
     const int l16 = lane & 15, lq = lane >> 4;
-    auto token_of = [&](int tj) { return now.j0 + wj * kSlab + tj * 16 + l16; };
-    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");             // the copies in flight: from here on stores count as well
-    uint8_t* slice = smem + fre + wave * kSlice;
-    float* bias_lds = reinterpret_cast<float*>(smem + fre + kOperand + wave * kSlice);
+    uint8_t* slice = smem + scratch_at + wave * kScratch;
+    // what was fetched is older than the copies that the loop's last wait left in flight, if there were enough of them
+    if (KIND != HEAD_WEIGHT && now.stages < 4) asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+    float4v add[F];
     if constexpr (LOGITS) {
 #pragma unroll
-      for (int q = 0; q < 2; q++)
-        if (q * 64 + lane < kSlab) bias_lds[q * 64 + lane] = bias_at[q];
-      wave_lds_fence();
+      for (int ti = 0; ti < F; ti++) {
+        if (r.bias) add[ti] = *reinterpret_cast<const float4v*>(slice + kBiasAt + (ti * 16 + lq * 4) * 4);
+        else {
+#pragma unroll
+          for (int e = 0; e < 4; e++) add[ti][e] = now.i0 + wi * kSlab + ti * 16 + lq * 4 + e < r.words ? 0.0f : -__builtin_inff();
+        }
+      }
     }
-    auto bias_of = [&](int ti) { return *reinterpret_cast<const float4v*>(bias_lds + ti * 16 + lq * 4); };
     if constexpr (KIND == HEAD_STATS) {
       const int64_t slab = now.i0 / kSlab + wi;
       const int base = (int)(slab * kSlab);
-      // (the accumulators are read once: vector instructions reach them through copies alone)
-      float4v y[kFrags][kFrags];
-      float m[kFrags], t[kFrags], s[kFrags], sum[kFrags];
+      constexpr int G = F / 2;                          // columns of fragments at a time, as far as registers go
 #pragma unroll
-      for (int tj = 0; tj < kFrags; tj++) { m[tj] = -__builtin_inff(); s[tj] = 0.0f; sum[tj] = 0.0f; }
+      for (int t0 = 0; t0 < F; t0 += G) {
+        // (the accumulators are read once: vector instructions reach them through copies alone)
+        float4v y[F][G];
+        float m[G], from[G], s[G], sum[G];
 #pragma unroll
-      for (int ti = 0; ti < kFrags; ti++) {
-        const float4v add = bias_of(ti);
+        for (int tj = 0; tj < G; tj++) { m[tj] = -__builtin_inff(); s[tj] = 0.0f; sum[tj] = 0.0f; }
 #pragma unroll
-        for (int tj = 0; tj < kFrags; tj++) {
+        for (int ti = 0; ti < F; ti++)
 #pragma unroll
-          for (int e = 0; e < 4; e++) {
-            y[ti][tj][e] = __builtin_fmaf(acc[ti][tj][e], r.scale, add[e]);
-            if constexpr (SMOOTH) sum[tj] += base + ti * 16 + lq * 4 + e < r.words ? y[ti][tj][e] : 0.0f;
-          }
-          m[tj] = fmaxf(fmaxf(m[tj], y[ti][tj][0]), y[ti][tj][1]);
-          m[tj] = fmaxf(fmaxf(m[tj], y[ti][tj][2]), y[ti][tj][3]);
-        }
-      }
-#pragma unroll
-      for (int tj = 0; tj < kFrags; tj++) {
-        m[tj] = over_quarters(m[tj], [](float a, float b) { return fmaxf(a, b); });
-        t[tj] = m[tj] == -__builtin_inff() ? 0.0f : m[tj];
-      }
-#pragma unroll
-      for (int ti = 0; ti < kFrags; ti++)
-#pragma unroll
-        for (int e = 0; e < 4; e++)
-#pragma unroll
-          for (int tj = 0; tj < kFrags; tj++) s[tj] += __builtin_amdgcn_exp2f(y[ti][tj][e] - t[tj]);
-#pragma unroll
-      for (int tj = 0; tj < kFrags; tj++) {
-        s[tj] = over_quarters(s[tj], [](float a, float b) { return a + b; });
-        if constexpr (SMOOTH) sum[tj] = over_quarters(sum[tj], [](float a, float b) { return a + b; });
-        const int64_t token = token_of(tj);
-        if (lq == 0) {
-          r.stats[slab * r.tokens_ld + token] = float2{m[tj], s[tj]};
-          if constexpr (SMOOTH) r.sums[slab * r.tokens_ld + token] = sum[tj];
-        }
-      }
-      if (r.target) {
-#pragma unroll
-        for (int tj = 0; tj < kFrags; tj++) {
-          const int at = target[tj] - base;
-          if (__any(at >= 0 && at < kSlab)) {
-#pragma unroll
-            for (int ti = 0; ti < kFrags; ti++)
-#pragma unroll
-              for (int e = 0; e < 4; e++)
-                if (at == ti * 16 + lq * 4 + e) r.picked[token_of(tj)] = y[ti][tj][e];
-          }
-        }
-      } else {
-        // the teacher's entries of these 96 words, four of a token at a time, from the token's row in LDS
-#pragma unroll
-        for (int tj = 0; tj < kFrags; tj++) {
-          const int many = (int)(listed[tj] >> 11 & 0x7ff), first = (int)(listed[tj] & 0x7ff);
-          if (__any(many > 0)) {
-            wave_lds_fence();
-#pragma unroll
-            for (int ti = 0; ti < kFrags; ti++)
-              *reinterpret_cast<float4v*>(slice + l16 * 384 + ((ti * 4 + lq) ^ ((l16 >> 1) & 7)) * 16) = y[ti][tj];
-            wave_lds_fence();
-            for (int n = lq; n < many; n += 4) {
-              const int64_t entry = token_of(tj) * r.entries + first + n;
-              const int at = n ? r.entry_words[entry] - base : (int)(listed[tj] >> 22);
-              r.picked[entry] = *reinterpret_cast<const float*>(slice + l16 * 384 + ((at >> 2) ^ ((l16 >> 1) & 7)) * 16 + (at & 3) * 4);
-            }
-          }
-        }
-      }
-    } else if constexpr (KIND == HEAD_SLOPE) {
-      // 32(j) x 96(i) pieces through the slice (rows of 192 bytes, chunks XOR-swizzled with the row), whole rows of them stored
-#pragma unroll
-      for (int tp = 0; tp < kFrags / 2; tp++) {
-        if (tp > 0) wave_lds_fence();
-#pragma unroll
-        for (int ti = 0; ti < kFrags; ti++) {
-          const float4v add = bias_of(ti);
-#pragma unroll
-          for (int t2 = 0; t2 < 2; t2++) {
-            const int tj = tp * 2 + t2;
-            T o[4];
+          for (int tj = 0; tj < G; tj++) {
 #pragma unroll
             for (int e = 0; e < 4; e++) {
-              float v = coef[tj].y * __builtin_amdgcn_exp2f(__builtin_fmaf(acc[ti][tj][e], r.scale, add[e]) - coef[tj].x);
-              if constexpr (SMOOTH) v = now.i0 + wi * kSlab + ti * 16 + lq * 4 + e < r.words ? v - level[tj] : 0.0f;
-              o[e] = from_float<T>(v);
+              y[ti][tj][e] = __builtin_fmaf(acc[ti][t0 + tj][e], r.scale, add[ti][e]);
+              if constexpr (SMOOTH) sum[tj] += base + ti * 16 + lq * 4 + e < r.words ? y[ti][tj][e] : 0.0f;
             }
-            *reinterpret_cast<Pack<T, 4>*>(slice + chunk_at(t2 * 16 + l16, ti * 2 + (lq >> 1)) + (lq & 1) * 8) = *reinterpret_cast<Pack<T, 4>*>(o);
+            m[tj] = fmaxf(fmaxf(m[tj], y[ti][tj][0]), y[ti][tj][1]);
+            m[tj] = fmaxf(fmaxf(m[tj], y[ti][tj][2]), y[ti][tj][3]);
           }
+#pragma unroll
+        for (int tj = 0; tj < G; tj++) {
+          m[tj] = over_quarters(m[tj], [](float a, float b) { return fmaxf(a, b); });
+          from[tj] = m[tj] == -__builtin_inff() ? 0.0f : m[tj];
         }
-        wave_lds_fence();
 #pragma unroll
-        for (int it = 0; it < 6; it++) {
-          const uint32_t piece = it * 64 + lane;
-          const int jl = piece / 12, ch = piece % 12;
-          const int4v v = *reinterpret_cast<const int4v*>(slice + chunk_at(jl, ch));
-          *reinterpret_cast<int4v*>((T*)r.slope + (now.j0 + wj * kSlab + tp * 32 + jl) * r.ld_slope + now.i0 + wi * kSlab + ch * 8) = v;
-        }
-      }
-    } else if (r.partial) {
+        for (int ti = 0; ti < F; ti++)
 #pragma unroll
-      for (int tj = 0; tj < kFrags; tj++) {
-        const int64_t row = now.j0 + wj * kSlab + tj * 16 + l16;
-        float* at = r.partial + ((int64_t)now.split * r.rows_j + row) * r.ld_out;
-        if (row < r.rows_j) {
+          for (int e = 0; e < 4; e++)
 #pragma unroll
-          for (int ti = 0; ti < kFrags; ti++) {
-            const int64_t col = now.i0 + wi * kSlab + ti * 16 + lq * 4;
-            if (col < r.ld_out) *reinterpret_cast<float4v*>(at + col) = acc[ti][tj];
+            for (int tj = 0; tj < G; tj++) s[tj] += __builtin_amdgcn_exp2f(y[ti][tj][e] - from[tj]);
+#pragma unroll
+        for (int tj = 0; tj < G; tj++) {
+          const int64_t token = now.j0 + wj * kSlab + (t0 + tj) * 16 + l16;
+          const int brought = *reinterpret_cast<const int*>(slice + kTokensAt + ((t0 + tj) * 16 + l16) * 4);
+          s[tj] = over_quarters(s[tj], [](float a, float b) { return a + b; });
+          if constexpr (SMOOTH) sum[tj] = over_quarters(sum[tj], [](float a, float b) { return a + b; });
+          if (lq == 0) {
+            r.stats[slab * r.tokens_ld + token] = float2{m[tj], s[tj]};
+            if constexpr (SMOOTH) r.sums[slab * r.tokens_ld + token] = sum[tj];
+          }
+          if (r.target) {
+            const int at = brought - base;
+            if (__any(at >= 0 && at < kSlab)) {
+#pragma unroll
+              for (int ti = 0; ti < F; ti++)
+#pragma unroll
+                for (int e = 0; e < 4; e++)
+                  if (at == ti * 16 + lq * 4 + e) r.picked[token] = y[ti][tj][e];
+            }
+          } else {
+            // the teacher's entries of these words, four of a token at a time, from the token's row in LDS, eight tokens in turn
+            const int many = brought >> 11 & 0x7ff, first = brought & 0x7ff;
+            if (__any(many > 0)) {
+#pragma unroll
+              for (int half = 0; half < 2; half++) {
+                uint8_t* row = slice + (l16 & 7) * (kSlab * 4);
+                wave_lds_fence();
+                if (l16 >> 3 == half) {
+#pragma unroll
+                  for (int ti = 0; ti < F; ti++) *reinterpret_cast<float4v*>(row + ((ti * 4 + lq) ^ (l16 & 7)) * 16) = y[ti][tj];
+                }
+                wave_lds_fence();
+                if (l16 >> 3 == half)
+                  for (int n = lq; n < many; n += 4) {
+                    const int64_t entry = token * r.entries + first + n;
+                    const int at = n ? r.entry_words[entry] - base : brought >> 22;
+                    r.picked[entry] = *reinterpret_cast<const float*>(row + ((at >> 2) ^ (l16 & 7)) * 16 + (at & 3) * 4);
+                  }
+              }
+            }
           }
         }
       }
     } else {
-      const float scale = *r.out_scale;
-      if constexpr (std::is_same<OutT, float>::value) {
-        const bool whole = r.ld_out % 4 == 0 && ((uintptr_t)r.out & 15) == 0;
+      // float32 as the accumulators lie, 16 bytes a lane
+      auto slots_of = [&](float* base, int64_t tile) { return base + tile * (kTile * kTile) + (wave * 64 + lane) * 4; };
+      if constexpr (!LOGITS) {
+        asm volatile("s_waitcnt vmcnt(0)" ::: "memory");         // the copies in flight: from here on stores count as well
+        if (r.add && pieces_of(now) == 1) {
+          const float* from = slots_of(r.sum, now.tile);
 #pragma unroll
-        for (int tj = 0; tj < kFrags; tj++) {
+          for (int ti = 0; ti < F; ti++)
+#pragma unroll
+            for (int tj = 0; tj < F; tj++) acc[ti][tj] += *reinterpret_cast<const float4v*>(from + (ti * F + tj) * (kThreads * 4));
+        }
+        if (pieces_of(now) > 1 || !r.last) {
+          float* to = pieces_of(now) > 1 ? slots_of(r.partial, (int64_t)now.piece * rest + now.tile - whole) : slots_of(r.sum, now.tile);
+#pragma unroll
+          for (int ti = 0; ti < F; ti++)
+#pragma unroll
+            for (int tj = 0; tj < F; tj++) *reinterpret_cast<float4v*>(to + (ti * F + tj) * (kThreads * 4)) = acc[ti][tj];
+          wave_lds_fence();
+          asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+          return;
+        }
+      }
+      const int64_t rows = KIND == HEAD_INPUT ? (int64_t)count : r.rows_j, cols = r.cols_out;
+      const float scale = LOGITS ? 1.0f : *r.out_scale;
+      if constexpr (!LOGITS && std::is_same<OutT, float>::value) {
+        const bool aligned = cols % 4 == 0 && ((uintptr_t)r.out & 15) == 0;
+#pragma unroll
+        for (int tj = 0; tj < F; tj++) {
           const int64_t row = now.j0 + wj * kSlab + tj * 16 + l16;
+          float* at = (float*)r.out + row * cols + now.i0 + wi * kSlab + lq * 4;
+          if (row < rows) {
 #pragma unroll
-          for (int ti = 0; ti < kFrags; ti++) {
-            const int64_t col = now.i0 + wi * kSlab + ti * 16 + lq * 4;
-            float* at = (float*)r.out + row * r.ld_out + col;
-            const float4v v = acc[ti][tj] * scale;
-            if (row < r.rows_j) {
-              if (whole && col + 4 <= r.cols_out) *reinterpret_cast<float4v*>(at) = v;
-              else {
+            for (int ti = 0; ti < F; ti++) {
+              const int64_t col = now.i0 + wi * kSlab + ti * 16 + lq * 4;
+              const float4v v = acc[ti][tj] * scale;
+              if (aligned && col < cols) *reinterpret_cast<float4v*>(at + ti * 16) = v;
+              else if (!aligned) {
 #pragma unroll
                 for (int e = 0; e < 4; e++)
-                  if (col + e < r.cols_out) at[e] = v[e];
+                  if (col + e < cols) at[ti * 16 + e] = v[e];
               }
             }
           }
         }
       } else {
-        const bool whole = r.ld_out % 8 == 0 && ((uintptr_t)r.out & 15) == 0;
+        // 16(j) x 128(i) pieces through the slice, chunks XOR-swizzled with the row, whole rows of them stored
+        const bool aligned = LOGITS || (cols % 8 == 0 && ((uintptr_t)r.out & 15) == 0);
+        T* out = (T*)(LOGITS ? r.slope : r.out);
+        const int64_t ld = LOGITS ? r.ld_slope : cols;
 #pragma unroll
-        for (int tp = 0; tp < kFrags / 2; tp++) {
-          if (tp > 0) wave_lds_fence();
+        for (int tj = 0; tj < F; tj++) {
+          float2 coef = {0, 0};
+          float level = 0.0f;
+          if constexpr (LOGITS) coef = *reinterpret_cast<const float2*>(slice + kTokensAt + (tj * 16 + l16) * 8);
+          if constexpr (LOGITS && SMOOTH) level = *reinterpret_cast<const float*>(slice + kLevelAt + (tj * 16 + l16) * 4);
+          if (tj > 0) wave_lds_fence();                          // behind the reads of the piece before
 #pragma unroll
-          for (int ti = 0; ti < kFrags; ti++)
+          for (int ti = 0; ti < F; ti++) {
+            T o[4];
 #pragma unroll
-            for (int t2 = 0; t2 < 2; t2++) {
-              T o[4];
-#pragma unroll
-              for (int e = 0; e < 4; e++) o[e] = from_float<T>(scaled(acc[ti][tp * 2 + t2][e], scale));
-              *reinterpret_cast<Pack<T, 4>*>(slice + chunk_at(t2 * 16 + l16, ti * 2 + (lq >> 1)) + (lq & 1) * 8) = *reinterpret_cast<Pack<T, 4>*>(o);
+            for (int e = 0; e < 4; e++) {
+              float v;
+              if constexpr (LOGITS) {
+                v = coef.y * __builtin_amdgcn_exp2f(__builtin_fmaf(acc[ti][tj][e], r.scale, add[ti][e]) - coef.x);
+                if constexpr (SMOOTH) v = now.i0 + wi * kSlab + ti * 16 + lq * 4 + e < r.words ? v - level : 0.0f;
+              } else v = scaled(acc[ti][tj][e], scale);
+              o[e] = from_float<T>(v);
             }
+            *reinterpret_cast<Pack<T, 4>*>(slice + chunk_at(l16, ti * 2 + (lq >> 1)) + (lq & 1) * 8) = *reinterpret_cast<Pack<T, 4>*>(o);
+          }
+          if (LOGITS && tj == 0) asm volatile("s_waitcnt vmcnt(0)" ::: "memory");    // the copies in flight, as above
           wave_lds_fence();
 #pragma unroll
-          for (int it = 0; it < 6; it++) {
+          for (int it = 0; it < CHUNKS / 4; it++) {
             const uint32_t piece = it * 64 + lane;
-            const int jl = piece / 12, ch = piece % 12;
-            const int64_t col = now.i0 + wi * kSlab + ch * 8, row = now.j0 + wj * kSlab + tp * 32 + jl;
+            const int jl = piece / CHUNKS, ch = piece % CHUNKS;
+            const int64_t row = now.j0 + wj * kSlab + tj * 16 + jl, col = now.i0 + wi * kSlab + ch * 8;
             const int4v v = *reinterpret_cast<const int4v*>(slice + chunk_at(jl, ch));
-            if (row < r.rows_j && col < r.cols_out) {
-              T* at = (T*)r.out + row * r.ld_out + col;
-              if (whole && col + 8 <= r.cols_out) __builtin_nontemporal_store(v, reinterpret_cast<int4v*>(at));
+            if constexpr (LOGITS) *reinterpret_cast<int4v*>(out + row * ld + col) = v;
+            else if (row < rows && col < cols) {
+              const int64_t to = KIND == HEAD_INPUT ? (int64_t)*reinterpret_cast<const int*>(slice + kTokensAt + (tj * 16 + jl) * 4) : row;
+              T* at = out + to * ld + col;
+              if (aligned) __builtin_nontemporal_store(v, reinterpret_cast<int4v*>(at));
               else {
 #pragma unroll
                 for (int e = 0; e < 8; e++)
-                  if (col + e < r.cols_out) at[e] = T{(uint16_t)((uint32_t)v[e >> 1] >> (e & 1) * 16)};
+                  if (col + e < cols) at[e] = T{(uint16_t)((uint32_t)v[e >> 1] >> (e & 1) * 16)};
               }
             }
           }
@@ -490,36 +514,50 @@ head_product(const HeadProduct p, const HeadResult r) {
     asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");           // the next copies go over what was read
   };
 
-  // ---- the sequence of stages.  Behind its end the copies go on from the last place (two stages that nobody reads): nothing in the loop
-  // depends on where the sequence ends.
-  uint32_t cur = 0, nxt = kStage, fre = 2 * kStage;              // buffers of this stage, the next and the one behind (= the one before)
-  copy_stage(cur);
-  copy_stage(nxt);
-  wait_copies_and_barrier<2 * kCopies, true>();
+  // ---- the sequence of stages.  Behind its end the copies go on from the last place (stages that nobody reads): nothing in the loop depends on where
+  // the sequence ends.
 #pragma unroll
-  for (int n = 0; n < READS; n++) read_one(0, n, cur, 0);
-  bool landed = false;                                           // the next stage has arrived already
+  for (int b = 0; b < kRing; b++) {
+#pragma unroll
+    for (int q = 0; q < 2 * kCopies; q++) copy_one(q, b * kStage);
+    copied();
+  }
+  wait_copies_and_barrier<(kRing - 1) * 2 * kCopies, true>();
+#pragma unroll
+  for (int n = 0; n < READS; n++) read_one(0, n, 0);
+  uint32_t cur = 0;                                              // buffer of the stage that is multiplied
+  int landed = 0;                                                // so many stages behind the next one have arrived already
+  // The next stage has arrived when the copies of those behind it are all that is in flight; and everyone has read this one.  (Loads complete in order: stores
+  // between them can only make this wait longer, and where there are many, all copies were waited for ahead of the first.)
+  auto arrive = [&]() {
+    if (KIND != HEAD_STATS && landed > 0) { wait_reads_and_barrier(); landed--; }
+    else wait_copies_and_barrier<(kRing - 2) * 2 * kCopies, true>();
+  };
+  auto stage = [&](auto set, auto is_first) __attribute__((always_inline)) {
+    const uint32_t nxt = cur + kStage == kRing * kStage ? 0u : cur + kStage;
+    arrive();
+    mma_stage(set, is_first, cur, nxt);
+    copied();
+    cur = nxt;
+  };
   for (int units = units_here;;) {
     fetch();
-#pragma unroll
-    for (int ti = 0; ti < kFrags; ti++)
-#pragma unroll
-      for (int tj = 0; tj < kFrags; tj++) acc[ti][tj] = float4v{0, 0, 0, 0};
-    int left = now.stages;
-    do {
-      mma_step(0, CA{}, fre, cur, 1);                            // with the copies of the stage behind the next one
-      copied();
-      if (landed) wait_reads_and_barrier();
-      else wait_copies_and_barrier<2 * kCopies, true>();
-      landed = false;
-      const uint32_t t = cur; cur = nxt; nxt = fre; fre = t;
-      mma_step(1, C0{}, 0, cur, 0);
-    } while (--left);
-    finish(fre);
+    // (the first stage adds to zero, and not to accumulators that were cleared: those the compiler would move about in the loop)
+    stage(std::integral_constant<int, 0>{}, std::true_type{});
+    stage(std::integral_constant<int, 1>{}, std::false_type{});
+    for (int left = now.stages - 1; left > 0; left--) {
+      stage(std::integral_constant<int, 0>{}, std::false_type{});
+      stage(std::integral_constant<int, 1>{}, std::false_type{});
+    }
+    finish();
     if (!--units) break;
-    landed = true;
+    landed = kRing - 1;
     advance(now);
+    // (once more: kept through finish() the first fragments of the next unit would be in the way of what that needs)
+#pragma unroll
+    for (int n = 0; n < READS; n++) read_one(0, n, cur);
   }
+  asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
 }
 
 }  // namespace

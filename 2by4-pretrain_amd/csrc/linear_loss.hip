@@ -3,9 +3,9 @@
 //   cross entropy   lse - (1 - s) z[target] - s mean(z) + c lse^2             u = z, lse = log sum exp u
 //   distillation    sum_k q_k (log q_k - u[i_k] + lse)                        u = z / temperature, q the teacher's probabilities of its listed words
 //
-// Forward: one product whose tiles leave a maximum and a sum of exponentials per token and 96 words behind, and the logits of the listed
+// Forward: one product whose tiles leave a maximum and a sum of exponentials per token and 128 words behind, and the logits of the listed
 // words; a small kernel joins them.  Backward: the product once more, P = dloss/dz in 16 bits for a piece of the vocabulary at a time (at most
-// 1 GiB of it), the listed words put right in it, then  dx += P W  and  dW = P^T x.  The product that is formed again is a quarter of the
+// 2 GiB of it), the listed words put right in it, then  dx += P W  and  dW = P^T x.  The product that is formed again is a quarter of the
 // arithmetic of a training step; kept, the logits would be the largest tensor of it.
 //
 // Tokens that do not count (their target is to be ignored, or no word of the teacher's is listed) are left out from the start: the others are
@@ -25,8 +25,8 @@ namespace {
 
 constexpr float kLog2e = 1.44269504088896340736f, kLn2 = 0.69314718055994530942f;
 constexpr int kMaxEntries = 1024;
-constexpr int64_t kSlopeBytes = (int64_t)1 << 30, kPartialBytes = (int64_t)1 << 29;
-constexpr int kMaxSplits = 64;
+constexpr int64_t kSlopeBytes = (int64_t)2 << 30;
+constexpr int kMostPieces = 1024;                                // tiles' pieces of a product: 256 MB
 
 // ---------------------------------------------------------------- which tokens count
 // A token's place among those that count, and back; the target of each, -2 one that no word has.
@@ -34,33 +34,46 @@ __global__ void __launch_bounds__(1024)
 count_tokens(const int64_t* __restrict__ targets, int64_t ignore, const int* __restrict__ flags, int tokens, int filled, int64_t words, int* __restrict__ count,
              int* __restrict__ row_of, int* __restrict__ place_of, int* __restrict__ target, float* __restrict__ loss) {
   __shared__ int sums[16];
-  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, each = (tokens + 1023) / 1024;
-  const int begin = min(tid * each, tokens), end = min(begin + each, tokens);
-  auto counts = [&](int t) { return targets ? targets[t] != ignore : flags[t] != 0; };
+  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, each = (tokens + 1023) / 1024 * 64;
+  const int begin = min(wave * each, tokens), end = min(begin + each, tokens);
+  auto counts = [&](int t) { return t < end && (targets ? targets[t] != ignore : flags[t] != 0); };
   int own = 0;
-  for (int t = begin; t < end; t++) own += counts(t);
-  int upto = own;
+  for (int t0 = begin; t0 < end; t0 += 256) {                    // four loads in flight
+    bool yes[4];
 #pragma unroll
-  for (int d = 1; d < 64; d *= 2) {
-    const int v = __shfl_up(upto, d);
-    if (lane >= d) upto += v;
+    for (int u = 0; u < 4; u++) yes[u] = counts(t0 + u * 64 + lane);
+#pragma unroll
+    for (int u = 0; u < 4; u++) own += __popcll(__ballot(yes[u]));
   }
-  if (lane == 63) sums[wave] = upto;
+  if (lane == 0) sums[wave] = own;
   __syncthreads();
-  int before = 0, total = 0;
+  int at = 0, total = 0;
   for (int w = 0; w < 16; w++) {
-    if (w < wave) before += sums[w];
+    if (w < wave) at += sums[w];
     total += sums[w];
   }
-  int at = before + upto - own;
-  for (int t = begin; t < end; t++) {
-    const bool yes = counts(t);
-    place_of[t] = yes ? at : -1;
-    if (!yes && loss) loss[t] = 0.0f;
-    if (yes) {
-      row_of[at] = t;
-      if (targets) target[at] = targets[t] >= 0 && targets[t] < words ? (int)targets[t] : -2;
-      at++;
+  for (int t0 = begin; t0 < end; t0 += 256) {
+    bool yes[4];
+    int64_t wanted[4];
+#pragma unroll
+    for (int u = 0; u < 4; u++) {
+      const int t = t0 + u * 64 + lane;
+      wanted[u] = targets && t < end ? targets[t] : -1;
+      yes[u] = counts(t);
+    }
+#pragma unroll
+    for (int u = 0; u < 4; u++) {
+      const int t = t0 + u * 64 + lane;
+      const uint64_t mask = __ballot(yes[u]);
+      const int place = at + __popcll(mask & ((1ull << lane) - 1));
+      at += __popcll(mask);
+      if (t < end) {
+        place_of[t] = yes[u] ? place : -1;
+        if (yes[u]) {
+          row_of[place] = t;
+          if (targets) target[place] = wanted[u] >= 0 && wanted[u] < words ? (int)wanted[u] : -2;
+        } else if (loss) loss[t] = 0.0f;
+      }
     }
   }
   for (int c = total + tid; c < filled; c += 1024) {
@@ -84,7 +97,7 @@ flag_tokens(const int64_t* __restrict__ indices, int64_t ld_indices, const L* __
 }
 
 // The entries of a token in ascending order of their words (one word listed twice: in the order of the list), the logarithm of the teacher's
-// probability of each, their sum, and where in the list the entries of 96 words begin.  A workgroup of one wave per token.
+// probability of each, their sum, and where in the list the entries of a slab of words begin.  A workgroup of one wave per token.
 template <typename L>
 __global__ void __launch_bounds__(64)
 list_entries(const int64_t* __restrict__ indices, int64_t ld_indices, const L* __restrict__ logits, int64_t ld_logits, const float* __restrict__ teacher_lse,
@@ -146,7 +159,7 @@ list_entries(const int64_t* __restrict__ indices, int64_t ld_indices, const L* _
     logq[to] = l;
     q += expf(l);
     const int slab = w / kSlab;
-    if (k == 0 || (int)(key[k - 1] >> 32) / kSlab != slab) {     // the first of its 96 words
+    if (k == 0 || (int)(key[k - 1] >> 32) / kSlab != slab) {     // the first of its slab
       int low = k, high = entries;                               // low: one of them, high: the first behind them
       while (high - low > 1) {
         const int mid = (low + high) / 2;
@@ -163,12 +176,12 @@ list_entries(const int64_t* __restrict__ indices, int64_t ld_indices, const L* _
 
 // ---------------------------------------------------------------- operands as the products read them
 // Rows of `cols` 16-bit elements, filled up with zeros to `ld_out` (a multiple of 8): row c of the result is row row_of[c] of the source (null: row c),
-// or zeros behind the last of *count, up to a whole tile.
+// or zeros behind the last of *count, up to a whole stage.
 __global__ void __launch_bounds__(256)
 pack_rows(const uint16_t* __restrict__ in, int64_t ld, int64_t rows, int64_t cols, bool aligned, const int* __restrict__ count, const int* __restrict__ row_of,
           uint16_t* __restrict__ out, int64_t ld_out) {
   const int64_t units = ld_out / 8;
-  if (count) rows = (int64_t)token_tiles(*count) * kTile;
+  if (count) rows = (int64_t)token_stages(*count) * kUnitK;
   for (int64_t u = (int64_t)blockIdx.x * 256 + threadIdx.x; u < rows * units; u += (int64_t)gridDim.x * 256) {
     const int64_t c = u / units, col = (u - c * units) * 8, row = row_of ? row_of[c] : c;
     int4v v = {0, 0, 0, 0};
@@ -211,7 +224,7 @@ token_losses(const float2* __restrict__ stats, const float* __restrict__ sums, i
   const int64_t c = (int64_t)blockIdx.x * per + (tid & (per - 1));
   const int n = *count;
   const bool counts = c < n;
-  if ((int64_t)blockIdx.x * per >= (int64_t)token_tiles(n) * kTile) return;
+  if ((int64_t)blockIdx.x * per >= n) return;
   float m = -__builtin_inff(), s = 0.0f, z = 0.0f;
   auto join = [](float& m, float& s, float m2, float s2) {
     const float top = fmaxf(m, m2), from = top == -__builtin_inff() ? 0.0f : top;
@@ -253,8 +266,8 @@ token_losses(const float2* __restrict__ stats, const float* __restrict__ sums, i
     __syncthreads();
   }
   if (share) return;
-  lse2[c] = counts ? lse : __builtin_inff();
   if (!counts) return;
+  lse2[c] = lse;
   if (entry_words) loss = mass[c] != mass[c] ? mass[c] : zs[tid];
   else {
     const float y = target[c] < 0 ? __builtin_nanf("") : picked[c], natural = lse * kLn2;
@@ -283,21 +296,24 @@ total_loss(const float* __restrict__ by_place, const int* __restrict__ count, bo
 // ---------------------------------------------------------------- gradient of the logits
 // Per token that counts: P = factor exp2(y - lse2) - level everywhere, less `pull` times the listed probabilities, all of it in units of the largest gradient of
 // a token's loss: of a mean P is 1 - p at the target, which rounding to 8 bits moves by 2^-9 where 4/3 of it (1 / 12288 less its power of
-// two) is moved by 2^-8.  By one workgroup; tokens behind the last get a factor of zero.
+// two) is moved by 2^-8.
+struct SlopeTerms { const float* grad; int reduction; LossTerms how; float inv_temperature; int to_exponent; };
+__device__ __forceinline__ float upstream_of(const SlopeTerms& t, int row, int n) {
+  const float g = t.reduction == TF24_REDUCE_NONE ? t.grad[row] : t.reduction == TF24_REDUCE_MEAN ? t.grad[0] / (float)n : t.grad[0];
+  return g * t.inv_temperature;
+}
+__device__ __forceinline__ float widened_by(const SlopeTerms& t, const float* mass, const float* lse2, int c) {
+  return mass ? mass[c] : 1.0f + 2.0f * t.how.z_loss * (lse2[c] * kLn2);
+}
+
+// The unit, where tokens differ: from the largest gradient of a token's loss, and the largest factor of one relative to it (what is not finite is that anyhow)
 __global__ void __launch_bounds__(1024)
-slope_terms(const float* __restrict__ grad, int reduction, LossTerms how, float inv_temperature, int to_exponent, const int* __restrict__ count,
-            const int* __restrict__ row_of, const int* __restrict__ target, const float* __restrict__ mass, const float* __restrict__ lse2,
-            float2* __restrict__ coef, float* __restrict__ level, float* __restrict__ pull, float* __restrict__ out_scale) {
+slope_unit(SlopeTerms terms, const int* __restrict__ count, const int* __restrict__ row_of, const float* __restrict__ mass, const float* __restrict__ lse2,
+           float* __restrict__ out_scale) {
   __shared__ float largest[1024];
-  const int tid = threadIdx.x, n = *count, filled = token_tiles(n) * kTile;
-  auto upstream = [&](int c) {
-    const float g = reduction == TF24_REDUCE_NONE ? grad[row_of[c]] : reduction == TF24_REDUCE_MEAN ? grad[0] / (float)n : grad[0];
-    return g * inv_temperature;
-  };
-  auto widened = [&](int c) { return mass ? mass[c] : 1.0f + 2.0f * how.z_loss * (lse2[c] * kLn2); };
-  // the largest gradient of a token's loss, and the largest factor of one relative to it (what is not finite is that anyhow)
+  const int tid = threadIdx.x, n = *count;
   auto most = [&](float v) {
-    largest[tid] = v < __builtin_inff() ? v : 0.0f;
+    largest[tid] = v;
     __syncthreads();
     for (int d = 512; d > 0; d /= 2) {
       if (tid < d) largest[tid] = fmaxf(largest[tid], largest[tid + d]);
@@ -307,27 +323,51 @@ slope_terms(const float* __restrict__ grad, int reduction, LossTerms how, float 
     __syncthreads();
     return top;
   };
+  auto finite = [](float v) { return v < __builtin_inff() ? v : 0.0f; };
   float v = 0.0f;
-  for (int c = tid; c < n; c += 1024) v = fmaxf(v, fabsf(upstream(c)));
+  for (int c = tid; c < n; c += 1024) v = fmaxf(v, finite(fabsf(upstream_of(terms, row_of[c], n))));
   float unit = most(v);
   if (unit == 0.0f) unit = 1.0f;
   v = 0.0f;
-  for (int c = tid; c < n; c += 1024) v = fmaxf(v, fabsf(upstream(c) / unit * widened(c)));
+  for (int c = tid; c < n; c += 1024) v = fmaxf(v, finite(fabsf(upstream_of(terms, row_of[c], n) / unit * widened_by(terms, mass, lse2, c))));
   v = most(v);
-  unit = ldexpf(unit, (v > 1.0f ? ilogbf(v) + 1 : 0) - to_exponent);
-  if (tid == 0) *out_scale = unit;
-  for (int c = tid; c < filled; c += 1024) {
-    float2 v = {__builtin_inff(), 0.0f};
-    float l = 0.0f, p = 0.0f;
-    if (c < n) {
-      const float g = upstream(c) / unit;
-      v = float2{lse2[c], g * widened(c)};
-      if (target && target[c] < 0) v.y = __builtin_nanf("");
-      l = g * (how.smoothing / (float)how.words);
-      p = g * (1.0f - how.smoothing);
-    }
-    coef[c] = v; pull[c] = p;
-    if (level) level[c] = l;
+  if (tid == 0) *out_scale = ldexpf(unit, (v > 1.0f ? ilogbf(v) + 1 : 0) - terms.to_exponent);
+}
+
+// The terms of 256 tokens; `alike`: all have the same gradient and a factor of one, which is the unit.  Tokens behind the last get a factor of zero, and rows of dx
+// that do not count are zero.
+template <typename T>
+__global__ void __launch_bounds__(256)
+slope_terms(SlopeTerms terms, bool alike, const int* __restrict__ count, const int* __restrict__ row_of, const int* __restrict__ target,
+            const float* __restrict__ mass, const float* __restrict__ lse2, float2* __restrict__ coef, float* __restrict__ level, float* __restrict__ pull,
+            float* __restrict__ out_scale, T* __restrict__ dx, int64_t width, const int* __restrict__ place_of, int64_t tokens) {
+  const int n = *count, c = blockIdx.x * 256 + threadIdx.x;
+  float unit;
+  if (alike) {
+    unit = n ? fabsf(upstream_of(terms, 0, n)) : 0.0f;
+    unit = ldexpf(unit > 0.0f && unit < __builtin_inff() ? unit : 1.0f, -terms.to_exponent);
+    if (c == 0) *out_scale = unit;
+  } else unit = *out_scale;
+  float2 v = {__builtin_inff(), 0.0f};
+  float l = 0.0f, p = 0.0f;
+  if (c < n) {
+    const float g = upstream_of(terms, row_of[c], n) / unit;
+    v = float2{lse2[c], g * widened_by(terms, mass, lse2, c)};
+    if (target && target[c] < 0) v.y = __builtin_nanf("");
+    l = g * (terms.how.smoothing / (float)terms.how.words);
+    p = g * (1.0f - terms.how.smoothing);
+  }
+  coef[c] = v; pull[c] = p;                                      // (tokens are filled up to whole workgroups)
+  if (level) level[c] = l;
+  if (!dx) return;
+  const int64_t row0 = (int64_t)blockIdx.x * 256 + (threadIdx.x & ~63);
+  const int lane = threadIdx.x & 63;
+  for (uint64_t left = __ballot(row0 + lane < tokens && place_of[min(row0 + lane, tokens - 1)] < 0); left; left &= left - 1) {
+    T* at = dx + (row0 + __builtin_ctzll(left)) * width;
+    if (width % 8 == 0 && (uintptr_t)dx % 16 == 0)
+      for (int64_t i = lane * 8; i < width; i += 512) *reinterpret_cast<uint4*>(at + i) = uint4{0, 0, 0, 0};
+    else
+      for (int64_t i = lane; i < width; i += 64) at[i] = T{0};
   }
 }
 
@@ -351,57 +391,6 @@ pull_listed(const int* __restrict__ count, const int* __restrict__ listed, const
   float v = coef[c].y * exp2f(picked[at] - coef[c].x) - pull[c] * q;
   if (level) v -= level[c];
   slope[c * ld + (w - first_word)] = from_float<T>(v);
-}
-
-// dx from the pieces: row by row of x, rows that do not count are zero.  `sum`: where the pieces of the vocabulary before this one were added up (null: there is
-// none), or, out null, where they go on.
-template <typename T>
-__global__ void __launch_bounds__(256)
-join_input(const float* __restrict__ partial, int splits, int64_t filled, int64_t ld, float* __restrict__ sum, bool first, const int* __restrict__ count,
-           const int* __restrict__ place_of, int64_t tokens, int64_t cols, const float* __restrict__ scale, T* __restrict__ out) {
-  const int64_t units = ld / 4, rows = out ? tokens : (int64_t)*count;
-  const float factor = *scale;
-  for (int64_t u = (int64_t)blockIdx.x * 256 + threadIdx.x; u < rows * units; u += (int64_t)gridDim.x * 256) {
-    const int64_t row = u / units, col = (u - row * units) * 4, c = out ? place_of[row] : row;
-    float4v v = {0, 0, 0, 0};
-    if (c >= 0) {
-      for (int s = 0; s < splits; s++) v += *reinterpret_cast<const float4v*>(partial + ((int64_t)s * filled + c) * ld + col);
-      if (!first) v += *reinterpret_cast<const float4v*>(sum + c * ld + col);
-    }
-    if (!out) {
-      *reinterpret_cast<float4v*>(sum + c * ld + col) = v;
-      continue;
-    }
-    T* at = out + row * cols + col;
-    T o[4];
-#pragma unroll
-    for (int e = 0; e < 4; e++) o[e] = from_float<T>(v[e] * factor);
-    if (cols % 4 == 0 && ((uintptr_t)out & 7) == 0) {
-      if (col < cols) *reinterpret_cast<Pack<T, 4>*>(at) = *reinterpret_cast<Pack<T, 4>*>(o);
-    } else {
-#pragma unroll
-      for (int e = 0; e < 4; e++)
-        if (col + e < cols) at[e] = o[e];
-    }
-  }
-}
-
-// dW of a piece of the vocabulary from the pieces of the tokens
-template <typename OutT>
-__global__ void __launch_bounds__(256)
-join_weight(const float* __restrict__ partial, int splits, const int* __restrict__ count, int64_t rows, int64_t ld, int64_t cols, const float* __restrict__ scale,
-            OutT* __restrict__ out) {
-  const int64_t units = ld / 4;
-  const float factor = *scale;
-  const int pieces = min(splits, token_stages(*count));
-  for (int64_t u = (int64_t)blockIdx.x * 256 + threadIdx.x; u < rows * units; u += (int64_t)gridDim.x * 256) {
-    const int64_t row = u / units, col = (u - row * units) * 4;
-    float4v v = {0, 0, 0, 0};
-    for (int s = 0; s < pieces; s++) v += *reinterpret_cast<const float4v*>(partial + ((int64_t)s * rows + row) * ld + col);
-#pragma unroll
-    for (int e = 0; e < 4; e++)
-      if (col + e < cols) out[row * cols + col + e] = from_float<OutT>(scaled(v[e], factor));
-  }
 }
 
 // db: columns of P, in `pieces` of the tokens, then over the pieces
@@ -465,10 +454,10 @@ State state_of(void* base, int64_t tokens, int64_t entries) {
   Carve part{(uint8_t*)base};
   const int64_t filled = up(tokens, kTile), many = filled * std::max<int64_t>(entries, 1);
   part(s.count, 4);
-  part(s.row_of, filled * 4);
+  part(s.row_of, filled * 4 + kOverread);
   part(s.place_of, filled * 4);
   part(s.lse2, filled * 4);
-  part(s.listed, many * 4);
+  part(s.listed, many * 4 + kOverread);
   part(s.picked, many * 4);
   if (entries) {
     part(s.logq, many * 4);
@@ -480,14 +469,14 @@ State state_of(void* base, int64_t tokens, int64_t entries) {
 
 struct Sizes {
   int64_t tokens, width, words, entries;                         // entries: of a token, 0: a target
-  int64_t filled, k, slabs, word_tiles;
+  int64_t filled, k, slabs, words_filled;
   bool pack_weight, smooth;
 };
 Sizes sizes_of(int64_t tokens, int64_t width, int64_t words, int64_t entries, bool smooth, const void* w, int64_t ldw) {
-  Sizes z{tokens, width, words, entries, up(tokens, kTile), up(width, kStageK), 0, (words + kTile - 1) / kTile, false, smooth};
-  z.slabs = z.word_tiles * 2;
+  Sizes z{tokens, width, words, entries, up(tokens, kTile), up(width, kUnitK), 0, up(words, kTile), false, smooth};
+  z.slabs = z.words_filled / kSlab;
   // rows of whole stages, 16-byte aligned, within reach of 32-bit offsets in a tile
-  z.pack_weight = width % kStageK || ldw % 8 || ldw > (1 << 22) || (uintptr_t)w % 16;
+  z.pack_weight = width % kUnitK || ldw % 8 || ldw > (1 << 22) || (uintptr_t)w % 16;
   return z;
 }
 
@@ -504,64 +493,53 @@ Forward forward_of(void* base, const Sizes& z) {
   Carve part{(uint8_t*)base};
   part(f.x, z.filled * z.k * 2);
   if (z.pack_weight) part(f.w, z.words * z.k * 2);
-  part(f.bias, z.word_tiles * kTile * 4);
+  part(f.bias, z.words_filled * 4 + kOverread);
   part(f.stats, z.slabs * z.filled * 8);
   if (z.smooth) part(f.sums, z.slabs * z.filled * 4);
   part(f.losses, z.filled * 4);
   if (z.entries) {
     part(f.flags, z.filled * 4);
-    part(f.slab_entries, z.slabs * z.filled * 4);
+    part(f.slab_entries, z.slabs * z.filled * 4 + kOverread);
   }
   f.bytes = part.used;
   return f;
 }
 
-// Pieces of a product's k: the number with the least rounds of the compute units x stages of a piece x 0.87 us + 0.32 us per MB of float32 results
-// (as measured on the dense weight gradient's pieces).
-int splits_of(int64_t tiles, int64_t stages, int64_t result_bytes, bool always_partial, int cus) {
-  int best = 1;
-  double least = 1e30;
-  for (int64_t s = 1; s <= std::min<int64_t>(kMaxSplits, stages); s++) {
-    if (s > 1 && s * result_bytes > kPartialBytes) break;
-    const double us = (double)((tiles * s + cus - 1) / cus) * (double)((stages + s - 1) / s) * 0.87 + (s > 1 || always_partial ? (double)(s * result_bytes) * 0.32e-6 : 0.0);
-    if (us < least) { least = us; best = (int)s; }
-  }
-  return best;
-}
+int64_t tiles_of(int64_t size) { return (size + kTile - 1) / kTile; }
 
 struct Backward {
   uint16_t *x, *w = nullptr;
-  float *bias, *level = nullptr, *pull, *out_scale, *partial_x = nullptr, *sum_x = nullptr, *partial_w = nullptr, *bias_sums = nullptr;
+  float *bias, *level = nullptr, *pull, *out_scale, *partial = nullptr, *sum_x = nullptr, *bias_sums = nullptr;
   float2* coef;
   uint8_t* slope;
-  int64_t piece_tiles, pieces, ld, bytes;
-  int splits_x, splits_w;
+  int64_t ld, pieces, bytes;                                     // words of a piece of the vocabulary, pieces
+  int groups, most_x = 0, most_w = 0;                            // workgroups of the products with a long k; pieces of their tiles
 };
 Backward backward_of(void* base, const Sizes& z, bool input, bool weight, bool bias) {
   Backward b;
   Carve part{(uint8_t*)base};
-  const int cus = compute_units();
-  const int64_t most = std::max<int64_t>(1, kSlopeBytes / (z.filled * 2 * kTile));
-  b.pieces = (z.word_tiles + most - 1) / most;
-  b.piece_tiles = (z.word_tiles + b.pieces - 1) / b.pieces;
-  b.pieces = (z.word_tiles + b.piece_tiles - 1) / b.piece_tiles;
-  b.ld = b.piece_tiles * kTile;
-  const int64_t width_tiles = (z.k + kTile - 1) / kTile;
-  b.splits_x = splits_of(width_tiles * (z.filled / kTile), b.ld / kStageK, z.filled * z.k * 4, true, cus);
-  b.splits_w = splits_of(width_tiles * b.piece_tiles, z.filled / kStageK, b.ld * z.k * 4, false, cus);
+  b.groups = std::max(1, compute_units() / 8) * 8;
+  const int64_t blocks = z.words_filled / kTile, at_once = std::max<int64_t>(1, kSlopeBytes / (z.filled * 2 * kTile));
+  b.pieces = (blocks + at_once - 1) / at_once;
+  b.ld = (blocks + b.pieces - 1) / b.pieces * kTile;
+  b.pieces = (z.words_filled + b.ld - 1) / b.ld;
+  const int64_t width_tiles = tiles_of(z.k);
+  auto most = [&](int64_t rest, int64_t stages) { return (int)std::min<int64_t>(kMostPieces, rest * stages); };
+  if (input) b.most_x = most(std::min<int64_t>(width_tiles * tiles_of(z.tokens), b.groups - 1), b.ld / kUnitK);     // (fewer tokens may count: another rest)
+  if (weight) {
+    const int64_t other = z.words_filled - (b.pieces - 1) * b.ld;                                  // the last piece
+    b.most_w = most(std::max(width_tiles * (b.ld / kTile) % b.groups, width_tiles * (other / kTile) % b.groups), z.filled / kUnitK);
+  }
   part(b.x, z.filled * z.k * 2);
   if (z.pack_weight) part(b.w, z.words * z.k * 2);
-  part(b.bias, z.word_tiles * kTile * 4);
-  part(b.coef, z.filled * 8);
-  if (z.smooth) part(b.level, z.filled * 4);
+  part(b.bias, z.words_filled * 4 + kOverread);
+  part(b.coef, z.filled * 8 + kOverread);
+  if (z.smooth) part(b.level, z.filled * 4 + kOverread);
   part(b.pull, z.filled * 4);
   part(b.out_scale, 4);
   part(b.slope, z.filled * b.ld * 2);
-  if (input) {
-    part(b.partial_x, b.splits_x * z.filled * z.k * 4);
-    if (b.pieces > 1) part(b.sum_x, z.filled * z.k * 4);
-  }
-  if (weight && b.splits_w > 1) part(b.partial_w, b.splits_w * b.ld * z.k * 4);
+  part(b.partial, (int64_t)std::max(b.most_x, b.most_w) * kTile * kTile * 4);
+  if (input && b.pieces > 1) part(b.sum_x, width_tiles * z.filled * kTile * 4);
   if (bias) part(b.bias_sums, kBiasPieces * b.ld * 4);
   b.bytes = part.used;
   return b;
@@ -576,7 +554,7 @@ int check_head(const char* fn, const void* x, int64_t ldx, const void* w, int64_
   if (tokens < 1 || tokens > (1 << 22) || width < 1 || width > (1 << 16) || words < 1 || words > (1 << 22))
     return fail(TF24_ERR_SHAPE, "%s: %lld tokens of %lld columns against %lld words: 1 to 2^22, 2^16 and 2^22 are supported", fn, (long long)tokens, (long long)width,
                 (long long)words);
-  if (up(tokens, kTile) / kTile * ((words + kTile - 1) / kTile) > (1 << 26))
+  if (tiles_of(tokens) * tiles_of(words) > (1 << 26))
     return fail(TF24_ERR_SHAPE, "%s: %lld tokens against %lld words are more than one launch takes", fn, (long long)tokens, (long long)words);
   if (entries < 0 || entries > kMaxEntries) return fail(TF24_ERR_SHAPE, "%s: %lld entries of a token, at most %d are supported", fn, (long long)entries, kMaxEntries);
   if (ldx < 0 || ldw < 0) return fail(TF24_ERR_STRIDE, "%s: negative leading dimension", fn);
@@ -653,10 +631,10 @@ extern "C" int tf24_linear_loss_forward(const void* x, int64_t ldx, const void* 
     });
   hipLaunchKernelGGL(count_tokens, dim3(1), dim3(1024), 0, s, targets, ignore, f.flags, (int)tokens, (int)z.filled, words, st.count, st.row_of, st.place_of, st.listed,
                      reduction == TF24_REDUCE_NONE ? loss : nullptr);
-  const bool with_bias = bias || words % kTile;
+  const bool with_bias = bias != nullptr;
   const int64_t cleared = entries ? z.slabs * z.filled / 4 : 0;
   if (with_bias || entries)
-    hipLaunchKernelGGL(prepare_words, dim3(blocks_for(std::max(with_bias ? z.word_tiles * kTile : 0, cleared))), dim3(256), 0, s, bias, bias_dtype, words, z.word_tiles * kTile, scale,
+    hipLaunchKernelGGL(prepare_words, dim3(blocks_for(std::max(with_bias ? z.words_filled : 0, cleared))), dim3(256), 0, s, bias, bias_dtype, words, z.words_filled, scale,
                        with_bias ? f.bias : nullptr, f.slab_entries, cleared);
   if (entries) {
     int padded = 2;
@@ -673,15 +651,15 @@ extern "C" int tf24_linear_loss_forward(const void* x, int64_t ldx, const void* 
   p.b = (const uint8_t*)f.x; p.ldb = z.k * 2;
   p.count = st.count;
   p.rows_i = words;
-  p.stages = (int)(z.k / kStageK); p.tiles_i = (int)z.word_tiles; p.tiles_j = (int)(z.filled / kTile); p.splits = 1;
+  p.stages = (int)(z.k / kUnitK); p.tiles_i = (int)tiles_of(words); p.tiles_j = (int)tiles_of(tokens);
   HeadResult r{};
   r.scale = scale; r.bias = with_bias ? f.bias : nullptr; r.tokens_ld = z.filled;
   r.stats = f.stats; r.sums = f.sums; r.picked = st.picked; r.words = words;
   if (entries) { r.slab_entries = f.slab_entries; r.entry_words = st.listed; r.entries = (int)entries; }
   else r.target = st.listed;
   if (int rc = launch_head_product(HEAD_STATS, dtype, z.smooth, false, p, r, stream)) return rc;
-  const int by = tokens <= 64 ? 0 : 4;
-  hipLaunchKernelGGL(token_losses, dim3((unsigned)(z.filled >> by)), dim3(256), 0, s, f.stats, f.sums, z.filled, LossTerms{smoothing, z_loss, words, (int)z.slabs, (int)entries},
+  const int by = tokens <= 64 ? 0 : tokens <= 4096 ? 2 : 4;       // (workgroups for every compute unit, then loads of whole lines)
+  hipLaunchKernelGGL(token_losses, dim3((unsigned)((tokens + (1 << by) - 1) >> by)), dim3(256), 0, s, f.stats, f.sums, z.filled, LossTerms{smoothing, z_loss, words, (int)z.slabs, (int)entries},
                      st.count, st.row_of, st.listed, st.picked, entries ? st.listed : nullptr, st.logq, st.mass, st.lse2, f.losses,
                      reduction == TF24_REDUCE_NONE ? loss : nullptr, by);
   if (reduction != TF24_REDUCE_NONE) hipLaunchKernelGGL(total_loss, dim3(1), dim3(1024), 0, s, f.losses, st.count, reduction == TF24_REDUCE_MEAN, loss);
@@ -717,26 +695,31 @@ extern "C" int tf24_linear_loss_backward(const float* grad_loss, const void* x, 
   hipStream_t s = (hipStream_t)stream;
   const float scale = kLog2e * inv_temperature;
   const LossTerms how{smoothing, z_loss, words, (int)z.slabs, (int)entries};
-  hipLaunchKernelGGL(slope_terms, dim3(1), dim3(1024), 0, s, grad_loss, reduction, how, inv_temperature, dtype == TF24_F16 ? 14 : 0, st.count, st.row_of,
-                     entries ? nullptr : st.listed, st.mass, st.lse2, b.coef, b.level, b.pull, b.out_scale);
-  const bool with_bias = bias || words % kTile;
+  const SlopeTerms terms{grad_loss, reduction, how, inv_temperature, dtype == TF24_F16 ? 14 : 0};
+  const bool alike = reduction != TF24_REDUCE_NONE && z_loss == 0.0f && !entries;
+  if (!alike) hipLaunchKernelGGL(slope_unit, dim3(1), dim3(1024), 0, s, terms, st.count, st.row_of, st.mass, st.lse2, b.out_scale);
+  auto set_terms = [&](auto* out) {
+    hipLaunchKernelGGL(slope_terms, dim3((unsigned)(z.filled / 256)), dim3(256), 0, s, terms, alike, st.count, st.row_of, entries ? nullptr : st.listed, st.mass, st.lse2, b.coef,
+                       b.level, b.pull, b.out_scale, out, width, st.place_of, tokens);
+  };
+  if (dtype == TF24_F16) set_terms((f16_t*)dx);
+  else set_terms((bf16_t*)dx);
+  const bool with_bias = bias != nullptr;
   if (with_bias)
-    hipLaunchKernelGGL(prepare_words, dim3(blocks_for(z.word_tiles * kTile)), dim3(256), 0, s, bias, bias_dtype, words, z.word_tiles * kTile, scale, b.bias, (uint32_t*)nullptr,
+    hipLaunchKernelGGL(prepare_words, dim3(blocks_for(z.words_filled)), dim3(256), 0, s, bias, bias_dtype, words, z.words_filled, scale, b.bias, (uint32_t*)nullptr,
                        (int64_t)0);
   pack(x, ldx, z.filled, width, st.count, st.row_of, b.x, z.k, s);
   if (b.w) pack(w, ldw, words, width, nullptr, nullptr, b.w, z.k, s);
   const uint8_t* w_at = (const uint8_t*)(b.w ? b.w : w);
   const int64_t w_ld = (b.w ? z.k : ldw) * 2;
-  const int token_tiles_most = (int)(z.filled / kTile), width_tiles = (int)((z.k + kTile - 1) / kTile);
   for (int64_t piece = 0; piece < b.pieces; piece++) {
-    const int64_t first_tile = piece * b.piece_tiles, tiles = std::min(b.piece_tiles, z.word_tiles - first_tile);
-    const int64_t first = first_tile * kTile, here = std::min(tiles * kTile, words - first);
+    const int64_t first = piece * b.ld, here = std::min(b.ld, words - first);
     HeadProduct p{};
     p.a = w_at + first * w_ld; p.lda = w_ld;
     p.b = (const uint8_t*)b.x; p.ldb = z.k * 2;
     p.count = st.count;
     p.rows_i = here;
-    p.stages = (int)(z.k / kStageK); p.tiles_i = (int)tiles; p.tiles_j = token_tiles_most; p.splits = 1;
+    p.stages = (int)(z.k / kUnitK); p.tiles_i = (int)tiles_of(here); p.tiles_j = (int)tiles_of(tokens);
     HeadResult r{};
     r.scale = scale; r.bias = with_bias ? b.bias + first : nullptr; r.tokens_ld = z.filled;
     r.coef = b.coef; r.level = b.level; r.slope = b.slope; r.ld_slope = b.ld; r.words = here;
@@ -748,44 +731,25 @@ extern "C" int tf24_linear_loss_backward(const float* grad_loss, const void* x, 
     };
     if (dtype == TF24_F16) put_right((f16_t*)b.slope);
     else put_right((bf16_t*)b.slope);
+    HeadProduct q{};
+    q.b = b.slope; q.ldb = b.ld * 2;
+    q.count = st.count;
+    q.rows_i = z.k; q.tiles_i = (int)tiles_of(z.k);
+    q.groups = b.groups;
+    HeadResult o{};
+    o.partial = b.partial; o.out_scale = b.out_scale; o.cols_out = width;
     if (dx) {
-      HeadProduct q{};
-      q.a = w_at + first * w_ld; q.lda = w_ld;
-      q.b = b.slope; q.ldb = b.ld * 2;
-      q.count = st.count;
-      q.rows_i = z.k; q.rows_k = here;
-      q.stages = (int)((here + kStageK - 1) / kStageK); q.tiles_i = width_tiles; q.tiles_j = token_tiles_most; q.splits = std::min(b.splits_x, q.stages);
-      HeadResult o{};
-      o.partial = b.partial_x; o.rows_j = z.filled; o.ld_out = z.k;
+      q.a = w_at + first * w_ld; q.lda = w_ld; q.rows_k = here;
+      q.stages = (int)((here + kUnitK - 1) / kUnitK); q.tiles_j = (int)tiles_of(tokens); q.most = b.most_x;
+      o.out = dx; o.row_of = st.row_of; o.sum = b.sum_x; o.add = piece > 0; o.last = piece == b.pieces - 1;
       if (int rc = launch_head_product(HEAD_INPUT, dtype, false, false, q, o, stream)) return rc;
-      const bool last = piece == b.pieces - 1;
-      auto join = [&](auto* out) {
-        hipLaunchKernelGGL(join_input, dim3(blocks_for(z.filled * z.k / 4)), dim3(256), 0, s, b.partial_x, q.splits, z.filled, z.k, b.sum_x, piece == 0, st.count, st.place_of,
-                           tokens, width, b.out_scale, last ? out : nullptr);
-      };
-      if (dtype == TF24_F16) join((f16_t*)dx);
-      else join((bf16_t*)dx);
     }
     if (dw) {
-      HeadProduct q{};
       q.a = (const uint8_t*)b.x; q.lda = z.k * 2;
-      q.b = b.slope; q.ldb = b.ld * 2;
-      q.count = st.count;
-      q.rows_i = z.k;
-      q.stages = (int)(z.filled / kStageK); q.tiles_i = width_tiles; q.tiles_j = (int)tiles; q.splits = b.splits_w;
-      HeadResult o{};
-      o.out = (uint8_t*)dw + first * width * dtype_size(dw_dtype); o.out_scale = b.out_scale;
-      o.rows_j = here; o.cols_out = width; o.ld_out = width;
-      if (b.partial_w) { o.partial = b.partial_w; o.ld_out = z.k; }
+      q.stages = (int)((tokens + kUnitK - 1) / kUnitK); q.tiles_j = (int)tiles_of(here); q.most = b.most_w;
+      if (share_out(q.tiles_i * q.tiles_j, q.stages, q.groups, q.most).pieces == 1) q.most = 0;    // no pieces, whatever number of tokens counts
+      o.out = (uint8_t*)dw + first * width * dtype_size(dw_dtype); o.sum = nullptr; o.add = false; o.last = true; o.rows_j = here;
       if (int rc = launch_head_product(HEAD_WEIGHT, dtype, false, dw_dtype == TF24_F32, q, o, stream)) return rc;
-      if (b.partial_w) {
-        auto join = [&](auto* out) {
-          hipLaunchKernelGGL(join_weight, dim3(blocks_for(here * z.k / 4)), dim3(256), 0, s, b.partial_w, b.splits_w, st.count, here, z.k, width, b.out_scale, out);
-        };
-        if (dw_dtype == TF24_F32) join((float*)o.out);
-        else if (dtype == TF24_F16) join((f16_t*)o.out);
-        else join((bf16_t*)o.out);
-      }
     }
     if (dbias) {
       auto sum = [&](auto* slope) {
