@@ -83,6 +83,10 @@ struct HeadResult {
 
 namespace {
 
+// eight 16-bit elements from anywhere (one load of 16 bytes, whatever the alignment)
+struct __attribute__((packed, aligned(2))) Unaligned8 { int4v v; };
+__device__ __forceinline__ int4v load8(const uint16_t* p) { return reinterpret_cast<const Unaligned8*>(p)->v; }
+
 __device__ __forceinline__ int token_stages(int count) { return max(1, (count + kUnitK - 1) / kUnitK); }
 __device__ __forceinline__ int token_tiles(int count) { return max(1, (count + kTile - 1) / kTile); }
 
@@ -152,7 +156,10 @@ head_product(const HeadProduct p, const HeadResult r) {
     const int gh = min(kRaster, tiles_i - u.group * kRaster);
     int col = (unsigned)u.in_group / kRaster;
     if (gh != kRaster) col = __builtin_amdgcn_readfirstlane((unsigned)u.in_group / (unsigned)gh);
-    u.i0 = (int64_t)(u.group * kRaster + (u.in_group - col * gh)) * kTile;
+    int row = u.in_group - col * gh;
+    // (a workgroup's tiles go round the rows: most of the words that a teacher lists are the frequent ones, in the first row of tiles)
+    if (LOGITS && gh == kRaster) row = (row + col) % kRaster;
+    u.i0 = (int64_t)(u.group * kRaster + row) * kTile;
     u.j0 = (int64_t)col * kTile;
   };
   auto unit_at = [&](int m) {
@@ -348,6 +355,8 @@ head_product(const HeadProduct p, const HeadResult r) {
         // (the accumulators are read once: vector instructions reach them through copies alone)
         float4v y[F][G];
         float m[G], from[G], s[G], sum[G];
+        constexpr int AHEAD = 2;
+        int brought[G], word[G][AHEAD] = {};
 #pragma unroll
         for (int tj = 0; tj < G; tj++) { m[tj] = -__builtin_inff(); s[tj] = 0.0f; sum[tj] = 0.0f; }
 #pragma unroll
@@ -363,6 +372,18 @@ head_product(const HeadProduct p, const HeadResult r) {
             m[tj] = fmaxf(fmaxf(m[tj], y[ti][tj][2]), y[ti][tj][3]);
           }
 #pragma unroll
+        for (int tj = 0; tj < G; tj++) brought[tj] = *reinterpret_cast<const int*>(slice + kTokensAt + ((t0 + tj) * 16 + l16) * 4);
+        if (!r.target) {                                         // the first entries' words, ahead of their use
+#pragma unroll
+          for (int tj = 0; tj < G; tj++) {
+            const int many = brought[tj] >> 11 & 0x7ff;
+            const int64_t entry = (now.j0 + wj * kSlab + (t0 + tj) * 16 + l16) * r.entries + (brought[tj] & 0x7ff);
+#pragma unroll
+            for (int u = 0; u < AHEAD; u++)
+              if (lq + 4 * u < many) word[tj][u] = r.entry_words[entry + lq + 4 * u];
+          }
+        }
+#pragma unroll
         for (int tj = 0; tj < G; tj++) {
           m[tj] = over_quarters(m[tj], [](float a, float b) { return fmaxf(a, b); });
           from[tj] = m[tj] == -__builtin_inff() ? 0.0f : m[tj];
@@ -376,7 +397,6 @@ head_product(const HeadProduct p, const HeadResult r) {
 #pragma unroll
         for (int tj = 0; tj < G; tj++) {
           const int64_t token = now.j0 + wj * kSlab + (t0 + tj) * 16 + l16;
-          const int brought = *reinterpret_cast<const int*>(slice + kTokensAt + ((t0 + tj) * 16 + l16) * 4);
           s[tj] = over_quarters(s[tj], [](float a, float b) { return a + b; });
           if constexpr (SMOOTH) sum[tj] = over_quarters(sum[tj], [](float a, float b) { return a + b; });
           if (lq == 0) {
@@ -384,7 +404,7 @@ head_product(const HeadProduct p, const HeadResult r) {
             if constexpr (SMOOTH) r.sums[slab * r.tokens_ld + token] = sum[tj];
           }
           if (r.target) {
-            const int at = brought - base;
+            const int at = brought[tj] - base;
             if (__any(at >= 0 && at < kSlab)) {
 #pragma unroll
               for (int ti = 0; ti < F; ti++)
@@ -394,23 +414,35 @@ head_product(const HeadProduct p, const HeadResult r) {
             }
           } else {
             // the teacher's entries of these words, four of a token at a time, from the token's row in LDS, eight tokens in turn
-            const int many = brought >> 11 & 0x7ff, first = brought & 0x7ff;
+            const int many = brought[tj] >> 11 & 0x7ff;
+            const int64_t entry = token * r.entries + (brought[tj] & 0x7ff);
             if (__any(many > 0)) {
 #pragma unroll
               for (int half = 0; half < 2; half++) {
                 uint8_t* row = slice + (l16 & 7) * (kSlab * 4);
+                auto pick = [&](int n, int word) {
+                  const int at = word - base;
+                  r.picked[entry + n] = *reinterpret_cast<const float*>(row + ((at >> 2) ^ (l16 & 7)) * 16 + (at & 3) * 4);
+                };
                 wave_lds_fence();
                 if (l16 >> 3 == half) {
 #pragma unroll
                   for (int ti = 0; ti < F; ti++) *reinterpret_cast<float4v*>(row + ((ti * 4 + lq) ^ (l16 & 7)) * 16) = y[ti][tj];
                 }
                 wave_lds_fence();
-                if (l16 >> 3 == half)
-                  for (int n = lq; n < many; n += 4) {
-                    const int64_t entry = token * r.entries + first + n;
-                    const int at = n ? r.entry_words[entry] - base : brought >> 22;
-                    r.picked[entry] = *reinterpret_cast<const float*>(row + ((at >> 2) ^ (l16 & 7)) * 16 + (at & 3) * 4);
+                if (l16 >> 3 == half) {
+#pragma unroll
+                  for (int u = 0; u < AHEAD; u++)
+                    if (lq + 4 * u < many) pick(lq + 4 * u, word[tj][u]);
+                  for (int n0 = lq + 4 * AHEAD; n0 < many; n0 += 16) {       // (four loads in flight)
+                    int more[4];
+#pragma unroll
+                    for (int u = 0; u < 4; u++) more[u] = r.entry_words[entry + min(n0 + 4 * u, many - 1)];
+#pragma unroll
+                    for (int u = 0; u < 4; u++)
+                      if (n0 + 4 * u < many) pick(n0 + 4 * u, more[u]);
                   }
+                }
               }
             }
           }

@@ -102,7 +102,7 @@ template <typename L>
 __global__ void __launch_bounds__(64)
 list_entries(const int64_t* __restrict__ indices, int64_t ld_indices, const L* __restrict__ logits, int64_t ld_logits, const float* __restrict__ teacher_lse,
              float inv_temperature, int entries, int padded, int64_t words, const int* __restrict__ count, const int* __restrict__ row_of,
-             int* __restrict__ entry_words, float* __restrict__ logq, float* __restrict__ mass, uint32_t* __restrict__ slab_entries, int64_t filled) {
+             int* __restrict__ entry_words, float* __restrict__ logq, float* __restrict__ mass, uint32_t* __restrict__ slab_entries, int64_t filled, int slab_words) {
   __shared__ uint64_t key[kMaxEntries];
   __shared__ float value[kMaxEntries];
   const int c = blockIdx.x, lane = threadIdx.x;
@@ -158,15 +158,15 @@ list_entries(const int64_t* __restrict__ indices, int64_t ld_indices, const L* _
     const float l = value[(uint32_t)at] - lse;
     logq[to] = l;
     q += expf(l);
-    const int slab = w / kSlab;
-    if (k == 0 || (int)(key[k - 1] >> 32) / kSlab != slab) {     // the first of its slab
+    const int slab = w / slab_words;
+    if (k == 0 || (int)(key[k - 1] >> 32) / slab_words != slab) {     // the first of its slab
       int low = k, high = entries;                               // low: one of them, high: the first behind them
       while (high - low > 1) {
         const int mid = (low + high) / 2;
-        if (key[mid] != ~0ull && (int)(key[mid] >> 32) / kSlab == slab) low = mid;
+        if (key[mid] != ~0ull && (int)(key[mid] >> 32) / slab_words == slab) low = mid;
         else high = mid;
       }
-      slab_entries[(int64_t)slab * filled + c] = (uint32_t)k | (uint32_t)(high - k) << 11 | (uint32_t)(w - slab * kSlab) << 22;
+      slab_entries[(int64_t)slab * filled + c] = (uint32_t)k | (uint32_t)(high - k) << 11 | (uint32_t)(w - slab * slab_words) << 22;
     }
   }
 #pragma unroll
@@ -178,7 +178,7 @@ list_entries(const int64_t* __restrict__ indices, int64_t ld_indices, const L* _
 // Rows of `cols` 16-bit elements, filled up with zeros to `ld_out` (a multiple of 8): row c of the result is row row_of[c] of the source (null: row c),
 // or zeros behind the last of *count, up to a whole stage.
 __global__ void __launch_bounds__(256)
-pack_rows(const uint16_t* __restrict__ in, int64_t ld, int64_t rows, int64_t cols, bool aligned, const int* __restrict__ count, const int* __restrict__ row_of,
+pack_rows(const uint16_t* __restrict__ in, int64_t ld, int64_t rows, int64_t cols, const int* __restrict__ count, const int* __restrict__ row_of,
           uint16_t* __restrict__ out, int64_t ld_out) {
   const int64_t units = ld_out / 8;
   if (count) rows = (int64_t)token_stages(*count) * kUnitK;
@@ -187,7 +187,7 @@ pack_rows(const uint16_t* __restrict__ in, int64_t ld, int64_t rows, int64_t col
     int4v v = {0, 0, 0, 0};
     if (row >= 0 && col < cols) {
       const uint16_t* at = in + row * ld + col;
-      if (aligned && col + 8 <= cols) v = *reinterpret_cast<const int4v*>(at);
+      if (col + 8 <= cols) v = load8(at);
       else {
 #pragma unroll
         for (int e = 0; e < 8; e++)
@@ -470,19 +470,19 @@ State state_of(void* base, int64_t tokens, int64_t entries) {
 struct Sizes {
   int64_t tokens, width, words, entries;                         // entries: of a token, 0: a target
   int64_t filled, k, slabs, words_filled;
-  bool pack_weight, smooth;
+  bool pack_weight, smooth, few;
 };
 Sizes sizes_of(int64_t tokens, int64_t width, int64_t words, int64_t entries, bool smooth, const void* w, int64_t ldw) {
-  Sizes z{tokens, width, words, entries, up(tokens, kTile), up(width, kUnitK), 0, up(words, kTile), false, smooth};
-  z.slabs = z.words_filled / kSlab;
+  Sizes z{tokens, width, words, entries, up(tokens, kTile), up(width, kUnitK), 0, up(words, kTile), false, smooth, tokens <= kFewTokens};
+  z.slabs = z.few ? (words + kFewSlab - 1) / kFewSlab : z.words_filled / kSlab;
   // rows of whole stages, 16-byte aligned, within reach of 32-bit offsets in a tile
   z.pack_weight = width % kUnitK || ldw % 8 || ldw > (1 << 22) || (uintptr_t)w % 16;
   return z;
 }
 
 struct Forward {
-  uint16_t *x, *w = nullptr;
-  float *bias, *sums = nullptr, *losses;
+  uint16_t *x = nullptr, *w = nullptr;
+  float *bias = nullptr, *sums = nullptr, *losses;
   float2* stats;
   int* flags = nullptr;
   uint32_t* slab_entries = nullptr;
@@ -491,9 +491,11 @@ struct Forward {
 Forward forward_of(void* base, const Sizes& z) {
   Forward f;
   Carve part{(uint8_t*)base};
-  part(f.x, z.filled * z.k * 2);
-  if (z.pack_weight) part(f.w, z.words * z.k * 2);
-  part(f.bias, z.words_filled * 4 + kOverread);
+  if (!z.few) {
+    part(f.x, z.filled * z.k * 2);
+    if (z.pack_weight) part(f.w, z.words * z.k * 2);
+    part(f.bias, z.words_filled * 4 + kOverread);
+  }
   part(f.stats, z.slabs * z.filled * 8);
   if (z.smooth) part(f.sums, z.slabs * z.filled * 4);
   part(f.losses, z.filled * 4);
@@ -568,7 +570,7 @@ int check_head(const char* fn, const void* x, int64_t ldx, const void* w, int64_
 }
 
 void pack(const void* in, int64_t ld, int64_t rows, int64_t cols, const int* count, const int* row_of, uint16_t* out, int64_t ld_out, hipStream_t s) {
-  hipLaunchKernelGGL(pack_rows, dim3(blocks_for(rows * (ld_out / 8))), dim3(256), 0, s, (const uint16_t*)in, ld, rows, cols, ld % 8 == 0 && (uintptr_t)in % 16 == 0, count, row_of,
+  hipLaunchKernelGGL(pack_rows, dim3(blocks_for(rows * (ld_out / 8))), dim3(256), 0, s, (const uint16_t*)in, ld, rows, cols, count, row_of,
                      out, ld_out);
 }
 
@@ -631,8 +633,8 @@ extern "C" int tf24_linear_loss_forward(const void* x, int64_t ldx, const void* 
     });
   hipLaunchKernelGGL(count_tokens, dim3(1), dim3(1024), 0, s, targets, ignore, f.flags, (int)tokens, (int)z.filled, words, st.count, st.row_of, st.place_of, st.listed,
                      reduction == TF24_REDUCE_NONE ? loss : nullptr);
-  const bool with_bias = bias != nullptr;
-  const int64_t cleared = entries ? z.slabs * z.filled / 4 : 0;
+  const bool with_bias = bias && !z.few;
+  const int64_t cleared = entries ? z.slabs * z.filled / 4 : 0;     // (filled is a multiple of 4)
   if (with_bias || entries)
     hipLaunchKernelGGL(prepare_words, dim3(blocks_for(std::max(with_bias ? z.words_filled : 0, cleared))), dim3(256), 0, s, bias, bias_dtype, words, z.words_filled, scale,
                        with_bias ? f.bias : nullptr, f.slab_entries, cleared);
@@ -641,23 +643,27 @@ extern "C" int tf24_linear_loss_forward(const void* x, int64_t ldx, const void* 
     while (padded < entries) padded *= 2;
     teacher([&](auto* logits) {
       hipLaunchKernelGGL(list_entries, dim3((unsigned)tokens), dim3(64), 0, s, indices, ld_indices, logits, ld_teacher, teacher_lse, inv_temperature, (int)entries, padded,
-                         words, st.count, st.row_of, st.listed, st.logq, st.mass, f.slab_entries, z.filled);
+                         words, st.count, st.row_of, st.listed, st.logq, st.mass, f.slab_entries, z.filled, z.few ? kFewSlab : kSlab);
     });
   }
-  pack(x, ldx, z.filled, width, st.count, st.row_of, f.x, z.k, s);
-  if (f.w) pack(w, ldw, words, width, nullptr, nullptr, f.w, z.k, s);
-  HeadProduct p{};
-  p.a = (const uint8_t*)(f.w ? f.w : w); p.lda = (f.w ? z.k : ldw) * 2;
-  p.b = (const uint8_t*)f.x; p.ldb = z.k * 2;
-  p.count = st.count;
-  p.rows_i = words;
-  p.stages = (int)(z.k / kUnitK); p.tiles_i = (int)tiles_of(words); p.tiles_j = (int)tiles_of(tokens);
   HeadResult r{};
-  r.scale = scale; r.bias = with_bias ? f.bias : nullptr; r.tokens_ld = z.filled;
-  r.stats = f.stats; r.sums = f.sums; r.picked = st.picked; r.words = words;
+  r.scale = scale; r.bias = f.bias && bias ? f.bias : nullptr; r.tokens_ld = z.filled; r.words = words;
+  r.stats = f.stats; r.sums = f.sums; r.picked = st.picked;
   if (entries) { r.slab_entries = f.slab_entries; r.entry_words = st.listed; r.entries = (int)entries; }
   else r.target = st.listed;
-  if (int rc = launch_head_product(HEAD_STATS, dtype, z.smooth, false, p, r, stream)) return rc;
+  if (z.few) {
+    if (int rc = launch_few_tokens(dtype, z.smooth, tokens, x, ldx, w, ldw, width, st.count, st.row_of, bias, bias_dtype, r, stream)) return rc;
+  } else {
+    pack(x, ldx, z.filled, width, st.count, st.row_of, f.x, z.k, s);
+    if (f.w) pack(w, ldw, words, width, nullptr, nullptr, f.w, z.k, s);
+    HeadProduct p{};
+    p.a = (const uint8_t*)(f.w ? f.w : w); p.lda = (f.w ? z.k : ldw) * 2;
+    p.b = (const uint8_t*)f.x; p.ldb = z.k * 2;
+    p.count = st.count;
+    p.rows_i = words;
+    p.stages = (int)(z.k / kUnitK); p.tiles_i = (int)tiles_of(words); p.tiles_j = (int)tiles_of(tokens);
+    if (int rc = launch_head_product(HEAD_STATS, dtype, z.smooth, false, p, r, stream)) return rc;
+  }
   const int by = tokens <= 64 ? 0 : tokens <= 4096 ? 2 : 4;       // (workgroups for every compute unit, then loads of whole lines)
   hipLaunchKernelGGL(token_losses, dim3((unsigned)((tokens + (1 << by) - 1) >> by)), dim3(256), 0, s, f.stats, f.sums, z.filled, LossTerms{smoothing, z_loss, words, (int)z.slabs, (int)entries},
                      st.count, st.row_of, st.listed, st.picked, entries ? st.listed : nullptr, st.logq, st.mass, st.lse2, f.losses,

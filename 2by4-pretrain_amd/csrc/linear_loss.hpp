@@ -1,4 +1,4 @@
-// What the files of the vocabulary head's losses share: the launches of its products (linear_loss_products.hip), made by linear_loss.hip.
+// What the files of the vocabulary head's losses share: the launches of its products (linear_loss_products.hip and linear_loss_few.hip), made by linear_loss.hip.
 #pragma once
 #include "tf24_common.hpp"
 
@@ -9,5 +9,10 @@ struct HeadResult;
 
 // smooth: with a sum of the logits (STATS) or a level that is subtracted (SLOPE); wide: float32 results (WEIGHT)
 int launch_head_product(int kind, int dtype, bool smooth, bool wide, const HeadProduct& p, const HeadResult& r, void* stream);
+
+// the forward product of up to 64 tokens (linear_loss_few.hip), operands as they lie: slabs of 64 words, bias as it is
+constexpr int kFewTokens = 64, kFewSlab = 64;
+int launch_few_tokens(int dtype, bool smooth, int64_t tokens, const void* x, int64_t ldx, const void* w, int64_t ldw, int64_t width, const int* count, const int* row_of,
+                      const void* bias, int bias_dtype, const HeadResult& r, void* stream);
 
 }  // namespace tf24

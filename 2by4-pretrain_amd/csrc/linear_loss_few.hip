@@ -1,0 +1,175 @@
+// The logits of few tokens (up to 64) against a whole vocabulary, and what linear_loss.hip wants of them: per token and slab of 64 words a maximum and a sum of
+// exponentials, and the logits of the listed words.
+//
+// Bound by memory: the weight is read once, straight into registers, and as it lies, whatever its rows' alignment (a copy of it in whole aligned stages, as the
+// tiles want it, costs three times the reading).  A workgroup takes 64 words; its four waves share the width out among them, 32 columns a step, so that
+// 16 waves and more of a compute unit have loads in flight, and add up their products through the LDS.  The tokens' rows come from the caches.
+#include "linear_loss.hpp"
+#include "head_tiles.hpp"
+
+namespace tf24 {
+namespace {
+
+constexpr int kWords = 64, kSteps = 4;                           // words of a workgroup; steps whose loads are in flight at once
+
+// the columns of a row that are left of eight
+__device__ __forceinline__ int4v load_up_to(const uint16_t* p, int64_t left) {
+  int4v v = {0, 0, 0, 0};
+#pragma unroll
+  for (int e = 0; e < 8; e++)
+    if (e < left) v[e >> 1] |= (int)((uint32_t)p[e] << (e & 1) * 16);
+  return v;
+}
+
+// Eight columns from dword to dword (a load that crosses dwords takes several times as long: 133 us for 37 tokens against 50257 x 1601), and the
+// last of them from the dword behind where they start in the middle of one.
+struct __attribute__((packed, aligned(4))) Dwords { int4v v; };
+struct Row {
+  const uint32_t* at;                                            // the dword of the row's first column
+  uint32_t shift;                                                // 16: its second half
+  __device__ __forceinline__ explicit Row(const uint16_t* p) : at((const uint32_t*)((uintptr_t)p & ~(uintptr_t)3)), shift(((uintptr_t)p & 2) * 8) {}
+  template <bool HALVES>
+  __device__ __forceinline__ int4v load(int64_t column) const {  // (a multiple of 8)
+    const uint32_t* p = at + column / 2;
+    int4v v = reinterpret_cast<const Dwords*>(p)->v;
+    if constexpr (HALVES) {
+      const uint32_t behind = p[shift ? 4 : 3];
+#pragma unroll
+      for (int e = 0; e < 4; e++) v[e] = (int)__builtin_amdgcn_alignbit(e < 3 ? (uint32_t)v[e + 1] : behind, (uint32_t)v[e], shift);
+    }
+    return v;
+  }
+};
+
+// N: fragments of 16 tokens.  HALVES: rows may start in the middle of a dword
+template <typename T, int N, bool SMOOTH, bool HALVES>
+__global__ void __launch_bounds__(256)
+few_tokens(const uint16_t* __restrict__ x, int64_t ldx, const uint16_t* __restrict__ w, int64_t ldw, int64_t width, const int* __restrict__ count,
+           const int* __restrict__ row_of, const void* __restrict__ bias, int bias_dtype, const HeadResult r) {
+  constexpr int STRIDE = kWords + 4;                             // floats of a token: 16 tokens start 16 bytes apart
+  __shared__ __attribute__((aligned(16))) float part[4][16 * N][STRIDE];
+  const int n = *count;
+  if (!n) return;
+  const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), l16 = lane & 15, lq = lane >> 4;
+  const int64_t word0 = (int64_t)blockIdx.x * kWords;
+  auto weight_row = [&](int f) { return w + min(word0 + f * 16 + l16, r.words - 1) * ldw + lq * 8; };
+  auto token_row = [&](int t) { return x + (int64_t)row_of[t * 16 + l16 < n ? t * 16 + l16 : 0] * ldx + lq * 8; };    // (columns of tokens behind the last are not used)
+  const Row a[4] = {Row(weight_row(0)), Row(weight_row(1)), Row(weight_row(2)), Row(weight_row(3))};
+  const Row b[4] = {Row(token_row(0)), Row(token_row(N > 1 ? 1 : 0)), Row(token_row(N > 2 ? 2 : 0)), Row(token_row(N > 3 ? 3 : 0))};
+  const int steps = (int)(width / 32), begin = wave * steps / 4, end = (wave + 1) * steps / 4;
+  float4v acc[4][N];
+#pragma unroll
+  for (int f = 0; f < 4; f++)
+#pragma unroll
+    for (int t = 0; t < N; t++) acc[f][t] = float4v{0, 0, 0, 0};
+  int s = begin;
+  for (; s + kSteps <= end; s += kSteps) {
+    int4v av[kSteps][4], bv[kSteps][N];
+#pragma unroll
+    for (int u = 0; u < kSteps; u++) {
+#pragma unroll
+      for (int f = 0; f < 4; f++) av[u][f] = a[f].template load<HALVES>((s + u) * 32);
+#pragma unroll
+      for (int t = 0; t < N; t++) bv[u][t] = b[t].template load<HALVES>((s + u) * 32);
+    }
+#pragma unroll
+    for (int u = 0; u < kSteps; u++)
+#pragma unroll
+      for (int f = 0; f < 4; f++)
+#pragma unroll
+        for (int t = 0; t < N; t++) acc[f][t] = mma(T{}, av[u][f], bv[u][t], acc[f][t]);
+  }
+  auto one = [&](auto load) {
+    int4v av[4], bv[N];
+#pragma unroll
+    for (int f = 0; f < 4; f++) av[f] = load(a[f], weight_row(f));
+#pragma unroll
+    for (int t = 0; t < N; t++) bv[t] = load(b[t], token_row(t));
+#pragma unroll
+    for (int f = 0; f < 4; f++)
+#pragma unroll
+      for (int t = 0; t < N; t++) acc[f][t] = mma(T{}, av[f], bv[t], acc[f][t]);
+  };
+  for (; s < end; s++) one([&](const Row& row, const uint16_t*) { return row.template load<HALVES>(s * 32); });
+  if (wave == 3 && width % 32) one([&](const Row&, const uint16_t* p) { return load_up_to(p + steps * 32, width - steps * 32 - lq * 8); });
+
+#pragma unroll
+  for (int f = 0; f < 4; f++)
+#pragma unroll
+    for (int t = 0; t < N; t++) *reinterpret_cast<float4v*>(&part[wave][t * 16 + l16][f * 16 + lq * 4]) = acc[f][t];
+  __syncthreads();
+  // four threads a token, 16 words each
+  const int token = tid >> 2, quarter = tid & 3;
+  if (token >= n || token >= 16 * N) return;                     // (whole groups of four)
+  float y[16], m = -__builtin_inff(), sum = 0.0f, total = 0.0f;
+#pragma unroll
+  for (int e = 0; e < 16; e++) {
+    const int c = quarter * 16 + e;
+    const int64_t word = word0 + c;
+    const float z = (part[0][token][c] + part[1][token][c]) + (part[2][token][c] + part[3][token][c]);
+    float add = 0.0f;
+    if (word >= r.words) add = -__builtin_inff();
+    else if (bias) add = (bias_dtype == TF24_F32 ? ((const float*)bias)[word] : bias_dtype == TF24_F16 ? to_float(((const f16_t*)bias)[word]) : to_float(((const bf16_t*)bias)[word])) * r.scale;
+    y[e] = __builtin_fmaf(z, r.scale, add);
+    m = fmaxf(m, y[e]);
+    if constexpr (SMOOTH) total += word < r.words ? y[e] : 0.0f;
+  }
+  m = fmaxf(m, __shfl_xor(m, 1));
+  m = fmaxf(m, __shfl_xor(m, 2));
+  const float from = m == -__builtin_inff() ? 0.0f : m;
+#pragma unroll
+  for (int e = 0; e < 16; e++) {
+    sum += __builtin_amdgcn_exp2f(y[e] - from);
+    part[0][token][quarter * 16 + e] = y[e];
+  }
+  sum += __shfl_xor(sum, 1);
+  sum += __shfl_xor(sum, 2);
+  if constexpr (SMOOTH) {
+    total += __shfl_xor(total, 1);
+    total += __shfl_xor(total, 2);
+  }
+  const int64_t at = (int64_t)blockIdx.x * r.tokens_ld + token;
+  if (quarter == 0) {
+    r.stats[at] = float2{m, sum};
+    if constexpr (SMOOTH) r.sums[at] = total;
+  }
+  wave_lds_fence();
+  if (r.target) {
+    const int64_t c = r.target[token] - word0;
+    if (quarter == 0 && c >= 0 && c < kWords) r.picked[token] = part[0][token][c];
+  } else {
+    const uint32_t listed = r.slab_entries[at];
+    const int first = (int)(listed & 0x7ff), many = (int)(listed >> 11 & 0x7ff);
+    for (int k = quarter; k < many; k += 4) {
+      const int64_t entry = (int64_t)token * r.entries + first + k;
+      r.picked[entry] = part[0][token][r.entry_words[entry] - word0];
+    }
+  }
+}
+
+}  // namespace
+
+int launch_few_tokens(int dtype, bool smooth, int64_t tokens, const void* x, int64_t ldx, const void* w, int64_t ldw, int64_t width, const int* count, const int* row_of,
+                      const void* bias, int bias_dtype, const HeadResult& r, void* stream) {
+  auto go = [&](auto type, auto n) {
+    using T = decltype(type);
+    auto launch = [&](auto smoothed, auto halves) {
+      hipLaunchKernelGGL((few_tokens<T, decltype(n)::value, decltype(smoothed)::value, decltype(halves)::value>), dim3((unsigned)((r.words + kWords - 1) / kWords)), dim3(256), 0, (hipStream_t)stream,
+                         (const uint16_t*)x, ldx, (const uint16_t*)w, ldw, width, count, row_of, bias, bias_dtype, r);
+    };
+    const bool halves = ldw % 2 || ldx % 2 || (uintptr_t)w % 4 || (uintptr_t)x % 4;
+    if (smooth && halves) launch(std::true_type{}, std::true_type{});
+    else if (smooth) launch(std::true_type{}, std::false_type{});
+    else if (halves) launch(std::false_type{}, std::true_type{});
+    else launch(std::false_type{}, std::false_type{});
+  };
+  auto sized = [&](auto type) {
+    if (tokens <= 16) go(type, std::integral_constant<int, 1>{});
+    else if (tokens <= 32) go(type, std::integral_constant<int, 2>{});
+    else go(type, std::integral_constant<int, 4>{});
+  };
+  if (dtype == TF24_F16) sized(f16_t{}); else sized(bf16_t{});
+  return check_launch("tf24_linear_loss");
+}
+
+}  // namespace tf24
