@@ -372,11 +372,13 @@ slope_terms(SlopeTerms terms, bool alike, const int* __restrict__ count, const i
 }
 
 // The listed words of a piece of the vocabulary in P: one thread per token, or per entry of one; of a word listed twice the first does both.
+// `rest` (null: no gradient of the bias is wanted): by word, what rounding takes from them, in units of 2^-32.  They are most of the bias's gradient, whose sum over
+// tokens is of rounded values otherwise; as whole numbers they can be added in any order.
 template <typename T>
 __global__ void __launch_bounds__(256)
 pull_listed(const int* __restrict__ count, const int* __restrict__ listed, const float* __restrict__ picked, const float* __restrict__ logq, int entries,
             const float2* __restrict__ coef, const float* __restrict__ level, const float* __restrict__ pull, int64_t first_word, int64_t words, T* __restrict__ slope,
-            int64_t ld) {
+            int64_t ld, unsigned long long* __restrict__ rest) {
   const int64_t at = (int64_t)blockIdx.x * 256 + threadIdx.x, c = at / entries;
   if (c >= *count) return;
   const int w = listed[at];
@@ -390,7 +392,15 @@ pull_listed(const int* __restrict__ count, const int* __restrict__ listed, const
   }
   float v = coef[c].y * exp2f(picked[at] - coef[c].x) - pull[c] * q;
   if (level) v -= level[c];
-  slope[c * ld + (w - first_word)] = from_float<T>(v);
+  const T rounded = from_float<T>(v);
+  slope[c * ld + (w - first_word)] = rounded;
+  if (rest) {
+    const float off = v - to_float(rounded);
+    if (fabsf(off) < 65536.0f) atomicAdd(rest + (w - first_word), (unsigned long long)(long long)(off * 4294967296.0f));     // (not of what is infinite or NaN)
+  }
+}
+__global__ void __launch_bounds__(256) clear_rest(unsigned long long* __restrict__ rest, int64_t words) {
+  for (int64_t w = (int64_t)blockIdx.x * 256 + threadIdx.x; w < words; w += (int64_t)gridDim.x * 256) rest[w] = 0;
 }
 
 // db: columns of P, in `pieces` of the tokens, then over the pieces
@@ -419,12 +429,12 @@ sum_columns(const T* __restrict__ slope, int64_t ld, const int* __restrict__ cou
   if ((int64_t)blockIdx.x * 256 + tid < ld) sums[blockIdx.y * ld + (int64_t)blockIdx.x * 256 + tid] = s;
 }
 __global__ void __launch_bounds__(256)
-join_bias(const float* __restrict__ sums, int64_t ld, int64_t words, const float* __restrict__ scale, void* __restrict__ out, int dtype) {
+join_bias(const float* __restrict__ sums, int64_t ld, int64_t words, const unsigned long long* __restrict__ rest, const float* __restrict__ scale, void* __restrict__ out, int dtype) {
   const int64_t w = (int64_t)blockIdx.x * 256 + threadIdx.x;
   if (w >= words) return;
-  float v = 0.0f;
+  float v = (float)((double)(long long)rest[w] * 0x1p-32);
   for (int p = 0; p < kBiasPieces; p++) v += sums[p * ld + w];
-  v *= *scale;
+  v = scaled(v, *scale);
   if (dtype == TF24_F32) ((float*)out)[w] = v;
   else if (dtype == TF24_F16) ((f16_t*)out)[w] = from_float<f16_t>(v);
   else ((bf16_t*)out)[w] = from_float<bf16_t>(v);
@@ -513,6 +523,7 @@ struct Backward {
   uint16_t *x, *w = nullptr;
   float *bias, *level = nullptr, *pull, *out_scale, *partial = nullptr, *sum_x = nullptr, *bias_sums = nullptr;
   float2* coef;
+  unsigned long long* bias_rest = nullptr;
   uint8_t* slope;
   int64_t ld, pieces, bytes;                                     // words of a piece of the vocabulary, pieces
   int groups, most_x = 0, most_w = 0;                            // workgroups of the products with a long k; pieces of their tiles
@@ -542,7 +553,10 @@ Backward backward_of(void* base, const Sizes& z, bool input, bool weight, bool b
   part(b.slope, z.filled * b.ld * 2);
   part(b.partial, (int64_t)std::max(b.most_x, b.most_w) * kTile * kTile * 4);
   if (input && b.pieces > 1) part(b.sum_x, width_tiles * z.filled * kTile * 4);
-  if (bias) part(b.bias_sums, kBiasPieces * b.ld * 4);
+  if (bias) {
+    part(b.bias_sums, kBiasPieces * b.ld * 4);
+    part(b.bias_rest, b.ld * 8);
+  }
   b.bytes = part.used;
   return b;
 }
@@ -731,9 +745,10 @@ extern "C" int tf24_linear_loss_backward(const float* grad_loss, const void* x, 
     r.coef = b.coef; r.level = b.level; r.slope = b.slope; r.ld_slope = b.ld; r.words = here;
     if (int rc = launch_head_product(HEAD_SLOPE, dtype, z.smooth, false, p, r, stream)) return rc;
     const int64_t many = std::max<int64_t>(entries, 1);
+    if (dbias) hipLaunchKernelGGL(clear_rest, dim3(blocks_for(here)), dim3(256), 0, s, b.bias_rest, here);
     auto put_right = [&](auto* slope) {
       hipLaunchKernelGGL(pull_listed, dim3((unsigned)((tokens * many + 255) / 256)), dim3(256), 0, s, st.count, st.listed, st.picked, st.logq, (int)many, b.coef,
-                         b.level, b.pull, first, here, slope, b.ld);
+                         b.level, b.pull, first, here, slope, b.ld, b.bias_rest);
     };
     if (dtype == TF24_F16) put_right((f16_t*)b.slope);
     else put_right((bf16_t*)b.slope);
@@ -763,7 +778,7 @@ extern "C" int tf24_linear_loss_backward(const float* grad_loss, const void* x, 
       };
       if (dtype == TF24_F16) sum((const f16_t*)b.slope);
       else sum((const bf16_t*)b.slope);
-      hipLaunchKernelGGL(join_bias, dim3((unsigned)((here + 255) / 256)), dim3(256), 0, s, b.bias_sums, b.ld, here, b.out_scale,
+      hipLaunchKernelGGL(join_bias, dim3((unsigned)((here + 255) / 256)), dim3(256), 0, s, b.bias_sums, b.ld, here, b.bias_rest, b.out_scale,
                          (void*)((uint8_t*)dbias + first * dtype_size(bias_dtype)), bias_dtype);
     }
   }

@@ -21,23 +21,24 @@ __device__ __forceinline__ int4v load_up_to(const uint16_t* p, int64_t left) {
   return v;
 }
 
-// Eight columns from dword to dword (a load that crosses dwords takes several times as long: 133 us for 37 tokens against 50257 x 1601), and the
-// last of them from the dword behind where they start in the middle of one.
+// A lane's eight columns of a step of a row, from dword to dword (loads that cross dwords take several times as long: 133 us for 37 tokens against 50257 x 1601).
+// Where rows start in the middle of a dword, the columns are moved down by half of one, and the last comes from the dword that follows: the first
+// of the lane 16 further on, or (the last quarter) of the next step.
 struct __attribute__((packed, aligned(4))) Dwords { int4v v; };
 struct Row {
-  const uint32_t* at;                                            // the dword of the row's first column
+  const uint32_t* at;                                            // the dword of the lane's first column
   uint32_t shift;                                                // 16: its second half
   __device__ __forceinline__ explicit Row(const uint16_t* p) : at((const uint32_t*)((uintptr_t)p & ~(uintptr_t)3)), shift(((uintptr_t)p & 2) * 8) {}
-  template <bool HALVES>
-  __device__ __forceinline__ int4v load(int64_t column) const {  // (a multiple of 8)
-    const uint32_t* p = at + column / 2;
-    int4v v = reinterpret_cast<const Dwords*>(p)->v;
-    if constexpr (HALVES) {
-      const uint32_t behind = p[shift ? 4 : 3];
+  __device__ __forceinline__ int4v load(int step) const { return reinterpret_cast<const Dwords*>(at + step * 16)->v; }
+  // in the lanes of the first quarter the dword that follows the steps before `step`, where their last column lies in it (else, as in the other lanes, whatever
+  // they have read already: there may be nothing behind it)
+  __device__ __forceinline__ uint32_t follower(int step, bool first_quarter) const { return at[(first_quarter && shift ? step : step - 1) * 16]; }
+  __device__ __forceinline__ int4v moved(int4v v, uint32_t next_first, bool first_quarter, int from_lane) const {
+    const uint32_t behind = (uint32_t)__builtin_amdgcn_ds_bpermute(from_lane * 4, (int)(first_quarter ? next_first : (uint32_t)v[0]));
+    int4v o;
 #pragma unroll
-      for (int e = 0; e < 4; e++) v[e] = (int)__builtin_amdgcn_alignbit(e < 3 ? (uint32_t)v[e + 1] : behind, (uint32_t)v[e], shift);
-    }
-    return v;
+    for (int e = 0; e < 4; e++) o[e] = (int)__builtin_amdgcn_alignbit(e < 3 ? (uint32_t)v[e + 1] : behind, (uint32_t)v[e], shift);
+    return o;
   }
 };
 
@@ -62,36 +63,54 @@ few_tokens(const uint16_t* __restrict__ x, int64_t ldx, const uint16_t* __restri
   for (int f = 0; f < 4; f++)
 #pragma unroll
     for (int t = 0; t < N; t++) acc[f][t] = float4v{0, 0, 0, 0};
-  int s = begin;
-  for (; s + kSteps <= end; s += kSteps) {
-    int4v av[kSteps][4], bv[kSteps][N];
+  const bool first_quarter = lq == 0;
+  const int from_lane = (lane + 16) & 63;
+  auto some = [&](auto many, int s) {                            // so many steps
+    constexpr int U = decltype(many)::value;
+    int4v av[U][4], bv[U][N];
+    uint32_t af[4], bf[N];
 #pragma unroll
-    for (int u = 0; u < kSteps; u++) {
+    for (int u = 0; u < U; u++) {
 #pragma unroll
-      for (int f = 0; f < 4; f++) av[u][f] = a[f].template load<HALVES>((s + u) * 32);
+      for (int f = 0; f < 4; f++) av[u][f] = a[f].load(s + u);
 #pragma unroll
-      for (int t = 0; t < N; t++) bv[u][t] = b[t].template load<HALVES>((s + u) * 32);
+      for (int t = 0; t < N; t++) bv[u][t] = b[t].load(s + u);
+    }
+    if constexpr (HALVES) {
+#pragma unroll
+      for (int f = 0; f < 4; f++) af[f] = a[f].follower(s + U, first_quarter);
+#pragma unroll
+      for (int t = 0; t < N; t++) bf[t] = b[t].follower(s + U, first_quarter);
+#pragma unroll
+      for (int u = 0; u < U; u++) {
+#pragma unroll
+        for (int f = 0; f < 4; f++) av[u][f] = a[f].moved(av[u][f], u + 1 < U ? (uint32_t)av[u + 1 < U ? u + 1 : u][f][0] : af[f], first_quarter, from_lane);
+#pragma unroll
+        for (int t = 0; t < N; t++) bv[u][t] = b[t].moved(bv[u][t], u + 1 < U ? (uint32_t)bv[u + 1 < U ? u + 1 : u][t][0] : bf[t], first_quarter, from_lane);
+      }
     }
 #pragma unroll
-    for (int u = 0; u < kSteps; u++)
+    for (int u = 0; u < U; u++)
 #pragma unroll
       for (int f = 0; f < 4; f++)
 #pragma unroll
         for (int t = 0; t < N; t++) acc[f][t] = mma(T{}, av[u][f], bv[u][t], acc[f][t]);
-  }
-  auto one = [&](auto load) {
+  };
+  int s = begin;
+  for (; s + kSteps <= end; s += kSteps) some(std::integral_constant<int, kSteps>{}, s);
+  for (; s < end; s++) some(std::integral_constant<int, 1>{}, s);
+  if (wave == 3 && width % 32) {                                 // the columns behind the last whole step
+    const int64_t left = width - steps * 32 - lq * 8;
     int4v av[4], bv[N];
 #pragma unroll
-    for (int f = 0; f < 4; f++) av[f] = load(a[f], weight_row(f));
+    for (int f = 0; f < 4; f++) av[f] = load_up_to(weight_row(f) + steps * 32, left);
 #pragma unroll
-    for (int t = 0; t < N; t++) bv[t] = load(b[t], token_row(t));
+    for (int t = 0; t < N; t++) bv[t] = load_up_to(token_row(t) + steps * 32, left);
 #pragma unroll
     for (int f = 0; f < 4; f++)
 #pragma unroll
       for (int t = 0; t < N; t++) acc[f][t] = mma(T{}, av[f], bv[t], acc[f][t]);
-  };
-  for (; s < end; s++) one([&](const Row& row, const uint16_t*) { return row.template load<HALVES>(s * 32); });
-  if (wave == 3 && width % 32) one([&](const Row&, const uint16_t* p) { return load_up_to(p + steps * 32, width - steps * 32 - lq * 8); });
+  }
 
 #pragma unroll
   for (int f = 0; f < 4; f++)
@@ -166,6 +185,7 @@ int launch_few_tokens(int dtype, bool smooth, int64_t tokens, const void* x, int
   auto sized = [&](auto type) {
     if (tokens <= 16) go(type, std::integral_constant<int, 1>{});
     else if (tokens <= 32) go(type, std::integral_constant<int, 2>{});
+    else if (tokens <= 48) go(type, std::integral_constant<int, 3>{});
     else go(type, std::integral_constant<int, 4>{});
   };
   if (dtype == TF24_F16) sized(f16_t{}); else sized(bf16_t{});

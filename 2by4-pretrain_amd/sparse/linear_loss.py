@@ -6,9 +6,12 @@
 
 The logits of 12 sequences of 1024 tokens over 50304 words are 2.5 GB in float32, and torch's own loss keeps them, their
 softmax and the gradient of both.  Here the forward pass keeps the logarithm of the sum of exponentials of each token, and the backward pass forms the
-logits once more, a piece of the vocabulary at a time.  Tokens that do not count take no part in the products.
+logits once more, a piece of the vocabulary at a time (2 GiB of 16-bit gradients at most, which are gone when it returns).  Tokens that do not count take no part
+in the products.
 The reference has no such operators; its recipe trains models that bring their own head (README.md:56-118).
 """
+from contextlib import nullcontext
+
 import torch
 from torch import autograd, nn
 
@@ -20,6 +23,11 @@ _REDUCTIONS = {"mean": N.REDUCE_MEAN, "sum": N.REDUCE_SUM, "none": N.REDUCE_NONE
 _HALF = (torch.float16, torch.bfloat16)
 _TYPES = (torch.float32, torch.float16, torch.bfloat16)
 _MAX_ENTRIES = 1024
+
+
+def _on_device_of(t):
+    """The tensor's device as the current one, for the sizes of workspaces and the launches that they are for."""
+    return nullcontext() if t.get_device() == torch.cuda.current_device() else torch.cuda.device(t.device)
 
 
 class _linear_loss(autograd.Function):
@@ -40,16 +48,17 @@ class _linear_loss(autograd.Function):
             return loss.zero_()
         lib, code, ptr = N.lib(), N.dtype_codes, N.ptr
         state = torch.empty(lib.tf24_linear_loss_state_bytes(tokens, entries), dtype=torch.uint8, device=x.device)
-        nbytes = lib.tf24_linear_loss_forward_workspace_bytes(tokens, width, words, entries, smoothing != 0.0, w.data_ptr(), ldw)
-        workspace = torch.empty(nbytes, dtype=torch.uint8, device=x.device)
         ld_indices = ld_teacher = 0
         if entries:
             indices, ld_indices = N.as_rows(indices)
             teacher_logits, ld_teacher = N.as_rows(teacher_logits)
-        N.launch(flat, lib.tf24_linear_loss_forward, flat.data_ptr(), ldx, w.data_ptr(), ldw, ptr(bias), N.F32 if bias is None else code[bias.dtype], code[dtype],
-                 tokens, width, words, ptr(target), ignore_index, ptr(indices), ld_indices, ptr(teacher_logits), ld_teacher,
-                 code[teacher_logits.dtype] if entries else N.F32, ptr(teacher_lse), entries, smoothing, z_loss, 1.0 / temperature, reduction, loss.data_ptr(),
-                 state.data_ptr(), state.numel(), workspace.data_ptr(), nbytes)
+        with _on_device_of(x):
+            nbytes = lib.tf24_linear_loss_forward_workspace_bytes(tokens, width, words, entries, smoothing != 0.0, w.data_ptr(), ldw)
+            workspace = torch.empty(nbytes, dtype=torch.uint8, device=x.device)
+            N.check(lib.tf24_linear_loss_forward(
+                flat.data_ptr(), ldx, w.data_ptr(), ldw, ptr(bias), N.F32 if bias is None else code[bias.dtype], code[dtype], tokens, width, words, ptr(target),
+                ignore_index, ptr(indices), ld_indices, ptr(teacher_logits), ld_teacher, code[teacher_logits.dtype] if entries else N.F32, ptr(teacher_lse), entries,
+                smoothing, z_loss, 1.0 / temperature, reduction, loss.data_ptr(), state.data_ptr(), state.numel(), workspace.data_ptr(), nbytes, N.stream_ptr()))
         if any(ctx.needs_input_grad[:3]):
             ctx.save_for_backward(x, weight if weight16 is weight else weight16, bias, state)
         return loss
@@ -74,11 +83,13 @@ class _linear_loss(autograd.Function):
             if bias is not None:
                 bias = N.as_it_was(what, bias, *bias_as, device).resolve_neg().contiguous()
             state = N.as_it_was(what, state, (lib.tf24_linear_loss_state_bytes(tokens, entries),), torch.uint8, device).contiguous()
-            nbytes = lib.tf24_linear_loss_backward_workspace_bytes(tokens, width, words, entries, smoothing != 0.0, w.data_ptr(), ldw, needs[0], needs[1], needs[2])
-            workspace = torch.empty(nbytes, dtype=torch.uint8, device=device)
-            N.launch(flat, lib.tf24_linear_loss_backward, grad_loss.data_ptr(), flat.data_ptr(), ldx, w.data_ptr(), ldw, ptr(bias),
-                     N.F32 if bias is None else code[bias.dtype], code[dtype], tokens, width, words, entries, smoothing, z_loss, 1.0 / temperature, reduction,
-                     state.data_ptr(), state.numel(), ptr(dx), ptr(dw), code[weight_dtype], ptr(db), workspace.data_ptr(), nbytes)
+            with _on_device_of(flat):
+                nbytes = lib.tf24_linear_loss_backward_workspace_bytes(tokens, width, words, entries, smoothing != 0.0, w.data_ptr(), ldw, needs[0], needs[1], needs[2])
+                workspace = torch.empty(nbytes, dtype=torch.uint8, device=device)
+                N.check(lib.tf24_linear_loss_backward(
+                    grad_loss.data_ptr(), flat.data_ptr(), ldx, w.data_ptr(), ldw, ptr(bias), N.F32 if bias is None else code[bias.dtype], code[dtype], tokens, width,
+                    words, entries, smoothing, z_loss, 1.0 / temperature, reduction, state.data_ptr(), state.numel(), ptr(dx), ptr(dw), code[weight_dtype], ptr(db),
+                    workspace.data_ptr(), nbytes, N.stream_ptr()))
         return dx, dw, db, *(None,) * 10
 
 
@@ -150,9 +161,9 @@ def linear_cross_entropy(x, weight, target, bias=None, *, ignore_index=-100, lab
     target = _beside(fn, "target", target, x.shape[:-1], x.device, False)
     reduction = _reduction(fn, reduction)
     smoothing, z_loss = _number(fn, "label_smoothing", label_smoothing, 0.0, 1.0), _number(fn, "z_loss", z_loss, 0.0, 1e30)
-    if not isinstance(ignore_index, int):
-        raise RuntimeError(f"{fn}: ignore_index {ignore_index!r} is not a whole number")
-    return _linear_loss.apply(x, weight, bias, dtype, target.long().contiguous(), ignore_index, None, None, None, smoothing, z_loss, 1.0, reduction)
+    if not isinstance(ignore_index, int) or not -2**63 <= ignore_index < 2**63:
+        raise RuntimeError(f"{fn}: ignore_index {ignore_index!r} is not a whole number of 64 bits")
+    return _linear_loss.apply(x, weight, bias, dtype, target.long().resolve_neg().contiguous(), ignore_index, None, None, None, smoothing, z_loss, 1.0, reduction)
 
 
 def linear_distillation(x, weight, indices, teacher_logits, bias=None, *, teacher_lse=None, temperature=1.0, reduction="mean"):

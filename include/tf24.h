@@ -557,8 +557,8 @@ int64_t tf24_linear_loss_forward_workspace_bytes(int64_t tokens, int64_t width, 
 /*
  * Its backward pass, from the gradient of the loss (one float, or [tokens]), the operands as they were and the state.  dx [tokens, width] of the operands' type
  * (zero rows for tokens that do not count), dw [words, width] of that type or F32, dbias [words] of the bias's; contiguous, each may be NULL.
- *   workspace  as many bytes as the function below says for the results that are wanted: at most 1 GiB of it for the gradient of the logits, 16-bit, of a piece
- *              of the vocabulary
+ *   workspace  as many bytes as the function below says for the results that are wanted: at most 2 GiB of it for the gradient of the logits, 16-bit, of a piece
+ *              of the vocabulary (256 words at least), 256 MB for pieces of the products
  */
 int tf24_linear_loss_backward(const float* grad_loss, const void* x, int64_t ldx, const void* w, int64_t ldw, const void* bias, int bias_dtype, int dtype,
                               int64_t tokens, int64_t width, int64_t words, int64_t entries, float smoothing, float z_loss, float inv_temperature,

@@ -119,9 +119,61 @@ def test_large_vocabulary(cuda, dtype):
             check_loss(sparse.linear_cross_entropy(x, w, target, b, reduction="none"), want, z, counts, x, w, b, "none")
 
 
+@pytest.mark.parametrize("dtype", [F16, BF16])
+@pytest.mark.parametrize("cols", [1, 31, 33, 64, 95, 257, 766])
+def test_few_tokens(cuda, cols, dtype):
+    """1 to 64 tokens, whose weight is read as it lies: every number of tokens that a variant begins and ends with, rows that start in the middle of a dword, tensors that
+    end with their last row, in front of which and behind which there are NaN."""
+    import sparse
+    words = 391
+    for tokens in (1, 2, 16, 17, 32, 33, 48, 49, 63, 64, 65):
+        gen, x, w, b = operands(cuda, tokens + cols, tokens, cols, words, dtype, BF16)
+        around = torch.full(((words + 2) * (cols + 1) + 2,), torch.nan, dtype=dtype, device=cuda)
+        for start, ld in ((1, cols), (2, cols), (1, cols + 1), (2, cols + 1)):
+            held = around.clone().as_strided((words, cols), (ld, 1), start)
+            held.copy_(w)
+            target = torch.randint(-1, words, (tokens,), generator=gen).to(cuda)
+            z = definition.logits(torch.where(target[:, None] == -1, 0, x), w, b)
+            want, _, counts = definition.cross_entropy(z, target, -1, 0.1, 1e-3)
+            with torch.no_grad():
+                loss = sparse.linear_cross_entropy(x, held, target, b, ignore_index=-1, label_smoothing=0.1, z_loss=1e-3, reduction="none")
+            check_loss(loss, want, z, counts, x, w, b, "none")
+            indices, logits = torch.randint(-1, words, (tokens, 70), generator=gen).to(cuda), draw(gen, tokens, 70).to(cuda)
+            z = definition.logits(x, w, b)
+            want, _, counts = definition.distillation(z, indices, logits, temperature=2.0)
+            with torch.no_grad():
+                check_loss(sparse.linear_distillation(x, held, indices, logits, b, temperature=2.0, reduction="none"), want, z, counts, x, w, b, "none", 2.0)
+
+
+@pytest.mark.parametrize("tokens,cols,words", [(520, 1100, 9000), (70, 264, 66000), (2100, 520, 700), (300, 40, 400)])
+def test_pieces_along_k(cuda, tokens, cols, words):
+    """Products of which some tiles are whole and others cut along k, all whole, all cut, and (few tokens count) another share of them than there is room for."""
+    for ignored in (0.0, 0.7, 0.995):
+        gen, x, w, b = operands(cuda, tokens, tokens, cols, words, BF16, F32)
+        target = torch.where(torch.rand(tokens, generator=gen) < ignored, -100, torch.randint(0, words, (tokens,), generator=gen)).to(cuda)
+        ce_check(cuda, x, w, b, target, "none")
+
+
+def test_gradient_of_a_bias_is_that_of_the_unrounded_logits(cuda):
+    """Of few tokens it is one listed word's probability mostly, rounded once and not twice; the order in which tokens come does not matter to the bit."""
+    gen, x, w, b = operands(cuda, 71, 90, 64, 50, BF16, F32)
+    target = torch.randint(0, 50, (90,), generator=gen).to(cuda)
+    z = definition.logits(x, w, b)
+    _, slope, counts = definition.cross_entropy(z, target)
+    grad = torch.tensor(1.0, device=cuda)
+    want = definition.gradients(slope, counts, grad, "sum", x, w, b)[2]
+    got = ce_step(x, w, b, target, grad, reduction="sum")[1][2]
+    # what is not listed is rounded to 8 bits: 2^-9 of each at most, about its root mean square over 90 tokens together; the listed words to 2^-32
+    others = slope.clone()
+    others[torch.arange(90, device=cuda), target] = 0
+    assert ((got.double() - want).abs() <= 2.0 ** -8 * others.abs().sum(0) + 2.0 ** -20).all()
+    again = [ce_step(x, w, b, target, grad, reduction="sum")[1][2] for _ in range(3)]
+    assert all(torch.equal(a, got) for a in again)
+
+
 def test_pieces_of_the_vocabulary(cuda):
     """More tokens than the gradient of all logits at once is formed for."""
-    tokens, cols, words = 30011, 72, 20000
+    tokens, cols, words = 30011, 72, 40000
     gen, x, w, b = operands(cuda, 3, tokens, cols, words, BF16, BF16)
     target = torch.where(torch.rand(tokens, generator=gen) < 0.1, -100, torch.randint(0, words, (tokens,), generator=gen)).to(cuda)
     ce_check(cuda, x, w, b, target)
@@ -431,6 +483,59 @@ def test_head_of_a_model(cuda):
         head(embedding(tokens), target, indices=indices, teacher_logits=logits)
 
 
+def test_two_threads(cuda):
+    """Calls at once from two threads, on streams of their own."""
+    import threading
+    gen, x, w, b = operands(cuda, 73, 500, 200, 3000, BF16, F32)
+    target = torch.randint(0, 3000, (500,), generator=gen).to(cuda)
+    indices, logits = torch.randint(0, 3000, (500, 9), generator=gen).to(cuda), draw(gen, 500, 9).to(cuda)
+    one = torch.tensor(1.0, device=cuda)
+    steps = (lambda: ce_step(x, w, b, target, one), lambda: kd_step(x, w, b, indices, logits, one))
+    want = [step() for step in steps]
+    torch.cuda.synchronize()
+    got = [[], []]
+
+    def run(i):
+        with torch.cuda.stream(torch.cuda.Stream()):
+            for _ in range(5):
+                got[i].append(steps[i]())
+            torch.cuda.current_stream().synchronize()
+
+    threads = [threading.Thread(target=run, args=(i,)) for i in range(2)]
+    [t.start() for t in threads]
+    [t.join() for t in threads]
+    for i in range(2):
+        assert len(got[i]) == 5 and all(torch.equal(r[0], want[i][0]) and all(torch.equal(a, c) for a, c in zip(r[1], want[i][1])) for r in got[i])
+
+
+def test_called_from_compiled_code(cuda):
+    """What the compiler cannot trace it leaves to Python."""
+    import sparse
+    gen, x, w, _ = operands(cuda, 79, 130, 64, 300, BF16)
+    target = torch.randint(0, 300, (130,), generator=gen).to(cuda)
+    want = ce_step(x, w, None, target, torch.tensor(2.0, device=cuda))
+    torch._dynamo.reset()
+    leaves = [x.clone().requires_grad_(), w.clone().requires_grad_()]
+    loss = torch.compile(lambda x, w: sparse.linear_cross_entropy(x, w, target) * 2, backend="eager")(*leaves)
+    loss.backward()
+    torch._dynamo.reset()
+    assert torch.equal(loss.detach(), want[0] * 2) and all(torch.equal(t.grad, g) for t, g in zip(leaves, want[1]))
+
+
+def test_saved_tensors_are_looked_at(cuda):
+    """What a hook hands back instead of a saved tensor is not read as what it is not; what it brings back from the host is."""
+    gen, x, w, _ = operands(cuda, 83, 40, 64, 300, BF16)
+    target = torch.randint(0, 300, (40,), generator=gen).to(cuda)
+    one = torch.tensor(1.0, device=cuda)
+    want = ce_step(x, w, None, target, one)
+    with torch.autograd.graph.saved_tensors_hooks(lambda t: t.cpu(), lambda t: t.to(cuda)):
+        got = ce_step(x, w, None, target, one)
+    assert all(torch.equal(a, c) for a, c in zip(got[1], want[1]))
+    for spoil in (lambda t: t[:1], lambda t: t.cpu(), lambda t: t.float()):
+        with torch.autograd.graph.saved_tensors_hooks(lambda t: t, spoil), pytest.raises(RuntimeError, match="saved"):
+            ce_step(x, w, None, target, one)
+
+
 def test_refusals(cuda):
     import sparse
     x, w, t = torch.zeros(4, 64, dtype=BF16, device=cuda), torch.zeros(10, 64, dtype=BF16, device=cuda), torch.zeros(4, dtype=torch.long, device=cuda)
@@ -440,7 +545,7 @@ def test_refusals(cuda):
                        (lambda: ce(x, w, t[:3]), "target"), (lambda: ce(x, w, t.float()), "dtype"), (lambda: ce(x.float(), w, t), "not supported"),
                        (lambda: ce(x.half(), w, t), "not supported"), (lambda: ce(x, w, t, torch.zeros(9, device=cuda)), "bias"), (lambda: ce(x, w, t, reduction="max"), "reduction"),
                        (lambda: ce(x, w, t, label_smoothing=1.5), "label_smoothing"), (lambda: ce(x, w, t, z_loss=-1.0), "z_loss"), (lambda: ce(x, w, t, z_loss=float("nan")), "z_loss"),
-                       (lambda: ce(x, w, t, ignore_index=None), "ignore_index"), (lambda: ce(x, w, None), "target"), (lambda: ce(x.long(), w, t), "dtype"),
+                       (lambda: ce(x, w, t, ignore_index=None), "ignore_index"), (lambda: ce(x, w, t, ignore_index=1 << 64), "ignore_index"), (lambda: ce(x, w, None), "target"), (lambda: ce(x.long(), w, t), "dtype"),
                        (lambda: kd(x, w, i[:, :0], l[:, :0]), "entries"), (lambda: kd(x, w, i, l[:, :1]), "teacher_logits"), (lambda: kd(x, w, i, l.requires_grad_()), "gradient"),
                        (lambda: kd(x, w, i, l.detach(), temperature=0.0), "temperature"), (lambda: kd(x, w, i, l.detach(), teacher_lse=l[:, 0][:2]), "teacher_lse"),
                        (lambda: kd(x, w, i.expand(4, 2).repeat(1, 600), l.detach().repeat(1, 600)), "entries")):
