@@ -28,9 +28,9 @@ constexpr int kRowBytes = kStageK * 2, kSlowRowBytes = kTile * 2, kOperand = kTi
 constexpr int kCopies = kOperand / 1024 / kWaves;                           // 1 KB copies per wave and operand of a stage
 constexpr int kOverread = 1024;                                             // what is copied for a tile's tokens or words is 1 KB of each kind
 constexpr int kRaster = 8;                                                  // tiles along i of a group
-// a wave's own LDS: 4 KB of results, then 1 KB each of the words' bias and what the tokens bring
+// a wave's own LDS: 4 KB of results (8 of logits), then 1 KB each of the words' bias and what the tokens bring
 constexpr int kLds = 160 * 1024, kScratch = (kLds - kRing * kStage) / kWaves, kBiasAt = 4096, kTokensAt = 5120, kLevelAt = 6144;
-static_assert(kCopies * 1024 * kWaves == kOperand && kScratch >= kLevelAt + 1024, "a stage's copies divide among the waves");
+static_assert(kCopies * 1024 * kWaves == kOperand && kScratch >= kLevelAt + 1024 && kScratch >= 16 * kSlab * 4, "a stage's copies divide among the waves");
 
 // 16-byte chunks of a row of 64 bytes are XOR-swizzled for reads of 16 bytes a lane, which go by lanes 0-3, 12-15, 20-23 and 24-27, then the
 // other 16 of the first 32, and so on: each such group touches every bank once ((row >> 2) & 3, which suits 16 lanes in a row, took twice the cycles)
@@ -349,6 +349,9 @@ head_product(const HeadProduct p, const HeadResult r) {
     if constexpr (KIND == HEAD_STATS) {
       const int64_t slab = now.i0 / kSlab + wi;
       const int base = (int)(slab * kSlab);
+      int brought_all[F];                                        // (from here on all of the wave's LDS is for the logits of listed words)
+#pragma unroll
+      for (int tj = 0; tj < F; tj++) brought_all[tj] = *reinterpret_cast<const int*>(slice + kTokensAt + (tj * 16 + l16) * 4);
       constexpr int G = F / 2;                          // columns of fragments at a time, as far as registers go
 #pragma unroll
       for (int t0 = 0; t0 < F; t0 += G) {
@@ -372,7 +375,7 @@ head_product(const HeadProduct p, const HeadResult r) {
             m[tj] = fmaxf(fmaxf(m[tj], y[ti][tj][2]), y[ti][tj][3]);
           }
 #pragma unroll
-        for (int tj = 0; tj < G; tj++) brought[tj] = *reinterpret_cast<const int*>(slice + kTokensAt + ((t0 + tj) * 16 + l16) * 4);
+        for (int tj = 0; tj < G; tj++) brought[tj] = brought_all[t0 + tj];
         if (!r.target) {                                         // the first entries' words, ahead of their use
 #pragma unroll
           for (int tj = 0; tj < G; tj++) {
@@ -413,36 +416,29 @@ head_product(const HeadProduct p, const HeadResult r) {
                   if (at == ti * 16 + lq * 4 + e) r.picked[token] = y[ti][tj][e];
             }
           } else {
-            // the teacher's entries of these words, four of a token at a time, from the token's row in LDS, eight tokens in turn
+            // the teacher's entries of these words, four of a token at a time, from the token's row in LDS
             const int many = brought[tj] >> 11 & 0x7ff;
             const int64_t entry = token * r.entries + (brought[tj] & 0x7ff);
             if (__any(many > 0)) {
+              uint8_t* row = slice + l16 * (kSlab * 4);
+              auto pick = [&](int n, int word) {
+                const int at = word - base;
+                r.picked[entry + n] = *reinterpret_cast<const float*>(row + ((at >> 2) ^ (l16 & 7)) * 16 + (at & 3) * 4);
+              };
+              wave_lds_fence();
 #pragma unroll
-              for (int half = 0; half < 2; half++) {
-                uint8_t* row = slice + (l16 & 7) * (kSlab * 4);
-                auto pick = [&](int n, int word) {
-                  const int at = word - base;
-                  r.picked[entry + n] = *reinterpret_cast<const float*>(row + ((at >> 2) ^ (l16 & 7)) * 16 + (at & 3) * 4);
-                };
-                wave_lds_fence();
-                if (l16 >> 3 == half) {
+              for (int ti = 0; ti < F; ti++) *reinterpret_cast<float4v*>(row + ((ti * 4 + lq) ^ (l16 & 7)) * 16) = y[ti][tj];
+              wave_lds_fence();
 #pragma unroll
-                  for (int ti = 0; ti < F; ti++) *reinterpret_cast<float4v*>(row + ((ti * 4 + lq) ^ (l16 & 7)) * 16) = y[ti][tj];
-                }
-                wave_lds_fence();
-                if (l16 >> 3 == half) {
+              for (int u = 0; u < AHEAD; u++)
+                if (lq + 4 * u < many) pick(lq + 4 * u, word[tj][u]);
+              for (int n0 = lq + 4 * AHEAD; n0 < many; n0 += 16) {           // (four loads in flight)
+                int more[4];
 #pragma unroll
-                  for (int u = 0; u < AHEAD; u++)
-                    if (lq + 4 * u < many) pick(lq + 4 * u, word[tj][u]);
-                  for (int n0 = lq + 4 * AHEAD; n0 < many; n0 += 16) {       // (four loads in flight)
-                    int more[4];
+                for (int u = 0; u < 4; u++) more[u] = r.entry_words[entry + min(n0 + 4 * u, many - 1)];
 #pragma unroll
-                    for (int u = 0; u < 4; u++) more[u] = r.entry_words[entry + min(n0 + 4 * u, many - 1)];
-#pragma unroll
-                    for (int u = 0; u < 4; u++)
-                      if (n0 + 4 * u < many) pick(n0 + 4 * u, more[u]);
-                  }
-                }
+                for (int u = 0; u < 4; u++)
+                  if (n0 + 4 * u < many) pick(n0 + 4 * u, more[u]);
               }
             }
           }

@@ -645,7 +645,7 @@ extern "C" int tf24_linear_loss_forward(const void* x, int64_t ldx, const void* 
     teacher([&](auto* logits) {
       hipLaunchKernelGGL(flag_tokens, dim3((unsigned)((tokens + 3) / 4)), dim3(256), 0, s, indices, ld_indices, logits, ld_teacher, (int)tokens, (int)entries, f.flags);
     });
-  hipLaunchKernelGGL(count_tokens, dim3(1), dim3(1024), 0, s, targets, ignore, f.flags, (int)tokens, (int)z.filled, words, st.count, st.row_of, st.place_of, st.listed,
+  if (!z.few || entries) hipLaunchKernelGGL(count_tokens, dim3(1), dim3(1024), 0, s, targets, ignore, f.flags, (int)tokens, (int)z.filled, words, st.count, st.row_of, st.place_of, st.listed,
                      reduction == TF24_REDUCE_NONE ? loss : nullptr);
   const bool with_bias = bias && !z.few;
   const int64_t cleared = entries ? z.slabs * z.filled / 4 : 0;     // (filled is a multiple of 4)
@@ -666,7 +666,8 @@ extern "C" int tf24_linear_loss_forward(const void* x, int64_t ldx, const void* 
   if (entries) { r.slab_entries = f.slab_entries; r.entry_words = st.listed; r.entries = (int)entries; }
   else r.target = st.listed;
   if (z.few) {
-    if (int rc = launch_few_tokens(dtype, z.smooth, tokens, x, ldx, w, ldw, width, st.count, st.row_of, bias, bias_dtype, r, stream)) return rc;
+    const FewTokens which{(int)tokens, (int)z.filled, targets, ignore, st.count, st.row_of, st.place_of, st.listed, reduction == TF24_REDUCE_NONE ? loss : nullptr};
+    if (int rc = launch_few_tokens(dtype, z.smooth, which, x, ldx, w, ldw, width, bias, bias_dtype, r, stream)) return rc;
   } else {
     pack(x, ldx, z.filled, width, st.count, st.row_of, f.x, z.k, s);
     if (f.w) pack(w, ldw, words, width, nullptr, nullptr, f.w, z.k, s);

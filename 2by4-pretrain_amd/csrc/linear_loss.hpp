@@ -12,7 +12,14 @@ int launch_head_product(int kind, int dtype, bool smooth, bool wide, const HeadP
 
 // the forward product of up to 64 tokens (linear_loss_few.hip), operands as they lie: slabs of 64 words, bias as it is
 constexpr int kFewTokens = 64, kFewSlab = 64;
-int launch_few_tokens(int dtype, bool smooth, int64_t tokens, const void* x, int64_t ldx, const void* w, int64_t ldw, int64_t width, const int* count, const int* row_of,
-                      const void* bias, int bias_dtype, const HeadResult& r, void* stream);
+struct FewTokens {
+  int tokens, filled;
+  const int64_t* targets;            // null: which tokens count has been found out already
+  int64_t ignore;
+  int *count, *row_of, *place_of, *listed;
+  float* loss;                       // of tokens that do not count, if there is one of each
+};
+int launch_few_tokens(int dtype, bool smooth, const FewTokens& which, const void* x, int64_t ldx, const void* w, int64_t ldw, int64_t width, const void* bias,
+                      int bias_dtype, const HeadResult& r, void* stream);
 
 }  // namespace tf24

@@ -45,16 +45,38 @@ struct Row {
 // N: fragments of 16 tokens.  HALVES: rows may start in the middle of a dword
 template <typename T, int N, bool SMOOTH, bool HALVES>
 __global__ void __launch_bounds__(256)
-few_tokens(const uint16_t* __restrict__ x, int64_t ldx, const uint16_t* __restrict__ w, int64_t ldw, int64_t width, const int* __restrict__ count,
-           const int* __restrict__ row_of, const void* __restrict__ bias, int bias_dtype, const HeadResult r) {
+few_tokens(const uint16_t* __restrict__ x, int64_t ldx, const uint16_t* __restrict__ w, int64_t ldw, int64_t width, const FewTokens which,
+           const void* __restrict__ bias, int bias_dtype, const HeadResult r) {
   constexpr int STRIDE = kWords + 4;                             // floats of a token: 16 tokens start 16 bytes apart
   __shared__ __attribute__((aligned(16))) float part[4][16 * N][STRIDE];
-  const int n = *count;
-  if (!n) return;
+  __shared__ int rows[kFewTokens], wanted[kFewTokens];           // of the tokens that count, and their targets
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), l16 = lane & 15, lq = lane >> 4;
   const int64_t word0 = (int64_t)blockIdx.x * kWords;
+  int n;
+  if (which.targets) {
+    // every workgroup finds out for itself which tokens count; the first one writes it down
+    const int64_t target = lane < which.tokens ? which.targets[lane] : which.ignore;
+    const bool yes = lane < which.tokens && target != which.ignore;
+    const uint64_t mask = __ballot(yes);
+    const int place = __popcll(mask & ((1ull << lane) - 1)), word = target >= 0 && target < r.words ? (int)target : -2;
+    n = __popcll(mask);
+    if (wave == 0 && yes) { rows[place] = lane; wanted[place] = word; }
+    if (blockIdx.x == 0 && wave == 0) {
+      if (lane < which.tokens) which.place_of[lane] = yes ? place : -1;
+      if (yes) { which.row_of[place] = lane; which.listed[place] = word; }
+      if (lane >= n) { which.row_of[lane] = -1; which.listed[lane] = -1; }
+      for (int c = 64 + lane; c < which.filled; c += 64) { which.row_of[c] = -1; which.listed[c] = -1; }
+      if (which.loss && lane < which.tokens && !yes) which.loss[lane] = 0.0f;
+      if (lane == 0) *which.count = n;
+    }
+  } else {
+    n = *which.count;
+    if (wave == 0 && lane < n) rows[lane] = which.row_of[lane];
+  }
+  if (!n) return;
+  __syncthreads();
   auto weight_row = [&](int f) { return w + min(word0 + f * 16 + l16, r.words - 1) * ldw + lq * 8; };
-  auto token_row = [&](int t) { return x + (int64_t)row_of[t * 16 + l16 < n ? t * 16 + l16 : 0] * ldx + lq * 8; };    // (columns of tokens behind the last are not used)
+  auto token_row = [&](int t) { return x + (int64_t)rows[t * 16 + l16 < n ? t * 16 + l16 : 0] * ldx + lq * 8; };    // (columns of tokens behind the last are not used)
   const Row a[4] = {Row(weight_row(0)), Row(weight_row(1)), Row(weight_row(2)), Row(weight_row(3))};
   const Row b[4] = {Row(token_row(0)), Row(token_row(N > 1 ? 1 : 0)), Row(token_row(N > 2 ? 2 : 0)), Row(token_row(N > 3 ? 3 : 0))};
   const int steps = (int)(width / 32), begin = wave * steps / 4, end = (wave + 1) * steps / 4;
@@ -153,8 +175,8 @@ few_tokens(const uint16_t* __restrict__ x, int64_t ldx, const uint16_t* __restri
     if constexpr (SMOOTH) r.sums[at] = total;
   }
   wave_lds_fence();
-  if (r.target) {
-    const int64_t c = r.target[token] - word0;
+  if (which.targets) {
+    const int64_t c = wanted[token] - word0;
     if (quarter == 0 && c >= 0 && c < kWords) r.picked[token] = part[0][token][c];
   } else {
     const uint32_t listed = r.slab_entries[at];
@@ -168,13 +190,13 @@ few_tokens(const uint16_t* __restrict__ x, int64_t ldx, const uint16_t* __restri
 
 }  // namespace
 
-int launch_few_tokens(int dtype, bool smooth, int64_t tokens, const void* x, int64_t ldx, const void* w, int64_t ldw, int64_t width, const int* count, const int* row_of,
-                      const void* bias, int bias_dtype, const HeadResult& r, void* stream) {
+int launch_few_tokens(int dtype, bool smooth, const FewTokens& which, const void* x, int64_t ldx, const void* w, int64_t ldw, int64_t width, const void* bias,
+                      int bias_dtype, const HeadResult& r, void* stream) {
   auto go = [&](auto type, auto n) {
     using T = decltype(type);
     auto launch = [&](auto smoothed, auto halves) {
       hipLaunchKernelGGL((few_tokens<T, decltype(n)::value, decltype(smoothed)::value, decltype(halves)::value>), dim3((unsigned)((r.words + kWords - 1) / kWords)), dim3(256), 0, (hipStream_t)stream,
-                         (const uint16_t*)x, ldx, (const uint16_t*)w, ldw, width, count, row_of, bias, bias_dtype, r);
+                         (const uint16_t*)x, ldx, (const uint16_t*)w, ldw, width, which, bias, bias_dtype, r);
     };
     const bool halves = ldw % 2 || ldx % 2 || (uintptr_t)w % 4 || (uintptr_t)x % 4;
     if (smooth && halves) launch(std::true_type{}, std::true_type{});
@@ -183,9 +205,9 @@ int launch_few_tokens(int dtype, bool smooth, int64_t tokens, const void* x, int
     else launch(std::false_type{}, std::false_type{});
   };
   auto sized = [&](auto type) {
-    if (tokens <= 16) go(type, std::integral_constant<int, 1>{});
-    else if (tokens <= 32) go(type, std::integral_constant<int, 2>{});
-    else if (tokens <= 48) go(type, std::integral_constant<int, 3>{});
+    if (which.tokens <= 16) go(type, std::integral_constant<int, 1>{});
+    else if (which.tokens <= 32) go(type, std::integral_constant<int, 2>{});
+    else if (which.tokens <= 48) go(type, std::integral_constant<int, 3>{});
     else go(type, std::integral_constant<int, 4>{});
   };
   if (dtype == TF24_F16) sized(f16_t{}); else sized(bf16_t{});
