@@ -13,6 +13,14 @@
 // tile, or a piece of its k) as ONE sequence of stages, so that the copies of the next unit run under the end of this one and under what is done
 // with its accumulators; for that there is an LDS area apart, to which what a tile needs of its tokens and words is copied as well.
 // The number of tokens that count lies in device memory: no call waits for it.
+//
+// Bound by the matrix units and the power they draw: at 8192 tokens, 128000 x 4096 bf16 they are busy for 74, 69, 64 and 70 % of the cycles of the four products at
+// 1.93 GHz (6.4, 6.7, 6.7 and 6.3 ms; 1.34, 1.28, 1.28 and 1.36 PFLOP/s; a library's product of the same sizes with nothing of a loss in it 5.9, 6.3 for dx, 7.4 for dW).
+// Short ones by what stands between the tiles, a quarter of STATS and SLOPE at a width of 768: 12288 tokens, 50304 x 768 0.94, 0.93, 0.82 + 0.05 and 0.70 + 0.02 ms
+// (1.01 to 1.35 PFLOP/s; the library 0.85, 1.33 for dx, 0.99 for dW).
+// 256 x 256 tiles against 192 x 192, both passes: 8192 tokens, 128000 x 4096 26.5 and 30.6 ms; 8192 tokens, 50304 x 1024 2.93 and 3.33; 1024 tokens, 50304 x 768 0.42
+// and 0.39 (788 tiles are 3.1 rounds on 256 compute units).  Two buffers of 64 elements of k against four
+// of 32: the forward pass of the first 6.9 and 6.4 ms.
 #pragma once
 #include "lds_copies.hpp"
 #include <algorithm>
@@ -92,7 +100,8 @@ __device__ __forceinline__ int token_tiles(int count) { return max(1, (count + k
 
 // How the tiles of a product with a long k go to `groups` workgroups: as many as fill whole rounds each in one piece, the rest cut along k into as many pieces as
 // cost least, in stages of kUnitK: rounds x stages of a piece, and for each piece of a tile 0.09 of one (256 KB written and read again), 4 for the pass that joins
-// them.  12288 tokens, 50304 x 768 bf16: see linear_loss.hip.
+// them.  With pieces and without, both passes: 1024 tokens, 50304 x 768 (12 and 591 tiles) 0.42 and 1.36 ms; 12288 tokens 3.53 and 3.89 ms; 8192 tokens, 128000 x 4096
+// 26.5 and 26.8.
 struct Share { int whole, rest, pieces; };
 __host__ __device__ inline Share share_out(int tiles, int stages, int groups, int most) {
   Share s{tiles / groups * groups, tiles % groups, 1};
@@ -157,7 +166,8 @@ head_product(const HeadProduct p, const HeadResult r) {
     int col = (unsigned)u.in_group / kRaster;
     if (gh != kRaster) col = __builtin_amdgcn_readfirstlane((unsigned)u.in_group / (unsigned)gh);
     int row = u.in_group - col * gh;
-    // (a workgroup's tiles go round the rows: most of the words that a teacher lists are the frequent ones, in the first row of tiles)
+    // (a workgroup's tiles go round the rows: most of the words that a teacher lists are the frequent ones, in the first row of tiles; 12288 tokens of 64 entries,
+    // forward pass 1.045 ms, as they come 1.076)
     if (LOGITS && gh == kRaster) row = (row + col) % kRaster;
     u.i0 = (int64_t)(u.group * kRaster + row) * kTile;
     u.j0 = (int64_t)col * kTile;

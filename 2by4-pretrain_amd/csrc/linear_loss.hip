@@ -15,6 +15,11 @@
 // 16-bit gradient of the logits is rounded to as well.  It is formed in units of the largest gradient of a token's loss (float16: of 2^-14 of it), which come
 // back behind the products, so that the small probabilities of a large batch do not vanish in float16.
 // All sums are float32 (the loss over tokens: float64), in an order that the sizes alone decide.
+//
+// Bound by the matrix units and, in long products, by the power that they may draw (zeros for operands: 22.4 ms instead of 26.5).  Both passes in bf16, floor at the
+// 1.52 PFLOP/s of a large library product (three products) and measured: 12288 tokens, 50304 x 768 1.87 and 3.52 ms; 8192 tokens, 128000 x 4096 16.9 and
+// 26.2 ms, four products at 1.31 PFLOP/s.  Everything but the four products: 0.14 and 0.15 ms.  The kernels' own figures stand beside them (us; head_tiles.hpp has
+// the products').
 #include "linear_loss.hpp"
 #include "head_tiles.hpp"
 #include <algorithm>
@@ -25,11 +30,12 @@ namespace {
 
 constexpr float kLog2e = 1.44269504088896340736f, kLn2 = 0.69314718055994530942f;
 constexpr int kMaxEntries = 1024;
-constexpr int64_t kSlopeBytes = (int64_t)2 << 30;
+constexpr int64_t kSlopeBytes = (int64_t)2 << 30;                // (8192 tokens, 128000 x 4096, both passes: 26.53 ms, with 512 MB 26.63)
 constexpr int kMostPieces = 1024;                                // tiles' pieces of a product: 256 MB
 
 // ---------------------------------------------------------------- which tokens count
-// A token's place among those that count, and back; the target of each, -2 one that no word has.
+// A token's place among those that count, and back; the target of each, -2 one that no word has.  One workgroup, so that places follow the tokens' order without a
+// second launch: 3 for 1024 tokens, 11 for 12288 (bound by the two passes' loads that wait for each other).
 __global__ void __launch_bounds__(1024)
 count_tokens(const int64_t* __restrict__ targets, int64_t ignore, const int* __restrict__ flags, int tokens, int filled, int64_t words, int* __restrict__ count,
              int* __restrict__ row_of, int* __restrict__ place_of, int* __restrict__ target, float* __restrict__ loss) {
@@ -84,7 +90,7 @@ count_tokens(const int64_t* __restrict__ targets, int64_t ignore, const int* __r
 }
 
 // ---------------------------------------------------------------- the teacher's entries
-// A token counts if one of its entries is used (its word is not negative) and has a logit above -infinity (or NaN).
+// A token counts if one of its entries is used (its word is not negative) and has a logit above -infinity (or NaN).  A wave per token: 5 for 8192 tokens of 64.
 template <typename L>
 __global__ void __launch_bounds__(256)
 flag_tokens(const int64_t* __restrict__ indices, int64_t ld_indices, const L* __restrict__ logits, int64_t ld_logits, int tokens, int entries, int* __restrict__ flags) {
@@ -97,7 +103,8 @@ flag_tokens(const int64_t* __restrict__ indices, int64_t ld_indices, const L* __
 }
 
 // The entries of a token in ascending order of their words (one word listed twice: in the order of the list), the logarithm of the teacher's
-// probability of each, their sum, and where in the list the entries of a slab of words begin.  A workgroup of one wave per token.
+// probability of each, their sum, and where in the list the entries of a slab of words begin.  A workgroup of one wave per token, which sorts them in LDS (a bitonic
+// network): 25 for 8192 tokens of 64 entries as for 4096 of 128, bound by the network's steps that wait for each other.
 template <typename L>
 __global__ void __launch_bounds__(64)
 list_entries(const int64_t* __restrict__ indices, int64_t ld_indices, const L* __restrict__ logits, int64_t ld_logits, const float* __restrict__ teacher_lse,
@@ -176,7 +183,8 @@ list_entries(const int64_t* __restrict__ indices, int64_t ld_indices, const L* _
 
 // ---------------------------------------------------------------- operands as the products read them
 // Rows of `cols` 16-bit elements, filled up with zeros to `ld_out` (a multiple of 8): row c of the result is row row_of[c] of the source (null: row c),
-// or zeros behind the last of *count, up to a whole stage.
+// or zeros behind the last of *count, up to a whole stage.  Bound by memory: 25 for 8192 x 4096 (5.4 TB/s); the weight of 50257 x 1601, whose rows are not aligned, 52
+// (6.2 TB/s, some of it from the caches).
 __global__ void __launch_bounds__(256)
 pack_rows(const uint16_t* __restrict__ in, int64_t ld, int64_t rows, int64_t cols, const int* __restrict__ count, const int* __restrict__ row_of,
           uint16_t* __restrict__ out, int64_t ld_out) {
@@ -214,7 +222,8 @@ prepare_words(const void* __restrict__ bias, int dtype, int64_t words, int64_t f
 // ---------------------------------------------------------------- losses of the tokens
 struct LossTerms { float smoothing, z_loss; int64_t words; int slabs, entries; };
 
-// 2^by tokens of a workgroup, the slabs of each shared out to 256 / 2^by threads
+// 2^by tokens of a workgroup, the slabs of each shared out to 256 / 2^by threads.  Bound by memory and, with few tokens, by the launch: 15 for 12288 tokens of 394
+// slabs (2.6 TB/s), 40 for 8192 tokens of 1000.
 __global__ void __launch_bounds__(256)
 token_losses(const float2* __restrict__ stats, const float* __restrict__ sums, int64_t filled, LossTerms how, const int* __restrict__ count, const int* __restrict__ row_of,
              const int* __restrict__ target, const float* __restrict__ picked, const int* __restrict__ entry_words, const float* __restrict__ logq,
@@ -278,6 +287,7 @@ token_losses(const float2* __restrict__ stats, const float* __restrict__ sums, i
   if (by_token) by_token[row_of[c]] = loss;
 }
 
+// One workgroup, in a fixed order: 5 for 12288 tokens
 __global__ void __launch_bounds__(1024)
 total_loss(const float* __restrict__ by_place, const int* __restrict__ count, bool mean, float* __restrict__ loss) {
   __shared__ double sums[1024];
@@ -306,7 +316,8 @@ __device__ __forceinline__ float widened_by(const SlopeTerms& t, const float* ma
   return mass ? mass[c] : 1.0f + 2.0f * t.how.z_loss * (lse2[c] * kLn2);
 }
 
-// The unit, where tokens differ: from the largest gradient of a token's loss, and the largest factor of one relative to it (what is not finite is that anyhow)
+// The unit, where tokens differ: from the largest gradient of a token's loss, and the largest factor of one relative to it (what is not finite is that anyhow).
+// 9 for 8192 tokens: two passes of one workgroup
 __global__ void __launch_bounds__(1024)
 slope_unit(SlopeTerms terms, const int* __restrict__ count, const int* __restrict__ row_of, const float* __restrict__ mass, const float* __restrict__ lse2,
            float* __restrict__ out_scale) {
@@ -335,7 +346,7 @@ slope_unit(SlopeTerms terms, const int* __restrict__ count, const int* __restric
 }
 
 // The terms of 256 tokens; `alike`: all have the same gradient and a factor of one, which is the unit.  Tokens behind the last get a factor of zero, and rows of dx
-// that do not count are zero.
+// that do not count are zero.  5 for 12288 tokens, 12 with 3000 rows of 1280 columns to clear.
 template <typename T>
 __global__ void __launch_bounds__(256)
 slope_terms(SlopeTerms terms, bool alike, const int* __restrict__ count, const int* __restrict__ row_of, const int* __restrict__ target,
@@ -373,7 +384,7 @@ slope_terms(SlopeTerms terms, bool alike, const int* __restrict__ count, const i
 
 // The listed words of a piece of the vocabulary in P: one thread per token, or per entry of one; of a word listed twice the first does both.
 // `rest` (null: no gradient of the bias is wanted): by word, what rounding takes from them, in units of 2^-32.  They are most of the bias's gradient, whose sum over
-// tokens is of rounded values otherwise; as whole numbers they can be added in any order.
+// tokens is of rounded values otherwise; as whole numbers they can be added in any order.  Bound by single accesses to P: 5 for 12288 targets, 17 for 8192 x 64 entries.
 template <typename T>
 __global__ void __launch_bounds__(256)
 pull_listed(const int* __restrict__ count, const int* __restrict__ listed, const float* __restrict__ picked, const float* __restrict__ logq, int entries,
@@ -403,7 +414,8 @@ __global__ void __launch_bounds__(256) clear_rest(unsigned long long* __restrict
   for (int64_t w = (int64_t)blockIdx.x * 256 + threadIdx.x; w < words; w += (int64_t)gridDim.x * 256) rest[w] = 0;
 }
 
-// db: columns of P, in `pieces` of the tokens, then over the pieces
+// db: columns of P, in `pieces` of the tokens, then over the pieces.  Bound by memory: 30 for 2000 tokens and 50257 words (6.7 TB/s, much of P still in the caches),
+// 5 for the pieces
 constexpr int kBiasPieces = 16;
 template <typename T>
 __global__ void __launch_bounds__(256)
@@ -483,10 +495,14 @@ struct Sizes {
   bool pack_weight, smooth, few;
 };
 Sizes sizes_of(int64_t tokens, int64_t width, int64_t words, int64_t entries, bool smooth, const void* w, int64_t ldw) {
-  Sizes z{tokens, width, words, entries, up(tokens, kTile), up(width, kUnitK), 0, up(words, kTile), false, smooth, tokens <= kFewTokens};
-  z.slabs = z.few ? (words + kFewSlab - 1) / kFewSlab : z.words_filled / kSlab;
+  Sizes z{tokens, width, words, entries, up(tokens, kTile), up(width, kUnitK), 0, up(words, kTile), false, smooth, false};
   // rows of whole stages, 16-byte aligned, within reach of 32-bit offsets in a tile
   z.pack_weight = width % kUnitK || ldw % 8 || ldw > (1 << 22) || (uintptr_t)w % 16;
+  // The kernel for few tokens and the tiles, forward pass in us: 50304 x 768 16 tokens 27 and 40, 48 36 and 41, 64 40 and 41; 50304 x 2048 48 tokens 68 and 64, 64
+  // 73 and 64; 128000 x 4096 16 tokens 237 and 271, 48 266 and 273, 64 286 and 273.  Where tiles need a copy of the weight first: 50257 x 1601 32 tokens 63
+  // and 122, 64 103 and 122.  One limit for both kinds of rows: results do not depend on strides and alignment.
+  z.few = tokens <= kFewTokens;
+  z.slabs = z.few ? (words + kFewSlab - 1) / kFewSlab : z.words_filled / kSlab;
   return z;
 }
 
@@ -645,8 +661,9 @@ extern "C" int tf24_linear_loss_forward(const void* x, int64_t ldx, const void* 
     teacher([&](auto* logits) {
       hipLaunchKernelGGL(flag_tokens, dim3((unsigned)((tokens + 3) / 4)), dim3(256), 0, s, indices, ld_indices, logits, ld_teacher, (int)tokens, (int)entries, f.flags);
     });
-  if (!z.few || entries) hipLaunchKernelGGL(count_tokens, dim3(1), dim3(1024), 0, s, targets, ignore, f.flags, (int)tokens, (int)z.filled, words, st.count, st.row_of, st.place_of, st.listed,
-                     reduction == TF24_REDUCE_NONE ? loss : nullptr);
+  if (!z.few || entries)
+    hipLaunchKernelGGL(count_tokens, dim3(1), dim3(1024), 0, s, targets, ignore, f.flags, (int)tokens, (int)z.filled, words, st.count, st.row_of, st.place_of, st.listed,
+                       reduction == TF24_REDUCE_NONE ? loss : nullptr);
   const bool with_bias = bias && !z.few;
   const int64_t cleared = entries ? z.slabs * z.filled / 4 : 0;     // (filled is a multiple of 4)
   if (with_bias || entries)
@@ -679,7 +696,9 @@ extern "C" int tf24_linear_loss_forward(const void* x, int64_t ldx, const void* 
     p.stages = (int)(z.k / kUnitK); p.tiles_i = (int)tiles_of(words); p.tiles_j = (int)tiles_of(tokens);
     if (int rc = launch_head_product(HEAD_STATS, dtype, z.smooth, false, p, r, stream)) return rc;
   }
-  const int by = tokens <= 64 ? 0 : tokens <= 4096 ? 2 : 4;       // (workgroups for every compute unit, then loads of whole lines)
+  // workgroups for every compute unit, then loads of whole lines (1, 4 and 16 tokens of a workgroup, us for 50304 words: 64 tokens 6, 10 and 22; 1024 tokens 9, 7
+  // and 22; 8192 tokens 32, 20 and 14)
+  const int by = tokens <= 64 ? 0 : tokens <= 4096 ? 2 : 4;
   hipLaunchKernelGGL(token_losses, dim3((unsigned)((tokens + (1 << by) - 1) >> by)), dim3(256), 0, s, f.stats, f.sums, z.filled, LossTerms{smoothing, z_loss, words, (int)z.slabs, (int)entries},
                      st.count, st.row_of, st.listed, st.picked, entries ? st.listed : nullptr, st.logq, st.mass, st.lse2, f.losses,
                      reduction == TF24_REDUCE_NONE ? loss : nullptr, by);

