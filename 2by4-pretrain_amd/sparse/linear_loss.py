@@ -173,7 +173,7 @@ def linear_distillation(x, weight, indices, teacher_logits, bias=None, *, teache
 
     indices [..., entries] (whole numbers) and teacher_logits [..., entries] are the words and the teacher's logits of each token, in any order, 1 to 1024
     of them.  teacher_lse [...] is the logarithm of the sum of exponentials of all of the teacher's logits / temperature; without it the listed words
-    share all of the probability.  An entry with a negative word is unused; a token without a used entry above -inf does not count: loss and gradient
+    share all of the probability.  An entry with a negative word is unused, one with a word past the last makes its token's loss and the gradients NaN; a token without a used entry above -inf does not count: loss and gradient
     zero, nothing of its x read.  A word listed twice has the probability of both.  x, weight, bias, reduction and gradients as in linear_cross_entropy; none for
     the teacher's.  (A loss that is to keep its size over temperatures is multiplied by temperature^2 by the caller.)"""
     fn = "linear_distillation"

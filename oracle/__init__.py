@@ -19,6 +19,7 @@ Pinning status (what fixes each function independently of this file):
   adamw_step_update      torch.optim.AdamW (amsgrad on/off) in phase 1, phase 1 at eps = 0 in phase 2, step-1 closed forms of Z
   gelu_glu_forward/_backward  torch's gelu(approximate='tanh') * x and autograd's gradient of it
   kept, norm, norm_backward   torch's float8_e4m3fn cast; torch's layer_norm / rms_norm in float64 and autograd's gradients
+  linear_loss.*          torch's cross_entropy and kl_div in float64, autograd and differences
   spmm_ref               dense masked fp32 product (definition); parity of the reference's CUTLASS
                          GEMM itself is unpinned (CUTLASS is an un-vendored, unpinned submodule)
 """
