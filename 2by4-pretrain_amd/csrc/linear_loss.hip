@@ -30,6 +30,7 @@ namespace {
 
 constexpr float kLog2e = 1.44269504088896340736f, kLn2 = 0.69314718055994530942f;
 constexpr int kMaxEntries = 1024;
+constexpr int64_t kMostBlocks = 1 << 16;                         // of entries, one to a thread: 2^22 x 1024 threads are more than one launch has
 constexpr int64_t kSlopeBytes = (int64_t)2 << 30;                // (8192 tokens, 128000 x 4096, both passes: 26.53 ms, with 512 MB 26.63)
 constexpr int kMostPieces = 1024;                                // tiles' pieces of a product: 256 MB
 
@@ -390,24 +391,26 @@ __global__ void __launch_bounds__(256)
 pull_listed(const int* __restrict__ count, const int* __restrict__ listed, const float* __restrict__ picked, const float* __restrict__ logq, int entries,
             const float2* __restrict__ coef, const float* __restrict__ level, const float* __restrict__ pull, int64_t first_word, int64_t words, T* __restrict__ slope,
             int64_t ld, unsigned long long* __restrict__ rest) {
-  const int64_t at = (int64_t)blockIdx.x * 256 + threadIdx.x, c = at / entries;
-  if (c >= *count) return;
-  const int w = listed[at];
-  if (w < first_word || w >= first_word + words) return;
-  float q = 1.0f;
-  if (logq) {
-    const int k = (int)(at - c * entries);
-    if (k && listed[at - 1] == w) return;
-    q = expf(logq[at]);
-    for (int j = 1; k + j < entries && listed[at + j] == w; j++) q += expf(logq[at + j]);
-  }
-  float v = coef[c].y * exp2f(picked[at] - coef[c].x) - pull[c] * q;
-  if (level) v -= level[c];
-  const T rounded = from_float<T>(v);
-  slope[c * ld + (w - first_word)] = rounded;
-  if (rest) {
-    const float off = v - to_float(rounded);
-    if (fabsf(off) < 65536.0f) atomicAdd(rest + (w - first_word), (unsigned long long)(long long)(off * 4294967296.0f));     // (not of what is infinite or NaN)
+  const int64_t listed_here = (int64_t)*count * entries;
+  for (int64_t at = (int64_t)blockIdx.x * 256 + threadIdx.x; at < listed_here; at += (int64_t)gridDim.x * 256) {
+    const int w = listed[at];
+    if (w < first_word || w >= first_word + words) continue;
+    const int64_t c = at / entries;
+    float q = 1.0f;
+    if (logq) {
+      const int k = (int)(at - c * entries);
+      if (k && listed[at - 1] == w) continue;
+      q = expf(logq[at]);
+      for (int j = 1; k + j < entries && listed[at + j] == w; j++) q += expf(logq[at + j]);
+    }
+    float v = coef[c].y * exp2f(picked[at] - coef[c].x) - pull[c] * q;
+    if (level) v -= level[c];
+    const T rounded = from_float<T>(v);
+    slope[c * ld + (w - first_word)] = rounded;
+    if (rest) {
+      const float off = v - to_float(rounded);
+      if (fabsf(off) < 65536.0f) atomicAdd(rest + (w - first_word), (unsigned long long)(long long)(off * 4294967296.0f));     // (not of what is infinite or NaN)
+    }
   }
 }
 __global__ void __launch_bounds__(256) clear_rest(unsigned long long* __restrict__ rest, int64_t words) {
@@ -767,7 +770,7 @@ extern "C" int tf24_linear_loss_backward(const float* grad_loss, const void* x, 
     const int64_t many = std::max<int64_t>(entries, 1);
     if (dbias) hipLaunchKernelGGL(clear_rest, dim3(blocks_for(here)), dim3(256), 0, s, b.bias_rest, here);
     auto put_right = [&](auto* slope) {
-      hipLaunchKernelGGL(pull_listed, dim3((unsigned)((tokens * many + 255) / 256)), dim3(256), 0, s, st.count, st.listed, st.picked, st.logq, (int)many, b.coef,
+      hipLaunchKernelGGL(pull_listed, dim3((unsigned)std::min<int64_t>((tokens * many + 255) / 256, kMostBlocks)), dim3(256), 0, s, st.count, st.listed, st.picked, st.logq, (int)many, b.coef,
                          b.level, b.pull, first, here, slope, b.ld, b.bias_rest);
     };
     if (dtype == TF24_F16) put_right((f16_t*)b.slope);

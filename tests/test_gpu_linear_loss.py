@@ -202,6 +202,41 @@ def kd_check(cuda, x, w, b, indices, logits, reduction="mean", seed=6, temperatu
     assert not grads[0].reshape(-1, x.shape[-1])[~counts].any()
 
 
+def test_more_than_2_31_elements(cuda):
+    """Rows of x, dx and the teacher's entries past 2^31 elements: few of the tokens count, the first and the last, and all of them."""
+    import sparse
+    tokens, cols, words = 2200003, 1000, 200
+    rows = torch.cat([torch.arange(1500), torch.arange(tokens - 1500, tokens)]).to(cuda)
+    gen, _, w, _ = operands(cuda, 77, 1, cols, words, BF16)
+    x = torch.empty(tokens, cols, dtype=BF16, device=cuda).normal_().requires_grad_()
+    target = torch.full((tokens,), -100, device=cuda)
+    target[rows] = torch.randint(0, words, (3000,), generator=gen).to(cuda)
+    one = torch.tensor(1.0, device=cuda)
+    few = x.detach()[rows]
+    for some in (True, False):
+        if not some:
+            target[target == -100] = 7
+        leaf = w.clone().requires_grad_()
+        loss = sparse.linear_cross_entropy(x, leaf, target, reduction="none")
+        z = definition.logits(few, w)
+        want, slope, counts = definition.cross_entropy(z, target[rows])
+        check_loss(loss.detach()[rows], want, z, counts, few, w, None, "none")
+        dx, dw = torch.autograd.grad(loss, (x, leaf), one.expand(tokens))
+        *wanted, p = definition.gradients(slope, counts, torch.ones(3000, device=cuda), "none", few, w)
+        check_grads((dx[rows], dw if some else None, None), wanted, p, few, w, None, counts, BF16)
+        if some:
+            assert not loss.detach()[1500:-1500].any() and not dx[1500:-1500].any()
+        del loss, dx, dw
+    indices = torch.randint(-1, words, (tokens, cols), device=cuda)
+    logits = torch.empty(tokens, cols, dtype=BF16, device=cuda).normal_()
+    loss = sparse.linear_distillation(x, w, indices, logits, reduction="none")
+    want, slope, counts = definition.distillation(z, indices[rows], logits[rows])
+    check_loss(loss.detach()[rows], want, z, counts, few, w, None, "none")
+    dx, = torch.autograd.grad(loss, x, one.expand(tokens))
+    *wanted, p = definition.gradients(slope, counts, torch.ones(3000, device=cuda), "none", few, w)
+    check_grads((dx[rows], None, None), wanted, p, few, w, None, counts, BF16)
+
+
 @pytest.mark.parametrize("dtype", [F16, BF16])
 @pytest.mark.parametrize("tokens,cols,words", SIZES)
 def test_distillation(cuda, tokens, cols, words, dtype):
