@@ -4,7 +4,7 @@
 // Bound by memory: the weight is read once, straight into registers, and as it lies, whatever its rows' alignment (a copy of it in whole aligned stages, as the
 // tiles want it, costs three times the reading).  A workgroup takes 64 words; its four waves share the width out among them, 32 columns a step, so that
 // 16 waves and more of a compute unit have loads in flight, and add up their products through the LDS.  The tokens' rows come from the caches.
-// One token, 50304 x 768 bf16 (77 MB): 19 us, 4.1 TB/s; 16 tokens, 128000 x 4096 (1 GB): 4.5 TB/s; 37 tokens, 50257 x 1601 float16, every other row in the middle of a
+// One token, 50304 x 768 bf16 (77 MB): 18 us, 4.3 TB/s; 16 tokens, 128000 x 4096 (1 GB): 185 us, 5.7 TB/s; 37 tokens, 50257 x 1601 float16, every other row in the middle of a
 // dword: 62 us, 2.6 TB/s, bound by the loads' passes over lines that 16 bytes from any address cross.
 #include "linear_loss.hpp"
 #include "head_tiles.hpp"
@@ -12,7 +12,7 @@
 namespace tf24 {
 namespace {
 
-constexpr int kWords = 64, kSteps = 4;                           // words of a workgroup; steps whose loads are in flight at once
+constexpr int kWords = 64;                                       // of a workgroup
 
 // the columns of a row that are left of eight
 __device__ __forceinline__ int4v load_up_to(const uint16_t* p, int64_t left) {
@@ -44,13 +44,20 @@ struct Row {
   }
 };
 
-// N: fragments of 16 tokens.  HALVES: rows may start in the middle of a dword
+// N: fragments of 16 tokens.  HALVES: rows may start in the middle of a dword.
+// kSteps: steps whose loads are in flight at once.  Two, and registers for two workgroups of a compute unit at least, against four: 16 tokens, 128000 x 4096 196 us
+// (so without the bound on registers; with it 225) and 238, 48 tokens 236 and 266.  Where the loads are to be moved, which takes registers of its own, four and
+// no bound against two of each: 37 tokens, 50257 x 1601 68 and 70, 64 tokens 79 and 96.
 template <typename T, int N, bool SMOOTH, bool HALVES>
-__global__ void __launch_bounds__(256)
+__global__ void __launch_bounds__(256, HALVES || N == 1 ? 1 : 2)
 few_tokens(const uint16_t* __restrict__ x, int64_t ldx, const uint16_t* __restrict__ w, int64_t ldw, int64_t width, const FewTokens which,
            const void* __restrict__ bias, int bias_dtype, const HeadResult r) {
   constexpr int STRIDE = kWords + 4;                             // floats of a token: 16 tokens start 16 bytes apart
-  __shared__ __attribute__((aligned(16))) float part[4][16 * N][STRIDE];
+  constexpr int kSteps = HALVES ? 4 : 2;
+  // The waves' parts of a sum: of all four where the LDS holds them beside those of other workgroups, else of two, to which the others add theirs (64 tokens, 50257 x
+  // 1601 102 us with four parts, 79 with two; 48 tokens, 50304 x 768 34 and 31; 32 tokens, 50257 x 1601 63 and 70).
+  constexpr int PARTS = N <= 2 ? 4 : 2;
+  __shared__ __attribute__((aligned(16))) float part[PARTS][16 * N][STRIDE];
   __shared__ int rows[kFewTokens], wanted[kFewTokens];           // of the tokens that count, and their targets
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), l16 = lane & 15, lq = lane >> 4;
   const int64_t word0 = (int64_t)blockIdx.x * kWords;
@@ -122,7 +129,8 @@ few_tokens(const uint16_t* __restrict__ x, int64_t ldx, const uint16_t* __restri
   };
   int s = begin;
   for (; s + kSteps <= end; s += kSteps) some(std::integral_constant<int, kSteps>{}, s);
-  for (; s < end; s++) some(std::integral_constant<int, 1>{}, s);
+  if (kSteps > 2 && s + 2 <= end) { some(std::integral_constant<int, 2>{}, s); s += 2; }
+  if (s < end) some(std::integral_constant<int, 1>{}, s);
   if (wave == 3 && width % 32) {                                 // the columns behind the last whole step
     const int64_t left = width - steps * 32 - lq * 8;
     int4v av[4], bv[N];
@@ -137,10 +145,18 @@ few_tokens(const uint16_t* __restrict__ x, int64_t ldx, const uint16_t* __restri
   }
 
 #pragma unroll
-  for (int f = 0; f < 4; f++)
+  for (int turn = 4 / PARTS - 1; turn >= 0; turn--) {            // (the last waves first)
+    if (wave / PARTS == turn) {
 #pragma unroll
-    for (int t = 0; t < N; t++) *reinterpret_cast<float4v*>(&part[wave][t * 16 + l16][f * 16 + lq * 4]) = acc[f][t];
-  __syncthreads();
+      for (int f = 0; f < 4; f++)
+#pragma unroll
+        for (int t = 0; t < N; t++) {
+          float4v* at = reinterpret_cast<float4v*>(&part[wave % PARTS][t * 16 + l16][f * 16 + lq * 4]);
+          *at = PARTS == 4 || turn ? acc[f][t] : acc[f][t] + *at;
+        }
+    }
+    __syncthreads();
+  }
   // four threads a token, 16 words each
   const int token = tid >> 2, quarter = tid & 3;
   if (token >= n || token >= 16 * N) return;                     // (whole groups of four)
@@ -149,7 +165,8 @@ few_tokens(const uint16_t* __restrict__ x, int64_t ldx, const uint16_t* __restri
   for (int e = 0; e < 16; e++) {
     const int c = quarter * 16 + e;
     const int64_t word = word0 + c;
-    const float z = (part[0][token][c] + part[1][token][c]) + (part[2][token][c] + part[3][token][c]);
+    float z = part[0][token][c] + part[1][token][c];
+    if constexpr (PARTS == 4) z += part[2][token][c] + part[3][token][c];
     float add = 0.0f;
     if (word >= r.words) add = -__builtin_inff();
     else if (bias) add = (bias_dtype == TF24_F32 ? ((const float*)bias)[word] : bias_dtype == TF24_F16 ? to_float(((const f16_t*)bias)[word]) : to_float(((const bf16_t*)bias)[word])) * r.scale;
