@@ -502,7 +502,7 @@ Sizes sizes_of(int64_t tokens, int64_t width, int64_t words, int64_t entries, bo
   // rows of whole stages, 16-byte aligned, within reach of 32-bit offsets in a tile
   z.pack_weight = width % kUnitK || ldw % 8 || ldw > (1 << 22) || (uintptr_t)w % 16;
   // The kernel for few tokens and the tiles, forward pass in us: 50304 x 768 1 token 25 and 40, 64 tokens 37 and 41; 128000 x 4096 16 tokens 195 and 266, 64 266
-  // and 269; 50304 x 2048 16 tokens 49 and 63, 64 72 and 64.  Where tiles need a copy of the weight first: 50257 x 1601 32 tokens 63 and 119, 64 79 and 119.  One
+  // and 269; 50304 x 2048 16 tokens 49 and 63, 64 72 and 64.  Where tiles need a copy of the weight first: 50257 x 1601 32 tokens 56 and 119, 64 72 and 119.  One
   // limit for both kinds of rows: results do not depend on strides and alignment.
   z.few = tokens <= kFewTokens;
   z.slabs = z.few ? (words + kFewSlab - 1) / kFewSlab : z.words_filled / kSlab;

@@ -5,7 +5,7 @@
 // tiles want it, costs three times the reading).  A workgroup takes 64 words; its four waves share the width out among them, 32 columns a step, so that
 // 16 waves and more of a compute unit have loads in flight, and add up their products through the LDS.  The tokens' rows come from the caches.
 // One token, 50304 x 768 bf16 (77 MB): 18 us, 4.3 TB/s; 16 tokens, 128000 x 4096 (1 GB): 185 us, 5.7 TB/s; 37 tokens, 50257 x 1601 float16, every other row in the middle of a
-// dword: 62 us, 2.6 TB/s, bound by the loads' passes over lines that 16 bytes from any address cross.
+// dword: 58 us, 2.8 TB/s, bound by what moves the tokens' and the weight's columns into place (one token: 43 us).
 #include "linear_loss.hpp"
 #include "head_tiles.hpp"
 
@@ -23,41 +23,54 @@ __device__ __forceinline__ int4v load_up_to(const uint16_t* p, int64_t left) {
   return v;
 }
 
-// A lane's eight columns of a step of a row, from dword to dword (loads that cross dwords take several times as long: 133 us for 37 tokens against 50257 x 1601).
-// Where rows start in the middle of a dword, the columns are moved down by half of one, and the last comes from the dword that follows: the first
-// of the lane 16 further on, or (the last quarter) of the next step.
-struct __attribute__((packed, aligned(4))) Dwords { int4v v; };
+// A step's 64 bytes of a row, 16 to each of the four lanes that share it.  What a load costs is the blocks of 64 bytes that it touches: rows that do not start at one
+// are loaded block by block, each once (16 bytes from wherever they start: 16 tokens, 50257 x 1601 62 us for 50, 37 tokens x 4097 195 for 151; two whole pieces of
+// 16 bytes for each: 139), and a step is put together from two of them: dword j of a lane's 16 bytes is dword j + `turn` of a
+// block that lies `quarters` (or one more) lanes further on, in the same block or in the next.  In the end halves of dwords are moved.
+template <bool MOVED>
 struct Row {
-  const uint32_t* at;                                            // the dword of the lane's first column
-  uint32_t shift;                                                // 16: its second half
-  __device__ __forceinline__ explicit Row(const uint16_t* p) : at((const uint32_t*)((uintptr_t)p & ~(uintptr_t)3)), shift(((uintptr_t)p & 2) * 8) {}
-  __device__ __forceinline__ int4v load(int step) const { return reinterpret_cast<const Dwords*>(at + step * 16)->v; }
-  // in the lanes of the first quarter the dword that follows the steps before `step`, where their last column lies in it (else, as in the other lanes, whatever
-  // they have read already: there may be nothing behind it)
-  __device__ __forceinline__ uint32_t follower(int step, bool first_quarter) const { return at[(first_quarter && shift ? step : step - 1) * 16]; }
-  __device__ __forceinline__ int4v moved(int4v v, uint32_t next_first, bool first_quarter, int from_lane) const {
-    const uint32_t behind = (uint32_t)__builtin_amdgcn_ds_bpermute(from_lane * 4, (int)(first_quarter ? next_first : (uint32_t)v[0]));
+  const uint8_t* at;                                             // the lane's 16 bytes of the first block
+  uint32_t turn, half;
+  int quarters, last;                                            // last: block that the row's part has something in
+  __device__ __forceinline__ Row(const uint16_t* p, int lq, int end) {
+    const uint32_t off = MOVED ? (uint32_t)(uintptr_t)p & 63 : 0;
+    at = (const uint8_t*)p - off + lq * 16;
+    turn = off >> 2 & 3; half = (off & 2) * 8; quarters = (int)(off >> 4);
+    last = off ? end : end - 1;
+  }
+  __device__ __forceinline__ int4v load(int step) const { return *reinterpret_cast<const int4v*>(at + step * 64); }
+  __device__ __forceinline__ int4v block(int step) const { return load(min(step, last)); }
+  __device__ __forceinline__ int4v turned(int4v v) const {
+    const int4v t = {turn & 2 ? v[2] : v[0], turn & 2 ? v[3] : v[1], turn & 2 ? v[0] : v[2], turn & 2 ? v[1] : v[3]};
+    return int4v{turn & 1 ? t[1] : t[0], turn & 1 ? t[2] : t[1], turn & 1 ? t[3] : t[2], turn & 1 ? t[0] : t[3]};
+  }
+  __device__ __forceinline__ int4v joined(int4v now, int4v next, int lq, int l16) const {      // both turned
+    uint32_t d[5];
+#pragma unroll
+    for (int j = 0; j < 5; j++) {
+      const int on = quarters + (j + (int)turn >= 4 ? 1 : 0);
+      d[j] = (uint32_t)__builtin_amdgcn_ds_bpermute((((lq + on) & 3) * 16 + l16) * 4, lq >= on ? now[j & 3] : next[j & 3]);
+    }
     int4v o;
 #pragma unroll
-    for (int e = 0; e < 4; e++) o[e] = (int)__builtin_amdgcn_alignbit(e < 3 ? (uint32_t)v[e + 1] : behind, (uint32_t)v[e], shift);
+    for (int i = 0; i < 4; i++) o[i] = (int)__builtin_amdgcn_alignbit(d[i + 1], d[i], half);
     return o;
   }
 };
 
-// N: fragments of 16 tokens.  HALVES: rows may start in the middle of a dword.
+// N: fragments of 16 tokens.  MOVED: rows do not all start at 16 bytes (where they do, but not at 64, the moving costs more than it saves: 16 tokens, 50304 x 776 31
+// us, moved 38).
 // kSteps: steps whose loads are in flight at once.  Two, and registers for two workgroups of a compute unit at least, against four: 16 tokens, 128000 x 4096 196 us
-// (so without the bound on registers; with it 225) and 238, 48 tokens 236 and 266.  Where the loads are to be moved, which takes registers of its own, four and
-// no bound against two of each: 37 tokens, 50257 x 1601 68 and 70, 64 tokens 79 and 96.
-template <typename T, int N, bool SMOOTH, bool HALVES>
-__global__ void __launch_bounds__(256, HALVES || N == 1 ? 1 : 2)
+// (so without the bound on registers; with it 225) and 238, 48 tokens 236 and 266.  Where steps are moved, which takes registers of its own, one against two: 37
+// tokens, 50257 x 1601 62 and 81, 64 tokens 72 and 93, and with the bound 68 and 63, 73 and 92.
+template <typename T, int N, bool SMOOTH, bool MOVED>
+__global__ void __launch_bounds__(256, MOVED || N == 1 ? 1 : 2)
 few_tokens(const uint16_t* __restrict__ x, int64_t ldx, const uint16_t* __restrict__ w, int64_t ldw, int64_t width, const FewTokens which,
            const void* __restrict__ bias, int bias_dtype, const HeadResult r) {
   constexpr int STRIDE = kWords + 4;                             // floats of a token: 16 tokens start 16 bytes apart
-  constexpr int kSteps = HALVES ? 4 : 2;
-  // The waves' parts of a sum: of all four where the LDS holds them beside those of other workgroups, else of two, to which the others add theirs (64 tokens, 50257 x
-  // 1601 102 us with four parts, 79 with two; 48 tokens, 50304 x 768 34 and 31; 32 tokens, 50257 x 1601 63 and 70).
-  constexpr int PARTS = N <= 2 ? 4 : 2;
-  __shared__ __attribute__((aligned(16))) float part[PARTS][16 * N][STRIDE];
+  constexpr int kSteps = MOVED ? 1 : 2;
+  // the parts of a sum that two waves have, to which the others add theirs (parts of all four: fewer workgroups; 48 tokens, 50304 x 768 33 us for 31)
+  __shared__ __attribute__((aligned(16))) float part[2][16 * N][STRIDE];
   __shared__ int rows[kFewTokens], wanted[kFewTokens];           // of the tokens that count, and their targets
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), l16 = lane & 15, lq = lane >> 4;
   const int64_t word0 = (int64_t)blockIdx.x * kWords;
@@ -84,60 +97,62 @@ few_tokens(const uint16_t* __restrict__ x, int64_t ldx, const uint16_t* __restri
   }
   if (!n) return;
   __syncthreads();
-  auto weight_row = [&](int f) { return w + min(word0 + f * 16 + l16, r.words - 1) * ldw + lq * 8; };
-  auto token_row = [&](int t) { return x + (int64_t)rows[t * 16 + l16 < n ? t * 16 + l16 : 0] * ldx + lq * 8; };    // (columns of tokens behind the last are not used)
-  const Row a[4] = {Row(weight_row(0)), Row(weight_row(1)), Row(weight_row(2)), Row(weight_row(3))};
-  const Row b[4] = {Row(token_row(0)), Row(token_row(N > 1 ? 1 : 0)), Row(token_row(N > 2 ? 2 : 0)), Row(token_row(N > 3 ? 3 : 0))};
   const int steps = (int)(width / 32), begin = wave * steps / 4, end = (wave + 1) * steps / 4;
+  auto weight_row = [&](int f) { return w + min(word0 + f * 16 + l16, r.words - 1) * ldw; };
+  auto token_row = [&](int t) { return x + (int64_t)rows[t * 16 + l16 < n ? t * 16 + l16 : 0] * ldx; };    // (columns of tokens behind the last are not used)
+  const Row<MOVED> a[4] = {Row<MOVED>(weight_row(0), lq, end), Row<MOVED>(weight_row(1), lq, end), Row<MOVED>(weight_row(2), lq, end), Row<MOVED>(weight_row(3), lq, end)};
+  const Row<MOVED> b[4] = {Row<MOVED>(token_row(0), lq, end), Row<MOVED>(token_row(N > 1 ? 1 : 0), lq, end), Row<MOVED>(token_row(N > 2 ? 2 : 0), lq, end), Row<MOVED>(token_row(N > 3 ? 3 : 0), lq, end)};
   float4v acc[4][N];
 #pragma unroll
   for (int f = 0; f < 4; f++)
 #pragma unroll
     for (int t = 0; t < N; t++) acc[f][t] = float4v{0, 0, 0, 0};
-  const bool first_quarter = lq == 0;
-  const int from_lane = (lane + 16) & 63;
+  int4v a0[4], b0[N];                                            // MOVED: the blocks that the steps from here on begin in
+  if (MOVED && begin < end) {
+#pragma unroll
+    for (int f = 0; f < 4; f++) a0[f] = a[f].turned(a[f].load(begin));
+#pragma unroll
+    for (int t = 0; t < N; t++) b0[t] = b[t].turned(b[t].load(begin));
+  }
   auto some = [&](auto many, int s) {                            // so many steps
     constexpr int U = decltype(many)::value;
     int4v av[U][4], bv[U][N];
-    uint32_t af[4], bf[N];
 #pragma unroll
     for (int u = 0; u < U; u++) {
 #pragma unroll
-      for (int f = 0; f < 4; f++) av[u][f] = a[f].load(s + u);
+      for (int f = 0; f < 4; f++) av[u][f] = MOVED ? a[f].block(s + u + 1) : a[f].load(s + u);
 #pragma unroll
-      for (int t = 0; t < N; t++) bv[u][t] = b[t].load(s + u);
+      for (int t = 0; t < N; t++) bv[u][t] = MOVED ? b[t].block(s + u + 1) : b[t].load(s + u);
     }
-    if constexpr (HALVES) {
 #pragma unroll
-      for (int f = 0; f < 4; f++) af[f] = a[f].follower(s + U, first_quarter);
+    for (int u = 0; u < U; u++) {
+      if constexpr (MOVED) {
+        auto move = [&](const Row<MOVED>& row, int4v& before, int4v& v) {
+          const int4v next = row.turned(v);
+          v = row.joined(before, next, lq, l16);
+          before = next;
+        };
 #pragma unroll
-      for (int t = 0; t < N; t++) bf[t] = b[t].follower(s + U, first_quarter);
+        for (int f = 0; f < 4; f++) move(a[f], a0[f], av[u][f]);
 #pragma unroll
-      for (int u = 0; u < U; u++) {
-#pragma unroll
-        for (int f = 0; f < 4; f++) av[u][f] = a[f].moved(av[u][f], u + 1 < U ? (uint32_t)av[u + 1 < U ? u + 1 : u][f][0] : af[f], first_quarter, from_lane);
-#pragma unroll
-        for (int t = 0; t < N; t++) bv[u][t] = b[t].moved(bv[u][t], u + 1 < U ? (uint32_t)bv[u + 1 < U ? u + 1 : u][t][0] : bf[t], first_quarter, from_lane);
+        for (int t = 0; t < N; t++) move(b[t], b0[t], bv[u][t]);
       }
-    }
-#pragma unroll
-    for (int u = 0; u < U; u++)
 #pragma unroll
       for (int f = 0; f < 4; f++)
 #pragma unroll
         for (int t = 0; t < N; t++) acc[f][t] = mma(T{}, av[u][f], bv[u][t], acc[f][t]);
+    }
   };
   int s = begin;
   for (; s + kSteps <= end; s += kSteps) some(std::integral_constant<int, kSteps>{}, s);
-  if (kSteps > 2 && s + 2 <= end) { some(std::integral_constant<int, 2>{}, s); s += 2; }
-  if (s < end) some(std::integral_constant<int, 1>{}, s);
+  if (kSteps > 1 && s < end) some(std::integral_constant<int, 1>{}, s);
   if (wave == 3 && width % 32) {                                 // the columns behind the last whole step
     const int64_t left = width - steps * 32 - lq * 8;
     int4v av[4], bv[N];
 #pragma unroll
-    for (int f = 0; f < 4; f++) av[f] = load_up_to(weight_row(f) + steps * 32, left);
+    for (int f = 0; f < 4; f++) av[f] = load_up_to(weight_row(f) + steps * 32 + lq * 8, left);
 #pragma unroll
-    for (int t = 0; t < N; t++) bv[t] = load_up_to(token_row(t) + steps * 32, left);
+    for (int t = 0; t < N; t++) bv[t] = load_up_to(token_row(t) + steps * 32 + lq * 8, left);
 #pragma unroll
     for (int f = 0; f < 4; f++)
 #pragma unroll
@@ -145,14 +160,14 @@ few_tokens(const uint16_t* __restrict__ x, int64_t ldx, const uint16_t* __restri
   }
 
 #pragma unroll
-  for (int turn = 4 / PARTS - 1; turn >= 0; turn--) {            // (the last waves first)
-    if (wave / PARTS == turn) {
+  for (int first = 2; first >= 0; first -= 2) {
+    if (wave - first == 0 || wave - first == 1) {
 #pragma unroll
       for (int f = 0; f < 4; f++)
 #pragma unroll
         for (int t = 0; t < N; t++) {
-          float4v* at = reinterpret_cast<float4v*>(&part[wave % PARTS][t * 16 + l16][f * 16 + lq * 4]);
-          *at = PARTS == 4 || turn ? acc[f][t] : acc[f][t] + *at;
+          float4v* at = reinterpret_cast<float4v*>(&part[wave - first][t * 16 + l16][f * 16 + lq * 4]);
+          *at = first ? acc[f][t] : acc[f][t] + *at;
         }
     }
     __syncthreads();
@@ -165,8 +180,7 @@ few_tokens(const uint16_t* __restrict__ x, int64_t ldx, const uint16_t* __restri
   for (int e = 0; e < 16; e++) {
     const int c = quarter * 16 + e;
     const int64_t word = word0 + c;
-    float z = part[0][token][c] + part[1][token][c];
-    if constexpr (PARTS == 4) z += part[2][token][c] + part[3][token][c];
+    const float z = part[0][token][c] + part[1][token][c];
     float add = 0.0f;
     if (word >= r.words) add = -__builtin_inff();
     else if (bias) add = (bias_dtype == TF24_F32 ? ((const float*)bias)[word] : bias_dtype == TF24_F16 ? to_float(((const f16_t*)bias)[word]) : to_float(((const bf16_t*)bias)[word])) * r.scale;
@@ -213,14 +227,14 @@ int launch_few_tokens(int dtype, bool smooth, const FewTokens& which, const void
                       int bias_dtype, const HeadResult& r, void* stream) {
   auto go = [&](auto type, auto n) {
     using T = decltype(type);
-    auto launch = [&](auto smoothed, auto halves) {
-      hipLaunchKernelGGL((few_tokens<T, decltype(n)::value, decltype(smoothed)::value, decltype(halves)::value>), dim3((unsigned)((r.words + kWords - 1) / kWords)), dim3(256), 0, (hipStream_t)stream,
+    auto launch = [&](auto smoothed, auto moved) {
+      hipLaunchKernelGGL((few_tokens<T, decltype(n)::value, decltype(smoothed)::value, decltype(moved)::value>), dim3((unsigned)((r.words + kWords - 1) / kWords)), dim3(256), 0, (hipStream_t)stream,
                          (const uint16_t*)x, ldx, (const uint16_t*)w, ldw, width, which, bias, bias_dtype, r);
     };
-    const bool halves = ldw % 2 || ldx % 2 || (uintptr_t)w % 4 || (uintptr_t)x % 4;
-    if (smooth && halves) launch(std::true_type{}, std::true_type{});
+    const bool moved = ldw % 8 || ldx % 8 || (uintptr_t)w % 16 || (uintptr_t)x % 16;
+    if (smooth && moved) launch(std::true_type{}, std::true_type{});
     else if (smooth) launch(std::true_type{}, std::false_type{});
-    else if (halves) launch(std::false_type{}, std::true_type{});
+    else if (moved) launch(std::false_type{}, std::true_type{});
     else launch(std::false_type{}, std::false_type{});
   };
   auto sized = [&](auto type) {
