@@ -36,8 +36,8 @@ constexpr int kRowBytes = kStageK * 2, kSlowRowBytes = kTile * 2, kOperand = kTi
 constexpr int kCopies = kOperand / 1024 / kWaves;                           // 1 KB copies per wave and operand of a stage
 constexpr int kOverread = 1024;                                             // what is copied for a tile's tokens or words is 1 KB of each kind
 constexpr int kRaster = 8;                                                  // tiles along i of a group
-// a wave's own LDS: 4 KB of results (8 of logits), then 1 KB each of the words' bias and what the tokens bring
-constexpr int kLds = 160 * 1024, kScratch = (kLds - kRing * kStage) / kWaves, kBiasAt = 4096, kTokensAt = 5120, kLevelAt = 6144;
+// a wave's own LDS: 4 KB of results (8 of logits), then 1 KB each of what the tile's columns bring and what its rows do
+constexpr int kLds = 160 * 1024, kScratch = (kLds - kRing * kStage) / kWaves, kColumnsAt = 4096, kTokensAt = 5120, kLevelAt = 6144;
 static_assert(kCopies * 1024 * kWaves == kOperand && kScratch >= kLevelAt + 1024 && kScratch >= 16 * kSlab * 4, "a stage's copies divide among the waves");
 
 // 16-byte chunks of a row of 64 bytes are XOR-swizzled for reads of 16 bytes a lane, which go by lanes 0-3, 12-15, 20-23 and 24-27, then the
@@ -76,10 +76,12 @@ struct HeadResult {
   int entries;
   // HEAD_SLOPE
   const float2* coef;                // [token] log-sum-exp, factor
-  const float* level;                // SMOOTH: [token] what is subtracted everywhere
+  const float* level;                // SMOOTH: [token] what is subtracted everywhere, a number of 16 bits
   void* slope;
   int64_t ld_slope;
   // HEAD_INPUT, HEAD_WEIGHT
+  const float* common;               // SMOOTH: [column, filled up to whole tiles with anything] what is subtracted from every row
+  const float* level_rest;           // INPUT, SMOOTH: so many times [token]
   float* partial;                    // [piece][tile of the rest][kTile^2], as the accumulators lie
   float* sum;                        // [tile][kTile^2]: what the pieces of the vocabulary before this one gave (add), and where it goes on (not last)
   bool add, last;
@@ -324,7 +326,7 @@ head_product(const HeadProduct p, const HeadResult r) {
     const int64_t token = now.j0 + wj * kSlab;
     if constexpr (KIND == HEAD_INPUT) g2l16((const uint8_t*)(r.row_of + token), off, to + kTokensAt);
     if constexpr (LOGITS) {
-      if (r.bias) g2l16((const uint8_t*)(r.bias + now.i0 + wi * kSlab), off, to + kBiasAt);
+      if (r.bias) g2l16((const uint8_t*)(r.bias + now.i0 + wi * kSlab), off, to + kColumnsAt);
       if constexpr (KIND == HEAD_STATS) {
         const uint8_t* from = r.target ? (const uint8_t*)(r.target + token) : (const uint8_t*)(r.slab_entries + (now.i0 / kSlab + wi) * r.tokens_ld + token);
         g2l16(from, off, to + kTokensAt);
@@ -332,6 +334,9 @@ head_product(const HeadProduct p, const HeadResult r) {
         g2l16((const uint8_t*)(r.coef + token), off, to + kTokensAt);
         if constexpr (SMOOTH) g2l16((const uint8_t*)(r.level + token), off, to + kLevelAt);
       }
+    } else if constexpr (SMOOTH) {
+      g2l16((const uint8_t*)(r.common + now.i0 + wi * kSlab), off, to + kColumnsAt);
+      if constexpr (KIND == HEAD_INPUT) g2l16((const uint8_t*)(r.level_rest + token), off, to + kLevelAt);
     }
   };
   constexpr int ROW16 = kSlab * 2, CHUNKS = kSlab / 8;             // 16-bit results go out by 16 rows, through the wave's 4 KB
@@ -349,7 +354,7 @@ head_product(const HeadProduct p, const HeadResult r) {
     if constexpr (LOGITS) {
 #pragma unroll
       for (int ti = 0; ti < F; ti++) {
-        if (r.bias) add[ti] = *reinterpret_cast<const float4v*>(slice + kBiasAt + (ti * 16 + lq * 4) * 4);
+        if (r.bias) add[ti] = *reinterpret_cast<const float4v*>(slice + kColumnsAt + (ti * 16 + lq * 4) * 4);
         else {
 #pragma unroll
           for (int e = 0; e < 4; e++) add[ti][e] = now.i0 + wi * kSlab + ti * 16 + lq * 4 + e < r.words ? 0.0f : -__builtin_inff();
@@ -475,6 +480,19 @@ head_product(const HeadProduct p, const HeadResult r) {
           wave_lds_fence();
           asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
           return;
+        }
+        if constexpr (SMOOTH) {
+          float times[F];
+#pragma unroll
+          for (int tj = 0; tj < F; tj++) times[tj] = KIND == HEAD_INPUT ? *reinterpret_cast<const float*>(slice + kLevelAt + (tj * 16 + l16) * 4) : 1.0f;
+#pragma unroll
+          for (int ti = 0; ti < F; ti++) {
+            const float4v common = *reinterpret_cast<const float4v*>(slice + kColumnsAt + (ti * 16 + lq * 4) * 4);
+#pragma unroll
+            for (int tj = 0; tj < F; tj++)
+#pragma unroll
+              for (int e = 0; e < 4; e++) acc[ti][tj][e] = __builtin_fmaf(-times[tj], common[e], acc[ti][tj][e]);
+          }
         }
       }
       const int64_t rows = KIND == HEAD_INPUT ? (int64_t)count : r.rows_j, cols = r.cols_out;

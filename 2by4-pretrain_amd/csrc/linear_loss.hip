@@ -308,6 +308,11 @@ total_loss(const float* __restrict__ by_place, const int* __restrict__ count, bo
 // Per token that counts: P = factor exp2(y - lse2) - level everywhere, less `pull` times the listed probabilities, all of it in units of the largest gradient of
 // a token's loss: of a mean P is 1 - p at the target, which rounding to 8 bits moves by 2^-9 where 4/3 of it (1 / 12288 less its power of
 // two) is moved by 2^-8.
+// The level, g smoothing / words, is nearly all of the gradient of a word that is far less probable.  Rounded in P it would be off in the same way for all of those words and
+// all tokens (by 0.39 % of it at worst in bfloat16), which no sum averages out.  So P has the nearest number of 16 bits in its place, and what is left of it comes to the results
+// in float32: dx is P W less the rest times the sum of W's rows, dW P^T x less the sum of x's rows times their rests, db the sum of P less that of the rests.  (Without a
+// level in P a word whose probability is near it would be off by more: by a step of p, not one of the difference.)  W is read once more for it: both passes of 2000 tokens against
+// 50257 x 1280 1150 and 1190, of one token against 50304 x 768 157 and 182.
 struct SlopeTerms { const float* grad; int reduction; LossTerms how; float inv_temperature; int to_exponent; };
 __device__ __forceinline__ float upstream_of(const SlopeTerms& t, int row, int n) {
   const float g = t.reduction == TF24_REDUCE_NONE ? t.grad[row] : t.reduction == TF24_REDUCE_MEAN ? t.grad[0] / (float)n : t.grad[0];
@@ -351,8 +356,8 @@ slope_unit(SlopeTerms terms, const int* __restrict__ count, const int* __restric
 template <typename T>
 __global__ void __launch_bounds__(256)
 slope_terms(SlopeTerms terms, bool alike, const int* __restrict__ count, const int* __restrict__ row_of, const int* __restrict__ target,
-            const float* __restrict__ mass, const float* __restrict__ lse2, float2* __restrict__ coef, float* __restrict__ level, float* __restrict__ pull,
-            float* __restrict__ out_scale, T* __restrict__ dx, int64_t width, const int* __restrict__ place_of, int64_t tokens) {
+            const float* __restrict__ mass, const float* __restrict__ lse2, float2* __restrict__ coef, float* __restrict__ level, float* __restrict__ level_rest,
+            float* __restrict__ pull, float* __restrict__ out_scale, T* __restrict__ dx, int64_t width, const int* __restrict__ place_of, int64_t tokens) {
   const int n = *count, c = blockIdx.x * 256 + threadIdx.x;
   float unit;
   if (alike) {
@@ -370,7 +375,10 @@ slope_terms(SlopeTerms terms, bool alike, const int* __restrict__ count, const i
     p = g * (1.0f - terms.how.smoothing);
   }
   coef[c] = v; pull[c] = p;                                      // (tokens are filled up to whole workgroups)
-  if (level) level[c] = l;
+  if (level) {
+    level[c] = to_float(from_float<T>(l));
+    level_rest[c] = l - level[c];                                // (exact)
+  }
   if (!dx) return;
   const int64_t row0 = (int64_t)blockIdx.x * 256 + (threadIdx.x & ~63);
   const int lane = threadIdx.x & 63;
@@ -417,23 +425,25 @@ __global__ void __launch_bounds__(256) clear_rest(unsigned long long* __restrict
   for (int64_t w = (int64_t)blockIdx.x * 256 + threadIdx.x; w < words; w += (int64_t)gridDim.x * 256) rest[w] = 0;
 }
 
-// db: columns of P, in `pieces` of the tokens, then over the pieces.  Bound by memory: 30 for 2000 tokens and 50257 words (6.7 TB/s, much of P still in the caches),
-// 5 for the pieces
-constexpr int kBiasPieces = 16;
+// Sums of the columns of an operand, in as many pieces of its rows (*count of them, or `rows`) as the grid is high: of P, for db; with smoothing of W, and of x with each
+// row times the rest of its level.  Bound by memory: P of 2000 tokens and 50257 words 30 (6.7 TB/s, much of it still in the caches)
+constexpr int kBiasPieces = 16, kOperandPieces = 64;
 template <typename T>
 __global__ void __launch_bounds__(256)
-sum_columns(const T* __restrict__ slope, int64_t ld, const int* __restrict__ count, float* __restrict__ sums) {
+sum_columns(const T* __restrict__ in, int64_t ld, int64_t cols, const int* __restrict__ count, int64_t rows, const float* __restrict__ times, float* __restrict__ sums) {
   __shared__ float part[8][256];
-  const int n = *count, tid = threadIdx.x, chunk = tid & 31, group = tid >> 5;
+  const int n = count ? *count : (int)rows, tid = threadIdx.x, chunk = tid & 31, group = tid >> 5;
   const int64_t col = (int64_t)blockIdx.x * 256 + chunk * 8;
-  const int begin = (int)((int64_t)blockIdx.y * n / kBiasPieces), end = (int)((int64_t)(blockIdx.y + 1) * n / kBiasPieces);
+  const int begin = (int)((int64_t)blockIdx.y * n / gridDim.y), end = (int)((int64_t)(blockIdx.y + 1) * n / gridDim.y);
   float v[8] = {};
-  if (col < ld)
+  if (col < cols)
+#pragma unroll 4
     for (int c = begin + group; c < end; c += 8) {
       Pack<T, 8> p;
-      p.load(slope + c * ld + col);
+      p.load(in + c * ld + col);
+      const float by = times ? times[c] : 1.0f;
 #pragma unroll
-      for (int e = 0; e < 8; e++) v[e] += to_float(p.v[e]);
+      for (int e = 0; e < 8; e++) v[e] = __builtin_fmaf(to_float(p.v[e]), by, v[e]);
     }
 #pragma unroll
   for (int e = 0; e < 8; e++) part[group][chunk * 8 + e] = v[e];
@@ -441,14 +451,25 @@ sum_columns(const T* __restrict__ slope, int64_t ld, const int* __restrict__ cou
   float s = 0.0f;
 #pragma unroll
   for (int g = 0; g < 8; g++) s += part[g][tid];
-  if ((int64_t)blockIdx.x * 256 + tid < ld) sums[blockIdx.y * ld + (int64_t)blockIdx.x * 256 + tid] = s;
+  if ((int64_t)blockIdx.x * 256 + tid < cols) sums[blockIdx.y * cols + (int64_t)blockIdx.x * 256 + tid] = s;
 }
+__global__ void __launch_bounds__(64) join_columns(const float* __restrict__ sums, int64_t cols, float* __restrict__ out) {
+  const int64_t col = (int64_t)blockIdx.x * 64 + threadIdx.x;
+  if (col >= cols) return;
+  float s = 0.0f;
+#pragma unroll 16
+  for (int p = 0; p < kOperandPieces; p++) s += sums[p * cols + col];
+  out[col] = s;
+}
+// db, over the pieces; `level_rests`: what the rests of all tokens' levels add up to, or null.  5 for 50257 words
 __global__ void __launch_bounds__(256)
-join_bias(const float* __restrict__ sums, int64_t ld, int64_t words, const unsigned long long* __restrict__ rest, const float* __restrict__ scale, void* __restrict__ out, int dtype) {
+join_bias(const float* __restrict__ sums, int64_t ld, int64_t words, const unsigned long long* __restrict__ rest, const float* __restrict__ level_rests, const float* __restrict__ scale,
+          void* __restrict__ out, int dtype) {
   const int64_t w = (int64_t)blockIdx.x * 256 + threadIdx.x;
   if (w >= words) return;
   float v = (float)((double)(long long)rest[w] * 0x1p-32);
   for (int p = 0; p < kBiasPieces; p++) v += sums[p * ld + w];
+  if (level_rests) v -= *level_rests;
   v = scaled(v, *scale);
   if (dtype == TF24_F32) ((float*)out)[w] = v;
   else if (dtype == TF24_F16) ((f16_t*)out)[w] = from_float<f16_t>(v);
@@ -540,7 +561,8 @@ int64_t tiles_of(int64_t size) { return (size + kTile - 1) / kTile; }
 
 struct Backward {
   uint16_t *x, *w = nullptr;
-  float *bias, *level = nullptr, *pull, *out_scale, *partial = nullptr, *sum_x = nullptr, *bias_sums = nullptr;
+  float *bias, *pull, *out_scale, *partial = nullptr, *sum_x = nullptr, *bias_sums = nullptr;
+  float *level = nullptr, *level_rest = nullptr, *level_rests = nullptr, *column_sums = nullptr, *sum_of_w = nullptr, *sum_of_x = nullptr;     // with smoothing
   float2* coef;
   unsigned long long* bias_rest = nullptr;
   uint8_t* slope;
@@ -566,7 +588,14 @@ Backward backward_of(void* base, const Sizes& z, bool input, bool weight, bool b
   if (z.pack_weight) part(b.w, z.words * z.k * 2);
   part(b.bias, z.words_filled * 4 + kOverread);
   part(b.coef, z.filled * 8 + kOverread);
-  if (z.smooth) part(b.level, z.filled * 4 + kOverread);
+  if (z.smooth) {
+    part(b.level, z.filled * 4 + kOverread);
+    part(b.level_rest, z.filled * 4 + kOverread);
+    part(b.level_rests, 4);
+    part(b.column_sums, kOperandPieces * z.k * 4);
+    part(b.sum_of_w, width_tiles * kTile * 4 + kOverread);
+    part(b.sum_of_x, width_tiles * kTile * 4 + kOverread);
+  }
   part(b.pull, z.filled * 4);
   part(b.out_scale, 4);
   part(b.slope, z.filled * b.ld * 2);
@@ -743,7 +772,7 @@ extern "C" int tf24_linear_loss_backward(const float* grad_loss, const void* x, 
   if (!alike) hipLaunchKernelGGL(slope_unit, dim3(1), dim3(1024), 0, s, terms, st.count, st.row_of, st.mass, st.lse2, b.out_scale);
   auto set_terms = [&](auto* out) {
     hipLaunchKernelGGL(slope_terms, dim3((unsigned)(z.filled / 256)), dim3(256), 0, s, terms, alike, st.count, st.row_of, entries ? nullptr : st.listed, st.mass, st.lse2, b.coef,
-                       b.level, b.pull, b.out_scale, out, width, st.place_of, tokens);
+                       b.level, b.level_rest, b.pull, b.out_scale, out, width, st.place_of, tokens);
   };
   if (dtype == TF24_F16) set_terms((f16_t*)dx);
   else set_terms((bf16_t*)dx);
@@ -755,6 +784,22 @@ extern "C" int tf24_linear_loss_backward(const float* grad_loss, const void* x, 
   if (b.w) pack(w, ldw, words, width, nullptr, nullptr, b.w, z.k, s);
   const uint8_t* w_at = (const uint8_t*)(b.w ? b.w : w);
   const int64_t w_ld = (b.w ? z.k : ldw) * 2;
+  auto sum_up = [&](const void* in, int64_t ld, int64_t cols, const int* count, int64_t rows, const float* times, int pieces, float* out) {
+    auto go = [&](auto* at) {
+      hipLaunchKernelGGL(sum_columns, dim3((unsigned)((cols + 255) / 256), pieces), dim3(256), 0, s, at, ld, cols, count, rows, times, out);
+    };
+    if (dtype == TF24_F16) go((const f16_t*)in);
+    else go((const bf16_t*)in);
+  };
+  if (z.smooth) {
+    auto column_sums = [&](const void* in, int64_t ld, const int* count, const float* times, float* out) {
+      sum_up(in, ld, z.k, count, words, times, kOperandPieces, b.column_sums);
+      hipLaunchKernelGGL(join_columns, dim3((unsigned)(z.k / 64)), dim3(64), 0, s, b.column_sums, z.k, out);
+    };
+    if (dx) column_sums(w_at, w_ld / 2, nullptr, nullptr, b.sum_of_w);
+    if (dw) column_sums(b.x, z.k, st.count, b.level_rest, b.sum_of_x);
+    if (dbias) hipLaunchKernelGGL(total_loss, dim3(1), dim3(1024), 0, s, b.level_rest, st.count, false, b.level_rests);
+  }
   for (int64_t piece = 0; piece < b.pieces; piece++) {
     const int64_t first = piece * b.ld, here = std::min(b.ld, words - first);
     HeadProduct p{};
@@ -786,22 +831,20 @@ extern "C" int tf24_linear_loss_backward(const float* grad_loss, const void* x, 
       q.a = w_at + first * w_ld; q.lda = w_ld; q.rows_k = here;
       q.stages = (int)((here + kUnitK - 1) / kUnitK); q.tiles_j = (int)tiles_of(tokens); q.most = b.most_x;
       o.out = dx; o.row_of = st.row_of; o.sum = b.sum_x; o.add = piece > 0; o.last = piece == b.pieces - 1;
-      if (int rc = launch_head_product(HEAD_INPUT, dtype, false, false, q, o, stream)) return rc;
+      o.common = b.sum_of_w; o.level_rest = b.level_rest;
+      if (int rc = launch_head_product(HEAD_INPUT, dtype, z.smooth, false, q, o, stream)) return rc;
     }
     if (dw) {
       q.a = (const uint8_t*)b.x; q.lda = z.k * 2;
       q.stages = (int)((tokens + kUnitK - 1) / kUnitK); q.tiles_j = (int)tiles_of(here); q.most = b.most_w;
       if (share_out(q.tiles_i * q.tiles_j, q.stages, q.groups, q.most).pieces == 1) q.most = 0;    // no pieces, whatever number of tokens counts
       o.out = (uint8_t*)dw + first * width * dtype_size(dw_dtype); o.sum = nullptr; o.add = false; o.last = true; o.rows_j = here;
-      if (int rc = launch_head_product(HEAD_WEIGHT, dtype, false, dw_dtype == TF24_F32, q, o, stream)) return rc;
+      o.common = b.sum_of_x;
+      if (int rc = launch_head_product(HEAD_WEIGHT, dtype, z.smooth, dw_dtype == TF24_F32, q, o, stream)) return rc;
     }
     if (dbias) {
-      auto sum = [&](auto* slope) {
-        hipLaunchKernelGGL(sum_columns, dim3((unsigned)((b.ld + 255) / 256), kBiasPieces), dim3(256), 0, s, slope, b.ld, st.count, b.bias_sums);
-      };
-      if (dtype == TF24_F16) sum((const f16_t*)b.slope);
-      else sum((const bf16_t*)b.slope);
-      hipLaunchKernelGGL(join_bias, dim3((unsigned)((here + 255) / 256)), dim3(256), 0, s, b.bias_sums, b.ld, here, b.bias_rest, b.out_scale,
+      sum_up(b.slope, b.ld, b.ld, st.count, 0, nullptr, kBiasPieces, b.bias_sums);
+      hipLaunchKernelGGL(join_bias, dim3((unsigned)((here + 255) / 256)), dim3(256), 0, s, b.bias_sums, b.ld, here, b.bias_rest, b.level_rests, b.out_scale,
                          (void*)((uint8_t*)dbias + first * dtype_size(bias_dtype)), bias_dtype);
     }
   }

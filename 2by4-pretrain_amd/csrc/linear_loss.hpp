@@ -7,7 +7,7 @@ namespace tf24 {
 struct HeadProduct;
 struct HeadResult;
 
-// smooth: with a sum of the logits (STATS) or a level that is subtracted (SLOPE); wide: float32 results (WEIGHT)
+// smooth: with a sum of the logits (STATS), less a level (SLOPE), less what all rows have in common (INPUT, WEIGHT); wide: float32 results (WEIGHT)
 int launch_head_product(int kind, int dtype, bool smooth, bool wide, const HeadProduct& p, const HeadResult& r, void* stream);
 
 // the forward product of up to kFewTokens tokens (linear_loss_few.hip), operands as they lie: slabs of kFewSlab words, bias as it is

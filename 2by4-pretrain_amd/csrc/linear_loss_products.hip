@@ -17,8 +17,9 @@ template <typename T>
 void launch_kind(int kind, bool smooth, bool wide, const HeadProduct& p, const HeadResult& r, hipStream_t s) {
   if (kind == HEAD_STATS) smooth ? launch<T, T, HEAD_STATS, true>(p, r, s) : launch<T, T, HEAD_STATS, false>(p, r, s);
   else if (kind == HEAD_SLOPE) smooth ? launch<T, T, HEAD_SLOPE, true>(p, r, s) : launch<T, T, HEAD_SLOPE, false>(p, r, s);
-  else if (kind == HEAD_INPUT) launch<T, T, HEAD_INPUT, false>(p, r, s);
-  else wide ? launch<T, float, HEAD_WEIGHT, false>(p, r, s) : launch<T, T, HEAD_WEIGHT, false>(p, r, s);
+  else if (kind == HEAD_INPUT) smooth ? launch<T, T, HEAD_INPUT, true>(p, r, s) : launch<T, T, HEAD_INPUT, false>(p, r, s);
+  else if (wide) smooth ? launch<T, float, HEAD_WEIGHT, true>(p, r, s) : launch<T, float, HEAD_WEIGHT, false>(p, r, s);
+  else smooth ? launch<T, T, HEAD_WEIGHT, true>(p, r, s) : launch<T, T, HEAD_WEIGHT, false>(p, r, s);
 }
 
 // What the pieces of the rest of a product's tiles add up to: block (tile of the rest, some of the fragments of one row).  Bound by memory: 144 tiles of 5 pieces, 189
@@ -54,6 +55,12 @@ join_pieces(const HeadProduct p, const HeadResult r) {
       continue;
     }
     if (j >= rows) continue;
+    if (r.common) {                                              // (filled up to whole tiles)
+      const float times = KIND == HEAD_INPUT ? r.level_rest[j] : 1.0f;
+      const float4v common = *reinterpret_cast<const float4v*>(r.common + i);
+#pragma unroll
+      for (int e = 0; e < 4; e++) v[e] = __builtin_fmaf(-times, common[e], v[e]);
+    }
     OutT* out = (OutT*)r.out + (KIND == HEAD_INPUT ? (int64_t)r.row_of[j] : j) * r.cols_out + i;
     OutT o[4];
 #pragma unroll
