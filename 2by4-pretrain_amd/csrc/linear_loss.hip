@@ -183,16 +183,18 @@ list_entries(const int64_t* __restrict__ indices, int64_t ld_indices, const L* _
 }
 
 // ---------------------------------------------------------------- operands as the products read them
-// Rows of `cols` 16-bit elements, filled up with zeros to `ld_out` (a multiple of 8): row c of the result is row row_of[c] of the source (null: row c),
-// or zeros behind the last of *count, up to a whole stage.  Bound by memory: 25 for 8192 x 4096 (5.4 TB/s); the weight of 50257 x 1601, whose rows are not aligned, 52
-// (6.2 TB/s, some of it from the caches).
+// Rows of `cols` 16-bit elements, filled up with zeros to `ld_out` (a multiple of 8): row c of the result is row row_of[c] of the source (null: row c).
+// Behind the last of *count, up to a whole stage, the first one stands once more (none: zeros).  P is 0 times an exponential there, which is 0 where the logits are numbers or
+// -inf: those of a row of zeros are NaN where a weight is -inf, those of a token that counts are not, or all that it gives is NaN.  Bound by memory: 25 for 8192 x 4096
+// (5.4 TB/s); the weight of 50257 x 1601, whose rows are not aligned, 52 (6.2 TB/s, some of it from the caches).
 __global__ void __launch_bounds__(256)
 pack_rows(const uint16_t* __restrict__ in, int64_t ld, int64_t rows, int64_t cols, const int* __restrict__ count, const int* __restrict__ row_of,
           uint16_t* __restrict__ out, int64_t ld_out) {
   const int64_t units = ld_out / 8;
-  if (count) rows = (int64_t)token_stages(*count) * kUnitK;
+  const int n = count ? *count : 0;
+  if (count) rows = (int64_t)token_stages(n) * kUnitK;
   for (int64_t u = (int64_t)blockIdx.x * 256 + threadIdx.x; u < rows * units; u += (int64_t)gridDim.x * 256) {
-    const int64_t c = u / units, col = (u - c * units) * 8, row = row_of ? row_of[c] : c;
+    const int64_t c = u / units, col = (u - c * units) * 8, row = row_of ? row_of[c < n ? c : 0] : c;
     int4v v = {0, 0, 0, 0};
     if (row >= 0 && col < cols) {
       const uint16_t* at = in + row * ld + col;
@@ -393,13 +395,16 @@ slope_terms(SlopeTerms terms, bool alike, const int* __restrict__ count, const i
 
 // The listed words of a piece of the vocabulary in P: one thread per token, or per entry of one; of a word listed twice the first does both.
 // `rest` (null: no gradient of the bias is wanted): by word, what rounding takes from them, in units of 2^-32.  They are most of the bias's gradient, whose sum over
-// tokens is of rounded values otherwise; as whole numbers they can be added in any order.  Bound by single accesses to P: 5 for 12288 targets, 17 for 8192 x 64 entries.
+// tokens is of rounded values otherwise; as whole numbers they can be added in any order.  Where no token counts, P of the stage of rows that the gradient of the weight
+// reads all the same is cleared: what the products made of rows of zeros is NaN where the weight or the bias is not finite.  Bound by single accesses to P: 5 for 12288 targets, 17 for 8192 x 64 entries.
 template <typename T>
 __global__ void __launch_bounds__(256)
 pull_listed(const int* __restrict__ count, const int* __restrict__ listed, const float* __restrict__ picked, const float* __restrict__ logq, int entries,
             const float2* __restrict__ coef, const float* __restrict__ level, const float* __restrict__ pull, int64_t first_word, int64_t words, T* __restrict__ slope,
             int64_t ld, unsigned long long* __restrict__ rest) {
   const int64_t listed_here = (int64_t)*count * entries;
+  if (!listed_here)
+    for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < kUnitK * ld / 8; i += (int64_t)gridDim.x * 256) reinterpret_cast<uint4*>(slope)[i] = uint4{0, 0, 0, 0};
   for (int64_t at = (int64_t)blockIdx.x * 256 + threadIdx.x; at < listed_here; at += (int64_t)gridDim.x * 256) {
     const int w = listed[at];
     if (w < first_word || w >= first_word + words) continue;

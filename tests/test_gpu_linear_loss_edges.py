@@ -50,3 +50,36 @@ def test_smoothing_of_words_that_are_not_expected(cuda, dtype, reduction, cols):
     assert ((dw.double() - want[1]).abs() <= bound).all(), ((dw.double() - want[1]).abs() - bound).max()
     bound = (tokens + 16) * E * (level.sum() + torch.zeros(words, dtype=torch.float64, device=cuda).index_add_(0, target, g * smoothing))
     assert ((db.double() - want[2]).abs() <= bound).all(), ((db.double() - want[2]).abs() - bound).max()
+
+
+@pytest.mark.parametrize("tokens", [3, 100, 300])
+def test_nothing_counts_before_weights_that_are_not_finite(cuda, tokens):
+    """Tokens that do not count give no gradient, whatever the weights and the bias have become."""
+    gen, x, w, b = operands(cuda, tokens, tokens, 72, 500, BF16, F32)
+    for value in (torch.nan, torch.inf, -torch.inf):
+        w[3, 5], b[7] = value, value
+        for reduction in ("mean", "none"):
+            grad = torch.ones(tokens if reduction == "none" else (), device=cuda)
+            for smoothing in (0.0, 0.1):
+                loss, grads = ce_step(x, w, b, torch.full((tokens,), -100, device=cuda), grad, reduction=reduction, label_smoothing=smoothing)
+                assert not loss.any() and not any(g.any() for g in grads[1:]) and not grads[0].any(), (value, reduction)
+            loss, grads = kd_step(x, w, b, torch.full((tokens, 2), -1, device=cuda), torch.zeros(tokens, 2, device=cuda), grad, reduction=reduction)
+            assert not loss.any() and not any(g.any() for g in grads), (value, reduction)
+
+
+@pytest.mark.parametrize("tokens", [3, 100, 256, 300])
+def test_words_with_a_logit_of_minus_infinity(cuda, tokens):
+    """A weight of -inf against positive x takes its word out as a bias of -inf does: probability 0, and a gradient of 0 for its row, as of a word whose bias is -inf."""
+    gen, x, w, _ = operands(cuda, tokens, tokens, 64, 300, BF16)
+    x[:, 7] = x[:, 7].abs() + 0.5
+    target = torch.randint(0, 200, (tokens,), generator=gen).to(cuda)
+    b = torch.zeros(300, device=cuda)
+    b[250] = -torch.inf
+    leaf = w.clone().requires_grad_()
+    import sparse
+    loss = sparse.linear_cross_entropy(x, leaf, target, b)
+    want, = torch.autograd.grad(loss, leaf)
+    w[250, 7] = -torch.inf
+    leaf = w.clone().requires_grad_()
+    got = sparse.linear_cross_entropy(x, leaf, target, torch.zeros_like(b))
+    assert torch.equal(got, loss) and torch.equal(torch.autograd.grad(got, leaf)[0], want) and not want[250].any()
