@@ -324,6 +324,9 @@ __device__ __forceinline__ float widened_by(const SlopeTerms& t, const float* ma
   return mass ? mass[c] : 1.0f + 2.0f * t.how.z_loss * (lse2[c] * kLn2);
 }
 
+// largest * 2^exponent, kept among float32's normal numbers: P is multiplied by the unit in the end, and nothing may become 0 times infinity on the way
+__device__ __forceinline__ float unit_of(float largest, int exponent) { return fminf(fmaxf(ldexpf(largest, exponent), 0x1p-126f), 0x1p127f); }
+
 // The unit, where tokens differ: from the largest gradient of a token's loss, and the largest factor of one relative to it (what is not finite is that anyhow).
 // 9 for 8192 tokens: two passes of one workgroup
 __global__ void __launch_bounds__(1024)
@@ -350,7 +353,7 @@ slope_unit(SlopeTerms terms, const int* __restrict__ count, const int* __restric
   v = 0.0f;
   for (int c = tid; c < n; c += 1024) v = fmaxf(v, finite(fabsf(upstream_of(terms, row_of[c], n) / unit * widened_by(terms, mass, lse2, c))));
   v = most(v);
-  if (tid == 0) *out_scale = ldexpf(unit, (v > 1.0f ? ilogbf(v) + 1 : 0) - terms.to_exponent);
+  if (tid == 0) *out_scale = unit_of(unit, (v > 1.0f ? ilogbf(v) + 1 : 0) - terms.to_exponent);
 }
 
 // The terms of 256 tokens; `alike`: all have the same gradient and a factor of one, which is the unit.  Tokens behind the last get a factor of zero, and rows of dx
@@ -364,7 +367,7 @@ slope_terms(SlopeTerms terms, bool alike, const int* __restrict__ count, const i
   float unit;
   if (alike) {
     unit = n ? fabsf(upstream_of(terms, 0, n)) : 0.0f;
-    unit = ldexpf(unit > 0.0f && unit < __builtin_inff() ? unit : 1.0f, -terms.to_exponent);
+    unit = unit_of(unit > 0.0f && unit < __builtin_inff() ? unit : 1.0f, -terms.to_exponent);
     if (c == 0) *out_scale = unit;
   } else unit = *out_scale;
   float2 v = {__builtin_inff(), 0.0f};
@@ -396,7 +399,8 @@ slope_terms(SlopeTerms terms, bool alike, const int* __restrict__ count, const i
 // The listed words of a piece of the vocabulary in P: one thread per token, or per entry of one; of a word listed twice the first does both.
 // `rest` (null: no gradient of the bias is wanted): by word, what rounding takes from them, in units of 2^-32.  They are most of the bias's gradient, whose sum over
 // tokens is of rounded values otherwise; as whole numbers they can be added in any order.  Where no token counts, P of the stage of rows that the gradient of the weight
-// reads all the same is cleared: what the products made of rows of zeros is NaN where the weight or the bias is not finite.  Bound by single accesses to P: 5 for 12288 targets, 17 for 8192 x 64 entries.
+// reads all the same is cleared: what the products made of rows of zeros is NaN where the weight or the bias is not finite.  Bound by single accesses to P: 5 for 12288
+// targets, 17 for 8192 x 64 entries.
 template <typename T>
 __global__ void __launch_bounds__(256)
 pull_listed(const int* __restrict__ count, const int* __restrict__ listed, const float* __restrict__ picked, const float* __restrict__ logq, int entries,

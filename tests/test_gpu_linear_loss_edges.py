@@ -83,3 +83,24 @@ def test_words_with_a_logit_of_minus_infinity(cuda, tokens):
     leaf = w.clone().requires_grad_()
     got = sparse.linear_cross_entropy(x, leaf, target, torch.zeros_like(b))
     assert torch.equal(got, loss) and torch.equal(torch.autograd.grad(got, leaf)[0], want) and not want[250].any()
+
+
+def test_gradients_at_the_ends_of_float32(cuda):
+    """Upstream gradients far below float32's normal numbers give gradients that are no larger, and no NaN; ones near its largest number the gradients that 16 bits hold."""
+    gen, x, w, b = operands(cuda, 3, 70, 64, 300, F16, F32)
+    target, indices, logits = torch.randint(0, 300, (70,), generator=gen).to(cuda), torch.randint(0, 300, (70, 4), generator=gen).to(cuda), draw(gen, 70, 4).to(cuda)
+    for dtype in (F16, BF16):
+        for size in (1e-37, 1e-40, 1e-44):
+            for reduction in ("sum", "none"):
+                grad = torch.tensor(size, device=cuda) if reduction == "sum" else torch.full((70,), size, device=cuda)
+                for _, grads in (ce_step(x.to(dtype), w.to(dtype), b, target, grad, reduction=reduction), kd_step(x.to(dtype), w.to(dtype), b, indices, logits, grad, reduction=reduction)):
+                    # (70 tokens, or 300 words, of at most 4 or so)
+                    assert all((g.double().abs() <= 2000 * size).all() for g in grads), (dtype, size, reduction)
+    # probabilities of a teacher that add up to e^0.5, the largest gradient of a token's loss times that past float32's largest number, that of the operands below it
+    x, w = x.to(BF16), w.to(BF16) * 2.0 ** -20
+    lse = torch.logsumexp(logits, 1) - 0.5
+    kw = dict(reduction="none", teacher_lse=lse)
+    unit, = (g[0] for _, g in (kd_step(x, w, None, indices, logits, torch.ones(70, device=cuda), **kw),))
+    large, = (g[0] for _, g in (kd_step(x, w, None, indices, logits, torch.full((70,), 2.0 ** 127, device=cuda), **kw),))
+    # (units that are a power of two apart: the same roundings)
+    assert torch.equal(large.double(), unit.double() * 2.0 ** 127)
