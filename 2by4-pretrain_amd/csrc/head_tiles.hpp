@@ -71,7 +71,7 @@ struct HeadResult {
   float* sums;                       // SMOOTH: [slab][token] sum of y
   const int* target;                 // [token], or null: the teacher's entries
   float* picked;                     // y of the target [token], of the entries [token][entries]
-  const uint32_t* slab_entries;      // [slab][token] first entry of the slab | entries << 11 | column of the first << 22
+  const uint32_t* slab_entries;      // [slab][token] first entry of the slab | entries << 11
   const int* entry_words;            // [token][entries] ascending
   int entries;
   // HEAD_SLOPE

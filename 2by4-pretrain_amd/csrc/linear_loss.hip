@@ -174,7 +174,7 @@ list_entries(const int64_t* __restrict__ indices, int64_t ld_indices, const L* _
         if (key[mid] != ~0ull && (int)(key[mid] >> 32) / slab_words == slab) low = mid;
         else high = mid;
       }
-      slab_entries[(int64_t)slab * filled + c] = (uint32_t)k | (uint32_t)(high - k) << 11 | (uint32_t)(w - slab * slab_words) << 22;
+      slab_entries[(int64_t)slab * filled + c] = (uint32_t)k | (uint32_t)(high - k) << 11;
     }
   }
 #pragma unroll
@@ -214,9 +214,8 @@ __global__ void __launch_bounds__(256)
 prepare_words(const void* __restrict__ bias, int dtype, int64_t words, int64_t filled, float scale, float* __restrict__ out, uint32_t* __restrict__ clear, int64_t cleared) {
   const int64_t first = (int64_t)blockIdx.x * 256 + threadIdx.x, step = (int64_t)gridDim.x * 256;
   for (int64_t i = first; out && i < filled; i += step) {
-    float v = 0.0f;
-    if (i >= words) v = -__builtin_inff();
-    else if (bias) v = (dtype == TF24_F32 ? ((const float*)bias)[i] : dtype == TF24_F16 ? to_float(((const f16_t*)bias)[i]) : to_float(((const bf16_t*)bias)[i])) * scale;
+    float v = -__builtin_inff();
+    if (i < words) v = (dtype == TF24_F32 ? ((const float*)bias)[i] : dtype == TF24_F16 ? to_float(((const f16_t*)bias)[i]) : to_float(((const bf16_t*)bias)[i])) * scale;
     out[i] = v;
   }
   for (int64_t i = first; i < cleared; i += step) reinterpret_cast<uint4*>(clear)[i] = uint4{0, 0, 0, 0};

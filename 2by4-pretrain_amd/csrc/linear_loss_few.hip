@@ -174,7 +174,7 @@ few_tokens(const uint16_t* __restrict__ x, int64_t ldx, const uint16_t* __restri
   }
   // four threads a token, 16 words each
   const int token = tid >> 2, quarter = tid & 3;
-  if (token >= n || token >= 16 * N) return;                     // (whole groups of four)
+  if (token >= n) return;                                        // (whole groups of four; n is 16 * N at most)
   float y[16], m = -__builtin_inff(), sum = 0.0f, total = 0.0f;
 #pragma unroll
   for (int e = 0; e < 16; e++) {

@@ -60,7 +60,7 @@ class _linear_loss(autograd.Function):
                 ignore_index, ptr(indices), ld_indices, ptr(teacher_logits), ld_teacher, code[teacher_logits.dtype] if entries else N.F32, ptr(teacher_lse), entries,
                 smoothing, z_loss, 1.0 / temperature, reduction, loss.data_ptr(), state.data_ptr(), state.numel(), workspace.data_ptr(), nbytes, N.stream_ptr()))
         if any(ctx.needs_input_grad[:3]):
-            ctx.save_for_backward(x, weight if weight16 is weight else weight16, bias, state)
+            ctx.save_for_backward(x, weight16, bias, state)
         return loss
 
     @staticmethod
