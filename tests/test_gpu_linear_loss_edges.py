@@ -52,6 +52,56 @@ def test_smoothing_of_words_that_are_not_expected(cuda, dtype, reduction, cols):
     assert ((db.double() - want[2]).abs() <= bound).all(), ((db.double() - want[2]).abs() - bound).max()
 
 
+@pytest.mark.parametrize("tokens,cols", [(32768, 512), (30011, 600)])
+@pytest.mark.parametrize("smoothing", [0.0, 0.1])
+def test_whole_tiles_over_pieces_of_the_vocabulary(cuda, tokens, cols, smoothing):
+    """The gradient of x from several pieces of the vocabulary: 256 tiles, each in one piece of k on a card of 256 compute units, and 354, some of which are cut."""
+    gen, x, w, b = operands(cuda, tokens, tokens, cols, 40000, BF16, F32)
+    target = torch.where(torch.rand(tokens, generator=gen) < 0.001, -100, torch.randint(0, 40000, (tokens,), generator=gen)).to(cuda)
+    ce_check(cuda, x, w, b, target, label_smoothing=smoothing)
+
+
+@pytest.mark.parametrize("words", [95, 96, 97, 255, 256, 257, 512, 671, 672, 673])
+@pytest.mark.parametrize("tokens", [255, 256, 257, 511, 512, 513])
+def test_ends_of_tiles(cuda, tokens, words):
+    """Tiles of 256 tokens and 256 words, stages of 64 words of which half may lie behind the last."""
+    gen, x, w, b = operands(cuda, tokens + words, tokens, 64 if words % 2 else 136, words, BF16 if tokens % 2 else F16, F32)
+    target = torch.randint(0, words, (tokens,), generator=gen).to(cuda)
+    ce_check(cuda, x, w, b, target, label_smoothing=0.1 if words % 3 else 0.0)
+    indices = torch.randint(-1, words, (tokens, 5), generator=gen).to(cuda)
+    kd_check(cuda, x, w, b, indices, draw(gen, tokens, 5).to(cuda))
+
+
+@pytest.mark.parametrize("counted", [0, 1, 63, 64, 65, 255, 256, 257, 512])
+def test_numbers_of_tokens_that_count(cuda, counted):
+    gen, x, w, b = operands(cuda, counted, 700, 320, 900, BF16, F32)
+    counts = torch.zeros(700, dtype=torch.bool)
+    counts[torch.randperm(700, generator=gen)[:counted]] = True
+    target = torch.where(counts, torch.randint(0, 900, (700,), generator=gen), -100).to(cuda)
+    ce_check(cuda, x, w, b, target, "none", label_smoothing=0.1)
+    ce_check(cuda, x, w, b, target)
+    indices = torch.where(counts[:, None], torch.randint(0, 900, (700, 7), generator=gen), -1).to(cuda)
+    kd_check(cuda, x, w, b, indices, draw(gen, 700, 7).to(cuda), "none")
+
+
+@pytest.mark.parametrize("tokens", [1, 40, 64, 300])
+def test_rows_that_do_not_count_are_not_read(cuda, tokens):
+    """Infinities and NaN in them reach neither the losses nor a gradient, through any kernel and both losses."""
+    gen, x, w, b = operands(cuda, tokens, tokens, 128, 1000, F16, F32)
+    skipped = torch.rand(tokens, generator=gen) < 0.5
+    skipped[0] = True
+    target = torch.where(skipped, -100, torch.randint(0, 1000, (tokens,), generator=gen)).to(cuda)
+    indices = torch.where(skipped[:, None], -1, torch.randint(0, 1000, (tokens, 6), generator=gen)).to(cuda)
+    logits = draw(gen, tokens, 6).to(cuda)
+    grad = torch.rand(tokens, generator=gen).to(cuda)
+    dirty = x.clone()
+    dirty[skipped.to(cuda)] = torch.tensor([torch.nan, torch.inf, -torch.inf, 65504.0], dtype=F16, device=cuda).repeat(32)
+    for step in (lambda v: ce_step(v, w, b, target, grad, reduction="none", label_smoothing=0.1), lambda v: kd_step(v, w, b, indices, logits, grad, reduction="none")):
+        clean, got = step(x), step(dirty)
+        assert torch.equal(clean[0], got[0]) and all(torch.equal(a, c) for a, c in zip(clean[1], got[1]))
+        assert all(t.isfinite().all() for t in (got[0], *got[1])) and not got[1][0][skipped.to(cuda)].any()
+
+
 @pytest.mark.parametrize("tokens", [3, 100, 300])
 def test_nothing_counts_before_weights_that_are_not_finite(cuda, tokens):
     """Tokens that do not count give no gradient, whatever the weights and the bias have become."""
@@ -104,3 +154,41 @@ def test_gradients_at_the_ends_of_float32(cuda):
     large, = (g[0] for _, g in (kd_step(x, w, None, indices, logits, torch.full((70,), 2.0 ** 127, device=cuda), **kw),))
     # (units that are a power of two apart: the same roundings)
     assert torch.equal(large.double(), unit.double() * 2.0 ** 127)
+
+
+def test_order_of_tokens(cuda):
+    """Permuted tokens give the same loss and the same gradients up to the order of float32 sums: at most as many additions as there are tokens or words, of the magnitudes
+    added, and a rounding of x's gradient.  The products that are added are the same."""
+    gen, x, w, b = operands(cuda, 71, 300, 64, 500, BF16, F32)
+    target = torch.randint(0, 40, (300,), generator=gen).to(cuda)
+    z = definition.logits(x, w, b)
+    _, slope, counts = definition.cross_entropy(z, target)
+    order = torch.randperm(300, generator=gen).to(cuda)
+    one = torch.tensor(1.0, device=cuda)
+    loss, (dx, dw, db) = ce_step(x, w.float(), b, target, one, reduction="sum")
+    other, (dx2, dw2, db2) = ce_step(x[order], w.float(), b, target[order], one, reduction="sum")
+    assert abs(loss - other) <= 2 * E * loss                       # (summed in float64, rounded once)
+    assert torch.equal(dx2, dx[order])
+    # (a factor of 1.01 for probabilities that are rounded to 8 bits)
+    assert ((dw - dw2).abs().double() <= 1.01 * 600 * E * (slope.abs().t() @ x.double().abs())).all()
+    assert ((db - db2).abs().double() <= 1.01 * 600 * E * slope.abs().sum(0)).all()
+
+
+def test_what_the_workspace_held_does_not_matter(cuda):
+    """NaN, zeros and large numbers in the memory that workspaces, states and results are made in: the same bits."""
+    gen, x, w, b = operands(cuda, 5, 333, 200, 5003, BF16, F32)
+    target = torch.where(torch.rand(333, generator=gen) < 0.3, -100, torch.randint(0, 5003, (333,), generator=gen)).to(cuda)
+    indices, logits = torch.where(torch.rand(333, 9, generator=gen) < 0.5, -1, torch.randint(0, 5003, (333, 9), generator=gen)).to(cuda), draw(gen, 333, 9).to(cuda)
+    grad = torch.rand(333, generator=gen).to(cuda)
+    first = None
+    for fill in (0, 255, 126):
+        torch.cuda.empty_cache()
+        held = [torch.full((1 << 28,), fill, dtype=torch.uint8, device=cuda)] + [torch.full((1 << 19,), fill, dtype=torch.uint8, device=cuda) for _ in range(64)]
+        del held
+        got = []
+        for some in (slice(None), slice(0, 50)):
+            for loss, grads in (ce_step(x[some], w, b, target[some], grad[some], reduction="none", label_smoothing=0.1, z_loss=1e-3), kd_step(x[some], w, b, indices[some], logits[some], grad[some], reduction="none")):
+                got += [loss, *grads]
+        if first is None:
+            first = got
+        assert all(torch.equal(a, c) for a, c in zip(got, first)), fill
