@@ -192,3 +192,57 @@ def test_what_the_workspace_held_does_not_matter(cuda):
         if first is None:
             first = got
         assert all(torch.equal(a, c) for a, c in zip(got, first)), fill
+
+
+@pytest.mark.parametrize("tokens,cols,words", [(70, 65536, 300), (3, 65536, 97), (100, 24, 1 << 22), (3, 24, 1 << 22), (1 << 22, 24, 100)])
+def test_largest_sizes(cuda, tokens, cols, words):
+    """2^16 columns, 2^22 words, 2^22 tokens; the last word and the last token among those that matter."""
+    gen, x, w, b = operands(cuda, 9, tokens, cols, words, BF16, F32)
+    target = torch.where(torch.rand(tokens, generator=gen) < 0.3, -100, torch.randint(0, words, (tokens,), generator=gen))
+    target[-1] = words - 1
+    target = target.to(cuda)
+    ce_check(cuda, x, w, b, target, label_smoothing=0.1)
+    indices = torch.randint(0, words, (tokens, 3), generator=gen)
+    indices[-1, 1] = words - 1
+    kd_check(cuda, x, w, b, indices.to(cuda), draw(gen, tokens, 3).to(cuda))
+
+
+def test_smoothing_of_any_layout_each_gradient_alone_and_replayed(cuda):
+    """Weights in wider rows, in the middle of a dword, expanded; gradients one by one; a captured step with eager work between its replays: the same bits."""
+    import sparse
+    gen, x, w, b = operands(cuda, 13, 300, 128, 3000, BF16, F32)
+    target = torch.where(torch.rand(300, generator=gen) < 0.3, -100, torch.randint(0, 3000, (300,), generator=gen)).to(cuda)
+    grad = torch.rand(300, generator=gen).to(cuda)
+    kw = dict(reduction="none", label_smoothing=0.1, z_loss=1e-3)
+    want = ce_step(x, w, b, target, grad, **kw)
+    for start, ld in ((24, 200), (3, 200), (1, 129)):
+        held = torch.full((3000 * ld + start,), torch.nan, dtype=BF16, device=cuda).as_strided((3000, 128), (ld, 1), start)
+        held.copy_(w)
+        got = ce_step(x, held, b, target, grad, **kw)
+        assert torch.equal(got[0], want[0]) and all(torch.equal(a, c) for a, c in zip(got[1], want[1]))
+    for i in range(3):
+        leaves = [t.detach().requires_grad_(i == n) for n, t in enumerate((x, w, b))]
+        got, = torch.autograd.grad(sparse.linear_cross_entropy(leaves[0], leaves[1], target, leaves[2], **kw), leaves[i], grad)
+        assert torch.equal(got, want[1][i])
+    same = w[:1].expand(3000, 128)
+    for a, c in zip(ce_step(x, same, b, target, grad, **kw)[1], ce_step(x, same.contiguous(), b, target, grad, **kw)[1]):
+        assert torch.equal(a, c)
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        ce_step(x, w, b, target, grad, **kw)
+    torch.cuda.synchronize()
+    held = [x.clone(), target.clone(), grad.clone()]
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out = ce_step(held[0], w, b, held[1], held[2], **kw)
+    for n in range(4):
+        batch = [t.roll(n, 0) for t in (x, target, grad)]
+        if n == 2:
+            batch[1] = torch.full_like(target, -100)
+        for h, t in zip(held, batch):
+            h.copy_(t)
+        graph.replay()
+        eager = ce_step(batch[0], w, b, batch[1], batch[2], **kw)
+        torch.cuda.synchronize()
+        assert torch.equal(out[0], eager[0]) and all(torch.equal(a, c) for a, c in zip(out[1], eager[1])), n
