@@ -313,7 +313,7 @@ total_loss(const float* __restrict__ by_place, const int* __restrict__ count, bo
 // all tokens (by 0.39 % of it at worst in bfloat16), which no sum averages out.  So P has the nearest number of 16 bits in its place, and what is left of it comes to the results
 // in float32: dx is P W less the rest times the sum of W's rows, dW P^T x less the sum of x's rows times their rests, db the sum of P less that of the rests.  (Without a
 // level in P a word whose probability is near it would be off by more: by a step of p, not one of the difference.)  W is read once more for it: both passes of 2000 tokens against
-// 50257 x 1280 1150 and 1190, of one token against 50304 x 768 157 and 182.
+// 50257 x 1280 1172 and 1204, of one token against 50304 x 768 156 and 176.
 struct SlopeTerms { const float* grad; int reduction; LossTerms how; float inv_temperature; int to_exponent; };
 __device__ __forceinline__ float upstream_of(const SlopeTerms& t, int row, int n) {
   const float g = t.reduction == TF24_REDUCE_NONE ? t.grad[row] : t.reduction == TF24_REDUCE_MEAN ? t.grad[0] / (float)n : t.grad[0];
@@ -433,14 +433,20 @@ __global__ void __launch_bounds__(256) clear_rest(unsigned long long* __restrict
   for (int64_t w = (int64_t)blockIdx.x * 256 + threadIdx.x; w < words; w += (int64_t)gridDim.x * 256) rest[w] = 0;
 }
 
-// Sums of the columns of an operand, in as many pieces of its rows (*count of them, or `rows`) as the grid is high: of P, for db; with smoothing of W, and of x with each
-// row times the rest of its level.  Bound by memory: P of 2000 tokens and 50257 words 30 (6.7 TB/s, much of it still in the caches)
+// Sums of the columns of one or two operands (blockIdx.z), in as many pieces of their rows (*count of them, or `rows`) as the grid is high: of P, for db; with smoothing of W,
+// and of x with each row times the rest of its level.  Bound by memory: P of 2000 tokens and 50257 words 30 (6.7 TB/s, much of it still in the caches), the weight of 50257 x
+// 1280 and 2000 rows of x 20 (6.7 TB/s, from the caches as well).
+struct ColumnSums { const void* in; int64_t ld; const int* count; int64_t rows; const float* times; float *pieces, *out; };
 constexpr int kBiasPieces = 16, kOperandPieces = 64;
 template <typename T>
 __global__ void __launch_bounds__(256)
-sum_columns(const T* __restrict__ in, int64_t ld, int64_t cols, const int* __restrict__ count, int64_t rows, const float* __restrict__ times, float* __restrict__ sums) {
+sum_columns(const ColumnSums one, const ColumnSums other, int64_t cols) {
   __shared__ float part[8][256];
-  const int n = count ? *count : (int)rows, tid = threadIdx.x, chunk = tid & 31, group = tid >> 5;
+  const ColumnSums& which = blockIdx.z ? other : one;
+  const T* in = (const T*)which.in;
+  const float* times = which.times;
+  const int64_t ld = which.ld;
+  const int n = which.count ? *which.count : (int)which.rows, tid = threadIdx.x, chunk = tid & 31, group = tid >> 5;
   const int64_t col = (int64_t)blockIdx.x * 256 + chunk * 8;
   const int begin = (int)((int64_t)blockIdx.y * n / gridDim.y), end = (int)((int64_t)(blockIdx.y + 1) * n / gridDim.y);
   float v[8] = {};
@@ -459,15 +465,16 @@ sum_columns(const T* __restrict__ in, int64_t ld, int64_t cols, const int* __res
   float s = 0.0f;
 #pragma unroll
   for (int g = 0; g < 8; g++) s += part[g][tid];
-  if ((int64_t)blockIdx.x * 256 + tid < cols) sums[blockIdx.y * cols + (int64_t)blockIdx.x * 256 + tid] = s;
+  if ((int64_t)blockIdx.x * 256 + tid < cols) which.pieces[blockIdx.y * cols + (int64_t)blockIdx.x * 256 + tid] = s;
 }
-__global__ void __launch_bounds__(64) join_columns(const float* __restrict__ sums, int64_t cols, float* __restrict__ out) {
+__global__ void __launch_bounds__(64) join_columns(const ColumnSums one, const ColumnSums other, int64_t cols) {
+  const ColumnSums& which = blockIdx.y ? other : one;
   const int64_t col = (int64_t)blockIdx.x * 64 + threadIdx.x;
   if (col >= cols) return;
   float s = 0.0f;
 #pragma unroll 16
-  for (int p = 0; p < kOperandPieces; p++) s += sums[p * cols + col];
-  out[col] = s;
+  for (int p = 0; p < kOperandPieces; p++) s += which.pieces[p * cols + col];
+  which.out[col] = s;
 }
 // db, over the pieces; `level_rests`: what the rests of all tokens' levels add up to, or null.  5 for 50257 words
 __global__ void __launch_bounds__(256)
@@ -600,7 +607,7 @@ Backward backward_of(void* base, const Sizes& z, bool input, bool weight, bool b
     part(b.level, z.filled * 4 + kOverread);
     part(b.level_rest, z.filled * 4 + kOverread);
     part(b.level_rests, 4);
-    part(b.column_sums, kOperandPieces * z.k * 4);
+    part(b.column_sums, 2 * kOperandPieces * z.k * 4);
     part(b.sum_of_w, width_tiles * kTile * 4 + kOverread);
     part(b.sum_of_x, width_tiles * kTile * 4 + kOverread);
   }
@@ -792,22 +799,19 @@ extern "C" int tf24_linear_loss_backward(const float* grad_loss, const void* x, 
   if (b.w) pack(w, ldw, words, width, nullptr, nullptr, b.w, z.k, s);
   const uint8_t* w_at = (const uint8_t*)(b.w ? b.w : w);
   const int64_t w_ld = (b.w ? z.k : ldw) * 2;
-  auto sum_up = [&](const void* in, int64_t ld, int64_t cols, const int* count, int64_t rows, const float* times, int pieces, float* out) {
-    auto go = [&](auto* at) {
-      hipLaunchKernelGGL(sum_columns, dim3((unsigned)((cols + 255) / 256), pieces), dim3(256), 0, s, at, ld, cols, count, rows, times, out);
-    };
-    if (dtype == TF24_F16) go((const f16_t*)in);
-    else go((const bf16_t*)in);
+  auto sum_up = [&](const ColumnSums& one, const ColumnSums* other, int64_t cols, int pieces) {
+    const dim3 grid((unsigned)((cols + 255) / 256), pieces, other ? 2 : 1);
+    if (dtype == TF24_F16) hipLaunchKernelGGL(sum_columns<f16_t>, grid, dim3(256), 0, s, one, other ? *other : one, cols);
+    else hipLaunchKernelGGL(sum_columns<bf16_t>, grid, dim3(256), 0, s, one, other ? *other : one, cols);
   };
-  if (z.smooth) {
-    auto column_sums = [&](const void* in, int64_t ld, const int* count, const float* times, float* out) {
-      sum_up(in, ld, z.k, count, words, times, kOperandPieces, b.column_sums);
-      hipLaunchKernelGGL(join_columns, dim3((unsigned)(z.k / 64)), dim3(64), 0, s, b.column_sums, z.k, out);
-    };
-    if (dx) column_sums(w_at, w_ld / 2, nullptr, nullptr, b.sum_of_w);
-    if (dw) column_sums(b.x, z.k, st.count, b.level_rest, b.sum_of_x);
-    if (dbias) hipLaunchKernelGGL(total_loss, dim3(1), dim3(1024), 0, s, b.level_rest, st.count, false, b.level_rests);
+  if (z.smooth && (dx || dw)) {
+    const ColumnSums of_w{w_at, w_ld / 2, nullptr, words, nullptr, b.column_sums, b.sum_of_w};
+    const ColumnSums of_x{b.x, z.k, st.count, 0, b.level_rest, b.column_sums + kOperandPieces * z.k, b.sum_of_x};
+    const ColumnSums& one = dx ? of_w : of_x;
+    sum_up(one, dx && dw ? &of_x : nullptr, z.k, kOperandPieces);
+    hipLaunchKernelGGL(join_columns, dim3((unsigned)(z.k / 64), dx && dw ? 2 : 1), dim3(64), 0, s, one, of_x, z.k);
   }
+  if (z.smooth && dbias) hipLaunchKernelGGL(total_loss, dim3(1), dim3(1024), 0, s, b.level_rest, st.count, false, b.level_rests);
   for (int64_t piece = 0; piece < b.pieces; piece++) {
     const int64_t first = piece * b.ld, here = std::min(b.ld, words - first);
     HeadProduct p{};
@@ -851,7 +855,7 @@ extern "C" int tf24_linear_loss_backward(const float* grad_loss, const void* x, 
       if (int rc = launch_head_product(HEAD_WEIGHT, dtype, z.smooth, dw_dtype == TF24_F32, q, o, stream)) return rc;
     }
     if (dbias) {
-      sum_up(b.slope, b.ld, b.ld, st.count, 0, nullptr, kBiasPieces, b.bias_sums);
+      sum_up(ColumnSums{b.slope, b.ld, st.count, 0, nullptr, b.bias_sums, nullptr}, nullptr, b.ld, kBiasPieces);
       hipLaunchKernelGGL(join_bias, dim3((unsigned)((here + 255) / 256)), dim3(256), 0, s, b.bias_sums, b.ld, here, b.bias_rest, b.level_rests, b.out_scale,
                          (void*)((uint8_t*)dbias + first * dtype_size(bias_dtype)), bias_dtype);
     }
