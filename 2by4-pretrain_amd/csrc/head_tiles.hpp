@@ -18,6 +18,8 @@
 // 1.93 GHz (6.4, 6.7, 6.7 and 6.3 ms; 1.34, 1.28, 1.28 and 1.36 PFLOP/s; a library's product of the same sizes with nothing of a loss in it 5.9, 6.3 for dx, 7.4 for dW).
 // Short ones by what stands between the tiles, a quarter of STATS and SLOPE at a width of 768: 12288 tokens, 50304 x 768 0.94, 0.93, 0.82 + 0.05 and 0.70 + 0.02 ms
 // (1.01 to 1.35 PFLOP/s; the library 0.85, 1.33 for dx, 0.99 for dW).
+// Registers: the accumulators leave 256 of a lane's 512.  The compiler keeps 4 to 9 more in memory for STATS and SLOPE (20 to 40 bytes a lane), 57 to 65 for INPUT and WEIGHT (172 to
+// 200): none in the loop over the stages, all where a unit begins and ends.  A reload there waits for the copies ahead of it, which is part of what stands between the tiles.
 // 256 x 256 tiles against 192 x 192, both passes: 8192 tokens, 128000 x 4096 26.5 and 30.6 ms; 8192 tokens, 50304 x 1024 2.93 and 3.33; 1024 tokens, 50304 x 768 0.42
 // and 0.39 (788 tiles are 3.1 rounds on 256 compute units).  Two buffers of 64 elements of k against four
 // of 32: the forward pass of the first 6.9 and 6.4 ms.

@@ -14,11 +14,11 @@
 // P is rounded to the operands' type as the operand of a matrix instruction: relative to each of its elements, which is what a
 // 16-bit gradient of the logits is rounded to as well.  It is formed in units of the largest gradient of a token's loss (float16: of 2^-14 of it), which come
 // back behind the products, so that the small probabilities of a large batch do not vanish in float16.
-// All sums are float32 (the loss over tokens: float64), in an order that the sizes alone decide.
+// All sums are float32 (the loss over tokens: float64), in an order that the sizes, the number of tokens that count and that of compute units decide.
 //
 // Bound by the matrix units and, in long products, by the power that they may draw (zeros for operands: 22.4 ms instead of 26.5).  Both passes in bf16, floor at the
-// 1.52 PFLOP/s of a large library product (three products) and measured: 12288 tokens, 50304 x 768 1.87 and 3.52 ms; 8192 tokens, 128000 x 4096 16.9 and
-// 26.2 ms, four products at 1.31 PFLOP/s.  Everything but the four products: 0.14 and 0.15 ms.  The kernels' own figures stand beside them (us; head_tiles.hpp has
+// 1.52 PFLOP/s of a large library product (three products) and measured (cards differ by 4 %; two figures that are compared are of one card): 12288 tokens, 50304 x 768 1.87
+// and 3.46 to 3.67 ms; 8192 tokens, 128000 x 4096 16.9 and 25.8 to 27.0 ms, four products at 1.27 to 1.33 PFLOP/s.  Everything but the four products: 0.14 and 0.15 ms.  The kernels' own figures stand beside them (us; head_tiles.hpp has
 // the products').
 #include "linear_loss.hpp"
 #include "head_tiles.hpp"

@@ -543,8 +543,9 @@ int tf24_linear16_suits(int64_t rows, int64_t k, int64_t tokens);
  *   reduction  tf24_reduction: loss float, one number (the mean over tokens that count; of none: 0) or [tokens] (0 for those that do not count)
  *   state      what the backward pass needs besides the operands: tf24_linear_loss_state_bytes(tokens, entries or 0), 16-byte aligned
  *   workspace  16-byte aligned, as many bytes as the function below says for the same sizes, `smooth` (smoothing is not 0), w and ldw
- * Nothing of the rows of x that do not count is read.  Sums in float32, in an order that the sizes alone decide.  The reference has no such
- * operator: the model that its recipe trains (README.md:56-118) brings its own head and loss.
+ * Nothing of the rows of x that do not count is read.  Sums in float32, in an order that the sizes, the number of tokens that count and that of the device's compute units
+ * decide, and no atomics on them: the same call gives the same bits.  The reference has no such operator: the model that its recipe trains (README.md:56-118) brings its own
+ * head and loss.
  */
 typedef enum { TF24_REDUCE_MEAN = 0, TF24_REDUCE_SUM = 1, TF24_REDUCE_NONE = 2 } tf24_reduction;
 int tf24_linear_loss_forward(const void* x, int64_t ldx, const void* w, int64_t ldw, const void* bias, int bias_dtype, int dtype, int64_t tokens, int64_t width,
